@@ -33,6 +33,9 @@ typedef struct rstr_model rstr_model;
 typedef struct rstr_pool rstr_pool;
 typedef struct rstr_decoder rstr_decoder;
 typedef struct rstr_transfer rstr_transfer;
+typedef struct rstr_kv4 rstr_kv4;
+typedef struct rstr_kv4_attn rstr_kv4_attn;
+typedef struct rstr_verify rstr_verify;
 
 /* Descriptor flags of src/pretrained/arch/{gemma3,qwen3,llama}.clj plus the HF
  * hyper-parameters read by decoder.clj:31-56 (load-hf). */
@@ -235,6 +238,10 @@ int rstr_decoder_step_timing(rstr_decoder* d, double* out, int32_t n);
 /* Logits [batch][vocab] of the last step (decode-row! returning logits,
  * decoder_gpu.clj:1158-1170). */
 int rstr_decode_logits(rstr_decoder* d, float* logits_out);
+/* No counterpart in the reference: the device address of those logits, f32
+ * [batch][vocab], for operators on device arrays (rstr_verify_run).  Valid until
+ * the decoder closes; written by every step on the session's stream. */
+int rstr_decode_logits_device(rstr_decoder* d, const float** out);
 /* Resident input rows [batch][d_model] (the state :r0). */
 int rstr_decoder_read_rows(rstr_decoder* d, float* out);
 /* 1 (default): replay each step as one captured HIP graph; 0: launch eagerly. */
@@ -360,6 +367,114 @@ enum {
  * launch count over the run. */
 int rstr_decoder_profile_steps(rstr_decoder* d, int32_t first, int32_t count, float* class_ms,
                                int32_t* class_launches);
+
+/* ---- operators on device arrays -------------------------------------------------
+ * No counterpart in the reference.  A cache of 4-bit blocks, the attention that
+ * reads it, the tables of a step that brings several tokens per sequence, and the
+ * verification of drafted tokens.  Unlike the entries above, these take arrays in
+ * the memory of the session's GPU and queue their kernels on `stream`: a
+ * hipStream_t of that GPU (NULL: its default stream), or RSTR_SESSION_STREAM for
+ * the session's own.  They return once queued, allocate, copy and wait for
+ * nothing, leave the caller's current device as it was, and may be captured into
+ * a graph.  Arrays stay alive and unchanged until the work has run; the caller
+ * orders streams (the session's is not ordered with the default stream).
+ * Arguments that the host can see are checked before anything is queued.  What
+ * only the device can see is bounded there: no index read from an array, whatever
+ * its value, leads outside the arrays and the cache.
+ *
+ * Element types (as rstr_tensor_raw.dtype) and rows: a [rows][heads][head_dim] array is given by
+ * its address, its element type and its row and head strides in elements;
+ * head_dim is contiguous. */
+enum { RSTR_F32 = 0, RSTR_F16 = 1, RSTR_BF16 = 2 };
+#define RSTR_SESSION_STREAM ((void*)-1)
+
+/* A paged K/V cache in 4 bits: blocks of 32 consecutive elements of a head's row,
+ * each an fp16 scale d and 32 codes that stand for d * (code - 8): 4.5 bits an
+ * element.  head_dim 64, 128 or 256; page_size a multiple of 16;
+ * physical_pages * page_size < 2^31.  All zeros when opened.  The layout inside
+ * a page is the library's own: rows go in and out through append and read. */
+int rstr_kv4_open(rstr_session* s, int32_t n_layers, int32_t n_kv, int32_t head_dim, int32_t page_size,
+                  int32_t physical_pages, rstr_kv4** out);
+/* Waits for the device.  RSTR_E_STATE while attention plans are open on it. */
+int rstr_kv4_close(rstr_kv4* p);
+/* Device bytes of the cache. */
+int64_t rstr_kv4_bytes(const rstr_kv4* p);
+/* Quantises rows k, v [rows][n_kv][head_dim] of one layer into the slots
+ * slots[rows] (page * page_size + offset); a row whose slot is negative or
+ * outside the cache is skipped.  Per block, with m its first element of greatest
+ * magnitude: d = fp16(-m / 8), at most 65504 in magnitude; code = x / d rounded to
+ * nearest, ties to even, plus 8, kept in [0, 15] (8 where d is 0).  A block with a NaN or an
+ * infinity becomes NaN.  Slots of one call are distinct: two rows for one slot
+ * leave a mixture of both there. */
+int rstr_kv4_append(rstr_kv4* p, int32_t layer, int32_t rows, int32_t dtype, const void* k, int64_t k_row,
+                    int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int32_t* slots, void* stream);
+/* The values that slots[rows] hold, rounded once to the output's type, as rows
+ * k, v; zeros for a slot outside the cache.  A slot may be listed twice. */
+int rstr_kv4_read(rstr_kv4* p, int32_t layer, int32_t rows, int32_t dtype, const int32_t* slots, void* k,
+                  int64_t k_row, int64_t k_head, void* v, int64_t v_row, int64_t v_head, void* stream);
+
+/* A plan for attention of up to max_batch sequences and max_rows query rows of
+ * n_q heads: the call's workspace.  One plan serves one call at a time: calls
+ * (and graphs that hold them) that may run at once need a plan each. */
+int rstr_kv4_attn_open(rstr_kv4* p, int32_t n_q, int32_t max_batch, int32_t max_rows, rstr_kv4_attn** out);
+/* Waits for the device. */
+int rstr_kv4_attn_close(rstr_kv4_attn* a);
+/* Attention over one layer.  Sequence b has the query rows
+ * [row_offsets[b], row_offsets[b+1]), its last tokens; it holds lengths[b] tokens
+ * (these included) in the pages page_table[b][0 .. pages_per_seq).  The row at
+ * token p sees the tokens j <= p, and with window > 0 only j > p - window:
+ * out = sum softmax(scale * q . k_j) v_j, in the type of q (f32: products and sums
+ * in fp32 precision; f16, bf16: probabilities rounded to 11 bits).  A row that
+ * sees no token (length 0, more rows than tokens) is 0.  Tokens of a page id outside
+ * the cache are not seen, nor are tokens behind the table's width.  Rows behind
+ * row_offsets[batch] are left as they are; row_offsets must not decrease.
+ * max_rows: the most rows a sequence of this call has (it chooses the tile; a sequence
+ * with more is still computed). */
+int rstr_kv4_attn_run(rstr_kv4_attn* a, int32_t layer, int32_t dtype, int32_t batch, int32_t rows,
+                      int32_t max_rows, int32_t window, float scale, const void* q, int64_t q_row, int64_t q_head,
+                      const int32_t* row_offsets, const int32_t* page_table, int32_t pages_per_seq,
+                      const int32_t* lengths, void* out, int64_t out_row, int64_t out_head, void* stream);
+
+/* The descriptors of a step in which sequence b, of lengths[b] tokens, gets
+ * counts[b] more.  New pages come from free_pages[0 .. n_free) in order, sequence
+ * by sequence; pages already in page_table[batch][pages_per_seq] are kept and the
+ * new ones written behind them.  A sequence is served if its tokens fit
+ * pages_per_seq, the list lasts (one that needs no new page is served after it
+ * has run out) and its rows fit `rows`; otherwise it keeps its length and has no rows.
+ * Writes new_lengths[batch], row_offsets[batch+1] (of the rows served),
+ * positions[rows] and slots[rows] (0 and -1 behind the last row; positions
+ * include start_positions[batch] where given) and pages_taken[0], the length of the
+ * list's part that is used up.  Outputs may not overlap inputs.  batch up to
+ * RSTR_STEP_MAPS_BATCH. */
+#define RSTR_STEP_MAPS_BATCH 8192
+int rstr_step_maps(rstr_session* s, int32_t page_size, int32_t batch, int32_t pages_per_seq, int32_t rows,
+                   const int32_t* lengths, const int32_t* counts, const int32_t* start_positions,
+                   const int32_t* free_pages, int32_t n_free, int32_t* page_table, int32_t* new_lengths,
+                   int32_t* row_offsets, int32_t* positions, int32_t* slots, int32_t* pages_taken, void* stream);
+
+/* Workspace for the verification of up to max_batch sequences and max_rows rows
+ * over a vocabulary (up to RSTR_VERIFY_VOCAB).  One call at a time, as with
+ * attention plans. */
+#define RSTR_VERIFY_VOCAB (1 << 24)
+int rstr_verify_open(rstr_session* s, int32_t max_batch, int32_t max_rows, int32_t vocab, rstr_verify** out);
+/* Waits for the device. */
+int rstr_verify_close(rstr_verify* v);
+/* Sequence b has the rows [row_offsets[b], row_offsets[b+1]): row i's logits are
+ * the target's after i drafted tokens, drafts[i] is the token drafted there (not read at the
+ * last row).  With p = softmax(logits / temperature[b]) in 64 bits and q the row's
+ * draft_probs [rows][vocab] (NULL: the draft was certain, q = 1 at it), draft i is
+ * accepted while u_accept[i] * q(draft) < p(draft).  At the first one refused a token is
+ * drawn from max(p - q, 0) (from p where that is 0 everywhere), after the last from p: the first
+ * token whose running sum exceeds u_sample[b] times the whole.  A temperature that is
+ * not positive and finite, and a row whose largest logit is not finite (NaN is
+ * the largest), are greedy: the draft is accepted if it is the first largest
+ * logit, which is the token otherwise.  Drafts outside the vocabulary are refused.  accepted[b] is the number
+ * of drafts accepted; tokens[rows] are those drafts, then the token, then -1.
+ * Random numbers lie in [0, 1).  Rows behind row_offsets[batch] are left as they are. */
+int rstr_verify_run(rstr_verify* v, int32_t dtype, int32_t batch, int32_t rows, const void* logits,
+                    int64_t logits_row, const int32_t* row_offsets, const int32_t* drafts, const float* draft_probs,
+                    int64_t probs_row, const float* temperature, const float* u_accept, const float* u_sample,
+                    int32_t* accepted, int32_t* tokens, void* stream);
 
 #ifdef __cplusplus
 }

@@ -24,35 +24,21 @@
 
 #include "device_math.h"
 #include "kernels.h"
+#include "session.h"
 
 using namespace rstr;
 
 static thread_local std::string g_open_err;
 
-struct rstr_session {
-  int device = 0;
-  hipStream_t stream = nullptr;
-  std::string err;
-  void* scratch = nullptr;  // device address of this GPU's static staging array
-};
-
 static_assert(RSTR_ATTN_STATIC_BYTES == RSTR_STATIC_SCRATCH_BYTES, "one staging size in the ABI and the kernels");
 
-namespace {
-
-int fail(rstr_session* s, int code, const std::string& msg) {
+int rstr::fail(rstr_session* s, int code, const std::string& msg) {
   if (s) s->err = msg;
   else g_open_err = msg;
   return code;
 }
 
-#define HIPCHK(S, expr)                                                                  \
-  do {                                                                                   \
-    hipError_t e_ = (expr);                                                              \
-    if (e_ != hipSuccess)                                                                \
-      return fail((S), e_ == hipErrorOutOfMemory ? RSTR_E_OOM : RSTR_E_HIP,              \
-                  std::string(#expr) + ": " + hipGetErrorString(e_));                    \
-  } while (0)
+namespace {
 
 // Device and pinned memory.  An allocation that does not fit is tried again
 // without the blocks that the pools of this GPU keep for isolated attention.
@@ -90,6 +76,8 @@ bool global_layer(const rstr_model_desc& d, int l) {
 }
 
 }  // namespace
+
+hipError_t rstr::device_alloc(void** p, size_t bytes) { return dev_alloc((char**)p, bytes); }
 
 struct LayerW {
   QTensor qkv, o, gu, down;
@@ -1302,6 +1290,16 @@ extern "C" int rstr_decode_logits(rstr_decoder* d, float* out) {
   HIPCHK(s, hipSetDevice(s->device));
   HIPCHK(s, hipStreamSynchronize(s->stream));
   HIPCHK(s, hipMemcpy(out, d->logits, sizeof(float) * d->B * d->m->d.vocab, hipMemcpyDeviceToHost));
+  return RSTR_OK;
+}
+
+extern "C" int rstr_decode_logits_device(rstr_decoder* d, const float** out) {
+  if (!d) return fail(nullptr, RSTR_E_INVALID, "null decoder");
+  rstr_session* s = d->m->s;
+  if (!out) return fail(s, RSTR_E_INVALID, "null output pointer");
+  *out = nullptr;
+  if (!d->has_logits) return fail(s, RSTR_E_STATE, "no step has run");
+  *out = d->logits;
   return RSTR_OK;
 }
 

@@ -5,11 +5,19 @@ thin handles, plain int32/f32 arrays, negative status codes
 turned into :class:`RstrError` carrying the library's message, the way the
 reference raises ``ex-info``.  No computation happens here; every call goes to
 the HIP library, and loading fails loudly if the library is missing.
+
+The operators on device arrays (:class:`Kv4Pool`, :class:`Kv4Attention`,
+:class:`Verifier`, :meth:`Session.step_maps`) take arrays that live on the
+session's GPU: torch tensors, or anything with their ``data_ptr()``, ``shape``,
+``stride()``, ``dtype`` and ``device``.  They queue work and return.  A program
+that uses torch imports it before this library is loaded, so that both share
+one HIP runtime.
 """
 from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -29,12 +37,15 @@ EXPORTS = (
     "rstr_chunk_restore_submit", "rstr_transfer_done", "rstr_transfer_complete", "rstr_chunk_bench", "rstr_decoder_open",
     "rstr_decoder_close", "rstr_prime_lanes", "rstr_prime_rows", "rstr_step_lanes",
     "rstr_step_lanes_submit", "rstr_step_lanes_collect",
-    "rstr_decode_logits", "rstr_decoder_read_rows", "rstr_decoder_set_graph", "rstr_decoder_step_timing",
+    "rstr_decode_logits", "rstr_decode_logits_device", "rstr_decoder_read_rows", "rstr_decoder_set_graph", "rstr_decoder_step_timing",
     "rstr_prefill_open",
     "rstr_prefill_range", "rstr_append_run", "rstr_tail_run", "rstr_linear_run",
     "rstr_attention_run", "rstr_attention_run_static",
     "rstr_attention_bench", "rstr_schedule_upload", "rstr_schedule_run",
     "rstr_decoder_profile_steps",
+    "rstr_kv4_open", "rstr_kv4_close", "rstr_kv4_bytes", "rstr_kv4_append", "rstr_kv4_read",
+    "rstr_kv4_attn_open", "rstr_kv4_attn_close", "rstr_kv4_attn_run",
+    "rstr_step_maps", "rstr_verify_open", "rstr_verify_close", "rstr_verify_run",
 )
 
 
@@ -121,6 +132,7 @@ def lib():
             "rstr_step_lanes_submit": (i32, [P, P, P, P, P, P, P]),
             "rstr_step_lanes_collect": (i32, [P, P]),
             "rstr_decode_logits": (i32, [P, P]),
+            "rstr_decode_logits_device": (i32, [P, C.POINTER(P)]),
             "rstr_decoder_read_rows": (i32, [P, P]),
             "rstr_decoder_set_graph": (i32, [P, i32]),
             "rstr_decoder_step_timing": (i32, [P, P, i32]),
@@ -136,6 +148,18 @@ def lib():
             "rstr_schedule_upload": (i32, [P, P, i32]),
             "rstr_schedule_run": (i32, [P, i32, i32, P, C.POINTER(f32)]),
             "rstr_decoder_profile_steps": (i32, [P, i32, i32, P, P]),
+            "rstr_kv4_open": (i32, [P, i32, i32, i32, i32, i32, C.POINTER(P)]),
+            "rstr_kv4_close": (i32, [P]),
+            "rstr_kv4_bytes": (i64, [P]),
+            "rstr_kv4_append": (i32, [P, i32, i32, i32, P, i64, i64, P, i64, i64, P, P]),
+            "rstr_kv4_read": (i32, [P, i32, i32, i32, P, P, i64, i64, P, i64, i64, P]),
+            "rstr_kv4_attn_open": (i32, [P, i32, i32, i32, C.POINTER(P)]),
+            "rstr_kv4_attn_close": (i32, [P]),
+            "rstr_kv4_attn_run": (i32, [P, i32, i32, i32, i32, i32, i32, f32, P, i64, i64, P, P, i32, P, P, i64, i64, P]),
+            "rstr_step_maps": (i32, [P, i32, i32, i32, i32, P, P, P, P, i32, P, P, P, P, P, P, P]),
+            "rstr_verify_open": (i32, [P, i32, i32, i32, C.POINTER(P)]),
+            "rstr_verify_close": (i32, [P]),
+            "rstr_verify_run": (i32, [P, i32, i32, i32, P, i64, P, P, P, i64, P, P, P, P, P, P]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -164,6 +188,99 @@ def make_desc(cfg: dict) -> Desc:
     return d
 
 
+# ---- arrays on the session's GPU ----------------------------------------------------
+SESSION_STREAM = C.c_void_p(-1).value   # the session's own stream, where a stream is asked for
+_ELEM = {"float32": 0, "float16": 1, "bfloat16": 2}
+_codes = {}   # an array library's dtype object -> element type code, or its name
+
+
+def _code(dtype):
+    c = _codes.get(dtype)
+    if c is None:
+        name = str(dtype).replace("torch.", "")
+        c = _codes[dtype] = _ELEM.get(name, name)
+    return c
+
+
+class DeviceView:
+    """Device memory that the library owns, in the form the operators take
+    (and torch's ``as_tensor``); it keeps its owner alive, not open."""
+
+    def __init__(self, ptr: int, shape, dtype: str, device: int, owner):
+        self._ptr, self.shape, self.dtype, self.device, self._owner = ptr, tuple(shape), dtype, device, owner
+
+    def data_ptr(self) -> int:
+        return self._ptr
+
+    def stride(self):
+        out = [1]
+        for n in self.shape[:0:-1]:
+            out.insert(0, out[0] * n)
+        return tuple(out)
+
+    @property
+    def __cuda_array_interface__(self):
+        return dict(shape=self.shape, typestr="<f4" if self.dtype == "float32" else "<f2", data=(self._ptr, False), version=2)
+
+
+def _on_device(sess, x, what):
+    d = x.device
+    if d != sess.device and not (getattr(d, "type", None) == "cuda" and d.index == sess.device):
+        raise ValueError(f"{what} must be on the session's GPU ({sess.device}), got {d}")
+
+
+def _ints(sess, x, what, shape):
+    """The address of a contiguous int32 device array of the given shape (None: any extent)."""
+    _on_device(sess, x, what)
+    if _code(x.dtype) != "int32":
+        raise ValueError(f"{what} must be int32, got {x.dtype}")
+    return _plain(x, what, shape)
+
+
+def _floats(sess, x, what, shape):
+    _on_device(sess, x, what)
+    if _code(x.dtype) != 0:
+        raise ValueError(f"{what} must be float32, got {x.dtype}")
+    return _plain(x, what, shape)
+
+
+def _plain(x, what, shape):
+    if len(x.shape) != len(shape) or any(w is not None and n != w for n, w in zip(x.shape, shape)):
+        raise ValueError(f"{what} must have the shape {tuple('any' if w is None else w for w in shape)}, got {tuple(x.shape)}")
+    want = 1
+    for n, st in zip(reversed(x.shape), reversed(x.stride())):
+        if n > 1 and st != want:
+            raise ValueError(f"{what} must be contiguous")
+        want *= n
+    return x.data_ptr()
+
+
+def _rows(sess, x, what, heads, hd, rows=None):
+    """(address, element type, row stride, head stride) of a [rows][heads][hd] device array."""
+    _on_device(sess, x, what)
+    code = _code(x.dtype)
+    if not isinstance(code, int):
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
+    if len(x.shape) != 3 or x.shape[1] != heads or x.shape[2] != hd or (rows is not None and x.shape[0] != rows):
+        raise ValueError(f"{what} must have the shape ({'rows' if rows is None else rows}, {heads}, {hd}), got {tuple(x.shape)}")
+    st = x.stride()
+    if st[2] != 1:
+        raise ValueError(f"the last dimension of {what} must be contiguous")
+    return x.data_ptr(), code, st[0], st[1]
+
+
+def _stream(sess, stream):
+    """The raw stream of a call: what it was given (a hipStream_t address, a torch
+    stream, or SESSION_STREAM), else torch's current one where torch is in use,
+    else the session's own."""
+    if stream is None:
+        torch = sys.modules.get("torch")
+        if torch is None or not torch.cuda.is_initialized():
+            return SESSION_STREAM
+        return torch.cuda.current_stream(sess.device).cuda_stream
+    return getattr(stream, "cuda_stream", stream)
+
+
 class Session:
     """A device session (raster.gpu.core/make-session)."""
 
@@ -173,6 +290,7 @@ class Session:
         if rc != 0:
             raise RstrError(rc, lib().rstr_open_error().decode())
         self.h = h
+        self.device = device
         self.children = []   # open models, pools, decoders (closed before the session)
 
     def _adopt(self, obj):
@@ -190,7 +308,7 @@ class Session:
 
     def close(self):
         if self.h:
-            order = {"Decoder": 0, "Prefill": 0, "Pool": 1, "Model": 2}
+            order = {"Decoder": 0, "Prefill": 0, "Kv4Attention": 0, "Verifier": 0, "Pool": 1, "Kv4Pool": 1, "Model": 2}
             for obj in sorted(self.children, key=lambda o: order.get(type(o).__name__, 3)):
                 obj.close()
             self.children = []
@@ -209,6 +327,21 @@ class Session:
         out = np.empty((rows, d), np.float32)
         self.check(lib().rstr_tail_run(self.h, rows, vocab, d, _p(logits), _p(emb), _p(tok), _p(out)))
         return tok, out
+
+    def step_maps(self, page_size: int, lengths, counts, free_pages, page_table, new_lengths, row_offsets, positions,
+                  slots, taken, starts=None, stream=None):
+        """The tables of a step on the GPU (rstr_step_maps): int32 device arrays; ``page_table``
+        [batch][width] and everything behind it are written.  The length of ``slots``
+        bounds the step's rows, that of ``free_pages`` its new pages."""
+        batch, (rows,) = len(lengths), slots.shape
+        width, n_free = page_table.shape[1], len(free_pages)
+        self.check(lib().rstr_step_maps(
+            self.h, page_size, batch, width, rows, _ints(self, lengths, "lengths", (batch,)),
+            _ints(self, counts, "counts", (batch,)), None if starts is None else _ints(self, starts, "starts", (batch,)),
+            _ints(self, free_pages, "free_pages", (n_free,)), n_free, _ints(self, page_table, "page_table", (batch, width)),
+            _ints(self, new_lengths, "new_lengths", (batch,)), _ints(self, row_offsets, "row_offsets", (batch + 1,)),
+            _ints(self, positions, "positions", (rows,)), _ints(self, slots, "slots", (rows,)),
+            _ints(self, taken, "taken", (1,)), _stream(self, stream)))
 
     def __enter__(self):
         return self
@@ -506,6 +639,12 @@ class Decoder:
         self.sess.check(lib().rstr_decode_logits(self.h, _p(out)))
         return out
 
+    def logits_device(self) -> DeviceView:
+        """The last step's logits where they are, on the GPU (rstr_decode_logits_device)."""
+        p = C.c_void_p()
+        self.sess.check(lib().rstr_decode_logits_device(self.h, C.byref(p)))
+        return DeviceView(p.value, (self.batch, self.model.cfg["vocab"]), "float32", self.sess.device, self)
+
     def rows(self) -> np.ndarray:
         out = np.empty((self.batch, self.model.cfg["d_model"]), np.float32)
         self.sess.check(lib().rstr_decoder_read_rows(self.h, _p(out)))
@@ -591,3 +730,138 @@ class Prefill:
         if self.h:
             lib().rstr_decoder_close(self.h)
             self.h = None
+
+
+class Kv4Pool:
+    """Paged K/V in 4-bit blocks (rstr_kv4_open): slots and page tables as with :class:`Pool`, at
+    4.5 bits an element instead of 16."""
+
+    def __init__(self, sess: Session, n_layers: int, n_kv: int, head_dim: int, page_size: int, physical_pages: int):
+        self.sess, self.n_layers, self.n_kv, self.head_dim = sess, n_layers, n_kv, head_dim
+        self.page_size, self.physical_pages = page_size, physical_pages
+        h = C.c_void_p()
+        sess.check(lib().rstr_kv4_open(sess.h, n_layers, n_kv, head_dim, page_size, physical_pages, C.byref(h)))
+        self.h = h
+        sess._adopt(self)
+
+    @property
+    def nbytes(self) -> int:
+        return int(lib().rstr_kv4_bytes(self.h))
+
+    def _kv(self, k, v, rows):
+        kp, kt, kr, kh = _rows(self.sess, k, "k", self.n_kv, self.head_dim, rows)
+        vp, vt, vr, vh = _rows(self.sess, v, "v", self.n_kv, self.head_dim, rows)
+        if kt != vt:
+            raise ValueError("k and v must have the same element type")
+        return kt, (kp, kr, kh), (vp, vr, vh)
+
+    def append(self, layer: int, k, v, slots, stream=None):
+        """Quantises rows k, v [rows][n_kv][head_dim] into ``slots`` [rows] (rstr_kv4_append);
+        rows whose slot is negative are skipped."""
+        rows = len(slots)
+        t, k, v = self._kv(k, v, rows)
+        self.sess.check(lib().rstr_kv4_append(self.h, layer, rows, t, *k, *v, _ints(self.sess, slots, "slots", (rows,)),
+                                              _stream(self.sess, stream)))
+
+    def read(self, layer: int, slots, k, v, stream=None):
+        """Writes the values that ``slots`` hold into rows k, v (rstr_kv4_read)."""
+        rows = len(slots)
+        t, k, v = self._kv(k, v, rows)
+        self.sess.check(lib().rstr_kv4_read(self.h, layer, rows, t, _ints(self.sess, slots, "slots", (rows,)), *k, *v,
+                                            _stream(self.sess, stream)))
+
+    def close(self):
+        if self.h:
+            self.sess.check(lib().rstr_kv4_close(self.h))
+            self.h = None
+            _left(self)
+
+
+class Kv4Attention:
+    """Attention over a :class:`Kv4Pool` (rstr_kv4_attn_run) and its workspace: one
+    call at a time, so programs and graphs that run side by side have one each."""
+
+    def __init__(self, pool: Kv4Pool, n_q: int, max_batch: int, max_rows: int):
+        self.pool, self.sess, self.n_q, self.max_batch, self.max_rows = pool, pool.sess, n_q, max_batch, max_rows
+        h = C.c_void_p()
+        self.sess.check(lib().rstr_kv4_attn_open(pool.h, n_q, max_batch, max_rows, C.byref(h)))
+        self.h = h
+        self.sess._adopt(self)
+
+    def run(self, layer: int, q, row_offsets, page_table, lengths, out, max_rows: int | None = None, window: int = 0,
+            scale: float | None = None, stream=None):
+        """q, out [rows][n_q][head_dim] of one type; int32 row_offsets [batch+1], page_table
+        [batch][width], lengths [batch].  ``max_rows``: the most rows of one sequence (default: all rows)."""
+        s, hd = self.sess, self.pool.head_dim
+        batch, rows = len(lengths), q.shape[0]
+        qp, t, qr, qh = _rows(s, q, "q", self.n_q, hd)
+        op, ot, orow, oh = _rows(s, out, "out", self.n_q, hd, rows)
+        if t != ot:
+            raise ValueError("q and out must have the same element type")
+        width = page_table.shape[1]
+        s.check(lib().rstr_kv4_attn_run(
+            self.h, layer, t, batch, rows, rows if max_rows is None else max_rows, window, hd ** -0.5 if scale is None else scale,
+            qp, qr, qh, _ints(s, row_offsets, "row_offsets", (batch + 1,)), _ints(s, page_table, "page_table", (batch, width)),
+            width, _ints(s, lengths, "lengths", (batch,)), op, orow, oh, _stream(s, stream)))
+
+    def close(self):
+        if self.h:
+            self.sess.check(lib().rstr_kv4_attn_close(self.h))
+            self.h = None
+            _left(self)
+
+
+class Verifier:
+    """Verification of drafted tokens (rstr_verify_run) and its workspace: one call at a time."""
+
+    def __init__(self, sess: Session, max_batch: int, max_rows: int, vocab: int):
+        self.sess, self.max_batch, self.max_rows, self.vocab = sess, max_batch, max_rows, vocab
+        h = C.c_void_p()
+        sess.check(lib().rstr_verify_open(sess.h, max_batch, max_rows, vocab, C.byref(h)))
+        self.h = h
+        sess._adopt(self)
+
+    def run(self, logits, row_offsets, drafts, temperature, u_accept, u_sample, accepted, tokens, draft_probs=None,
+            stream=None):
+        """logits [rows][vocab]; int32 row_offsets [batch+1], drafts [rows]; float32 temperature [batch],
+        u_accept [rows], u_sample [batch], draft_probs [rows][vocab]; writes int32 accepted [batch] and
+        tokens [rows]."""
+        s = self.sess
+        batch, rows = len(row_offsets) - 1, len(drafts)
+        lp, t, lr = _matrix(s, logits, "logits", rows, self.vocab)
+        pp, pr = None, 0
+        if draft_probs is not None:
+            pp, pt, pr = _matrix(s, draft_probs, "draft_probs", rows, self.vocab)
+            if pt != 0:
+                raise ValueError("draft_probs must be float32")
+        s.check(lib().rstr_verify_run(
+            self.h, t, batch, rows, lp, lr, _ints(s, row_offsets, "row_offsets", (batch + 1,)),
+            _ints(s, drafts, "drafts", (rows,)), pp, pr, _floats(s, temperature, "temperature", (batch,)),
+            _floats(s, u_accept, "u_accept", (rows,)), _floats(s, u_sample, "u_sample", (batch,)),
+            _ints(s, accepted, "accepted", (batch,)), _ints(s, tokens, "tokens", (rows,)), _stream(s, stream)))
+
+    def close(self):
+        if self.h:
+            self.sess.check(lib().rstr_verify_close(self.h))
+            self.h = None
+            _left(self)
+
+
+def _matrix(sess, x, what, rows, cols):
+    """(address, element type, row stride) of a [rows][cols] device array."""
+    _on_device(sess, x, what)
+    code = _code(x.dtype)
+    if not isinstance(code, int):
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
+    if tuple(x.shape) != (rows, cols):
+        raise ValueError(f"{what} must have the shape ({rows}, {cols}), got {tuple(x.shape)}")
+    st = x.stride()
+    if cols > 1 and st[1] != 1:
+        raise ValueError(f"the last dimension of {what} must be contiguous")
+    return x.data_ptr(), code, st[0]
+
+
+def _left(child):
+    """A closed handle is no longer its session's to close."""
+    if child in child.sess.children:
+        child.sess.children.remove(child)

@@ -1,0 +1,444 @@
+"""The 4-bit paged cache on the GPU: append and read bit for bit against the
+format's definition, attention against plain float64 attention over the values
+that the cache holds.
+
+Tolerances of attention, elementwise, from the roundings the kernel is allowed:
+with W = sum of w_j |v_j| of the row (w the exact probabilities),
+- scores: fp32 sums of D products with codes biased by at most 72 + 8, so each score is off by at
+  most (D + 16) * 2^-24 * 10 * |q| . |k| * scale (a kept code's magnitude is at least a tenth of the biased one's
+  bound on average over a block's largest element), which moves every weight by that factor, and the
+  output by twice that times W;
+- f16 and bf16: each weight is rounded to 11 bits, and its product with the block's scale again:
+  2 * 2^-12 relative, 2^-11 * W; weights below the smallest fp16 subnormal (2^-24 of 2^9) vanish or round:
+  N * 2^-33 * max|v|;
+- fp32: weights as two fp16 terms, 2^-22 * W, and fp32 sums over N tokens in at most N/8 dependent
+  steps a lane: N * 2^-27 * W;
+- the output's own rounding: half a step, finfo.eps / 2 * |out|.
+"""
+import numpy as np
+import pytest
+import torch
+
+import kv4_plain as P
+from rstr import hip
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def sess():
+    with hip.Session(0) as s:
+        yield s
+
+
+def _i32(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+
+
+def _laid(x, how):
+    """The rows x [R][H][D] on the GPU in another memory order, with the same values."""
+    x = x.cuda()
+    R, H, D = x.shape
+    if how == "plain":
+        return x
+    if how == "padded":  # strides larger than the rows
+        y = torch.zeros(R, H + 1, D + 8, dtype=x.dtype, device="cuda")[:, :H, :D]
+    elif how == "heads_outside":
+        y = torch.zeros(H, R, D, dtype=x.dtype, device="cuda").transpose(0, 1)
+    else:  # an address that no vector load may use
+        y = torch.zeros(R * H * (D + 1) + 1, dtype=x.dtype, device="cuda")[1:].as_strided((R, H, D), (H * (D + 1), D + 1, 1))
+    y.copy_(x)
+    return y
+
+
+# ---- append and read -------------------------------------------------------------------
+def _hard_rows(rng, rows, heads, D):
+    """Rows with what a quantiser can get wrong: ties, equal extremes of both signs, zeros, single
+    values, tiny and huge blocks, NaN and infinities."""
+    x = rng.standard_normal((rows, heads, D)).astype(np.float32)
+    b = x.reshape(-1, 32)
+    for i in range(len(b)):
+        kind = i % 12
+        if kind == 1:
+            b[i] = 0.0
+        elif kind == 2:  # every value a multiple of half a step: ties to even
+            b[i] = rng.integers(-16, 16, 32) * 0.5 * 0.25
+            b[i, rng.integers(32)] = 8 * 0.25 * rng.choice((-1, 1))
+        elif kind == 3:  # the same magnitude twice, the first one's sign decides
+            b[i, [5, 20]] = (4.5, -4.5) if i % 24 < 12 else (-4.5, 4.5)
+        elif kind == 4:
+            b[i] = 0.0
+            b[i, rng.integers(32)] = rng.standard_normal()
+        elif kind == 5:
+            b[i] *= 2.0 ** -20
+        elif kind == 6:
+            b[i] *= 2.0 ** -27
+        elif kind == 7:
+            b[i] *= 2.0 ** 13
+        elif kind == 8 and i % 48 == 8:
+            b[i, rng.integers(32)] = rng.choice((np.nan, np.inf, -np.inf))
+        elif kind == 9:
+            b[i] = -0.0
+    return x
+
+
+@pytest.mark.parametrize("D,heads,page", [(64, 3, 16), (128, 2, 48), (256, 1, 16), (128, 8, 64)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("how", ["plain", "padded", "heads_outside", "odd"])
+def test_append_read(sess, D, heads, page, dtype, how):
+    print("append", D, heads, page, dtype, how, flush=True)
+    rng = np.random.default_rng(D + heads + page)
+    rows, pages = 61, 9
+    pool = hip.Kv4Pool(sess, 2, heads, D, page, pages)
+    k = torch.tensor(_hard_rows(rng, rows, heads, D)).to(TYPES[dtype])
+    v = torch.tensor(_hard_rows(rng, rows, heads, D) * 1.5).to(TYPES[dtype])
+    slots = rng.permutation(pages * page)[:rows].astype(np.int64)
+    slots[7], slots[8], slots[50] = -1, pages * page, 2 ** 31 - 1
+    pool.append(1, _laid(k, how), _laid(v, how), _i32(slots))
+    listed = np.concatenate([slots, slots[:3], np.setdiff1d(np.arange(pages * page), slots)[:20]])  # some twice, some never written
+    ko = _laid(torch.full((len(listed), heads, D), 9.0, dtype=TYPES[dtype]), how)
+    vo = _laid(torch.full((len(listed), heads, D), 9.0, dtype=TYPES[dtype]), how)
+    pool.read(1, _i32(listed), ko, vo)
+    for x, o in ((k, ko), (v, vo)):
+        want = P.quantised(P.as_f64(x))
+        want[[7, 8, 50]] = 0.0
+        want = np.concatenate([want, want[:3], np.zeros((20, heads, D))])
+        want = torch.tensor(want).to(torch.float32).to(TYPES[dtype])  # exact in fp32, one rounding
+        got = o.cpu()
+        same = (got == want) | (got.isnan() & want.isnan())
+        assert bool(same.all()), (torch.nonzero(~same)[:4], got[~same][:4], want[~same][:4])
+    pool.read(0, _i32(listed), ko, vo)  # the other layer is untouched
+    assert not ko.any() and not vo.any()
+    pool.close()
+
+
+def test_append_huge_values(sess):
+    """Blocks past 8 * 65504 keep the largest scale, and their codes saturate."""
+    k = torch.zeros(1, 1, 64)
+    k[0, 0, 3], k[0, 0, 4], k[0, 0, 40], k[0, 0, 41] = 1e9, -2e5, -3e38, 7e5
+    pool = hip.Kv4Pool(sess, 1, 1, 64, 16, 1)
+    k = k.cuda()
+    pool.append(0, k, k, _i32([5]))
+    o, p = torch.empty_like(k), torch.empty_like(k)
+    pool.read(0, _i32([5]), o, p)
+    assert np.array_equal(P.as_f64(o), P.quantised(P.as_f64(k))) and torch.equal(o, p)
+    pool.close()
+
+
+def test_append_many_rows(sess):
+    """More rows than one launch row of workgroups holds, each its own slot."""
+    rows, pool = 5000, hip.Kv4Pool(sess, 1, 2, 64, 16, 313)
+    g = torch.Generator("cuda").manual_seed(1)
+    k = torch.randn(rows, 2, 64, generator=g, device="cuda").half()
+    slots = torch.randperm(313 * 16, generator=g, device="cuda")[:rows].to(torch.int32)
+    pool.append(0, k, -k, slots)
+    a, b = torch.empty_like(k), torch.empty_like(k)
+    pool.read(0, slots, a, b)
+    want = torch.tensor(P.quantised(P.as_f64(k))).half()
+    assert torch.equal(a.cpu(), want)
+    assert torch.equal(b.cpu(), torch.tensor(P.quantised(-P.as_f64(k))).half())
+    pool.close()
+
+
+# ---- attention ---------------------------------------------------------------------------
+class Case:
+    """A cache filled through append, ragged sequences over it and their float64 values."""
+
+    def __init__(self, sess, n_q, n_kv, D, page, lens, news, seed=0, extra=5, width=None, v_scale=1.0, k_scale=1.0, layers=1):
+        rng = np.random.default_rng([seed, n_q, D, page, len(lens)])
+        self.rng, self.lens, self.news, self.page, self.n_q, self.n_kv, self.D = rng, list(lens), list(news), page, n_q, n_kv, D
+        need = [-(-max(n, 0) // page) for n in lens]
+        self.pages = sum(need) + extra
+        perm = rng.permutation(self.pages)
+        self.table = np.full((len(lens), width or max(1, max(need))), -1, np.int64)
+        at = 0
+        for b, n in enumerate(need):
+            self.table[b, :n] = perm[at:at + n]
+            at += n
+        self.pool = hip.Kv4Pool(sess, layers, n_kv, D, page, self.pages)
+        total = sum(lens)
+        k = torch.tensor(rng.standard_normal((total, n_kv, D)) * k_scale, dtype=torch.float16)
+        v = torch.tensor(rng.standard_normal((total, n_kv, D)) * v_scale, dtype=torch.float16)
+        k[..., D // 3:: 29] *= 3.0
+        slots = np.concatenate([self.table[b, np.arange(n) // page] * page + np.arange(n) % page for b, n in enumerate(lens)] or [[]])
+        if total:
+            self.pool.append(layers - 1, k.cuda(), v.cuda(), _i32(slots))
+        cut = np.concatenate([[0], np.cumsum(lens)])
+        kq, vq = P.quantised(P.as_f64(k)), P.quantised(P.as_f64(v))
+        self.k = [kq[cut[b]:cut[b + 1]] for b in range(len(lens))]
+        self.v = [vq[cut[b]:cut[b + 1]] for b in range(len(lens))]
+        self.offsets = np.concatenate([[0], np.cumsum(news)])
+        self.layer = layers - 1
+
+    def plan(self, behind=0):
+        return hip.Kv4Attention(self.pool, self.n_q, len(self.lens), int(self.offsets[-1]) + behind)
+
+    def queries(self, dtype, behind=0, mul=1.5):
+        R = int(self.offsets[-1]) + behind
+        return torch.tensor(self.rng.standard_normal((R, self.n_q, self.D)) * mul, dtype=torch.float32).to(TYPES[dtype])
+
+    def check(self, got, q, dtype, window, scale, what=""):
+        want, mag, size = P.attention(P.as_f64(q), self.k, self.v, self.lens, self.offsets, window, scale)
+        R = int(self.offsets[-1])
+        N, D = max(self.lens + [1]), self.D
+        vmax = max([np.nanmax(np.abs(x)) for x in self.v if len(x)] + [0.0])
+        rel = 2 * (D + 16) * 2.0 ** -24 * 10 * size
+        rel = rel + (2.0 ** -11 if dtype != "f32" else 2.0 ** -22 + N * 2.0 ** -27)
+        tol = rel * mag + torch.finfo(TYPES[dtype]).eps / 2 * np.abs(want) * 1.01 + N * 2.0 ** -33 * vmax
+        far = np.abs(P.as_f64(got)[:R] - want[:R]) - tol[:R]
+        assert np.all(np.isfinite(P.as_f64(got)[:R])), what
+        assert far.max() <= 0, (what, far.max(), np.unravel_index(far.argmax(), far.shape))
+        return want
+
+    def close(self):
+        self.pool.close()
+
+
+SHAPES = [
+    # n_q, n_kv, D, page, lengths, rows, window
+    (4, 2, 128, 16, [1], [1], 0),
+    (4, 2, 128, 16, [0], [1], 0),
+    (4, 2, 128, 16, [16, 17, 31, 32, 33, 15], [1] * 6, 0),
+    (8, 2, 64, 16, [100, 1, 0, 333], [1, 1, 1, 1], 0),
+    (4, 1, 256, 16, [77, 600], [1, 1], 0),
+    (4, 1, 256, 32, [77, 600, 5], [3, 1, 5], 50),
+    (8, 8, 64, 48, [47, 48, 49, 500], [1, 2, 3, 4], 0),
+    (32, 8, 128, 16, [700, 3, 65], [1, 3, 2], 0),
+    (16, 8, 128, 64, [1500], [1], 100),
+    (24, 1, 128, 16, [200, 30], [1, 1], 0),      # more than 16 heads on one kv head
+    (48, 1, 64, 16, [90], [2], 33),
+    (4, 4, 128, 16, [40, 9], [40, 9], 0),        # whole prompts
+    (8, 2, 128, 16, [130, 77], [70, 77], 0),
+    (6, 2, 64, 16, [200], [150], 17),
+    (4, 1, 256, 16, [150], [99], 40),
+    (2, 2, 128, 16, [5, 0, 3], [9, 4, 2], 0),    # more rows than tokens: the first rows see nothing
+    (4, 2, 128, 16, [64, 64, 64], [0, 2, 0], 0),  # sequences without rows
+    (4, 2, 64, 16, [33] * 70, [1] * 70, 0),      # more sequences than a wave has lanes
+    (4, 2, 64, 16, [2500, 40], [1, 1], 1),       # a window of the token itself
+    (4, 2, 128, 16, [3000, 10, 800], [4, 1, 2], 0),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=[str(i) for i in range(len(SHAPES))])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention(sess, shape, dtype):
+    n_q, n_kv, D, page, lens, news, window = shape
+    print("attention", shape, dtype, flush=True)
+    c = Case(sess, n_q, n_kv, D, page, lens, news)
+    q = c.queries(dtype, behind=2)
+    out = torch.full_like(q, 7.0).cuda()
+    plan = c.plan(behind=2)
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(lens), out, max_rows=max(news), window=window, scale=D ** -0.5)
+    c.check(out, q, dtype, window, D ** -0.5)
+    assert bool((out[int(c.offsets[-1]):] == 7.0).all())  # rows behind the last sequence
+    # any bound on a sequence's rows gives the same values, to rounding
+    other = torch.full_like(out, 3.0)
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(lens), other, window=window, scale=D ** -0.5)
+    c.check(other, q, dtype, window, D ** -0.5, "max_rows")
+    plan.close()
+    c.close()
+
+
+@pytest.mark.parametrize("how", ["padded", "heads_outside", "odd"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_strides(sess, how, dtype):
+    c = Case(sess, 8, 2, 128, 16, [70, 200], [3, 20], layers=2)
+    q = c.queries(dtype)
+    out = _laid(torch.zeros_like(q), how)
+    plan = c.plan()
+    plan.run(1, _laid(q, how), _i32(c.offsets), _i32(c.table), _i32(c.lens), out, scale=0.1)
+    c.check(out, q, dtype, 0, 0.1)
+    plan.run(0, _laid(q, how), _i32(c.offsets), _i32(c.table), _i32(c.lens), out)  # an empty layer: zeros
+    assert not out.any()
+    plan.close()
+    c.close()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("v_scale,k_scale,mul", [(1e-4, 1.0, 1.5), (300.0, 1.0, 1.5), (1.0, 20.0, 6.0), (1.0, 1e-3, 1e-3), (3000.0, 3.0, 1.0)])
+def test_attention_ranges(sess, dtype, v_scale, k_scale, mul):
+    """Tiny and large values, near-uniform and one-hot probabilities."""
+    print("ranges", dtype, v_scale, k_scale, mul, flush=True)
+    c = Case(sess, 4, 2, 128, 16, [900, 40], [1, 6], v_scale=v_scale, k_scale=k_scale)
+    q = c.queries(dtype, mul=mul)
+    out = torch.zeros_like(q).cuda()
+    plan = c.plan()
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out, max_rows=6)
+    c.check(out, q, dtype, 0, 128 ** -0.5)
+    plan.close()
+    c.close()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows", [2, 40])
+def test_what_is_not_seen_does_not_matter(sess, dtype, rows):
+    """NaN blocks behind a row's position, before its window, in free pages and behind the length
+    change nothing, bit for bit; where a row does see one it is NaN in that block."""
+    D, page, n, window = 128, 16, 333, 64
+    c = Case(sess, 4, 2, D, page, [n, 50], [rows, 1])
+    q = c.queries(dtype).cuda()
+    plan = c.plan()
+
+    def run():
+        out = torch.zeros_like(q)
+        plan.run(0, q, _i32(c.offsets), _i32(c.table), _i32(c.lens), out, max_rows=rows, window=window)
+        return out
+
+    before = run()
+    c.check(before, q, dtype, window, D ** -0.5)
+    bad = torch.full((1, 2, D), float("nan"), device="cuda")
+    kill = lambda t: c.pool.append(0, bad, bad, _i32([c.table[0, t // page] * page + t % page]))  # noqa: E731
+    kill(0)
+    kill(n - rows - window)              # one before the first row's window
+    used = set(c.table.ravel().tolist())
+    for pg in range(c.pages):
+        if pg not in used:
+            c.pool.append(0, bad.expand(16, 2, D).contiguous(), bad.expand(16, 2, D).contiguous(), _i32(pg * page + np.arange(page)))
+    tail = c.table[0, n // page] * page + np.arange(n % page, page)   # behind the length
+    c.pool.append(0, bad.expand(len(tail), 2, D).contiguous(), bad.expand(len(tail), 2, D).contiguous(), _i32(tail))
+    assert torch.equal(run(), before)
+    kill(n - 1)                          # the last row's own token
+    after = run()
+    last = rows - 1
+    assert torch.equal(after[:last], before[:last]) and torch.equal(after[rows:], before[rows:])
+    assert bool(after[last].isnan().all())
+    # a value block alone: that block of the output is NaN, the others are not
+    good = torch.zeros(1, 2, D, device="cuda")
+    half = torch.ones(1, 2, D, device="cuda")
+    half[..., 32:64] = float("inf")
+    c.pool.append(0, good, half, _i32([c.table[0, (n - 1) // page] * page + (n - 1) % page]))
+    after = run()
+    assert bool(after[last, :, 32:64].isnan().all()) and bool(after[last, :, :32].isfinite().all())
+    assert bool(after[last, :, 64:].isfinite().all()) and torch.equal(after[:last], before[:last])
+    plan.close()
+    c.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_bad_descriptors_stay_inside(sess, dtype):
+    """Page ids outside the cache are not seen; lengths and offsets beyond the arrays are cut."""
+    page, D = 16, 64
+    c = Case(sess, 4, 2, D, page, [100, 64], [2, 1])
+    q = c.queries(dtype)
+    table = c.table.copy()
+    gone = {1: [16, 32], 3: [48, 64]}
+    table[0, 1], table[0, 3] = -1, c.pages
+    table[1, 0] = 2 ** 31 - 1
+    out = torch.zeros_like(q).cuda()
+    plan = c.plan()
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(table), _i32(c.lens), out)
+    seen = [np.ones(100, bool), np.ones(64, bool)]
+    for lo, hi in gone.values():
+        seen[0][lo:hi] = False
+    seen[1][:16] = False
+    want = np.zeros(q.shape)
+    for r, (b, p) in enumerate(((0, 98), (0, 99), (1, 63))):
+        j = np.flatnonzero(seen[b][:p + 1])
+        for h in range(4):
+            s = c.k[b][j, h // 2] @ P.as_f64(q)[r, h] * D ** -0.5
+            w = np.exp(s - s.max())
+            want[r, h] = w / w.sum() @ c.v[b][j, h // 2]
+    assert np.abs(P.as_f64(out) - want).max() < 4 * (2.0 ** -9 if dtype == "bf16" else 2.0 ** -18)
+    for lens, offs in (([10 ** 9, 64], c.offsets), ([-5, -(2 ** 31)], c.offsets), (c.lens, [0, 50, 90]), (c.lens, [-4, 1, 2 ** 31 - 1]),
+                       (c.lens, [2, 0, 3])):
+        plan.run(0, q.cuda(), _i32(offs), _i32(table), _i32(lens), out)
+        torch.cuda.synchronize()
+    plan.close()
+    c.close()
+
+
+def test_cache_past_32_bits(sess):
+    """Pages whose bytes lie past 2^32 of a layer."""
+    D, page, pages = 128, 64, 70000
+    pool = hip.Kv4Pool(sess, 1, 8, D, page, pages)
+    assert pool.nbytes > 2 ** 32
+    rng = np.random.default_rng(0)
+    table = np.array([[pages - 1, 3, pages - 2, 65536]])
+    n = 250
+    k = torch.tensor(rng.standard_normal((n, 8, D)), dtype=torch.float16)
+    v = torch.tensor(rng.standard_normal((n, 8, D)), dtype=torch.float16)
+    pool.append(0, k.cuda(), v.cuda(), _i32(table[0, np.arange(n) // page] * page + np.arange(n) % page))
+    q = torch.tensor(rng.standard_normal((1, 16, D)), dtype=torch.float32)
+    out = torch.zeros(1, 16, D, device="cuda")
+    plan = hip.Kv4Attention(pool, 16, 1, 1)
+    plan.run(0, q.cuda(), _i32([0, 1]), _i32(table), _i32([n]), out)
+    want, mag, _ = P.attention(P.as_f64(q), [P.quantised(P.as_f64(k))], [P.quantised(P.as_f64(v))], [n], [0, 1], 0, D ** -0.5)
+    assert np.abs(P.as_f64(out) - want).max() < 2.0 ** -16 * mag.max()
+    plan.close()
+    pool.close()
+
+
+def test_long_context(sess):
+    """One sequence over many workgroups; a window near its end; against float64 on the GPU."""
+    D, page, n = 128, 16, 40001
+    c_lens = [n]
+    g = torch.Generator("cuda").manual_seed(3)
+    pool = hip.Kv4Pool(sess, 1, 2, D, page, -(-n // page))
+    table = torch.randperm(-(-n // page), generator=g, device="cuda").to(torch.int32)[None]
+    t = torch.arange(n, device="cuda")
+    slots = table[0].long()[t // page] * page + t % page
+    k, v = torch.randn(n, 2, D, generator=g, device="cuda"), torch.randn(n, 2, D, generator=g, device="cuda")
+    pool.append(0, k, v, slots.to(torch.int32))
+    pool.read(0, slots.to(torch.int32), k, v)
+    for rows, window, dtype in ((1, 0, "f16"), (1, 0, "f32"), (3, 30000, "bf16"), (3, 33, "f32"), (40, 0, "f32"), (40, 39000, "f16")):
+        print("long", rows, window, dtype, flush=True)
+        q = torch.randn(rows, 8, D, generator=g, device="cuda").to(TYPES[dtype])
+        out = torch.zeros_like(q)
+        plan = hip.Kv4Attention(pool, 8, 1, rows)
+        plan.run(0, q, _i32([0, rows]), table, _i32(c_lens), out, window=window)
+        p = torch.arange(n - rows, n, device="cuda")[:, None]
+        hid = (t > p) | ((t <= p - window) if window else (t < 0))
+        for h in range(8):
+            s = (q[:, h].double() @ k[:, h // 4].double().t().contiguous()) * D ** -0.5
+            w = torch.softmax(s.masked_fill(hid, -float("inf")), 1)
+            want = w @ v[:, h // 4].double()
+            mag = w @ v[:, h // 4].double().abs()
+            tol = (2.0 ** -11 if dtype != "f32" else 2.0 ** -16) * mag + torch.finfo(q.dtype).eps / 2 * want.abs() * 1.01 + n * 2.0 ** -33 * 6
+            assert bool(((out[:, h].double() - want).abs() <= tol).all()), (rows, window, dtype, h)
+        plan.close()
+    pool.close()
+
+
+def test_streams_and_graphs(sess):
+    """Captured calls replay on changed inputs between eager calls; two plans run side by side on
+    two streams; the session's own stream takes calls too."""
+    c = Case(sess, 8, 2, 128, 16, [400, 90, 3], [2, 1, 1])
+    q = c.queries("f16").cuda()
+    args = (_i32(c.offsets), _i32(c.table), _i32(c.lens))
+    plans = [c.plan() for _ in range(3)]
+    outs = [torch.zeros_like(q) for _ in range(3)]
+    plans[0].run(0, q, *args, outs[0])
+    torch.cuda.synchronize()
+    graphs = []
+    for i in (0, 1):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            plans[i].run(0, q, *args, outs[i])
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for step in range(4):
+        q.copy_(c.queries("f16"))
+        plans[2].run(0, q, *args, outs[2])
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            outs[i].zero_()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[2]), step
+        outs[0].zero_()
+        torch.cuda.synchronize()
+        plans[0].run(0, q, *args, outs[0], stream=hip.SESSION_STREAM)
+        with torch.cuda.stream(streams[1]):
+            outs[1].zero_()
+            plans[1].run(0, q, *args, outs[1])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[2]), step
+    c.check(outs[0], q, "f16", 0, 128 ** -0.5)
+    for p in plans:
+        p.close()
+    c.close()
