@@ -8,9 +8,9 @@ with W = sum of w_j |v_j| of the row (w the exact probabilities),
   most (D + 16) * 2^-24 * 10 * |q| . |k| * scale (a kept code's magnitude is at least a tenth of the biased one's
   bound on average over a block's largest element), which moves every weight by that factor, and the
   output by twice that times W;
-- f16 and bf16: each weight is rounded to 11 bits, and its product with the block's scale again:
-  2 * 2^-12 relative, 2^-11 * W; weights below the smallest fp16 subnormal (2^-24 of 2^9) vanish or round:
-  N * 2^-33 * max|v|;
+- f16 and bf16: each weight is rounded to fp16's 11 bits, half a step of which is up to 2^-11 of it
+  (finfo.eps / 2), and its product with the block's scale again: 2 * 2^-11 = 2^-10 of W; weights below the
+  smallest fp16 subnormal (2^-24 of 2^9) vanish or round: N * 2^-33 * max|v|;
 - fp32: weights as two fp16 terms, 2^-22 * W, and fp32 sums over N tokens in at most N/8 dependent
   steps a lane: N * 2^-27 * W;
 - the output's own rounding: half a step, finfo.eps / 2 * |out|.
@@ -185,7 +185,7 @@ class Case:
         N, D = max(self.lens + [1]), self.D
         vmax = max([np.nanmax(np.abs(x)) for x in self.v if len(x)] + [0.0])
         rel = 2 * (D + 16) * 2.0 ** -24 * 10 * size
-        rel = rel + (2.0 ** -11 if dtype != "f32" else 2.0 ** -22 + N * 2.0 ** -27)
+        rel = rel + (2.0 ** -10 if dtype != "f32" else 2.0 ** -22 + N * 2.0 ** -27)
         tol = rel * mag + torch.finfo(TYPES[dtype]).eps / 2 * np.abs(want) * 1.01 + N * 2.0 ** -33 * vmax
         far = np.abs(P.as_f64(got)[:R] - want[:R]) - tol[:R]
         assert np.all(np.isfinite(P.as_f64(got)[:R])), what
@@ -395,7 +395,7 @@ def test_long_context(sess):
             w = torch.softmax(s.masked_fill(hid, -float("inf")), 1)
             want = w @ v[:, h // 4].double()
             mag = w @ v[:, h // 4].double().abs()
-            tol = (2.0 ** -11 if dtype != "f32" else 2.0 ** -16) * mag + torch.finfo(q.dtype).eps / 2 * want.abs() * 1.01 + n * 2.0 ** -33 * 6
+            tol = (2.0 ** -10 if dtype != "f32" else 2.0 ** -16) * mag + torch.finfo(q.dtype).eps / 2 * want.abs() * 1.01 + n * 2.0 ** -33 * 6
             assert bool(((out[:, h].double() - want).abs() <= tol).all()), (rows, window, dtype, h)
         plan.close()
     pool.close()
