@@ -111,6 +111,7 @@ extern "C" int rstr_kv4_open(rstr_session* s, int32_t n_layers, int32_t n_kv, in
   if (!kv4_head_dim(head_dim)) return fail(s, RSTR_E_INVALID, "4-bit cache head dim must be 64, 128 or 256");
   if (page_size % 16) return fail(s, RSTR_E_INVALID, "4-bit cache page size must be a multiple of 16");
   if ((int64_t)page_size * physical_pages > 0x7FFFFFFF) return fail(s, RSTR_E_INVALID, "4-bit cache slots must fit in 31 bits");
+  if ((double)kv4_record_bytes(head_dim, page_size) * n_kv > 4e9) return fail(s, RSTR_E_INVALID, "4-bit cache pages must be smaller than 4 GB");
   std::unique_ptr<rstr_kv4> p(new (std::nothrow) rstr_kv4());
   if (!p) return fail(s, RSTR_E_OOM, "4-bit cache handle");
   p->s = s;

@@ -11,9 +11,9 @@
 // layer base + (page * n_kv + head) * record, holds ps tokens (ps % 16 == 0):
 //   K codes   dword (token, block b, g = k/8 of the block): eight codes.  Code
 //             2i is nibble i, code 2i+1 nibble 4+i, so (w >> 4i) & 0x000F000F
-//             is a pair of neighbours.  Order [token][b / BQ][g][b % BQ], BQ =
-//             min(D/32, 4): the 16 tokens x 128 dims of a matrix operand are 16
-//             bytes a lane.
+//             is a pair of neighbours.  Order [token / 16][b / BQ][g][token % 16][b % BQ],
+//             BQ = min(D/32, 4): a matrix operand of 16 tokens x 128 dims is 1 KB, 16
+//             bytes a lane in the lanes' order.
 //   V codes   halfword (token group tg = token/4, block pair bp, c = k%16, j =
 //             token%4): nibbles of dims c and 16+c of block 2bp, then of block
 //             2bp+1.  Order [tg][bp / BP][c][bp % BP][j], BP = min(D/64, 2): four

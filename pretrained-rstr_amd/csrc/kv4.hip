@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/rstr_hip.h"
 #include "device_math.h"
@@ -70,7 +71,7 @@ struct Rec {
   static constexpr int BP = D / 64 < 2 ? D / 64 : 2;  // V: block pairs a lane loads together
   // byte offsets of a K code dword, a V code halfword (its j = 0) and a scale
   static __device__ __forceinline__ int k(int tok, int b, int g) {
-    return tok * (D / 2) + (b / BQ) * (16 * BQ) + g * (4 * BQ) + (b % BQ) * 4;
+    return (tok >> 4) * (8 * D) + (b / BQ) * (256 * BQ) + g * (64 * BQ) + (tok & 15) * (4 * BQ) + (b % BQ) * 4;
   }
   static __device__ __forceinline__ int v(int tg, int bp, int c) {
     return tg * (2 * D) + (bp / BP) * (128 * BP) + c * (8 * BP) + (bp % BP) * 8;
@@ -271,9 +272,16 @@ hipError_t rows_type(hipStream_t st, bool append, const Kv4Layer& c, int dtype, 
 // whole; else (O, mref, l) of its piece, and k_kv4_merge joins the pieces in
 // order.
 constexpr int kTile = 32;
+constexpr int kStart = 6;  // what beginning an item costs, in tiles
 
 template <class E> struct Terms { static constexpr int n = 1; };
 template <> struct Terms<F32> { static constexpr int n = 2; };
+
+// Waves a SIMD: what the registers of a form allow.
+constexpr int attn_waves(int hd, int nt, int terms) { return hd == 256 ? 1 : nt == 1 && terms == 1 ? 3 : 2; }
+
+// Tiles of a wave's ring: what 160 KB of LDS hold for that many waves.
+constexpr int attn_ring(int hd, int nt, int terms) { return attn_waves(hd, nt, terms) == 3 && hd == 128 ? 2 : 4; }
 
 // The sequences of a call, as every wave sees them.
 struct Lines {
@@ -295,7 +303,7 @@ __device__ __forceinline__ Seq sequence(const Lines& L, int b) {
   s.lo = lo > 0 ? (int)lo / kTile : 0;  // first tile
   s.tiles = max((int)(((int64_t)s.len + kTile - 1) / kTile) - s.lo, 0);
   s.nct = (int)(((int64_t)s.m * L.group + L.cols - 1) / L.cols);
-  s.units = (int64_t)L.n_kv * s.nct * (L.whole ? 1 : s.tiles);
+  s.units = (int64_t)L.n_kv * s.nct * (L.whole ? 1 : s.tiles + kStart);
   return s;
 }
 
@@ -326,8 +334,14 @@ __device__ __forceinline__ int64_t part_of(int64_t total, int workers, int least
 }
 
 // Pieces of items that several waves share: two a wave (the end of an item
-// that an earlier wave began, the beginning of one that later waves end).
+// that an earlier wave began, the beginning of one that later waves end).  The wave
+// that begins an item leaves what the merge needs to know of it.
+struct Begun {
+  int b, h, ct, w, pieces;  // w: the wave; pieces: 0 where it ended the item too
+};
 struct Pieces {
+  int* n_items;
+  Begun* begun;  // [items]
   float2* ml;   // [2 * workers][cols] (mref, l)
   float* acc;   // [2 * workers][cols][D]
 };
@@ -346,97 +360,99 @@ __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t* o) {
   }
 }
 
-// Pair i of a dword's eight codes, minus 8, as two fp16.
-__device__ __forceinline__ h2 code_pair(uint32_t w, int i) {
-  const uint32_t x = i < 2 ? w : w >> 8;
-  if (i & 1) {
-    const h2 bias = {(_Float16)-72.0f, (_Float16)-72.0f};
-    return __builtin_bit_cast(h2, (x & 0x00F000F0u) | 0x54005400u) + bias;
+// Masks and exponents of the code expansion in registers: an instruction that
+// selects and merges takes no literals, and with literals it is two.
+struct Magic {
+  uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u, e1024 = 0x64006400u, e64 = 0x54005400u;
+  __device__ __forceinline__ Magic() {
+    asm("" : "+s"(lo));
+    asm("" : "+s"(hi));
+    asm("" : "+v"(e1024));
+    asm("" : "+v"(e64));
   }
-  const h2 bias = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-  return __builtin_bit_cast(h2, (x & 0x000F000Fu) | 0x64006400u) + bias;
+};
+// Pair i of a dword's eight codes c as two fp16, c - 8: 1024 + c (i even) or 64 + c
+// (odd) from the bits, less that bias.  (Fewer instructions leave the bias in the
+// products, or take the codes as fp16 subnormals, c * 2^-24: both were exact only to 2^-14
+// of a block's scale, and no faster.)
+__device__ __forceinline__ h2 code_pair(const Magic& m, uint32_t w, int i) {
+  const uint32_t x = i < 2 ? w : w >> 8;
+  const _Float16 b = (i & 1) ? (_Float16)-72.0f : (_Float16)-1032.0f;
+  return __builtin_bit_cast(h2, (i & 1) ? (x & m.hi) | m.e64 : (x & m.lo) | m.e1024) + h2{b, b};
 }
 __device__ __forceinline__ h8 pack8(h2 a, h2 b, h2 c, h2 d) {
   return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 __device__ __forceinline__ float half_of(uint32_t w, int i) { return (float)__builtin_bit_cast(h2, w)[i]; }
 
+// Codes and scales of a tile's keys or values, by half of 16 tokens.
 template <int D>
 struct TileRegs {
   static constexpr int NB = D / 32;
-  uint32_t k[2][NB], v[2][NB], ks[2][2 * NB], vs[2][2 * NB];
+  uint32_t c[2][NB], s[2][2 * NB];
 };
 
-// A wave's walk over the 16-token halves of consecutive tiles: page ids of 64
-// table entries at a time, one a lane, and the offset inside the current page.
-struct Walk {
-  const int32_t* row;
-  int pages, n_pages, ps;  // of the cache; of the sequence; tokens a page
-  int ids, first, pg, off;
-  __device__ __forceinline__ void fill() {
-    const int i = first + (threadIdx.x & 63);
-    ids = i < n_pages ? row[i] : -1;
-    if (ids < 0 || ids >= pages) ids = -1;
-  }
-  __device__ __forceinline__ void start(int token) {
-    pg = token / ps;
-    off = token - pg * ps;
-    first = pg;
-    fill();
-  }
-  __device__ __forceinline__ int page() const { return __builtin_amdgcn_readlane(ids, pg - first); }
-  __device__ __forceinline__ void next() {
-    off += 16;
-    if (off == ps) {
-      off = 0;
-      pg++;
-      if (pg - first == 64) {
-        first = pg;
-        fill();
-      }
-    }
-  }
+// The ring of tiles that a wave keeps in LDS (bytes): K codes, V codes, then the
+// scales of both, each as its halves of 16 tokens lie in the records.
+template <int D>
+struct Ring {
+  static constexpr int CODES = 16 * D, SCALES = 2 * D, TILE = 2 * CODES + 2 * SCALES;
+  static constexpr int LOADS = D == 64 ? 3 : 2 * (D / 64) + 1;  // instructions a tile
 };
+#define RSTR_LDS(p) ((__attribute__((address_space(3))) void*)(p))
+typedef const __attribute__((address_space(4))) int32_t* TablePtr;  // read-only for the kernel: scalar loads
 
-template <int D, int NT, class E>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
+// s_waitcnt vmcnt(N) alone.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+template <int D, int NT, int NS, class E>
+__global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
     k_kv4_attn(Kv4Attn a, const int32_t* __restrict__ ro, const int32_t* __restrict__ lens, const int32_t* __restrict__ table,
-               const uint8_t* __restrict__ base, Pieces pc, int64_t* __restrict__ firsts, int workers, int least, bool whole) {
+               const uint8_t* __restrict__ base, Pieces pc, int workers, int least, bool whole) {
   typedef Rec<D> R;
   typedef typename E::T T;
   constexpr int NB = D / 32, COLS = 16 * NT, TERMS = Terms<E>::n;
+  const Magic magic;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int w = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
   const int group = a.n_q / a.c.n_kv, ps = a.c.page_size;
   const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), whole};
 
-  if (w >= workers) {  // one wave more than workers: the sequences' first units, for the merge
-    if (w > workers || whole) return;
-    int64_t run = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-      const int64_t n = b0 + lane < a.batch ? sequence(L, b0 + lane).units : 0;
-      const int64_t in = wave_scan_i64(n);
-      if (b0 + lane < a.batch) firsts[b0 + lane] = run + in - n;
-      run += shfl64(in, 63);
-    }
-    if (lane == 0) firsts[a.batch] = run;
-    return;
-  }
   int64_t mine = 0;
-  for (int b = lane; b < a.batch; b += 64) mine += sequence(L, b).units;
+  int items = 0;
+  for (int b = lane; b < a.batch; b += 64) {
+    const Seq s = sequence(L, b);
+    mine += s.units;
+    items += L.n_kv * s.nct;
+  }
+  if (w == 0 && !whole) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) items += __shfl_xor(items, d, 64);
+    if (lane == 0) *pc.n_items = items;
+  }
   const int64_t total = uniform64(wave_sum_i64(mine));
   const int64_t part = part_of(total, workers, least);
   int64_t u = (int64_t)w * part;
   const int64_t u_end = min(u + part, total);
   if (u >= u_end) return;
-  int b = 0;            // the sequence that unit u lies in, and its first unit
+  int b = 0, item0 = 0;  // the sequence that unit u lies in, its first item and unit
   int64_t first = 0;
   for (int64_t run = 0;; b += 64) {
-    const int64_t n = b + lane < a.batch ? sequence(L, b + lane).units : 0;
+    const Seq s = sequence(L, min(b + lane, a.batch - 1));
+    const bool in_batch = b + lane < a.batch;
+    const int64_t n = in_batch ? s.units : 0;
+    const int m = in_batch ? L.n_kv * s.nct : 0;
     const int64_t in = wave_scan_i64(n);
     const uint64_t over = __ballot(run + in > u);
+    const int f = over ? __ffsll((unsigned long long)over) - 1 : 64;
+    int before = lane < f ? m : 0;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d, 64);
+    item0 = uniform(item0 + before);
     if (over) {
-      const int f = __ffsll((unsigned long long)over) - 1;
       first = uniform64(run + shfl64(in - n, f));
       b = uniform(b + f);
       break;
@@ -444,14 +460,20 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
     run += shfl64(in, 63);
   }
 
+  typedef Ring<D> G;
+  __shared__ __attribute__((aligned(16))) uint8_t rings[4][NS][G::TILE];
+  uint8_t(*ring)[G::TILE] = rings[uniform(threadIdx.x >> 6)];
   const int64_t rec = kv4_record_bytes(D, ps);
-  const int kl = R::k(col, 0, g), vl = R::vbase(ps) + R::v(g, 0, col), sl = R::s(g, 0);
-  const int ksb = R::ksbase(ps) + sl, vsb = R::vsbase(ps) + sl;
+  // where a lane's pieces lie in a tile of the ring, and where the lane's scales come from
+  const uint32_t k_at = lane * (4 * R::BQ), v_at = G::CODES + R::v(g, 0, col), ks_at = 2 * G::CODES + g * (8 * NB), vs_at = ks_at + G::SCALES;
+  constexpr int SL = D / 16;  // lanes that load the scales of one half
+  const uint32_t sc_off = (lane & (2 * SL) ? R::vsbase(ps) : R::ksbase(ps)) + (lane % SL) * 16;
 
   while (u < u_end) {
     const Seq s = sequence(L, b);
     if (u >= first + s.units) {  // behind b: the next sequence that has units
       first += s.units;
+      item0 += L.n_kv * s.nct;
       b++;
       for (;; b += 64) {
         const uint64_t some = __ballot(b + lane < a.batch && sequence(L, b + lane).units > 0);
@@ -463,13 +485,15 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
       continue;
     }
     const int64_t rel = u - first;
-    const int per_item = whole ? 1 : s.tiles;
+    const int per_item = whole ? 1 : s.tiles + kStart;
     const int64_t item = rel / per_item;
     const int at = (int)(rel - item * per_item);
     const int h = (int)(item / s.nct), ct = (int)(item - (int64_t)h * s.nct);
     const int n = (int)min((int64_t)(per_item - at), u_end - u);
     const bool begins = at == 0, ends = at + n == per_item;
     u += n;
+    if (begins && !whole && lane == 0)
+      pc.begun[item0 + (int)item] = Begun{b, h, ct, w, ends ? 0 : (int)((u - n + per_item - 1) / part - w + 1)};
 
     // the columns' rows and what they see
     const int c0 = ct * COLS, p0 = s.len - s.m;
@@ -488,12 +512,13 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
     }
     const int hi_last = max(p0 + rl + 1, 0), hi_first = max(p0 + rf + 1, 0);
     const int lo_first = a.window > 0 ? max(p0 + rf + 1 - a.window, 0) : 0, lo_last = a.window > 0 ? max(p0 + rl + 1 - a.window, 0) : 0;
-    int t0 = s.lo + (whole ? 0 : at), t1 = whole ? s.lo + s.tiles : t0 + n;
+    int t0 = s.lo + (whole ? 0 : max(at - kStart, 0)), t1 = s.lo + (whole ? s.tiles : max(at + n - kStart, 0));
     t0 = max(t0, lo_first / kTile);
     t1 = min(t1, (hi_last + kTile - 1) / kTile);
 
     f4 acc[NT][2 * NB];
-    float mref[NT], l[NT], kcol[NT], fs[NT];
+    float mref[NT], kcol[NT], fs[NT];
+    f4 l[NT];             // one term: all four the sum of p; two: the lane's own part in the first
     int elim[NT];         // exponents of the V scales seen so far are no larger; fs = 2^(15 - elim)
     bool scaled = false;  // some column's fs is below 1
     h8 q[NT][TERMS][NB];
@@ -502,11 +527,84 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 #pragma unroll
       for (int i = 0; i < 2 * NB; i++) acc[t][i] = f4{0, 0, 0, 0};
       mref[t] = -1e30f;
-      l[t] = 0.0f;
+      l[t] = f4{0, 0, 0, 0};
       elim[t] = TERMS == 1 ? 15 : 0;
       fs[t] = __builtin_amdgcn_ldexpf(1.0f, 15 - elim[t]);
     }
     if (t0 < t1) {
+      // Tiles come into the ring NS - 1 ahead, straight into LDS; behind the last one, and
+      // for a page that is not there, from page 0, so that the count of loads in
+      // flight is known.  Page ids are read one tile ahead of their loads.
+      const TablePtr row = (TablePtr)(table + (int64_t)b * a.pps);
+      const int n_pages = (int)(((int64_t)s.len + ps - 1) / ps);
+      int pg = t0 * kTile / ps, off = t0 * kTile - pg * ps, slot = 0;
+      const uint8_t* head = base + (int64_t)h * rec;
+      const uint32_t page_bytes = (uint32_t)(a.c.n_kv * rec);
+      int id[2], id_off[2];
+      const auto look = [&] {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int v = row[min(pg, n_pages - 1)];
+          id[j] = pg < n_pages ? v : -1;
+          id_off[j] = off;
+          off += 16;
+          if (off == ps) { off = 0; pg++; }
+        }
+      };
+      uint32_t lost = 0;  // halves whose page is not there: two bits a tile, the tile computed lowest
+      const auto issue = [&] {
+        const uint8_t* r[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const bool ok = (uint32_t)id[j] < (uint32_t)a.c.pages;
+          r[j] = head + (uint64_t)(uint32_t)(ok ? id[j] : 0) * page_bytes;
+          if (!ok) lost |= 1u << (2 * (NS - 1) + j);
+        }
+        uint8_t* to = ring[slot];
+        slot = slot + 1 == NS ? 0 : slot + 1;
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+          const uint32_t start = kv ? R::vbase(ps) : 0;
+          if constexpr (D == 64) {  // half a wave a half
+            const uint8_t* p = lane < 32 ? r[0] + (uint32_t)id_off[0] * (D / 2) : r[1] + (uint32_t)id_off[1] * (D / 2);
+            __builtin_amdgcn_global_load_lds((const void*)(p + (start + (lane & 31) * 16)), RSTR_LDS(to + kv * G::CODES), 16, 0, 0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+              for (int i = 0; i < D / 128; i++)
+                __builtin_amdgcn_global_load_lds((const void*)(r[j] + (start + (uint32_t)id_off[j] * (D / 2) + i * 1024 + lane * 16)),
+                                                 RSTR_LDS(to + kv * G::CODES + (j * (D / 128) + i) * 1024), 16, 0, 0);
+          }
+        }
+        const bool second = (lane & SL) != 0;
+        const uint8_t* p = second ? r[1] + (uint32_t)id_off[1] * SL : r[0] + (uint32_t)id_off[0] * SL;
+        if (lane < 4 * SL) __builtin_amdgcn_global_load_lds((const void*)(p + sc_off), RSTR_LDS(to + 2 * G::CODES), 16, 0, 0);
+        look();
+      };
+      // a tile's codes or scales from the ring, by half
+      const auto codes = [&](const uint8_t* at, uint32_t (&o)[2][NB]) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          if constexpr (NB == 8) {
+            load_dwords<4>(at + j * 8 * D, o[j]);
+          } else {
+            load_dwords<NB>(at + j * 8 * D, o[j]);
+          }
+        }
+      };
+      const auto scales = [&](const uint8_t* at, uint32_t (&o)[2][2 * NB]) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) load_dwords<2 * NB>(at + j * D, o[j]);
+      };
+      int now = 0;  // the ring's tile that is computed
+      look();
+#pragma unroll
+      for (int i = 0; i < NS - 1; i++) {
+        lost >>= 2;
+        issue();
+      }
+
       const bool vec = vec_rows(a.q, sizeof(T));
 #pragma unroll
       for (int t = 0; t < NT; t++) {
@@ -538,141 +636,143 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
           }
       }
 
-      Walk walk;
-      walk.row = table + (int64_t)b * a.pps;
-      walk.pages = a.c.pages;
-      walk.n_pages = (int)(((int64_t)s.len + ps - 1) / ps);
-      walk.ps = ps;
-      walk.start(t0 * kTile);
-      int gone = 0;  // halves of the tile just loaded whose page is not there (bits)
-      const auto load = [&](TileRegs<D>& x) {
-        gone = 0;
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          int pg = walk.page();
-          if (pg < 0) { gone |= 1 << j; pg = 0; }
-          const uint8_t* r = base + ((int64_t)pg * a.c.n_kv + h) * rec;
-          const int code = walk.off * (D / 2), scl = walk.off * (D / 16);
-          if constexpr (NB == 8) {
-            load_dwords<4>(r + (code + kl), x.k[j]);
-            load_dwords<4>(r + (code + kl + 16 * R::BQ), x.k[j] + 4);
-            load_dwords<4>(r + (code + vl), x.v[j]);
-            load_dwords<4>(r + (code + vl + 128 * R::BP), x.v[j] + 4);
-          } else {
-            load_dwords<NB>(r + (code + kl), x.k[j]);
-            load_dwords<NB>(r + (code + vl), x.v[j]);
-          }
-          load_dwords<2 * NB>(r + (scl + ksb), x.ks[j]);
-          load_dwords<2 * NB>(r + (scl + vsb), x.vs[j]);
-          walk.next();
-        }
-      };
+      const uint32_t one = 0x3C003C00u;
+      const h8 ones = __builtin_bit_cast(h8, u32x4{one, one, one, one});
 
-      const auto compute = [&](const TileRegs<D>& x, int tile, int lost) {
+      for (int tile = t0; tile < t1; tile++) {
+        // the slot filled next was read a tile ago: those reads have returned
+        lost >>= 2;
+        issue();
+        wait_loads<(NS - 1) * G::LOADS>();
+        asm volatile("" ::: "memory");
+        const uint8_t* at = ring[now];
+        now = now + 1 == NS ? 0 : now + 1;
+        TileRegs<D> xk, xv;
+        codes(at + k_at, xk.c);
+        if constexpr (NB == 8) {
+          load_dwords<4>(at + k_at + 1024, xk.c[0] + 4);
+          load_dwords<4>(at + k_at + 1024 + 8 * D, xk.c[1] + 4);
+        }
+        scales(at + ks_at, xk.s);
         const int tok0 = tile * kTile;
-        const bool edge = lost || tok0 < lo_last || tok0 + kTile > hi_first;
-        h8 kq[2][NB];
+        const bool edge = (lost & 3) || tok0 < lo_last || tok0 + kTile > hi_first;
+        float sc[NT][8];  // scores over 2^e of their column's queries, before the scale
+        {
+          h8 kq[2][NB];
 #pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-          for (int bk = 0; bk < NB; bk++)
-            kq[j][bk] = pack8(code_pair(x.k[j][bk], 0), code_pair(x.k[j][bk], 1), code_pair(x.k[j][bk], 2), code_pair(x.k[j][bk], 3));
-        float sc[NT][8];
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            f4 sum = {0, 0, 0, 0};
+          for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int bk = 0; bk < NB; bk++) {
-              const f4 zero = {0, 0, 0, 0};
-              f4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[j][bk], q[t][0][bk], zero, 0, 0, 0);
-              if constexpr (TERMS == 2) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[j][bk], q[t][1][bk], d, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 4; i++) sum[i] = __builtin_fmaf(half_of(x.ks[j][2 * bk + (i >> 1)], i & 1), d[i], sum[i]);
+              const uint32_t w = xk.c[j][bk];
+              kq[j][bk] = pack8(code_pair(magic, w, 0), code_pair(magic, w, 1), code_pair(magic, w, 2), code_pair(magic, w, 3));
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) sc[t][4 * j + i] = sum[i] * kcol[t];
-          }
-        uint32_t see[NT];  // bit 4j + i: token 16j + 4g + i of the tile is seen
+          for (int t = 0; t < NT; t++) {
+            f4 d[2][NB];
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-          see[t] = 0xFF;
-          if (edge) {
-            see[t] = 0;
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+              for (int bk = 0; bk < NB; bk++) {
+                d[j][bk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[j][bk], q[t][0][bk], f4{0, 0, 0, 0}, 0, 0, 0);
+                if constexpr (TERMS == 2) d[j][bk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[j][bk], q[t][1][bk], d[j][bk], 0, 0, 0);
+              }
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
               for (int i = 0; i < 4; i++) {
-                const int tok = tok0 + 16 * j + 4 * g + i;
-                const bool ok = tok >= lo[t] && tok < hi[t] && !((lost >> j) & 1);
-                if (ok) see[t] |= 1u << (4 * j + i);
-                else sc[t][4 * j + i] = -INFINITY;
+                float sum = __builtin_fmaf(half_of(xk.s[j][i >> 1], i & 1), d[j][0][i], 0.0f);
+#pragma unroll
+                for (int bk = 1; bk < NB; bk++) sum = __builtin_fmaf(half_of(xk.s[j][2 * bk + (i >> 1)], i & 1), d[j][bk][i], sum);
+                sc[t][4 * j + i] = sum;
               }
           }
         }
-        // does a score pass what mref allows, or a scale of V what 2^a allows?
-        bool grow = false;
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          float m = sc[t][0];
-#pragma unroll
-          for (int i = 1; i < 8; i++) m = fmaxf(m, sc[t][i]);
-          grow |= m - mref[t] > 14.0f;
+        codes(at + v_at, xv.c);
+        if constexpr (NB == 8) {
+          load_dwords<4>(at + v_at + 256, xv.c[0] + 4);
+          load_dwords<4>(at + v_at + 256 + 8 * D, xv.c[1] + 4);
         }
-        uint32_t ors[2][2];  // of the bits of the scales, by half and token pair
+        scales(at + vs_at, xv.s);
+        // exponents of 2 against mref: -infinity where a token is not seen
+        float e2[NT][8];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) e2[t][i] = __builtin_fmaf(sc[t][i], kcol[t], -mref[t]);
+        // the largest exponent of a V scale, from above: of all bits together (exponents
+        // to 15 have no bit that 15 has not), and exactly where that is more than 15
+        const auto exponent = [](uint32_t o) { return (int)(((o | (o >> 16)) >> 10) & 31); };
+        uint32_t ors = 0;
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-          for (int i = 0; i < 2; i++) {
-            ors[j][i] = x.vs[j][i];
-#pragma unroll
-            for (int bk = 1; bk < NB; bk++) ors[j][i] |= x.vs[j][2 * bk + i];
-          }
-        // the largest exponent, from above: of all bits together (exponents to 15 have no
-        // bit that 15 has not), and exactly where that is more than 15
+          for (int i = 0; i < 2 * NB; i++) ors |= xv.s[j][i];
         int exps[NT];
-        const uint32_t o = ors[0][0] | ors[0][1] | ors[1][0] | ors[1][1];
-        const int all = (int)(((o | (o >> 16)) >> 10) & 31);
-        const bool large = __ballot(all > 15) != 0;
+        uint32_t see[NT];  // bit i: the lane's token i is seen by its column
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-          exps[t] = all;
-          if (edge) {
-            uint32_t k = 0;
+          see[t] = 0xFF;
+          exps[t] = exponent(ors);
+        }
+        if (edge) {
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+          for (int t = 0; t < NT; t++) {
+            uint32_t m = 0, pairs[4], o = 0;
 #pragma unroll
-              for (int i = 0; i < 4; i++)
-                if ((see[t] >> (4 * j + i)) & 1) k |= ors[j][i >> 1] >> (16 * (i & 1));
-            exps[t] = (int)((k >> 10) & 31);
-          }
-          if (large) {
-            int e = 0;
+            for (int i = 0; i < 8; i++) {
+              const int tok = tok0 + 16 * (i >> 2) + 4 * g + (i & 3);
+              const bool ok = tok >= lo[t] && tok < hi[t] && !((lost >> (i >> 2)) & 1);
+              m |= ok ? 1u << i : 0u;
+              if (!ok) e2[t][i] = -INFINITY;
+            }
+            see[t] = m;
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < 4; i++) {
+              pairs[i] = ((m >> (2 * i)) & 1 ? 0xFFFFu : 0) | ((m >> (2 * i + 1)) & 1 ? 0xFFFF0000u : 0);
 #pragma unroll
               for (int bk = 0; bk < NB; bk++) {
-                const int k = (int)((x.vs[i >> 2][2 * bk + ((i >> 1) & 1)] >> (16 * (i & 1) + 10)) & 31);
-                if (((see[t] >> i) & 1) && k < 31) e = max(e, k);
+                // 0 * NaN of a token that is not seen: scales of no token of this column become 0
+                if constexpr (NT == 1) xv.s[i >> 1][2 * bk + (i & 1)] &= pairs[i];
+                o |= xv.s[i >> 1][2 * bk + (i & 1)] & pairs[i];
               }
-            exps[t] = e;
+            }
+            exps[t] = exponent(o);
           }
-          grow |= exps[t] > elim[t];
+        }
+        // does a score pass what mref allows, or a scale of V what fs does?
+        bool grow = false;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          float m = e2[t][0];
+#pragma unroll
+          for (int i = 1; i < 8; i++) m = fmaxf(m, e2[t][i]);
+          grow |= m > 14.0f || exps[t] > elim[t];
         }
         if (__ballot(grow)) {
           bool big = false;
 #pragma unroll
           for (int t = 0; t < NT; t++) {
-            float m = sc[t][0];
+            float m = -INFINITY;
+            int e = exps[t];
+            if (e > 15) e = 0;
 #pragma unroll
-            for (int i = 1; i < 8; i++) m = fmaxf(m, sc[t][i]);
+            for (int i = 0; i < 8; i++) {
+              const bool ok = (see[t] >> i) & 1;
+              if (ok) m = fmaxf(m, sc[t][i] * kcol[t]);
+              if (exps[t] > 15 && ok)
+#pragma unroll
+                for (int bk = 0; bk < NB; bk++) {
+                  const int k = (int)((xv.s[i >> 2][2 * bk + ((i >> 1) & 1)] >> (16 * (i & 1) + 10)) & 31);
+                  if (k < 31) e = max(e, k);
+                }
+            }
             m = xor_max<32>(xor_max<16>(m));
-            int e = max(exps[t], elim[t]);
+            e = max(e, elim[t]);
             e = max(e, __shfl_xor(e, 16, 64));
             e = max(e, __shfl_xor(e, 32, 64));
             if (e <= 15) { e |= e >> 1; e |= e >> 2; }
-            const float now = fmaxf(mref[t], m - 10.0f);
+            // a column that needs no change has none: it does not depend on its neighbours
+            const float now = m - mref[t] > 14.0f ? m - 10.0f : mref[t];
             const float keep = __builtin_amdgcn_exp2f(mref[t] - now);
             mref[t] = now;
             l[t] *= keep;
@@ -682,6 +782,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
             big |= e > 15;
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) acc[t][i] *= less;
+#pragma unroll
+            for (int i = 0; i < 8; i++) e2[t][i] = (see[t] >> i) & 1 ? __builtin_fmaf(sc[t][i], kcol[t], -mref[t]) : -INFINITY;
           }
           scaled = __ballot(big) != 0;
         }
@@ -689,16 +791,32 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
         for (int t = 0; t < NT; t++) {
           float p[8];
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            p[i] = __builtin_amdgcn_exp2f(sc[t][i] - mref[t]);
-            l[t] += p[i];
-          }
+          for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(e2[t][i]);
           h2 ph[2][2];
-          if constexpr (TERMS == 1)
+          if constexpr (TERMS == 1) {
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
               for (int i = 0; i < 2; i++) ph[j][i] = h2{(_Float16)p[4 * j + 2 * i], (_Float16)p[4 * j + 2 * i + 1]};
+            l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pack8(ph[0][0], ph[0][1], ph[1][0], ph[1][1]), l[t], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) l[t][0] += p[i];
+          }
+          // scales of V, below 2 by fs, where a column is wide enough of them
+          uint32_t vs[2][2 * NB];
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) vs[j][i] = xv.s[j][i];
+          if (TERMS == 1 && scaled) {
+            asm volatile("");  // stays a branch
+            const h2 f = {(_Float16)fs[t], (_Float16)fs[t]};
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+              for (int i = 0; i < 2 * NB; i++) vs[j][i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, vs[j][i]) * f);
+          }
 #pragma unroll
           for (int bk = 0; bk < NB; bk++) {
             h8 pd[TERMS];
@@ -708,20 +826,19 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
               for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                  h2 d = __builtin_bit_cast(h2, x.vs[j][2 * bk + i]);
-                  if (scaled) d *= h2{(_Float16)fs[t], (_Float16)fs[t]};
-                  y[j][i] = ph[j][i] * d;
-                  if (edge) {  // 0 * NaN of a token that is not seen
-                    const uint32_t keep = ((see[t] >> (4 * j + 2 * i)) & 1 ? 0xFFFFu : 0) | ((see[t] >> (4 * j + 2 * i + 1)) & 1 ? 0xFFFF0000u : 0);
-                    y[j][i] = __builtin_bit_cast(h2, __builtin_bit_cast(uint32_t, y[j][i]) & keep);
+                  y[j][i] = ph[j][i] * __builtin_bit_cast(h2, vs[j][2 * bk + i]);
+                  if constexpr (NT > 1) {
+                    const uint32_t m = see[t] >> (4 * j + 2 * i);
+                    const uint32_t pair = (m & 1 ? 0xFFFFu : 0) | (m & 2 ? 0xFFFF0000u : 0);
+                    if (edge) y[j][i] = __builtin_bit_cast(h2, __builtin_bit_cast(uint32_t, y[j][i]) & pair);
                   }
                 }
               pd[0] = pack8(y[0][0], y[0][1], y[1][0], y[1][1]);
             } else {
 #pragma unroll
               for (int i = 0; i < 8; i++) {
-                float y = p[i] * fs[t] * half_of(x.vs[i >> 2][2 * bk + ((i >> 1) & 1)], i & 1);
-                if (edge && !((see[t] >> i) & 1)) y = 0.0f;
+                float y = p[i] * fs[t] * half_of(vs[i >> 2][2 * bk + ((i >> 1) & 1)], i & 1);
+                if (NT > 1 && edge && !((see[t] >> i) & 1)) y = 0.0f;
                 const _Float16 top = (_Float16)y;
                 pd[0][i] = top;
                 pd[1][i] = (_Float16)(y - (float)top);
@@ -730,27 +847,17 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
 #pragma unroll
             for (int hh = 0; hh < 2; hh++) {
               const int pr = (bk & 1) * 2 + hh, dw = (bk >> 1) * 2;
-              const h8 vq = pack8(code_pair(x.v[0][dw], pr), code_pair(x.v[0][dw + 1], pr), code_pair(x.v[1][dw], pr), code_pair(x.v[1][dw + 1], pr));
+              const auto pair = [&](int j, int k) { return code_pair(magic, xv.c[j][dw + k], pr); };
+              const h8 vq = pack8(pair(0, 0), pair(0, 1), pair(1, 0), pair(1, 1));
               f4& o = acc[t][2 * bk + hh];
               o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pd[0], o, 0, 0, 0);
               if constexpr (TERMS == 2) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pd[1], o, 0, 0, 0);
             }
           }
         }
-      };
-
-      TileRegs<D> x, y;
-      load(x);
-      int lost = gone;
-      for (int tile = t0;;) {
-        int next = 0;
-        if (tile + 1 < t1) { load(y); next = gone; }
-        compute(x, tile, lost);
-        if (++tile >= t1) break;
-        if (tile + 1 < t1) { load(x); lost = gone; }
-        compute(y, tile, next);
-        if (++tile >= t1) break;
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the slot is free
       }
+      wait_loads<0>();  // the next part's loads into the ring come behind these
     }
 
     // O on the scale of l
@@ -765,7 +872,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
     const int64_t slot = (begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w) * COLS;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const float sum = xor_add<32>(xor_add<16>(l[t]));
+      const float sum = TERMS == 1 ? l[t][0] : xor_add<32>(xor_add<16>(l[t][0]));
       if (!valid[t]) continue;
       if (begins && ends) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -795,62 +902,75 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2)
   }
 }
 
-// One workgroup per (query row, head): the pieces of an item that several waves
-// computed, joined in their order (a wave takes every n-th piece); zeros for a
-// row whose item has no tiles.
+// Joins the pieces of an item that several waves computed, in their order: a workgroup
+// an item and `per` columns (more for every gridDim.y), its waves by column and by piece.
 template <int D, class E>
-__global__ void k_kv4_merge(Kv4Attn a, Lines L, Pieces pc, const int64_t* __restrict__ firsts, int workers, int least) {
+__global__ void k_kv4_merge(Kv4Attn a, Lines L, Pieces pc, int per) {
   constexpr int V = D / 64;  // dims a lane
+  typedef typename E::T T;
   __shared__ float part[16][D];
   __shared__ float pl[16];
-  const int row = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  int lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (L.ro[mid] <= row) lo = mid; else hi = mid;
-  }
-  const int b = lo;
-  const Seq s = sequence(L, b);
-  if (row < s.r0 || row >= s.r0 + s.m) return;
-  typename E::T* dst = (typename E::T*)a.out.p + (int64_t)row * a.out.row + (int64_t)hq * a.out.head;
-  if (s.tiles == 0) {
-    for (int i = threadIdx.x; i < D; i += blockDim.x) dst[i] = E::put(0.0f);
-    return;
-  }
-  const int h = hq / L.group, c = (row - s.r0) * L.group + hq % L.group, ct = c / L.cols;
-  const int64_t part_units = part_of(firsts[a.batch], workers, least);
-  const int64_t u0 = firsts[b] + ((int64_t)h * s.nct + ct) * s.tiles, u1 = u0 + s.tiles - 1;
-  const int64_t w0 = u0 / part_units, w1 = u1 / part_units;
-  if (w0 == w1) return;  // written as a whole
-  const int n = (int)(w1 - w0 + 1), cc = c % L.cols;
-  const auto slot = [&](int i) { return (i == 0 ? 2 * w0 + 1 : 2 * (w0 + i)) * L.cols + cc; };
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) {
-    const float2 x = pc.ml[slot(i)];
-    if (x.y != 0.0f) m = fmaxf(m, x.x);
-  }
-  m = wave_max(m);
-  float acc[V] = {}, l = 0.0f;
-  for (int i = wave; i < n; i += waves) {
-    const int64_t k = slot(i);
-    const float2 x = pc.ml[k];
-    if (x.y == 0.0f) continue;
-    const float f = __builtin_amdgcn_exp2f(x.x - m);
-    l = __builtin_fmaf(f, x.y, l);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x >= *pc.n_items) return;
+  const Begun it = pc.begun[blockIdx.x];
+  const int n = it.pieces;
+  if (n == 0) return;
+  const int64_t w0 = it.w;
+  const Seq s = sequence(L, it.b);
+  const int c0 = it.ct * L.cols, cols = min(L.cols, s.m * L.group - c0);
+  const auto slot = [&](int i, int c) { return (i == 0 ? 2 * w0 + 1 : 2 * (w0 + i)) * L.cols + c; };
+  const int share = (blockDim.x >> 6) / per, mine = wave % share;  // waves a column
+  for (int at = blockIdx.y * per; at < cols; at += gridDim.y * per) {  // the same for all waves
+    const int c = at + wave / share;
+    float acc[V] = {}, l = 0.0f;
+    if (c < cols) {
+      float m = -INFINITY;
+      for (int i0 = mine; i0 == mine || i0 < n; i0 += 8 * share) {
+        float2 x[8];
+        float v[8][V];
 #pragma unroll
-    for (int j = 0; j < V; j++) acc[j] = __builtin_fmaf(f, pc.acc[k * D + lane * V + j], acc[j]);
-  }
+        for (int k = 0; k < 8; k++) {  // all loads before the first use
+          const int64_t p = slot(min(i0 + k * share, n - 1), c);
+          x[k] = pc.ml[p];
 #pragma unroll
-  for (int j = 0; j < V; j++) part[wave][lane * V + j] = acc[j];
-  if (lane == 0) pl[wave] = l;
-  __syncthreads();
-  for (int i = threadIdx.x; i < D; i += blockDim.x) {
-    float o = 0.0f, sum = 0.0f;
-    for (int k = 0; k < waves; k++) {
-      o += part[k][i];
-      sum += pl[k];
+          for (int j = 0; j < V; j++) v[k][j] = pc.acc[p * D + lane * V + j];
+        }
+        if (i0 == mine) {
+          for (int i = lane; i < n; i += 64) {
+            const float2 y = pc.ml[slot(i, c)];
+            if (y.y != 0.0f) m = fmaxf(m, y.x);
+          }
+          m = wave_max(m);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const bool some = i0 + k * share < n && x[k].y != 0.0f;
+          const float f = some ? __builtin_amdgcn_exp2f(x[k].x - m) : 0.0f;
+          l = __builtin_fmaf(f, some ? x[k].y : 0.0f, l);
+#pragma unroll
+          for (int j = 0; j < V; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
+        }
+      }
     }
-    dst[i] = E::put(sum == 0.0f ? 0.0f : o / sum);
+    if (share > 1) {
+#pragma unroll
+      for (int j = 0; j < V; j++) part[wave][lane * V + j] = acc[j];
+      if (lane == 0) pl[wave] = l;
+      __syncthreads();
+      if (mine == 0)
+        for (int k = 1; k < share; k++) {
+#pragma unroll
+          for (int j = 0; j < V; j++) acc[j] += part[wave + k][lane * V + j];
+          l += pl[wave + k];
+        }
+      __syncthreads();
+    }
+    if (c < cols && mine == 0) {
+      const int cc = c0 + c, r = cc / L.group;
+      T* dst = (T*)a.out.p + (int64_t)(s.r0 + r) * a.out.row + ((int64_t)it.h * L.group + cc % L.group) * a.out.head + lane * V;
+#pragma unroll
+      for (int j = 0; j < V; j++) dst[j] = E::put(l == 0.0f ? 0.0f : acc[j] / l);
+    }
   }
 }
 
@@ -875,42 +995,48 @@ int compute_units() {
   return n[dev];
 }
 
-constexpr int kMaxWaves = 2;  // a SIMD, of the attention kernel's
 constexpr int kLeast = 4;     // tiles a wave takes at least
 
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Workspace: the sequences' first units, then the pieces of up to `workers` waves.
-size_t attn_bytes(int batch, int64_t workers, int cols, int hd) {
-  return align256(sizeof(int64_t) * ((size_t)batch + 1)) + align256(sizeof(float2) * 2 * workers * cols) +
-         sizeof(float) * 2 * workers * cols * hd;
+// Items of a call, at most.
+int64_t attn_items(int n_q, int n_kv, int batch, int rows, int cols) {
+  return n_kv * ((int64_t)rows * (n_q / n_kv) / cols + std::min(batch, rows));
+}
+// Workspace: what up to `workers` waves leave of items that they share.
+size_t attn_bytes(int64_t items, int64_t workers, int cols, int hd) {
+  return 256 + align256(sizeof(Begun) * items) + align256(sizeof(float2) * 2 * workers * cols) + sizeof(float) * 2 * workers * cols * hd;
 }
 
 template <int D, int NT, class E>
 hipError_t attn_tiles(hipStream_t st, const Kv4Attn& a) {
   const int cols = 16 * NT, group = a.n_q / a.c.n_kv;
   const int64_t cap = std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0);
-  const int64_t items = a.c.n_kv * ((int64_t)a.rows * group / cols + std::min(a.batch, a.rows));  // at most
+  const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
   const int64_t tiles = (cap + kTile - 1) / kTile;
   const bool whole = tiles <= kLeast;
-  const int64_t most = (int64_t)compute_units() * 4 * kMaxWaves;
-  const int64_t want = whole ? items : (items * tiles + kLeast - 1) / kLeast;
+  const int64_t most = (int64_t)compute_units() * 4 * attn_waves(D, NT, Terms<E>::n);
+  const int64_t want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
   const int workers = (int)((std::min(most, want) + 3) / 4 * 4), least = whole ? 1 : kLeast;
   char* ws = (char*)a.ws;
-  int64_t* firsts = (int64_t*)ws;
-  ws += align256(sizeof(int64_t) * ((size_t)a.batch + 1));
   Pieces pc;
+  pc.n_items = (int*)ws;
+  ws += 256;
+  pc.begun = (Begun*)ws;
+  ws += align256(sizeof(Begun) * items);
   pc.ml = (float2*)ws;
   ws += align256(sizeof(float2) * 2 * workers * cols);
   pc.acc = (float*)ws;
-  hipLaunchKernelGGL((k_kv4_attn<D, NT, E>), dim3((unsigned)(workers / 4 + (whole ? 0 : 1))), dim3(256), 0, st, a, a.row_offsets, a.lengths,
-                     a.page_table, a.c.base, pc, firsts, workers, least, whole);
+  hipLaunchKernelGGL((k_kv4_attn<D, NT, attn_ring(D, NT, Terms<E>::n), E>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths,
+                     a.page_table, a.c.base, pc, workers, least, whole);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || whole) return e;
   const Lines L{a.row_offsets, a.lengths, a.rows, a.c.n_kv, group, a.window, cols, cap, false};
-  const int64_t heads = (int64_t)a.rows * a.n_q;
-  const int threads = heads <= 1024 ? 1024 : 256;  // few rows have many pieces each
-  hipLaunchKernelGGL((k_kv4_merge<D, E>), dim3((unsigned)a.rows, (unsigned)a.n_q), dim3(threads), 0, st, a, L, pc, firsts, workers, least);
+  // items of many pieces have a workgroup a column, of very many a large one
+  const int pieces = (int)(workers / items), per = pieces >= 4 ? 1 : 4;
+  const int64_t columns = std::min<int64_t>(cols, (int64_t)a.max_rows * group);
+  hipLaunchKernelGGL((k_kv4_merge<D, E>), dim3((unsigned)items, (unsigned)((columns + per - 1) / per)), dim3(pieces >= 16 ? 1024 : 256), 0,
+                     st, a, L, pc, per);
   return hipGetLastError();
 }
 
@@ -925,10 +1051,7 @@ hipError_t attn_type(hipStream_t st, const Kv4Attn& a) {
 }  // namespace
 
 size_t kv4_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows) {
-  (void)n_q;
-  (void)n_kv;
-  (void)rows;
-  return attn_bytes(batch, (int64_t)compute_units() * 4 * kMaxWaves, hd == 256 ? 16 : 32, hd);
+  return attn_bytes(attn_items(n_q, n_kv, batch, rows, 16), (int64_t)compute_units() * 4 * 3, hd == 256 ? 16 : 32, hd);
 }
 
 hipError_t launch_kv4_attn(hipStream_t st, int dtype, const Kv4Attn& a) {
