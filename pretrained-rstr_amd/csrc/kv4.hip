@@ -274,11 +274,14 @@ hipError_t rows_type(hipStream_t st, bool append, const Kv4Layer& c, int dtype, 
 constexpr int kTile = 32;
 constexpr int kStart = 6;  // what beginning an item costs, in tiles
 
-template <class E> struct Terms { static constexpr int n = 1; };
-template <> struct Terms<F32> { static constexpr int n = 2; };
+// Terms of a weight; ONCE: p * d is rounded once, from fp32.  bf16 results round to 8
+// bits anyway, so there p is rounded to fp16 and multiplied by pairs.
+template <class E> struct Terms { static constexpr int n = 1; static constexpr bool ONCE = true; };
+template <> struct Terms<F32> { static constexpr int n = 2; static constexpr bool ONCE = true; };
+template <> struct Terms<BF16> { static constexpr int n = 1; static constexpr bool ONCE = false; };
 
 // Waves a SIMD: what the registers of a form allow.
-constexpr int attn_waves(int hd, int nt, int terms) { return hd == 256 ? 1 : nt == 1 && terms == 1 ? 3 : 2; }
+constexpr int attn_waves(int hd, int nt, int terms) { return hd == 256 ? 1 : nt == 1 ? 3 : 2; }
 
 // Tiles of a wave's ring: what 160 KB of LDS hold for that many waves.
 constexpr int attn_ring(int hd, int nt, int terms) { return attn_waves(hd, nt, terms) == 3 && hd == 128 ? 2 : 4; }
@@ -415,6 +418,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   typedef Rec<D> R;
   typedef typename E::T T;
   constexpr int NB = D / 32, COLS = 16 * NT, TERMS = Terms<E>::n;
+  constexpr bool ONCE = Terms<E>::ONCE;
   const Magic magic;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int w = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -518,7 +522,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 
     f4 acc[NT][2 * NB];
     float mref[NT], kcol[NT], fs[NT];
-    f4 l[NT];             // one term: all four the sum of p; two: the lane's own part in the first
+    f4 l[NT];             // ONCE: the lane's own part of the sum of p in the first; else the sum, in all four
     int elim[NT];         // exponents of the V scales seen so far are no larger; fs = 2^(15 - elim)
     bool scaled = false;  // some column's fs is below 1
     h8 q[NT][TERMS][NB];
@@ -793,34 +797,49 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 #pragma unroll
           for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(e2[t][i]);
           h2 ph[2][2];
-          if constexpr (TERMS == 1) {
+          uint32_t vs[2][2 * NB];  // scales of V, below 2 by fs, where there are such
+          if constexpr (ONCE) {
+            l[t][0] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            if (TERMS == 2 || scaled) {
+              if constexpr (TERMS == 1) asm volatile("");  // stays a branch
+#pragma unroll
+              for (int i = 0; i < 8; i++) p[i] *= fs[t];
+            }
+          } else {
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
               for (int i = 0; i < 2; i++) ph[j][i] = h2{(_Float16)p[4 * j + 2 * i], (_Float16)p[4 * j + 2 * i + 1]};
             l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pack8(ph[0][0], ph[0][1], ph[1][0], ph[1][1]), l[t], 0, 0, 0);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) l[t][0] += p[i];
-          }
-          // scales of V, below 2 by fs, where a column is wide enough of them
-          uint32_t vs[2][2 * NB];
-#pragma unroll
-          for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int i = 0; i < 2 * NB; i++) vs[j][i] = xv.s[j][i];
-          if (TERMS == 1 && scaled) {
-            asm volatile("");  // stays a branch
-            const h2 f = {(_Float16)fs[t], (_Float16)fs[t]};
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-              for (int i = 0; i < 2 * NB; i++) vs[j][i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, vs[j][i]) * f);
+              for (int i = 0; i < 2 * NB; i++) vs[j][i] = xv.s[j][i];
+            if (scaled) {
+              asm volatile("");  // stays a branch
+              const h2 f = {(_Float16)fs[t], (_Float16)fs[t]};
+#pragma unroll
+              for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 2 * NB; i++) vs[j][i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, vs[j][i]) * f);
+            }
           }
 #pragma unroll
           for (int bk = 0; bk < NB; bk++) {
             h8 pd[TERMS];
-            if constexpr (TERMS == 1) {
+            if constexpr (ONCE) {
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                float y = p[i] * half_of(xv.s[i >> 2][2 * bk + ((i >> 1) & 1)], i & 1);
+                if (NT > 1 && edge && !((see[t] >> i) & 1)) y = 0.0f;  // 0 * NaN of a token that is not seen
+                // two terms: one product, not one for each term, of which the compiler would round
+                // one to fp32 and then fp16 and the other to fp16 at once
+                if constexpr (TERMS == 2) asm("" : "+v"(y));
+                const _Float16 top = (_Float16)y;
+                pd[0][i] = top;
+                if constexpr (TERMS == 2) pd[1][i] = (_Float16)(y - (float)top);
+              }
+            } else {
               h2 y[2][2];
 #pragma unroll
               for (int j = 0; j < 2; j++)
@@ -834,15 +853,6 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
                   }
                 }
               pd[0] = pack8(y[0][0], y[0][1], y[1][0], y[1][1]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                float y = p[i] * fs[t] * half_of(vs[i >> 2][2 * bk + ((i >> 1) & 1)], i & 1);
-                if (NT > 1 && edge && !((see[t] >> i) & 1)) y = 0.0f;
-                const _Float16 top = (_Float16)y;
-                pd[0][i] = top;
-                pd[1][i] = (_Float16)(y - (float)top);
-              }
             }
 #pragma unroll
             for (int hh = 0; hh < 2; hh++) {
@@ -872,7 +882,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
     const int64_t slot = (begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w) * COLS;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const float sum = TERMS == 1 ? l[t][0] : xor_add<32>(xor_add<16>(l[t][0]));
+      const float sum = ONCE ? xor_add<32>(xor_add<16>(l[t][0])) : l[t][0];
       if (!valid[t]) continue;
       if (begins && ends) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;

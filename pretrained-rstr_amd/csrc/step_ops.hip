@@ -137,7 +137,8 @@ __global__ void __launch_bounds__(kMapsThreads) k_step_maps(StepMaps a) {
 // ---- draft verification -----------------------------------------------------------------
 // Target probabilities p = softmax(x / T) of every row, in 64 bits: a drawn number
 // is compared with sums over the vocabulary, and 1e-7 of such a sum covers as many
-// borders between tokens as the vocabulary has.
+// borders between tokens as the vocabulary has.  The exponentials are good to 1e-12, and
+// so are the sums: one draw in ten million meets a border that two forms see differently.
 //   1. k_verify_rows: per (row, chunk of the vocabulary) the maximum, its first
 //      index and the sum of exp((x - max) / T).
 //   2. k_verify_pick: per (sequence, chunk): every row's sums joined, the first
@@ -147,13 +148,33 @@ __global__ void __launch_bounds__(kMapsThreads) k_step_maps(StepMaps a) {
 //      the token inside it.
 constexpr int kChunk = 4096, kVT = 256, kPer = kChunk / kVT;
 
+// 2^t for t <= 0, to 3e-13 of itself: t = n + f with |f| <= 1/2, and the series of 2^f
+// (coefficients ln(2)^k / k!) to the tenth power, whose rest is below 2^-41.
+__device__ __forceinline__ double pow2(double t) {
+  t = fmax(t, -1100.0);  // 0, and -infinity - -infinity is none
+  const double n = __builtin_rint(t), f = t - n;
+  double p = 7.0549116208011233e-09;
+  p = __builtin_fma(p, f, 1.0178086009239699e-07);
+  p = __builtin_fma(p, f, 1.3215486790144309e-06);
+  p = __builtin_fma(p, f, 1.5252733804059840e-05);
+  p = __builtin_fma(p, f, 1.5403530393381610e-04);
+  p = __builtin_fma(p, f, 1.3333558146428443e-03);
+  p = __builtin_fma(p, f, 9.6181291076284772e-03);
+  p = __builtin_fma(p, f, 5.5504108664821580e-02);
+  p = __builtin_fma(p, f, 2.4022650695910072e-01);
+  p = __builtin_fma(p, f, 6.9314718055994531e-01);
+  p = __builtin_fma(p, f, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)n);
+}
+constexpr double kLog2e = 1.4426950408889634;
+
 struct RowStat {
   double sum;   // of exp((x - top) / T) over the chunk; 0 where T <= 0
   float top;    // NaN if the chunk holds one
   int32_t at;   // first index of top (of the first NaN)
 };
 struct SeqPick {
-  double top, z, scale;  // p(v) = exp((x_v - top) * scale) / z
+  double top, z, scale;  // p(v) = 2^((x_v - top) * scale) / z
   int32_t row;           // the row the token is drawn from
   int32_t draft;         // >= 0: that token's probability is left out (a draft without probabilities)
   int32_t greedy;        // >= 0: the token itself
@@ -190,6 +211,32 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
+// The elements that a thread takes of a chunk: 16 bytes at a time, neighbours for
+// neighbouring threads.  token_of(v0, i): the token of a thread's i-th element.
+template <class E>
+__device__ __forceinline__ int token_of(int v0, int i) {
+  constexpr int PER = 16 / sizeof(typename E::T);
+  return v0 + ((i / PER) * kVT + (int)threadIdx.x) * PER + i % PER;
+}
+template <class E>
+__device__ __forceinline__ void load_chunk(const typename E::T* x, int v0, int v1, float (&val)[kPer]) {
+  typedef typename E::T T;
+  constexpr int PER = 16 / sizeof(T);
+  if (v1 - v0 == kChunk && ((uintptr_t)(x + v0) % 16) == 0) {
+    T t[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer / PER; i++) ((u32x4*)t)[i] = *(const u32x4*)(x + v0 + (i * kVT + (int)threadIdx.x) * PER);
+#pragma unroll
+    for (int i = 0; i < kPer; i++) val[i] = E::get(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int v = token_of<E>(v0, i);
+      val[i] = v < v1 ? E::get(x[v]) : -INFINITY;
+    }
+  }
+}
+
 template <class E>
 __global__ void __launch_bounds__(kVT) k_verify_rows(Verify a, RowStat* __restrict__ stats) {
   const int row = blockIdx.x, chunk = blockIdx.y, tid = threadIdx.x, chunks = gridDim.y;
@@ -201,10 +248,10 @@ __global__ void __launch_bounds__(kVT) k_verify_rows(Verify a, RowStat* __restri
   float val[kPer];
   float top = -INFINITY;
   int at = 0x7FFFFFFF;
+  load_chunk<E>(x, v0, v1, val);
 #pragma unroll
   for (int i = 0; i < kPer; i++) {
-    const int v = v0 + i * kVT + tid;
-    val[i] = v < v1 ? E::get(x[v]) : -INFINITY;
+    const int v = token_of<E>(v0, i);
     if (v < v1 && beats(val[i], v, top, at)) { top = val[i]; at = v; }
   }
 #pragma unroll
@@ -224,9 +271,9 @@ __global__ void __launch_bounds__(kVT) k_verify_rows(Verify a, RowStat* __restri
     if (beats(st[w], si[w], top, at)) { top = st[w]; at = si[w]; }
   double sum = 0.0;
   if (draws(T) && top > -INFINITY && top < INFINITY) {
-    const double k = 1.0 / (double)T, t = (double)top;
+    const double k = kLog2e / (double)T, t = (double)top;
 #pragma unroll
-    for (int i = 0; i < kPer; i++) sum += exp(((double)val[i] - t) * k);
+    for (int i = 0; i < kPer; i++) sum += pow2(((double)val[i] - t) * k);
   }
   sum = wave_sum64(sum);
   if ((tid & 63) == 0) ss[wave] = sum;
@@ -249,16 +296,15 @@ __device__ __forceinline__ void join_row(const RowStat* s, int chunks, double k,
   }
   z = 0.0;
   for (int c = lane; c < chunks; c += 64)
-    if (s[c].sum > 0.0) z += s[c].sum * exp(((double)s[c].top - (double)top) * k);
+    if (s[c].sum > 0.0) z += s[c].sum * pow2(((double)s[c].top - (double)top) * k);
   z = wave_sum64(z);
 }
 
-// What token v of the picked row weighs, times z.
-template <class E>
-__device__ __forceinline__ double weight(const Verify& a, const SeqPick& s, int v) {
-  const double e = exp(((double)E::get(((const typename E::T*)a.logits)[(int64_t)s.row * a.logits_row + v]) - s.top) * s.scale);
+// What a token of logit x and draft probability q weighs in the picked row, times z.
+__device__ __forceinline__ double weight(const SeqPick& s, float x, float q, int v) {
+  const double e = pow2(((double)x - s.top) * s.scale);
   if (s.from_probs) {
-    const double w = e - (double)a.probs[(int64_t)s.row * a.probs_row + v] * s.z;
+    const double w = e - (double)q * s.z;
     return w > 0.0 ? w : 0.0;
   }
   return v == s.draft ? 0.0 : e;
@@ -274,7 +320,7 @@ __global__ void __launch_bounds__(kVT) k_verify_pick(Verify a, const RowStat* __
     return;
   }
   const float T = a.temperature[b];
-  const double k = draws(T) ? 1.0 / (double)T : 0.0;
+  const double k = draws(T) ? kLog2e / (double)T : 0.0;
   __shared__ SeqPick pick;
   __shared__ int refused[kVT / 64], kept;
   __shared__ double ss[kVT / 64];
@@ -299,7 +345,7 @@ __global__ void __launch_bounds__(kVT) k_verify_pick(Verify a, const RowStat* __
           ok = d == at;
         } else if (inside) {
           const double q = a.probs ? (double)a.probs[(int64_t)row * a.probs_row + d] : 1.0;
-          const double p = exp(((double)E::get(((const typename E::T*)a.logits)[(int64_t)row * a.logits_row + d]) - (double)top) * k) / z;
+          const double p = pow2(((double)E::get(((const typename E::T*)a.logits)[(int64_t)row * a.logits_row + d]) - (double)top) * k) / z;
           ok = (double)a.u_accept[row] * q < p;
         }
         stop = !ok;
@@ -332,7 +378,23 @@ __global__ void __launch_bounds__(kVT) k_verify_pick(Verify a, const RowStat* __
   if (pick.greedy >= 0) return;
   double sum = 0.0;
   const int v0 = chunk * kChunk, v1 = min(v0 + kChunk, a.vocab);
-  for (int v = v0 + tid; v < v1; v += kVT) sum += weight<E>(a, pick, v);
+  const SeqPick s = pick;
+  float val[kPer], q[kPer];
+  load_chunk<E>((const typename E::T*)a.logits + (int64_t)s.row * a.logits_row, v0, v1, val);
+  if (s.from_probs) {
+    const float* p = a.probs + (int64_t)s.row * a.probs_row;
+    if constexpr (sizeof(typename E::T) == 4) {
+      load_chunk<LF32>(p, v0, v1, q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; i++) q[i] = token_of<E>(v0, i) < v1 ? p[token_of<E>(v0, i)] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    const int v = token_of<E>(v0, i);
+    if (v < v1) sum += weight(s, val[i], s.from_probs ? q[i] : 0.0f, v);
+  }
   sum = wave_sum64(sum);
   if ((tid & 63) == 0) ss[wave] = sum;
   __syncthreads();
@@ -362,7 +424,7 @@ __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* _
     const RowStat* st = stats + (int64_t)s.row * chunks;
     const auto mass = [&](int i) {
       if (!plain) return c[i];
-      return st[i].sum > 0.0 ? st[i].sum * exp(((double)st[i].top - s.top) * s.scale) : 0.0;
+      return st[i].sum > 0.0 ? st[i].sum * pow2(((double)st[i].top - s.top) * s.scale) : 0.0;
     };
     if (plain) total = s.z;
     const double t = (double)a.u_sample[b] * total;
@@ -404,7 +466,10 @@ __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* _
   double w[kPer], sum = 0.0;
 #pragma unroll
   for (int i = 0; i < kPer; i++) {
-    w[i] = v0 + i < v1 ? weight<E>(a, s, v0 + i) : 0.0;
+    w[i] = 0.0;
+    if (v0 + i < v1)
+      w[i] = weight(s, E::get(((const typename E::T*)a.logits)[(int64_t)s.row * a.logits_row + v0 + i]),
+                    s.from_probs ? a.probs[(int64_t)s.row * a.probs_row + v0 + i] : 0.0f, v0 + i);
     sum += w[i];
   }
   double in = sum;

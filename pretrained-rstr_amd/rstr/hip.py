@@ -223,30 +223,33 @@ class DeviceView:
         return dict(shape=self.shape, typestr="<f4" if self.dtype == "float32" else "<f2", data=(self._ptr, False), version=2)
 
 
-def _on_device(sess, x, what):
+def _device_of(x):
+    """The GPU that an array lives on (its ordinal; None: not on one)."""
     d = x.device
-    if d != sess.device and not (getattr(d, "type", None) == "cuda" and d.index == sess.device):
-        raise ValueError(f"{what} must be on the session's GPU ({sess.device}), got {d}")
+    return d if isinstance(d, int) else d.index if getattr(d, "type", None) == "cuda" else None
 
 
-def _ints(sess, x, what, shape):
-    """The address of a contiguous int32 device array of the given shape (None: any extent)."""
+def _on_device(sess, x, what):
+    if _device_of(x) != sess.device:
+        raise ValueError(f"{what} must be on the session's GPU ({sess.device}), got {x.device}")
+
+
+# These run before every call, a dozen of them a call: one expression decides the usual case, and
+# only what fails it is looked at closely.
+
+
+def _flat(sess, x, what, shape, code, name):
+    """The address of a contiguous device array of that element type and shape."""
+    try:
+        if _codes[x.dtype] == code and x.get_device() == sess.device and x.shape == shape and x.is_contiguous():
+            return x.data_ptr()
+    except (AttributeError, KeyError):
+        pass
     _on_device(sess, x, what)
-    if _code(x.dtype) != "int32":
-        raise ValueError(f"{what} must be int32, got {x.dtype}")
-    return _plain(x, what, shape)
-
-
-def _floats(sess, x, what, shape):
-    _on_device(sess, x, what)
-    if _code(x.dtype) != 0:
-        raise ValueError(f"{what} must be float32, got {x.dtype}")
-    return _plain(x, what, shape)
-
-
-def _plain(x, what, shape):
-    if len(x.shape) != len(shape) or any(w is not None and n != w for n, w in zip(x.shape, shape)):
-        raise ValueError(f"{what} must have the shape {tuple('any' if w is None else w for w in shape)}, got {tuple(x.shape)}")
+    if _code(x.dtype) != code:
+        raise ValueError(f"{what} must be {name}, got {x.dtype}")
+    if tuple(x.shape) != shape:
+        raise ValueError(f"{what} must have the shape {shape}, got {tuple(x.shape)}")
     want = 1
     for n, st in zip(reversed(x.shape), reversed(x.stride())):
         if n > 1 and st != want:
@@ -255,30 +258,49 @@ def _plain(x, what, shape):
     return x.data_ptr()
 
 
+def _ints(sess, x, what, shape):
+    return _flat(sess, x, what, shape, "int32", "int32")
+
+
+def _floats(sess, x, what, shape):
+    return _flat(sess, x, what, shape, 0, "float32")
+
+
 def _rows(sess, x, what, heads, hd, rows=None):
     """(address, element type, row stride, head stride) of a [rows][heads][hd] device array."""
-    _on_device(sess, x, what)
-    code = _code(x.dtype)
-    if not isinstance(code, int):
+    on = getattr(x, "get_device", None)
+    if on is None or on() != sess.device:
+        _on_device(sess, x, what)
+    code = _codes.get(x.dtype)
+    if code is None:
+        code = _code(x.dtype)
+    if code.__class__ is not int:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
-    if len(x.shape) != 3 or x.shape[1] != heads or x.shape[2] != hd or (rows is not None and x.shape[0] != rows):
-        raise ValueError(f"{what} must have the shape ({'rows' if rows is None else rows}, {heads}, {hd}), got {tuple(x.shape)}")
-    st = x.stride()
-    if st[2] != 1:
+    shape = x.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != hd or (rows is not None and shape[0] != rows):
+        raise ValueError(f"{what} must have the shape ({'rows' if rows is None else rows}, {heads}, {hd}), got {tuple(shape)}")
+    row, head, one = x.stride()
+    if one != 1:
         raise ValueError(f"the last dimension of {what} must be contiguous")
-    return x.data_ptr(), code, st[0], st[1]
+    return x.data_ptr(), code, row, head
+
+
+_raw_stream = None   # torch's current stream of a device, once torch uses the GPU
 
 
 def _stream(sess, stream):
     """The raw stream of a call: what it was given (a hipStream_t address, a torch
     stream, or SESSION_STREAM), else torch's current one where torch is in use,
     else the session's own."""
-    if stream is None:
+    global _raw_stream
+    if stream is not None:
+        return getattr(stream, "cuda_stream", stream)
+    if _raw_stream is None:
         torch = sys.modules.get("torch")
         if torch is None or not torch.cuda.is_initialized():
             return SESSION_STREAM
-        return torch.cuda.current_stream(sess.device).cuda_stream
-    return getattr(stream, "cuda_stream", stream)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(sess.device)
 
 
 class Session:
@@ -849,7 +871,9 @@ class Verifier:
 
 def _matrix(sess, x, what, rows, cols):
     """(address, element type, row stride) of a [rows][cols] device array."""
-    _on_device(sess, x, what)
+    on = getattr(x, "get_device", None)
+    if on is None or on() != sess.device:
+        _on_device(sess, x, what)
     code = _code(x.dtype)
     if not isinstance(code, int):
         raise ValueError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")

@@ -271,6 +271,27 @@ def test_attention_ranges(sess, dtype, v_scale, k_scale, mul):
     c.close()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_fp32_is_fp32(sess, D, rows):
+    """fp32 queries: the whole output within 2^-19 of its norm.  A weight is off by its exponent's
+    rounding, at most half a step of a number below 16 (2^-21) in each of the sum, the scale and the
+    difference, times ln 2: 2^-19.9 together if all agree; its two fp16 terms keep 2^-22."""
+    print("fp32", D, rows, flush=True)
+    for seed in range(6):
+        c = Case(sess, 4, 2, D, 16, [1500 + 83 * seed], [rows], seed=seed)
+        q = c.queries("f32")
+        out = torch.zeros_like(q).cuda()
+        plan = c.plan()
+        plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out)
+        want, _, _ = P.attention(P.as_f64(q), c.k, c.v, c.lens, c.offsets, 0, D ** -0.5)
+        for h in range(4):
+            off = np.linalg.norm((P.as_f64(out) - want)[:, h]) / np.linalg.norm(want[:, h])
+            assert off < 2.0 ** -19, (seed, h, off)
+        plan.close()
+        c.close()
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("rows", [2, 40])
 def test_what_is_not_seen_does_not_matter(sess, dtype, rows):
