@@ -163,7 +163,7 @@ static int kv4_rows_args(rstr_kv4* p, int32_t layer, int32_t rows, int32_t dtype
   TRY(check_rows(s, "key", k, size));
   TRY(check_rows(s, "value", v, size));
   TRY(check_ints(s, "slots", slots));
-  if ((int64_t)rows * p->n_kv * (p->hd / 8) > (int64_t)256 * 0x7FFFFFFF) return fail(s, RSTR_E_INVALID, "too many rows for one call");
+  if (((int64_t)rows / 4 + 8) * p->n_kv * (p->hd / 8) > 0x7FFFFFFF) return fail(s, RSTR_E_INVALID, "too many rows for one call");
   return RSTR_OK;
 }
 

@@ -84,131 +84,374 @@ struct Rec {
 
 __device__ __forceinline__ float h2f(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
 
-// ---- append -------------------------------------------------------------------------
-// One thread quantises 8 elements; the four threads of a block agree on its
-// scale.  Eight threads (64 elements, two blocks) hold the nibbles of eight V
-// columns between them and exchange them, so that each writes two halfwords.
+// ---- append and read ------------------------------------------------------------------
+// A thread takes 8 elements of four rows: four that may lie in one group of four tokens,
+// whose V codes are then written (read) as 8 bytes a column instead of 2, and a
+// workgroup four quads of four heads, the 16 tokens that lines of K are made of (lines
+// written in parts by several chips' caches cost far more than their bytes).  So that they
+// do where a prompt's rows fill consecutive slots, the quads begin where the first slot's
+// 16 do.  K: 8 neighbours of a block (blockIdx.y 0); V: columns 2i, 2i + 1 of a block pair,
+// that is 2 neighbours at four places, so that a thread holds whole halfwords.
 //
-// x / d is decided exactly: r = x - c * d is exact in fp32 near a half step
-// (both are multiples of the smaller operand's last place, and |r| < d), so the
-// estimate's nearest integer is corrected where |r| passes d / 2 and a tie goes
-// to the even code.
-template <int D, class E, bool VEC>
-__global__ void __launch_bounds__(256) k_kv4_append(Kv4Layer L, int rows, Rows kr, Rows vr, const int32_t* __restrict__ slots) {
-  typedef Rec<D> R;
-  constexpr int TPR = D / 8;  // threads a row
-  const bool is_v = blockIdx.y != 0;
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int t = (int)(gid % TPR);
-  const int64_t rh = gid / TPR;
-  const int h = (int)(rh % L.n_kv);
-  const int64_t row = rh / L.n_kv;
-  const bool live = row < rows;  // lanes behind the last row still take part in the exchanges
-  const int slot = live ? slots[row] : -1;
-  const Rows src = is_v ? vr : kr;
-  float x[8] = {};
-  if (live) load8<E, VEC>((const typename E::T*)src.p + row * src.row + h * src.head + t * 8, x);
-  // the block's element of greatest magnitude, the first of equals
-  float m = 0.0f;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    if (fabsf(x[i]) > fabsf(m)) m = x[i];
-    bad |= !(fabsf(x[i]) < INFINITY);
+// Few rows take one row a thread: 128 rows of 8 heads are then 4.2 us instead of 8.8.
+//
+// Codes: x / d is the product with d's reciprocal, corrected once by its residual, and adding
+// 1.5 * 2^23 rounds it to the nearest integer, ties to even, and leaves that in the low bits.
+// The corrected quotient is x / d rounded to fp32, so it is a half only where x / d is, or
+// is nearer to one than fp32 tells.  Quotients of two numbers of 11 bits are not, so for fp16 and
+// bf16 rows that is exact; for fp32 rows, where some lane's quotient is a half,
+// the codes are decided by r = x - c * d, which is exact there.
+//
+// The first element of greatest magnitude.  16-bit elements have room below their bits
+// for the place and the sign: one integer maximum.  fp32: the larger of maximum and
+// -minimum; only where these are equal does the order of the elements matter.
+struct Extreme {
+  float m;
+  int at;
+  __device__ __forceinline__ void meet(float om, int oat) {
+    const bool other = fabsf(om) > fabsf(m) || (fabsf(om) == fabsf(m) && oat < at);
+    m = other ? om : m;
+    at = other ? oat : at;
   }
-  float o = xor_lane<1>(m);
-  m = (fabsf(o) > fabsf(m) || (fabsf(o) == fabsf(m) && (t & 1))) ? o : m;
-  o = xor_lane<2>(m);
-  m = (fabsf(o) > fabsf(m) || (fabsf(o) == fabsf(m) && (t & 2))) ? o : m;
-  const uint64_t any_bad = __ballot(bad);
-  bad = (any_bad >> ((threadIdx.x & 63) & ~3)) & 0xF;
-  uint16_t db = f2h_bits(__builtin_amdgcn_fmed3f(m * -0.125f, -65504.0f, 65504.0f));
-  if ((db & 0x7FFFu) == 0) db = 0;
-  if (bad) db = 0x7E00u;
-  const float d = h2f(db);
-  const float id = d != 0.0f ? 1.0f / d : 0.0f, hd = fabsf(d) * 0.5f;
-  int c[8];
+};
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float min_nan(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v, uint32_t o) { return o > v ? o : v; }
+// Of a block spread over aligned groups of G lanes, N elements a lane, element i at
+// place(i) of the block: the first element of greatest magnitude; `bad` if one is
+// a NaN or infinite.
+template <class E, int N, int G, class P>
+__device__ __forceinline__ float extreme(const float* x, P place, bool& bad) {
+  if constexpr (sizeof(typename E::T) == 2) {
+    uint32_t k = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    float q = __builtin_rintf(__builtin_amdgcn_fmed3f(x[i] * id, -9.0f, 8.0f));
-    const float r = __builtin_fmaf(-q, d, x[i]);
-    const float up = (r < 0.0f) == (d < 0.0f) ? 1.0f : -1.0f;
-    const bool odd = ((int)q & 1) != 0;
-    if (fabsf(r) > hd || (fabsf(r) == hd && odd)) q += up;
-    c[i] = d != 0.0f && !bad ? (int)__builtin_amdgcn_fmed3f(q, -8.0f, 7.0f) + 8 : 8;
-  }
-  const int64_t limit = (int64_t)L.pages * L.page_size;
-  const bool put = slot >= 0 && slot < limit;
-  const int page = put ? slot / L.page_size : 0, tok = put ? slot % L.page_size : 0;
-  uint8_t* rec = L.base + ((int64_t)page * L.n_kv + h) * kv4_record_bytes(D, L.page_size);
-  const int b = t >> 2;
-  if (!is_v) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) w |= (uint32_t)c[2 * i] << (4 * i) | (uint32_t)c[2 * i + 1] << (16 + 4 * i);
-    if (put) *(uint32_t*)(rec + R::k(tok, b, t & 3)) = w;
-  } else {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) w |= (uint32_t)c[i] << (4 * i);
-    const int par = t & 1, n = (t >> 1) & 3;  // columns 8 * par + i; nibble n of a halfword
-    uint32_t h0 = 0, h1 = 0;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const uint32_t o4 = (uint32_t)__shfl((int)w, ((threadIdx.x & 63) & ~7) + 2 * k + par, 64) >> (8 * n);
-      h0 |= (o4 & 0xFu) << (4 * k);
-      h1 |= ((o4 >> 4) & 0xFu) << (4 * k);
+    for (int i = 0; i < N; i++) {
+      const uint32_t u = __float_as_uint(x[i]);
+      k = dpp_max(k, __builtin_rotateleft32(u, 1) | (uint32_t)(31 - place(i)) << 1);
     }
-    if (put) {
-      uint8_t* at = rec + R::vbase(L.page_size) + (tok & 3) * 2;
-      *(uint16_t*)(at + R::v(tok >> 2, t >> 3, 8 * par + 2 * n)) = (uint16_t)h0;
-      *(uint16_t*)(at + R::v(tok >> 2, t >> 3, 8 * par + 2 * n + 1)) = (uint16_t)h1;
-    }
+    k = dpp_max(k, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, 0xB1, 0xF, 0xF, true));
+    k = dpp_max(k, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, 0x4E, 0xF, 0xF, true));
+    if constexpr (G == 8) k = dpp_max(k, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, 0x141, 0xF, 0xF, true));
+    bad = k >= 0xFF000000u;
+    return __uint_as_float(__builtin_rotateright32(k & ~0x3Eu, 1));
   }
-  if (put && (t & 3) == 0)
-    *(uint16_t*)(rec + (is_v ? R::vsbase(L.page_size) : R::ksbase(L.page_size)) + R::s(tok >> 2, b) + (tok & 3) * 2) = db;
+  float hi = x[0], lo = x[0];
+#pragma unroll
+  for (int i = 1; i < N; i++) {
+    hi = max_nan(hi, x[i]);
+    lo = min_nan(lo, x[i]);
+  }
+  hi = max_nan(hi, xor_lane<1>(hi));
+  lo = min_nan(lo, xor_lane<1>(lo));
+  hi = max_nan(hi, xor_lane<2>(hi));
+  lo = min_nan(lo, xor_lane<2>(lo));
+  if constexpr (G == 8) {
+    hi = max_nan(hi, half_mirror_lane(hi));
+    lo = min_nan(lo, half_mirror_lane(lo));
+  }
+  bad = !(hi < INFINITY && lo > -INFINITY);
+  float m = hi > -lo ? hi : lo;
+  if (__ballot(hi == -lo && hi > 0.0f)) {
+    Extreme e{x[0], place(0)};
+#pragma unroll
+    for (int i = 1; i < N; i++) e.meet(x[i], place(i));
+    e.meet(xor_lane<1>(e.m), __builtin_amdgcn_update_dpp(0, e.at, 0xB1, 0xF, 0xF, true));
+    e.meet(xor_lane<2>(e.m), __builtin_amdgcn_update_dpp(0, e.at, 0x4E, 0xF, 0xF, true));
+    if constexpr (G == 8) e.meet(half_mirror_lane(e.m), __builtin_amdgcn_update_dpp(0, e.at, 0x141, 0xF, 0xF, true));
+    if (hi == -lo) m = e.m;
+  }
+  return m;
 }
 
-// ---- read ---------------------------------------------------------------------------
-// One thread gives 8 elements back; d * (c - 8) is exact in fp32 (11 + 4 bits)
-// and rounded once to the output's type.
-template <int D, class E, bool VEC>
-__global__ void __launch_bounds__(256) k_kv4_read(Kv4Layer L, int rows, Rows kr, Rows vr, const int32_t* __restrict__ slots) {
-  typedef Rec<D> R;
-  constexpr int TPR = D / 8;
-  const bool is_v = blockIdx.y != 0;
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int t = (int)(gid % TPR);
-  const int64_t rh = gid / TPR;
-  const int h = (int)(rh % L.n_kv);
-  const int64_t row = rh / L.n_kv;
-  if (row >= rows) return;
-  const int slot = slots[row];
-  float x[8] = {};
-  if (slot >= 0 && slot < (int64_t)L.pages * L.page_size) {
-    const int page = slot / L.page_size, tok = slot % L.page_size, b = t >> 2;
-    const uint8_t* rec = L.base + ((int64_t)page * L.n_kv + h) * kv4_record_bytes(D, L.page_size);
-    const int sb = is_v ? R::vsbase(L.page_size) : R::ksbase(L.page_size);
-    const float d = h2f(*(const uint16_t*)(rec + sb + R::s(tok >> 2, b) + (tok & 3) * 2));
-    if (!is_v) {
-      const uint32_t w = *(const uint32_t*)(rec + R::k(tok, b, t & 3));
+struct Scale {
+  uint16_t bits;
+  float d, id;
+  __device__ __forceinline__ Scale(float m, bool bad) {
+    bits = f2h_bits(__builtin_amdgcn_fmed3f(m * -0.125f, -65504.0f, 65504.0f));
+    if ((bits & 0x7FFFu) == 0) bits = 0;
+    d = h2f(bits);
+    if (bad) bits = 0x7E00u;
+    id = bad || d == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(d);
+  }
+  __device__ __forceinline__ float quotient(float x) const {
+    const float t = x * id;
+    return __builtin_fmaf(__builtin_fmaf(-t, d, x), id, t);
+  }
+  static __device__ __forceinline__ uint32_t nearest(float t) {
+    return __float_as_uint(__builtin_amdgcn_fmed3f(t + (0x1.8p23f + 8.0f), 0x1.8p23f, 0x1.8p23f + 15.0f)) & 0xFu;
+  }
+  __device__ __forceinline__ uint32_t exact(float x) const {
+    float q = __builtin_rintf(__builtin_amdgcn_fmed3f(x * id, -9.0f, 8.0f));
+    const float r = __builtin_fmaf(-q, d, x), up = (r < 0.0f) == (d < 0.0f) ? 1.0f : -1.0f, half = fabsf(d) * 0.5f;
+    const bool odd = ((int)q & 1) != 0;
+    if (fabsf(r) > half || (fabsf(r) == half && odd)) q += up;
+    return (uint32_t)((int)__builtin_amdgcn_fmed3f(q, -8.0f, 7.0f) + 8);
+  }
+  // N elements' codes, put(i, code) for each; 8, that is 0, where there is no scale.
+  template <class E, int N, class F>
+  __device__ __forceinline__ void codes(const float* x, bool bad, F put) const {
+    float y[N];
+    uint32_t c[N];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        x[2 * i] = d * (float)((int)((w >> (4 * i)) & 0xF) - 8);
-        x[2 * i + 1] = d * (float)((int)((w >> (16 + 4 * i)) & 0xF) - 8);
+    for (int i = 0; i < N; i++) y[i] = x[i];
+    if (__ballot(bad)) {
+#pragma unroll
+      for (int i = 0; i < N; i++) y[i] = bad ? 0.0f : y[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = quotient(y[i]);
+#pragma unroll
+    for (int i = 0; i < N; i++) c[i] = nearest(y[i]);
+    if constexpr (sizeof(typename E::T) == 4) {
+      bool half = false;
+#pragma unroll
+      for (int i = 0; i < N; i++) half |= __builtin_amdgcn_fractf(y[i]) == 0.5f;
+      if (__ballot(half)) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+          if (!bad && id != 0.0f) c[i] = exact(x[i]);
       }
-    } else {
-      const uint8_t* at = rec + R::vbase(L.page_size) + (tok & 3) * 2;
-      const int par = t & 1, n = (t >> 1) & 3;
+    }
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const uint32_t w = *(const uint16_t*)(at + R::v(tok >> 2, t >> 3, 8 * par + i));
-        x[i] = d * (float)((int)((w >> (4 * n)) & 0xF) - 8);
+    for (int i = 0; i < N; i++) put(i, c[i]);
+  }
+};
+
+// N rows from `row` on, their slots (-1: none) and whether these are one group of tokens.
+template <int N>
+struct Quad {
+  int row, slot[N];
+  bool group;
+  __device__ __forceinline__ Quad(const int32_t* slots, int rows, int quad, int64_t limit) {
+    row = quad * N;
+    if constexpr (N == 4) {
+      const int first = slots[0];
+      row -= first > 0 ? first & 15 : 0;
+    }
+    group = N == 4;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int r = row + i;
+      const int s = r >= 0 && r < rows ? slots[r] : -1;
+      slot[i] = s >= 0 && s < limit ? s : -1;
+      group = group && slot[i] >= 0 && slot[i] == slot[0] + i;
+    }
+    group = group && (slot[0] & 3) == 0;
+  }
+  // the row that is loaded in row i's place: one that is there
+  __device__ __forceinline__ int64_t read(int i, int rows) const { return min(max(row + i, 0), rows - 1); }
+  __device__ __forceinline__ bool live(int i, int rows) const { return row + i >= 0 && row + i < rows; }
+};
+
+// The record and token of a slot.
+struct Place {
+  uint8_t* rec;
+  int tok;
+  __device__ __forceinline__ Place(const Kv4Layer& L, int hd, int h, int slot) {
+    const uint32_t page = (uint32_t)slot / (uint32_t)L.page_size;
+    tok = slot - (int)(page * (uint32_t)L.page_size);
+    rec = L.base + ((int64_t)page * L.n_kv + h) * kv4_record_bytes(hd, L.page_size);
+  }
+};
+
+// Two neighbours, aligned to both where VEC.
+template <class E, bool VEC>
+__device__ __forceinline__ void load2(const typename E::T* p, float* x) {
+  struct __attribute__((aligned(2 * sizeof(typename E::T)))) Pair { typename E::T a, b; };
+  if constexpr (VEC) {
+    const Pair t = *(const Pair*)p;
+    x[0] = E::get(t.a);
+    x[1] = E::get(t.b);
+  } else {
+    x[0] = E::get(p[0]);
+    x[1] = E::get(p[1]);
+  }
+}
+template <class E, bool VEC>
+__device__ __forceinline__ void store2(typename E::T* p, const float* x) {
+  struct __attribute__((aligned(2 * sizeof(typename E::T)))) Pair { typename E::T a, b; };
+  if constexpr (VEC) {
+    *(Pair*)p = Pair{E::put(x[0]), E::put(x[1])};
+  } else {
+    p[0] = E::put(x[0]);
+    p[1] = E::put(x[1]);
+  }
+}
+
+template <int D, class E, bool VEC, int N>
+__global__ void __launch_bounds__(256) k_kv4_append(Kv4Layer L, int rows, int quads, Rows kr, Rows vr, const int32_t* __restrict__ slots) {
+  typedef Rec<D> R;
+  typedef typename E::T T;
+  constexpr int TPR = D / 8;  // threads a quad and head
+  const bool is_v = blockIdx.y != 0;
+  const uint32_t gid = blockIdx.x * 256u + threadIdx.x, qh = gid / TPR;
+  constexpr uint32_t SIDE = N == 4 ? 4 : 1;  // quads before the next head's
+  const uint32_t hq = qh / SIDE, side = hq / (uint32_t)L.n_kv;
+  const int t = (int)(gid % TPR), quad = (int)(side * SIDE + qh % SIDE), h = (int)(hq - side * (uint32_t)L.n_kv);
+  const int ps = L.page_size;
+  // lanes behind the last quad take part in the exchanges
+  const Quad<N> Q(slots, quad < quads ? rows : 0, quad, (int64_t)L.pages * ps);
+  if (!is_v) {
+    float x[N][8];
+#pragma unroll
+    for (int i = 0; i < N; i++) load8<E, VEC>((const T*)kr.p + Q.read(i, rows) * kr.row + (int64_t)h * kr.head + t * 8, x[i]);
+    const int b = t >> 2, g = t & 3;
+    uint16_t sc[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      bool bad;
+      const float m = extreme<E, 8, 4>(x[i], [&](int j) { return g * 8 + j; }, bad);
+      const Scale s(m, bad);
+      sc[i] = s.bits;
+      uint32_t w = 0;
+      s.template codes<E, 8>(x[i], bad, [&](int j, uint32_t c) { w |= c << (4 * (j >> 1) + 16 * (j & 1)); });
+      if (Q.slot[i] >= 0) {
+        const Place p(L, D, h, Q.slot[i]);
+        *(uint32_t*)(p.rec + R::k(p.tok, b, g)) = w;
+        if (!Q.group && g == 0) *(uint16_t*)(p.rec + R::ksbase(ps) + R::s(p.tok >> 2, b) + (p.tok & 3) * 2) = s.bits;
+      }
+    }
+    if constexpr (N == 4)
+    if (Q.group && g == 0) {
+      const Place p(L, D, h, Q.slot[0]);
+      *(u32x2*)(p.rec + R::ksbase(ps) + R::s(p.tok >> 2, b)) = u32x2{sc[0] | (uint32_t)sc[1] << 16, sc[2] | (uint32_t)sc[3] << 16};
+    }
+    return;
+  }
+  const int bp = t >> 3, c = (t & 7) * 2;
+  float x[N][2][4];  // row, block of the pair, (half, column)
+#pragma unroll
+  for (int i = 0; i < N; i++)
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      load2<E, VEC>((const T*)vr.p + Q.read(i, rows) * vr.row + (int64_t)h * vr.head + bp * 64 + k * 16 + c, &x[i][k >> 1][2 * (k & 1)]);
+    }
+  uint16_t sc[2][N], cols[2][N];  // block or column, row
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const float* y = x[i][k];
+      bool bad;
+      const float m = extreme<E, 4, 8>(y, [&](int j) { return c + (j & 1) + 16 * (j >> 1); }, bad);
+      const Scale s(m, bad);
+      sc[k][i] = s.bits;
+      s.template codes<E, 4>(y, bad, [&](int j, uint32_t c) { w[j & 1] |= c << (8 * k + 4 * (j >> 1)); });
+    }
+    cols[0][i] = (uint16_t)w[0];
+    cols[1][i] = (uint16_t)w[1];
+    if (!Q.group && Q.slot[i] >= 0) {
+      const Place p(L, D, h, Q.slot[i]);
+      uint8_t* at = p.rec + (p.tok & 3) * 2;
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        *(uint16_t*)(at + R::vbase(ps) + R::v(p.tok >> 2, bp, c + k)) = cols[k][i];
+        if ((t & 7) == 0) *(uint16_t*)(at + R::vsbase(ps) + R::s(p.tok >> 2, 2 * bp + k)) = sc[k][i];
       }
     }
   }
-  const Rows dst = is_v ? vr : kr;
-  store8<E, VEC>((typename E::T*)dst.p + row * dst.row + h * dst.head + t * 8, x);
+  if constexpr (N == 4)
+  if (Q.group) {
+    const Place p(L, D, h, Q.slot[0]);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      *(u32x2*)(p.rec + R::vbase(ps) + R::v(p.tok >> 2, bp, c + k)) =
+          u32x2{cols[k][0] | (uint32_t)cols[k][1] << 16, cols[k][2] | (uint32_t)cols[k][3] << 16};
+      if ((t & 7) == 0)
+        *(u32x2*)(p.rec + R::vsbase(ps) + R::s(p.tok >> 2, 2 * bp + k)) =
+            u32x2{sc[k][0] | (uint32_t)sc[k][1] << 16, sc[k][2] | (uint32_t)sc[k][3] << 16};
+    }
+  }
+}
+
+// d * (c - 8) is exact in fp32 (11 + 4 bits) and rounded once to the output's type.
+template <int D, class E, bool VEC, int N>
+__global__ void __launch_bounds__(256) k_kv4_read(Kv4Layer L, int rows, int quads, Rows kr, Rows vr, const int32_t* __restrict__ slots) {
+  typedef Rec<D> R;
+  typedef typename E::T T;
+  constexpr int TPR = D / 8;
+  const bool is_v = blockIdx.y != 0;
+  const uint32_t gid = blockIdx.x * 256u + threadIdx.x, qh = gid / TPR;
+  constexpr uint32_t SIDE = N == 4 ? 4 : 1;  // quads before the next head's
+  const uint32_t hq = qh / SIDE, side = hq / (uint32_t)L.n_kv;
+  const int t = (int)(gid % TPR), quad = (int)(side * SIDE + qh % SIDE), h = (int)(hq - side * (uint32_t)L.n_kv);
+  const int ps = L.page_size;
+  if (quad >= quads) return;
+  const Quad<N> Q(slots, rows, quad, (int64_t)L.pages * ps);
+  if (!is_v) {
+    const int b = t >> 2, g = t & 3;
+    uint32_t w[N];
+    uint16_t sc[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      w[i] = 0x88888888u;
+      sc[i] = 0;
+      if (Q.slot[i] >= 0) {
+        const Place p(L, D, h, Q.slot[i]);
+        w[i] = *(const uint32_t*)(p.rec + R::k(p.tok, b, g));
+        sc[i] = *(const uint16_t*)(p.rec + R::ksbase(ps) + R::s(p.tok >> 2, b) + (p.tok & 3) * 2);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (!Q.live(i, rows)) continue;
+      const float d = h2f(sc[i]);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        x[2 * j] = d * (float)((int)((w[i] >> (4 * j)) & 0xF) - 8);
+        x[2 * j + 1] = d * (float)((int)((w[i] >> (16 + 4 * j)) & 0xF) - 8);
+      }
+      store8<E, VEC>((T*)kr.p + (int64_t)(Q.row + i) * kr.row + (int64_t)h * kr.head + t * 8, x);
+    }
+    return;
+  }
+  const int bp = t >> 3, c = (t & 7) * 2;
+  uint16_t cols[2][N], sc[2][N];
+  bool loaded = false;
+  if constexpr (N == 4)
+  if (Q.group) {
+    loaded = true;
+    const Place p(L, D, h, Q.slot[0]);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const u32x2 a = *(const u32x2*)(p.rec + R::vbase(ps) + R::v(p.tok >> 2, bp, c + k));
+      const u32x2 s = *(const u32x2*)(p.rec + R::vsbase(ps) + R::s(p.tok >> 2, 2 * bp + k));
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        cols[k][i] = (uint16_t)(a[i >> 1] >> (16 * (i & 1)));
+        sc[k][i] = (uint16_t)(s[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  }
+  if (!loaded) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        cols[k][i] = 0x8888;
+        sc[k][i] = 0;
+        if (Q.slot[i] >= 0) {
+          const Place p(L, D, h, Q.slot[i]);
+          const uint8_t* at = p.rec + (p.tok & 3) * 2;
+          cols[k][i] = *(const uint16_t*)(at + R::vbase(ps) + R::v(p.tok >> 2, bp, c + k));
+          sc[k][i] = *(const uint16_t*)(at + R::vsbase(ps) + R::s(p.tok >> 2, 2 * bp + k));
+        }
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    if (!Q.live(i, rows)) continue;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {  // block k >> 1 of the pair, half k & 1
+      const float d = h2f(sc[k >> 1][i]);
+      float x[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) x[j] = d * (float)((int)((cols[j][i] >> (4 * k)) & 0xF) - 8);
+      store2<E, VEC>((T*)vr.p + (int64_t)(Q.row + i) * vr.row + (int64_t)h * vr.head + bp * 64 + k * 16 + c, x);
+    }
+  }
 }
 
 __host__ __device__ inline bool vec_rows(const Rows& r, int size) {
@@ -218,12 +461,19 @@ __host__ __device__ inline bool vec_rows(const Rows& r, int size) {
 template <int D, class E>
 hipError_t rows_launch(hipStream_t st, bool append, const Kv4Layer& c, int rows, const Rows& k, const Rows& v,
                        const int32_t* slots) {
-  const int64_t threads = (int64_t)rows * c.n_kv * (D / 8);
+  // a row a thread while that does not fill the chip twice over; else four, the first quad
+  // beginning up to 15 rows before the first row
+  const bool few = (int64_t)rows * c.n_kv * (D / 8) * 2 < (int64_t)1 << 19;
+  const int quads = few ? rows : (int)(((int64_t)rows + 15 + 15) / 16) * 4;
+  const int64_t threads = (int64_t)quads * c.n_kv * (D / 8);
   const dim3 grid((unsigned)((threads + 255) / 256), 2);
   const bool vec = vec_rows(k, sizeof(typename E::T)) && vec_rows(v, sizeof(typename E::T));
-  auto f = append ? (vec ? k_kv4_append<D, E, true> : k_kv4_append<D, E, false>)
-                  : (vec ? k_kv4_read<D, E, true> : k_kv4_read<D, E, false>);
-  hipLaunchKernelGGL(f, grid, dim3(256), 0, st, c, rows, k, v, slots);
+#define RSTR_ROWS(N)                                                                            \
+  (append ? (vec ? k_kv4_append<D, E, true, N> : k_kv4_append<D, E, false, N>)                  \
+          : (vec ? k_kv4_read<D, E, true, N> : k_kv4_read<D, E, false, N>))
+  auto f = few ? RSTR_ROWS(1) : RSTR_ROWS(4);
+#undef RSTR_ROWS
+  hipLaunchKernelGGL(f, grid, dim3(256), 0, st, c, rows, quads, k, v, slots);
   return hipGetLastError();
 }
 template <class E>
