@@ -675,10 +675,18 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   const int group = a.n_q / a.c.n_kv, ps = a.c.page_size;
   const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), whole};
 
-  int64_t mine = 0;
-  int items = 0;
-  for (int b = lane; b < a.batch; b += 64) {
-    const Seq s = sequence(L, b);
+  // the sequences, 64 at a time, one a lane
+  const auto chunk_of = [&](int b0) {
+    Seq s = sequence(L, min(b0 + lane, a.batch - 1));
+    if (b0 + lane >= a.batch) s.nct = 0, s.units = 0;
+    return s;
+  };
+  int b0 = 0;
+  Seq seqs = chunk_of(0);
+  int64_t mine = seqs.units;
+  int items = L.n_kv * seqs.nct;
+  for (int b = 64; b < a.batch; b += 64) {
+    const Seq s = chunk_of(b);
     mine += s.units;
     items += L.n_kv * s.nct;
   }
@@ -692,26 +700,24 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   int64_t u = (int64_t)w * part;
   const int64_t u_end = min(u + part, total);
   if (u >= u_end) return;
-  int b = 0, item0 = 0;  // the sequence that unit u lies in, its first item and unit
+  int at_seq = 0, item0 = 0;  // the sequence that unit u lies in (of seqs), its first item and unit
   int64_t first = 0;
-  for (int64_t run = 0;; b += 64) {
-    const Seq s = sequence(L, min(b + lane, a.batch - 1));
-    const bool in_batch = b + lane < a.batch;
-    const int64_t n = in_batch ? s.units : 0;
-    const int m = in_batch ? L.n_kv * s.nct : 0;
-    const int64_t in = wave_scan_i64(n);
+  for (int64_t run = 0;;) {
+    const int64_t in = wave_scan_i64(seqs.units);
     const uint64_t over = __ballot(run + in > u);
     const int f = over ? __ffsll((unsigned long long)over) - 1 : 64;
-    int before = lane < f ? m : 0;
+    int before = lane < f ? L.n_kv * seqs.nct : 0;
 #pragma unroll
     for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d, 64);
     item0 = uniform(item0 + before);
     if (over) {
-      first = uniform64(run + shfl64(in - n, f));
-      b = uniform(b + f);
+      first = uniform64(run + shfl64(in - seqs.units, f));
+      at_seq = uniform(f);
       break;
     }
     run += shfl64(in, 63);
+    b0 += 64;
+    seqs = chunk_of(b0);
   }
 
   typedef Ring<D> G;
@@ -724,20 +730,24 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   const uint32_t sc_off = (lane & (2 * SL) ? R::vsbase(ps) : R::ksbase(ps)) + (lane % SL) * 16;
 
   while (u < u_end) {
-    const Seq s = sequence(L, b);
-    if (u >= first + s.units) {  // behind b: the next sequence that has units
-      first += s.units;
+    const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at_seq); };
+    const Seq s{of(seqs.r0), of(seqs.m), of(seqs.len), of(seqs.lo), of(seqs.tiles), of(seqs.nct), 0};
+    const int64_t units = (int64_t)L.n_kv * s.nct * (whole ? 1 : s.tiles + kStart);
+    if (u >= first + units) {  // behind it: the next sequence that has units
+      first += units;
       item0 += L.n_kv * s.nct;
-      b++;
-      for (;; b += 64) {
-        const uint64_t some = __ballot(b + lane < a.batch && sequence(L, b + lane).units > 0);
+      for (int from = at_seq + 1;; from = 0) {
+        const uint64_t some = from < 64 ? __ballot(seqs.units > 0) >> from << from : 0;
         if (some) {
-          b = uniform(b + __ffsll((unsigned long long)some) - 1);
+          at_seq = uniform(__ffsll((unsigned long long)some) - 1);
           break;
         }
+        b0 += 64;
+        seqs = chunk_of(b0);
       }
       continue;
     }
+    const int b = b0 + at_seq;
     const int64_t rel = u - first;
     const int per_item = whole ? 1 : s.tiles + kStart;
     const int64_t item = rel / per_item;

@@ -58,42 +58,43 @@ __global__ void __launch_bounds__(kMapsThreads) k_step_maps(StepMaps a) {
   const int tid = threadIdx.x, per = (a.batch + kMapsThreads - 1) / kMapsThreads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
   const int64_t cap = (int64_t)a.pps * a.page_size;
-  const auto ask = [&](int b, int& n, int& m, int& need) {
-    n = a.lengths[b];
-    m = a.counts[b];
-    if (n < 0 || m < 0 || (int64_t)n + m > cap) m = 0;
-    need = m == 0 ? 0 : (int)(((int64_t)n + m + a.page_size - 1) / a.page_size - ((int64_t)n + a.page_size - 1) / a.page_size);
+  const auto pages_of = [&](uint32_t n) {
+    const uint32_t p = n / (uint32_t)a.page_size;
+    return (int)(p + (n != p * (uint32_t)a.page_size ? 1 : 0));
   };
-  int n, m, need;
-  // pages: a sequence is served while the list of free pages lasts
+  // what each sequence asks for: pages and rows
   int64_t sum = 0, total;
   for (int b = b0; b < b1; b++) {
-    ask(b, n, m, need);
+    const int n = a.lengths[b], c = a.counts[b];
+    const int m = n < 0 || c < 0 || (int64_t)n + c > cap ? 0 : c;
+    const int need = m == 0 ? 0 : pages_of((uint32_t)n + (uint32_t)m) - pages_of((uint32_t)n);
+    page0[b] = need;
+    row0[b] = m;
     sum += need;
   }
+  // pages: a sequence is served while the list of free pages lasts
   int64_t at = block_scan(sum, tmp, &total) - sum;
   int64_t rows = 0;
   for (int b = b0; b < b1; b++) {
-    ask(b, n, m, need);
+    const int need = page0[b];
     page0[b] = (int)min(at, (int64_t)a.n_free);
     at += need;
-    rows += need == 0 || at <= a.n_free ? m : 0;
+    if (need != 0 && at > a.n_free) row0[b] = 0;
+    rows += row0[b];
   }
-  // rows: and while the row arrays do
+  // rows: and while the row arrays do.  A sequence with rows has its pages up to where the
+  // next sequence's begin.
   if (tid < 2) smax[tid] = 0;
   int64_t r = block_scan(rows, tmp, &total) - rows;
   int64_t granted_rows = 0, granted_pages = 0;
   for (int b = b0; b < b1; b++) {
-    ask(b, n, m, need);
-    const bool pages_ok = need == 0 || (int64_t)page0[b] + need <= a.n_free;
-    const int mm = pages_ok ? m : 0;
-    const bool ok = mm > 0 && r + mm <= a.rows;
+    const int m = row0[b], end = b + 1 < b1 ? page0[b + 1] : (int)min(at, (int64_t)a.n_free);
     row0[b] = (int)min(r, (int64_t)a.rows);
-    if (ok) {
-      granted_rows = r + mm;
-      if (need > 0) granted_pages = (int64_t)page0[b] + need;
+    if (m > 0 && r + m <= a.rows) {
+      granted_rows = r + m;
+      if (end > page0[b]) granted_pages = end;
     }
-    r += mm;
+    r += m;
   }
   if (granted_rows) atomicMax((unsigned long long*)&smax[0], (unsigned long long)granted_rows);
   if (granted_pages) atomicMax((unsigned long long*)&smax[1], (unsigned long long)granted_pages);
@@ -119,17 +120,17 @@ __global__ void __launch_bounds__(kMapsThreads) k_step_maps(StepMaps a) {
     if (i < n_rows) {
       const int b = last_not_above(row0, a.batch, (int)i);
       const int have = a.lengths[b], t = have + ((int)i - row0[b]);
-      const int old = (int)(((int64_t)have + a.page_size - 1) / a.page_size), pg = t / a.page_size;
+      const int old = pages_of((uint32_t)have), pg = (int)((uint32_t)t / (uint32_t)a.page_size);
       const int page = pg < old ? a.page_table[(int64_t)b * a.pps + pg] : a.free_pages[page0[b] + (pg - old)];
       pos = t + (a.starts ? a.starts[b] : 0);
-      slot = page < 0 ? -1 : page * a.page_size + t % a.page_size;
+      slot = page < 0 ? -1 : page * a.page_size + (t - pg * a.page_size);
     }
     a.positions[i] = pos;
     a.slots[i] = slot;
   }
   for (int64_t e = (int64_t)blockIdx.x * kMapsThreads + tid; e < n_pages; e += step) {
     const int b = last_not_above(page0, a.batch, (int)e);
-    const int old = (int)(((int64_t)a.lengths[b] + a.page_size - 1) / a.page_size);
+    const int old = pages_of((uint32_t)a.lengths[b]);
     a.page_table[(int64_t)b * a.pps + old + ((int)e - page0[b])] = a.free_pages[e];
   }
 }
@@ -175,7 +176,7 @@ struct RowStat {
 };
 struct SeqPick {
   double top, z, scale;  // p(v) = 2^((x_v - top) * scale) / z
-  int32_t row;           // the row the token is drawn from
+  int32_t row;           // the row the token is drawn from; -1: the sequence has none
   int32_t draft;         // >= 0: that token's probability is left out (a draft without probabilities)
   int32_t greedy;        // >= 0: the token itself
   int32_t from_probs;    // 1: max(p - q, 0) of the draft's probabilities
@@ -185,15 +186,17 @@ struct LF32 { typedef float T; static __device__ __forceinline__ float get(T x) 
 struct LF16 { typedef _Float16 T; static __device__ __forceinline__ float get(T x) { return (float)x; } };
 struct LBF16 { typedef uint16_t T; static __device__ __forceinline__ float get(T x) { return __uint_as_float((uint32_t)x << 16); } };
 
-// (value, index) order of the greedy tail: NaN above every number, then the
-// larger value, then the lower index.
-__device__ __forceinline__ bool beats(float x, int i, float y, int j) {
-  const bool nx = x != x, ny = y != y;
-  if (nx || ny) return nx && (!ny || i < j);
-  return x > y || (x == y && i < j);
-}
-
+// The last sequence that begins at or before a row: all offsets at once, one a lane, where
+// they are few (one wait for memory instead of one for every halving).
 __device__ __forceinline__ int seq_of(const Verify& a, int row) {
+  if (a.batch <= 512) {
+    int n = 0;
+    for (int b = 0; b < a.batch; b += 64) {
+      const int i = b + (threadIdx.x & 63);
+      n += __popcll(__ballot(i < a.batch && a.row_offsets[i] <= row));
+    }
+    return max(n - 1, 0);
+  }
   int lo = 0, hi = a.batch;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -205,10 +208,29 @@ __device__ __forceinline__ int seq_of(const Verify& a, int row) {
 // A temperature that draws; anything else (0, below, not finite) is greedy.
 __device__ __forceinline__ bool draws(float T) { return T > 0.0f && T < INFINITY; }
 
+// Sum over the wave's lanes, without the LDS crossbar (see wave_tree_sum).
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int M>
+__device__ __forceinline__ double swap_add64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  float l0, l1, h0, h1;
+  lane_pair<M>(__uint_as_float((uint32_t)u), l0, l1);
+  lane_pair<M>(__uint_as_float((uint32_t)(u >> 32)), h0, h1);
+  return __builtin_bit_cast(double, (uint64_t)__float_as_uint(h0) << 32 | __float_as_uint(l0)) +
+         __builtin_bit_cast(double, (uint64_t)__float_as_uint(h1) << 32 | __float_as_uint(l1));
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
-  return v;
+  v += dpp64<0xB1>(v);
+  v += dpp64<0x4E>(v);
+  v += dpp64<0x141>(v);
+  v += dpp64<0x128>(v);
+  return swap_add64<32>(swap_add64<16>(v));
 }
 
 // The elements that a thread takes of a chunk: 16 bytes at a time, neighbours for
@@ -237,6 +259,23 @@ __device__ __forceinline__ void load_chunk(const typename E::T* x, int v0, int v
   }
 }
 
+// kPer neighbours from v0 on.
+template <class E>
+__device__ __forceinline__ void load_run(const typename E::T* x, int v0, int v1, float (&val)[kPer]) {
+  typedef typename E::T T;
+  constexpr int PER = 16 / sizeof(T);
+  if (v1 - v0 >= kPer && ((uintptr_t)(x + v0) % 16) == 0) {
+    T t[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer / PER; i++) ((u32x4*)t)[i] = ((const u32x4*)(x + v0))[i];
+#pragma unroll
+    for (int i = 0; i < kPer; i++) val[i] = E::get(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; i++) val[i] = v0 + i < v1 ? E::get(x[v0 + i]) : 0.0f;
+  }
+}
+
 template <class E>
 __global__ void __launch_bounds__(kVT) k_verify_rows(Verify a, RowStat* __restrict__ stats) {
   const int row = blockIdx.x, chunk = blockIdx.y, tid = threadIdx.x, chunks = gridDim.y;
@@ -249,26 +288,33 @@ __global__ void __launch_bounds__(kVT) k_verify_rows(Verify a, RowStat* __restri
   float top = -INFINITY;
   int at = 0x7FFFFFFF;
   load_chunk<E>(x, v0, v1, val);
-#pragma unroll
-  for (int i = 0; i < kPer; i++) {
-    const int v = token_of<E>(v0, i);
-    if (v < v1 && beats(val[i], v, top, at)) { top = val[i]; at = v; }
-  }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float o = __shfl_xor(top, d, 64);
-    const int oi = __shfl_xor(at, d, 64);
-    if (beats(o, oi, top, at)) { top = o; at = oi; }
-  }
   __shared__ float st[kVT / 64];
   __shared__ int si[kVT / 64];
   __shared__ double ss[kVT / 64];
   const int wave = tid >> 6;
-  if ((tid & 63) == 0) { st[wave] = top; si[wave] = at; }
-  __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kVT / 64; w++)
-    if (beats(st[w], si[w], top, at)) { top = st[w]; at = si[w]; }
+  for (int i = 0; i < kPer; i++) top = __builtin_elementwise_maximum(top, val[i]);  // NaN if there is one
+  bool nan = top != top;
+  top = wave_max(top);  // of the other lanes
+  nan = __ballot(nan) != 0;
+  if ((tid & 63) == 0) st[wave] = nan ? __builtin_nanf("") : top;
+  __syncthreads();
+  top = st[0];
+#pragma unroll
+  for (int w = 1; w < kVT / 64; w++) top = __builtin_elementwise_maximum(top, st[w]);
+  if (!draws(T) || !(top > -INFINITY && top < INFINITY)) {  // greedy: where the maximum is first
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; i--) {
+      const int v = token_of<E>(v0, i);
+      if (v < v1 && (val[i] == top || (val[i] != val[i] && top != top))) at = min(at, v);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) at = min(at, __shfl_xor(at, d, 64));
+    if ((tid & 63) == 0) si[wave] = at;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kVT / 64; w++) at = min(at, si[w]);
+  }
   double sum = 0.0;
   if (draws(T) && top > -INFINITY && top < INFINITY) {
     const double k = kLog2e / (double)T, t = (double)top;
@@ -281,20 +327,24 @@ __global__ void __launch_bounds__(kVT) k_verify_rows(Verify a, RowStat* __restri
   if (tid == 0) stats[(int64_t)row * chunks + chunk] = RowStat{ss[0] + ss[1] + ss[2] + ss[3], top, at};
 }
 
-// A row's chunks joined by one wave: maximum, first index, normaliser.
-__device__ __forceinline__ void join_row(const RowStat* s, int chunks, double k, float& top, int& at, double& z) {
+// A row's chunks joined by one wave: maximum and normaliser, and where the row is greedy
+// the maximum's first index.
+__device__ __forceinline__ void join_row(const RowStat* s, int chunks, double k, float& top, int& at, double& z, bool& cold) {
   const int lane = threadIdx.x & 63;
   top = -INFINITY;
+  for (int c = lane; c < chunks; c += 64) top = __builtin_elementwise_maximum(top, s[c].top);
+  const bool nan = __ballot(top != top) != 0;
+  top = nan ? __builtin_nanf("") : wave_max(top);
+  cold = k == 0.0 || !(top > -INFINITY && top < INFINITY);
   at = 0x7FFFFFFF;
-  for (int c = lane; c < chunks; c += 64)
-    if (beats(s[c].top, s[c].at, top, at)) { top = s[c].top; at = s[c].at; }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float o = __shfl_xor(top, d, 64);
-    const int oi = __shfl_xor(at, d, 64);
-    if (beats(o, oi, top, at)) { top = o; at = oi; }
-  }
   z = 0.0;
+  if (cold) {
+    for (int c = lane; c < chunks; c += 64)
+      if (s[c].top == top || (nan && s[c].top != s[c].top)) at = min(at, s[c].at);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) at = min(at, __shfl_xor(at, d, 64));
+    return;
+  }
   for (int c = lane; c < chunks; c += 64)
     if (s[c].sum > 0.0) z += s[c].sum * pow2(((double)s[c].top - (double)top) * k);
   z = wave_sum64(z);
@@ -316,7 +366,10 @@ __global__ void __launch_bounds__(kVT) k_verify_pick(Verify a, const RowStat* __
   const int b = blockIdx.x, chunk = blockIdx.y, chunks = gridDim.y, tid = threadIdx.x, wave = tid >> 6;
   const int r0 = max(a.row_offsets[b], 0), r1 = min(a.row_offsets[b + 1], a.rows);
   if (r1 <= r0) {
-    if (chunk == 0 && tid == 0) a.accepted[b] = 0;
+    if (chunk == 0 && tid == 0) {
+      a.accepted[b] = 0;
+      picks[b].row = -1;
+    }
     return;
   }
   const float T = a.temperature[b];
@@ -330,24 +383,27 @@ __global__ void __launch_bounds__(kVT) k_verify_pick(Verify a, const RowStat* __
     bool stop = false;
     SeqPick mine = {};
     if (row < r1) {
+      // what the draft's test reads, asked for before the row's chunks are joined
+      const bool last = row == r1 - 1;
+      const int d = last ? -1 : a.drafts[row];
+      const bool inside = d >= 0 && d < a.vocab;
+      float u = 0.0f, q = 1.0f, x = 0.0f;
+      if (inside) {
+        u = a.u_accept[row];
+        x = E::get(((const typename E::T*)a.logits)[(int64_t)row * a.logits_row + d]);
+        if (a.probs) q = a.probs[(int64_t)row * a.probs_row + d];
+      }
       float top;
       int at;
       double z;
-      join_row(stats + (int64_t)row * chunks, chunks, k, top, at, z);
-      const bool cold = !draws(T) || !(top > -INFINITY && top < INFINITY);
+      bool cold;
+      join_row(stats + (int64_t)row * chunks, chunks, k, top, at, z, cold);
       mine = SeqPick{(double)top, z, k, row, -1, cold ? at : -1, 0};
       stop = true;
-      if (row < r1 - 1) {
-        const int d = a.drafts[row];
-        const bool inside = d >= 0 && d < a.vocab;
+      if (!last) {
         bool ok = false;
-        if (cold) {
-          ok = d == at;
-        } else if (inside) {
-          const double q = a.probs ? (double)a.probs[(int64_t)row * a.probs_row + d] : 1.0;
-          const double p = pow2(((double)E::get(((const typename E::T*)a.logits)[(int64_t)row * a.logits_row + d]) - (double)top) * k) / z;
-          ok = (double)a.u_accept[row] * q < p;
-        }
+        if (cold) ok = d == at;
+        else if (inside) ok = (double)u * (double)q < pow2(((double)x - (double)top) * k) / z;
         stop = !ok;
         mine.draft = a.probs ? -1 : d;
         mine.from_probs = a.probs ? 1 : 0;
@@ -405,9 +461,8 @@ template <class E>
 __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* __restrict__ stats, const SeqPick* __restrict__ picks,
                                                       const double* __restrict__ sums, int chunks) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int r0 = max(a.row_offsets[b], 0), r1 = min(a.row_offsets[b + 1], a.rows);
-  if (r1 <= r0) return;
   SeqPick s = picks[b];
+  if (s.row < 0) return;
   if (s.greedy >= 0) {
     if (tid == 0) a.tokens[s.row] = s.greedy;
     return;
@@ -417,13 +472,15 @@ __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* _
   const double* c = sums + (int64_t)b * chunks;
   bool plain = false;  // nothing is left of p - q: the token comes from p
   if (wave == 0) {
-    double total = 0.0;
-    for (int i = lane; i < chunks; i += 64) total += c[i];
+    // the first 64 chunks' sums stay in registers: most vocabularies have no more
+    const double c0 = lane < chunks ? c[lane] : 0.0;
+    double total = c0;
+    for (int i = lane + 64; i < chunks; i += 64) total += c[i];
     total = wave_sum64(total);
     plain = !(total > 0.0);
     const RowStat* st = stats + (int64_t)s.row * chunks;
     const auto mass = [&](int i) {
-      if (!plain) return c[i];
+      if (!plain) return i < 64 ? c0 : c[i];
       return st[i].sum > 0.0 ? st[i].sum * pow2(((double)st[i].top - s.top) * s.scale) : 0.0;
     };
     if (plain) total = s.z;
@@ -464,12 +521,12 @@ __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* _
   if (chosen >> 30) { s.from_probs = 0; s.draft = -1; }
   const int v0 = chunk * kChunk + tid * kPer, v1 = min(chunk * kChunk + kChunk, a.vocab);
   double w[kPer], sum = 0.0;
+  float x[kPer], q[kPer];
+  load_run<E>((const typename E::T*)a.logits + (int64_t)s.row * a.logits_row, v0, v1, x);
+  if (s.from_probs) load_run<LF32>(a.probs + (int64_t)s.row * a.probs_row, v0, v1, q);
 #pragma unroll
   for (int i = 0; i < kPer; i++) {
-    w[i] = 0.0;
-    if (v0 + i < v1)
-      w[i] = weight(s, E::get(((const typename E::T*)a.logits)[(int64_t)s.row * a.logits_row + v0 + i]),
-                    s.from_probs ? a.probs[(int64_t)s.row * a.probs_row + v0 + i] : 0.0f, v0 + i);
+    w[i] = v0 + i < v1 ? weight(s, x[i], s.from_probs ? q[i] : 0.0f, v0 + i) : 0.0;
     sum += w[i];
   }
   double in = sum;
