@@ -29,11 +29,7 @@ struct F16 {
 struct BF16 {
   typedef uint16_t T;
   static __device__ __forceinline__ float get(T x) { return __uint_as_float((uint32_t)x << 16); }
-  static __device__ __forceinline__ T put(float x) {  // to nearest, ties to even
-    uint32_t u = __float_as_uint(x);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (T)((u >> 16) | 0x40u);
-    return (T)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
-  }
+  static __device__ __forceinline__ T put(float x) { return __builtin_bit_cast(T, (__bf16)x); }
 };
 
 template <class E, bool VEC>
@@ -541,7 +537,9 @@ struct Lines {
   const int32_t *ro, *lens;
   int rows, n_kv, group, window, cols;  // cols: of a column tile
   int64_t cap;                          // tokens that a page table row can hold
+  int start;                            // what beginning an item costs, in tiles
   bool whole;                           // one unit an item
+  __device__ __forceinline__ int per_item(int tiles) const { return whole ? 1 : tiles + start; }
 };
 struct Seq {
   int r0, m, len, lo, tiles, nct;
@@ -556,7 +554,7 @@ __device__ __forceinline__ Seq sequence(const Lines& L, int b) {
   s.lo = lo > 0 ? (int)lo / kTile : 0;  // first tile
   s.tiles = max((int)(((int64_t)s.len + kTile - 1) / kTile) - s.lo, 0);
   s.nct = (int)(((int64_t)s.m * L.group + L.cols - 1) / L.cols);
-  s.units = (int64_t)L.n_kv * s.nct * (L.whole ? 1 : s.tiles + kStart);
+  s.units = (int64_t)L.n_kv * s.nct * L.per_item(s.tiles);
   return s;
 }
 
@@ -564,6 +562,11 @@ __device__ __forceinline__ int64_t shfl64(int64_t v, int lane) { return __shfl((
 __device__ __forceinline__ int64_t wave_sum_i64(int64_t v) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) v += __shfl_xor((long long)v, d, 64);
+  return v;
+}
+__device__ __forceinline__ int wave_sum_i32(int v) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
   return v;
 }
 __device__ __forceinline__ int64_t wave_scan_i64(int64_t v) {
@@ -580,12 +583,6 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
   return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
 }
 
-// Units a wave takes, of `total` over `workers` waves.
-__device__ __forceinline__ int64_t part_of(int64_t total, int workers, int least) {
-  const int64_t n = (total + workers - 1) / workers;
-  return n > least ? n : least;
-}
-
 // Pieces of items that several waves share: two a wave (the end of an item
 // that an earlier wave began, the beginning of one that later waves end).  The wave
 // that begins an item leaves what the merge needs to know of it.
@@ -597,6 +594,103 @@ struct Pieces {
   Begun* begun;  // [items]
   float2* ml;   // [2 * workers][cols] (mref, l)
   float* acc;   // [2 * workers][cols][D]
+};
+
+// a / b of numbers below 2^53 (units of work), in an eighth of the instructions that 64-bit division is.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  const int64_t q = (int64_t)((double)a * __builtin_amdgcn_rcp((double)b));
+  const int64_t r = a - q * b;
+  return r < 0 ? q - 1 : r >= b ? q + 1 : q;
+}
+
+// The parts of items that a wave (or a workgroup) works on, in their order.  A wave holds the sequences
+// 64 at a time, one a lane.
+struct Line {
+  const Lines& L;
+  int batch, w, items;  // items: of the call
+  int64_t part, u, u_end;
+  // the part that next() came to: its item, and n of the item's units from `at` on
+  Seq s;
+  int b, h, ct, at, n, item, pieces;  // pieces of the item, 0 where there is one
+  bool begins, ends;
+
+  __device__ __forceinline__ Line(const Lines& lines, int n_seqs, int worker, int workers, int least) : L(lines), batch(n_seqs), w(worker) {
+    seqs = chunk_of(0);
+    int64_t mine = seqs.units;
+    items = L.n_kv * seqs.nct;
+    for (int i = 64; i < batch; i += 64) {
+      const Seq x = chunk_of(i);
+      mine += x.units;
+      items += L.n_kv * x.nct;
+    }
+    items = wave_sum_i32(items);
+    const int64_t total = uniform64(wave_sum_i64(mine));
+    part = quotient(total + workers - 1, workers);
+    part = part > least ? part : least;
+    u = (int64_t)w * part;
+    u_end = min(u + part, total);
+    if (u >= u_end) return;
+    for (int64_t run = 0;;) {
+      const int64_t in = wave_scan_i64(seqs.units);
+      const uint64_t over = __ballot(run + in > u);
+      const int f = over ? __ffsll((unsigned long long)over) - 1 : 64;
+      item0 = uniform(item0 + wave_sum_i32((int)(threadIdx.x & 63) < f ? L.n_kv * seqs.nct : 0));
+      if (over) {
+        first = uniform64(run + shfl64(in - seqs.units, f));
+        at_seq = uniform(f);
+        return;
+      }
+      run += shfl64(in, 63);
+      b0 += 64;
+      seqs = chunk_of(b0);
+    }
+  }
+
+  __device__ __forceinline__ bool next() {
+    while (u < u_end) {
+      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at_seq); };
+      s = Seq{of(seqs.r0), of(seqs.m), of(seqs.len), of(seqs.lo), of(seqs.tiles), of(seqs.nct), 0};
+      const int per_item = L.per_item(s.tiles);
+      const int64_t units = (int64_t)L.n_kv * s.nct * per_item;
+      if (u < first + units) {
+        b = b0 + at_seq;
+        const int64_t rel = u - first, i = quotient(rel, per_item);
+        at = (int)(rel - i * per_item);
+        h = (int)i / s.nct;
+        ct = (int)(i - (int64_t)h * s.nct);
+        item = item0 + (int)i;
+        n = (int)min((int64_t)(per_item - at), u_end - u);
+        begins = at == 0;
+        ends = at + n == per_item;
+        pieces = ends ? 0 : (int)(quotient(u + per_item - 1, part) - w + 1);
+        u += n;
+        return true;
+      }
+      first += units;  // behind it: the next sequence that has units
+      item0 += L.n_kv * s.nct;
+      for (int from = at_seq + 1;; from = 0) {
+        const uint64_t some = from < 64 ? __ballot(seqs.units > 0) >> from << from : 0;
+        if (some) {
+          at_seq = uniform(__ffsll((unsigned long long)some) - 1);
+          break;
+        }
+        b0 += 64;
+        seqs = chunk_of(b0);
+      }
+    }
+    return false;
+  }
+
+ private:
+  Seq seqs;
+  int b0 = 0, at_seq = 0, item0 = 0;  // the sequence that unit u lies in (of seqs), its first item and unit
+  int64_t first = 0;
+  __device__ __forceinline__ Seq chunk_of(int from) const {
+    const int at = from + (int)(threadIdx.x & 63);
+    Seq x = sequence(L, min(at, batch - 1));
+    if (at >= batch) x.nct = 0, x.units = 0;
+    return x;
+  }
 };
 
 template <int N>
@@ -673,52 +767,10 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int w = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
   const int group = a.n_q / a.c.n_kv, ps = a.c.page_size;
-  const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), whole};
+  const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), kStart, whole};
 
-  // the sequences, 64 at a time, one a lane
-  const auto chunk_of = [&](int b0) {
-    Seq s = sequence(L, min(b0 + lane, a.batch - 1));
-    if (b0 + lane >= a.batch) s.nct = 0, s.units = 0;
-    return s;
-  };
-  int b0 = 0;
-  Seq seqs = chunk_of(0);
-  int64_t mine = seqs.units;
-  int items = L.n_kv * seqs.nct;
-  for (int b = 64; b < a.batch; b += 64) {
-    const Seq s = chunk_of(b);
-    mine += s.units;
-    items += L.n_kv * s.nct;
-  }
-  if (w == 0 && !whole) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) items += __shfl_xor(items, d, 64);
-    if (lane == 0) *pc.n_items = items;
-  }
-  const int64_t total = uniform64(wave_sum_i64(mine));
-  const int64_t part = part_of(total, workers, least);
-  int64_t u = (int64_t)w * part;
-  const int64_t u_end = min(u + part, total);
-  if (u >= u_end) return;
-  int at_seq = 0, item0 = 0;  // the sequence that unit u lies in (of seqs), its first item and unit
-  int64_t first = 0;
-  for (int64_t run = 0;;) {
-    const int64_t in = wave_scan_i64(seqs.units);
-    const uint64_t over = __ballot(run + in > u);
-    const int f = over ? __ffsll((unsigned long long)over) - 1 : 64;
-    int before = lane < f ? L.n_kv * seqs.nct : 0;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d, 64);
-    item0 = uniform(item0 + before);
-    if (over) {
-      first = uniform64(run + shfl64(in - seqs.units, f));
-      at_seq = uniform(f);
-      break;
-    }
-    run += shfl64(in, 63);
-    b0 += 64;
-    seqs = chunk_of(b0);
-  }
+  Line line(L, a.batch, w, workers, least);
+  if (w == 0 && !whole && lane == 0) *pc.n_items = line.items;
 
   typedef Ring<D> G;
   __shared__ __attribute__((aligned(16))) uint8_t rings[4][NS][G::TILE];
@@ -729,35 +781,11 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   constexpr int SL = D / 16;  // lanes that load the scales of one half
   const uint32_t sc_off = (lane & (2 * SL) ? R::vsbase(ps) : R::ksbase(ps)) + (lane % SL) * 16;
 
-  while (u < u_end) {
-    const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at_seq); };
-    const Seq s{of(seqs.r0), of(seqs.m), of(seqs.len), of(seqs.lo), of(seqs.tiles), of(seqs.nct), 0};
-    const int64_t units = (int64_t)L.n_kv * s.nct * (whole ? 1 : s.tiles + kStart);
-    if (u >= first + units) {  // behind it: the next sequence that has units
-      first += units;
-      item0 += L.n_kv * s.nct;
-      for (int from = at_seq + 1;; from = 0) {
-        const uint64_t some = from < 64 ? __ballot(seqs.units > 0) >> from << from : 0;
-        if (some) {
-          at_seq = uniform(__ffsll((unsigned long long)some) - 1);
-          break;
-        }
-        b0 += 64;
-        seqs = chunk_of(b0);
-      }
-      continue;
-    }
-    const int b = b0 + at_seq;
-    const int64_t rel = u - first;
-    const int per_item = whole ? 1 : s.tiles + kStart;
-    const int64_t item = rel / per_item;
-    const int at = (int)(rel - item * per_item);
-    const int h = (int)(item / s.nct), ct = (int)(item - (int64_t)h * s.nct);
-    const int n = (int)min((int64_t)(per_item - at), u_end - u);
-    const bool begins = at == 0, ends = at + n == per_item;
-    u += n;
-    if (begins && !whole && lane == 0)
-      pc.begun[item0 + (int)item] = Begun{b, h, ct, w, ends ? 0 : (int)((u - n + per_item - 1) / part - w + 1)};
+  while (line.next()) {
+    const Seq& s = line.s;
+    const int b = line.b, h = line.h, ct = line.ct, at = line.at, n = line.n;
+    const bool begins = line.begins, ends = line.ends;
+    if (begins && !whole && lane == 0) pc.begun[line.item] = Begun{b, h, ct, w, line.pieces};
 
     // the columns' rows and what they see
     const int c0 = ct * COLS, p0 = s.len - s.m;
@@ -1172,6 +1200,441 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   }
 }
 
+// ---- attention of prompts ---------------------------------------------------------------
+// Many columns, fp16 or bf16, head dim 128: the waves of a workgroup take 32 columns each of
+// one sequence and kv head and share the expansion of its tiles.  They write the codes of the
+// next 64 tokens into LDS as matrix operands: K as c - 8 (fp16), or with its scale (bf16,
+// whose queries and results have 8 bits, K then 11); V with its scale, rounded to fp16, so that
+// O += V^T P^T takes P as it is.  A wave of k_kv4_attn spends 150 of its 300 vector instructions a
+// tile on the expansion; here it is a quarter of 200.  Parts, pieces and the merge are
+// those of k_kv4_attn with a workgroup in the place of a wave.
+//
+// 512 rows of 32 heads at 4096 tokens (8 kv heads, bf16): 80 us (k_kv4_attn: 112), a fifth of
+// the matrix rate.  A step of 64 tokens takes 3.3 us, of which matrix
+// instructions are 0.9 and vector instructions 1.7; before its first one a part waits 10 us
+// for its sequence, its pages, queries and codes, one after the other.  Four waves a workgroup, two of
+// those a CU: 87 us.  One wave of a SIMD expanding while the other multiplies: 84.
+//
+// Scales of 2^13 and more would pass fp16's range in V (c - 8): the first step that brings one
+// turns the part's scales down by 2^4 for good.  A NaN scale of V is expanded as 0, which
+// spares the columns that do not see its token, and written into O of those that do.
+constexpr int kPromptStart = 8;  // what beginning an item costs, in tiles
+
+template <int WAVES, class E>
+__global__ void __launch_bounds__(64 * WAVES, 2)
+    k_kv4_prompt(Kv4Attn a, const int32_t* __restrict__ ro, const int32_t* __restrict__ lens, const int32_t* __restrict__ table,
+                 const uint8_t* __restrict__ base, Pieces pc, int workers, int least) {
+  constexpr int D = 128, NB = 4, NT = 2, COLS = 32 * WAVES, SUB = WAVES / 4;  // SUB tiles at a time
+  constexpr bool SCALED_K = std::is_same<E, BF16>::value;
+  typedef Rec<D> R;
+  typedef typename E::T T;
+  const Magic magic;
+  struct Tile {
+    h8 k[2][NB][64], v[NB][2][64];
+    u32x2 ks[2][4][NB];       // K scales of four tokens: half, token group, block
+    u32x4 vs[2][4][NB / 2];   // V scales: half, token group, two blocks
+    uint32_t about[4];        // what each of the four waves that expanded it found
+  };
+  enum { LARGE = 1, NOT_FINITE = 2, GONE = 4 };
+  __shared__ Tile tiles[2][SUB];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int w = blockIdx.x, group = a.n_q / a.c.n_kv, ps = a.c.page_size;
+  const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), kPromptStart, false};
+  Line line(L, a.batch, w, workers, least);
+  if (w == 0 && threadIdx.x == 0) *pc.n_items = line.items;
+
+  const int64_t rec = kv4_record_bytes(D, ps);
+  const uint32_t page_bytes = (uint32_t)(a.c.n_kv * rec);
+  // a thread's part of a step: 8 bytes of codes of K and of V, of half j of tile `sub`
+  const int sub = wave >> 2, j = (wave >> 1) & 1, r = threadIdx.x & 127;
+  const int kg = r >> 5, ktok = (r >> 1) & 15, kb = (r & 1) * 2;  // K: eight dims of blocks kb, kb + 1
+  const int vt = r >> 5, vc = (r >> 1) & 15, vp = r & 1;          // V: token group, column, block pair
+
+  while (line.next()) {
+    const Seq& s = line.s;
+    const int h = line.h, c0 = line.ct * COLS, p0 = s.len - s.m;
+    const bool begins = line.begins, ends = line.ends;
+    if (begins && threadIdx.x == 0) pc.begun[line.item] = Begun{line.b, h, line.ct, w, line.pieces};
+    const auto row_of = [&](int c) { return min(s.m - 1, c / group); };
+    const int rf = row_of(c0), rl = row_of(c0 + COLS - 1);
+    const int cw = c0 + wave * 16 * NT, wf = row_of(cw), wl = row_of(cw + 16 * NT - 1);  // the wave's rows
+    // a column's row and head; found anew where they are needed, as keeping them costs registers of the loop
+    struct Column {
+      int row, head;
+    };
+    const auto column = [&](int t) {
+      int cc = cw + t * 16 + col;
+      asm("" : "+v"(cc));
+      const int row = cc / group;
+      return Column{row, h * group + (cc - row * group)};
+    };
+    int hi[NT], lo[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int row = column(t).row;
+      hi[t] = row < s.m ? max(p0 + row + 1, 0) : 0;
+      lo[t] = a.window > 0 ? max(p0 + row + 1 - a.window, 0) : 0;
+    }
+    const auto first_seen = [&](int row) { return a.window > 0 ? max(p0 + row + 1 - a.window, 0) : 0; };
+    const auto end_seen = [&](int row) { return max(p0 + row + 1, 0); };
+    const int t0 = max(s.lo + max(line.at - kPromptStart, 0), first_seen(rf) / kTile);
+    const int t1 = min(s.lo + max(line.at + line.n - kPromptStart, 0), (end_seen(rl) + kTile - 1) / kTile);
+    const bool any = cw < s.m * group;  // the wave has columns
+    const int w_lo = first_seen(wf), w_hi = any ? end_seen(wl) : 0, w_lo_last = first_seen(wl), w_hi_first = end_seen(wf);
+
+    f4 acc[NT][2 * NB], l[NT];
+    float mref[NT], kcol[NT];
+    h8 q[NT][NB];
+    float turn = 1.0f;  // of the item's scales
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+      for (int i = 0; i < 2 * NB; i++) acc[t][i] = f4{0, 0, 0, 0};
+      l[t] = f4{0, 0, 0, 0};
+      mref[t] = -1e30f;
+      kcol[t] = 0.0f;
+    }
+    if (t0 < t1) {
+      const TablePtr rowp = (TablePtr)(table + (int64_t)line.b * a.pps);
+      const int n_pages = (int)(((int64_t)s.len + ps - 1) / ps);
+      const uint8_t* head = base + (int64_t)h * rec;
+      // the wave's 16 tokens of a step: page and token in it, and the id, read a step ahead of its use
+      int pg, off, id, id_off;
+      bool id_there;
+      const auto look = [&] {
+        id = rowp[min(pg, n_pages - 1)];
+        id_there = pg < n_pages;
+        id_off = off;
+        off += SUB * kTile;
+        while (off >= ps) { off -= ps; pg++; }
+      };
+      const auto start = [&](int step) {
+        const int tok = (step + sub) * kTile + 16 * j;
+        pg = tok / ps;
+        off = tok - pg * ps;
+        look();
+      };
+      // a thread's part, loaded a step ahead of its expansion
+      u32x2 kc, vcode;
+      uint16_t ks[2];
+      u32x4 vs;
+      bool there = false;
+      const auto fetch = [&] {
+        there = id_there && (uint32_t)id < (uint32_t)a.c.pages;
+        const uint32_t off0 = (uint32_t)id_off;
+        const uint8_t* p = head + (uint64_t)(uint32_t)(there ? id : 0) * page_bytes;
+        kc = *(const u32x2*)(p + (off0 * (D / 2) + r * 8));
+        vcode = *(const u32x2*)(p + (R::vbase(ps) + off0 * (D / 2) + r * 8));
+        const uint32_t so = off0 * (D / 16);
+        ks[0] = *(const uint16_t*)(p + (R::ksbase(ps) + so + R::s(ktok >> 2, kb) + (ktok & 3) * 2));
+        ks[1] = *(const uint16_t*)(p + (R::ksbase(ps) + so + R::s(ktok >> 2, kb + 1) + (ktok & 3) * 2));
+        vs = *(const u32x4*)(p + (R::vsbase(ps) + so + R::s(vt, 2 * vp)));
+        look();
+      };
+      // its expansion into buffer i
+      const auto expand = [&](int i, int step) {
+        Tile& x = tiles[i][sub];
+        const int tok = (step + sub) * kTile + 16 * j;  // of the wave's first
+        uint16_t kd[2] = {ks[0], ks[1]};
+        uint32_t vd[4] = {vs[0], vs[1], vs[2], vs[3]};
+        if (!there || tok + 16 > s.len) {  // scales of no token are 0
+#pragma unroll
+          for (int n = 0; n < 2; n++) kd[n] = there && tok + ktok < s.len ? kd[n] : 0;
+#pragma unroll
+          for (int n = 0; n < 4; n++) {
+            const int at = tok + 4 * vt + 2 * (n & 1);
+            vd[n] &= there ? (at + 1 < s.len ? 0xFFFFFFFFu : at < s.len ? 0xFFFFu : 0u) : 0u;
+          }
+        }
+        if (vc == 0) x.vs[j][vt][vp] = u32x4{vd[0], vd[1], vd[2], vd[3]};
+        // the largest scale
+        typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+        const auto abs2 = [](uint32_t v) { return __builtin_bit_cast(us2, v & 0x7FFF7FFFu); };
+        us2 e = __builtin_elementwise_max(__builtin_elementwise_max(abs2(vd[0]), abs2(vd[1])), __builtin_elementwise_max(abs2(vd[2]), abs2(vd[3])));
+        if constexpr (SCALED_K) e = __builtin_elementwise_max(e, abs2(kd[0] | (uint32_t)kd[1] << 16));
+        uint32_t about = there ? 0 : GONE;
+        if (__ballot(max(e[0], e[1]) >= 0x7000)) {  // 2^13 and more, or not finite: hardly ever
+          asm volatile("");
+          bool large = false, odd = false;
+#pragma unroll
+          for (int n = 0; n < 8; n++) {
+            const uint32_t d = (vd[n >> 1] >> (16 * (n & 1))) & 0x7FFFu;
+            odd |= d >= 0x7C00u;
+            large |= d >= 0x7000u && d < 0x7C00u;
+            if (d >= 0x7C00u) vd[n >> 1] &= n & 1 ? 0xFFFFu : 0xFFFF0000u;
+          }
+          if constexpr (SCALED_K)
+#pragma unroll
+            for (int n = 0; n < 2; n++) large |= (kd[n] & 0x7FFFu) >= 0x7000u && (kd[n] & 0x7FFFu) < 0x7C00u;
+          about |= (__ballot(large) && turn == 1.0f ? LARGE : 0) | (__ballot(odd) ? NOT_FINITE : 0);
+        }
+        if (lane == 0) x.about[wave & 3] = about;
+        if (turn != 1.0f) {
+          const h2 down = {(_Float16)turn, (_Float16)turn};
+#pragma unroll
+          for (int n = 0; n < 4; n++) vd[n] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, vd[n]) * down);
+          if constexpr (SCALED_K)
+#pragma unroll
+            for (int n = 0; n < 2; n++) kd[n] = __builtin_bit_cast(uint16_t, (_Float16)(__builtin_bit_cast(_Float16, kd[n]) * down[0]));
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          h2 p[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            p[k] = code_pair(magic, kc[n], k);
+            if constexpr (SCALED_K) p[k] *= __builtin_bit_cast(h2, (uint32_t)kd[n] * 0x10001u);
+          }
+          x.k[j][kb + n][kg * 16 + ktok] = pack8(p[0], p[1], p[2], p[3]);
+          if constexpr (!SCALED_K)
+            if (kg == 0) ((uint16_t*)&x.ks[j][ktok >> 2][kb + n])[ktok & 3] = kd[n];
+        }
+#pragma unroll
+        for (int n = 0; n < 4; n++) {  // block 2 vp + n / 2, its half n % 2
+          const h2 y0 = code_pair(magic, vcode[0], n) * __builtin_bit_cast(h2, vd[2 * (n >> 1)]);
+          const h2 y1 = code_pair(magic, vcode[1], n) * __builtin_bit_cast(h2, vd[2 * (n >> 1) + 1]);
+          ((u32x2*)&x.v[2 * vp + (n >> 1)][n & 1][vt * 16 + vc])[j] = u32x2{__builtin_bit_cast(uint32_t, y0), __builtin_bit_cast(uint32_t, y1)};
+        }
+      };
+
+      start(t0);
+      fetch();
+      const bool vec = vec_rows(a.q, sizeof(T));
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float x[NB][8], big = 0.0f;
+        const Column c = column(t);
+#pragma unroll
+        for (int bk = 0; bk < NB; bk++) {
+          if (c.row < s.m) {
+            const T* src = (const T*)a.q.p + (int64_t)(s.r0 + c.row) * a.q.row + (int64_t)c.head * a.q.head + bk * 32 + g * 8;
+            if (vec) load8<E, true>(src, x[bk]); else load8<E, false>(src, x[bk]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[bk][i] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[bk][i]));
+        }
+        big = xor_max<32>(xor_max<16>(big));
+        const int e = __builtin_amdgcn_frexp_expf(big);
+        kcol[t] = __builtin_amdgcn_ldexpf(a.scale * 1.4426950408889634f, e);
+#pragma unroll
+        for (int bk = 0; bk < NB; bk++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) q[t][bk][i] = (_Float16)__builtin_amdgcn_ldexpf(x[bk][i], -e);
+      }
+      const uint32_t one = 0x3C003C00u;
+      const h8 ones = __builtin_bit_cast(h8, u32x4{one, one, one, one});
+
+      const auto compute = [&](int buf, int step) {
+#pragma unroll 1
+        for (int i = 0; i < SUB; i++) {
+          const Tile& x = tiles[buf][i];
+          const int tok0 = (step + i) * kTile;
+          if (step + i >= t1 || tok0 >= w_hi || tok0 + kTile <= w_lo) continue;
+          const u32x4 about = *(const u32x4*)x.about;
+          const uint32_t lost = uniform((about[0] & GONE) / GONE | (about[2] & GONE) / GONE << 1);
+          const bool edge = lost || tok0 < w_lo_last || tok0 + kTile > w_hi_first;
+          float sc[NT][8];
+          {
+            h8 kq[2][NB];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+              for (int bk = 0; bk < NB; bk++) kq[i][bk] = x.k[i][bk][lane];
+            if constexpr (SCALED_K) {
+              f4 d[NT][2] = {};
+#pragma unroll
+              for (int bk = 0; bk < NB; bk++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                  for (int t = 0; t < NT; t++) d[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[i][bk], q[t][bk], d[t][i], 0, 0, 0);
+#pragma unroll
+              for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) sc[t][i] = d[t][i >> 2][i & 3];
+            } else {
+#pragma unroll
+              for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                  f4 d[NB];
+#pragma unroll
+                  for (int bk = 0; bk < NB; bk++) d[bk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[i][bk], q[t][bk], f4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                  for (int n = 0; n < 4; n++) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int bk = 0; bk < NB; bk++) sum = __builtin_fmaf(half_of(x.ks[i][g][bk][n >> 1], n & 1), d[bk][n], sum);
+                    sc[t][4 * i + n] = sum;
+                  }
+                }
+            }
+          }
+          h8 v[NB][2];
+#pragma unroll
+          for (int bk = 0; bk < NB; bk++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) v[bk][hh] = x.v[bk][hh][lane];
+          asm volatile("" ::: "memory");  // these loads run while the weights are computed
+          uint32_t see[NT];
+          float e2[NT][8];
+          bool grow = false;
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            see[t] = 0xFF;
+#pragma unroll
+            for (int i = 0; i < 8; i++) e2[t][i] = __builtin_fmaf(sc[t][i], kcol[t], -mref[t]);
+          }
+          if (edge) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              see[t] = 0;
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const int tok = tok0 + 16 * (i >> 2) + 4 * g + (i & 3);
+                const bool ok = (tok >= lo[t]) & (tok < hi[t]) & !((lost >> (i >> 2)) & 1);
+                see[t] |= ok ? 1u << i : 0u;
+                if (!ok) e2[t][i] = -INFINITY;
+              }
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            float m = e2[t][0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) m = fmaxf(m, e2[t][i]);
+            grow |= m > 14.0f;
+          }
+          if (__ballot(grow)) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              asm volatile("" : "+v"(see[t]));  // its bits are looked at here only
+              float m = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 8; i++)
+                if ((see[t] >> i) & 1) m = fmaxf(m, sc[t][i] * kcol[t]);
+              m = xor_max<32>(xor_max<16>(m));
+              const float now = m - mref[t] > 14.0f ? m - 10.0f : mref[t];
+              const float keep = __builtin_amdgcn_exp2f(mref[t] - now);
+              mref[t] = now;
+              l[t] *= keep;
+#pragma unroll
+              for (int i = 0; i < 2 * NB; i++) acc[t][i] *= keep;
+#pragma unroll
+              for (int i = 0; i < 8; i++) e2[t][i] = (see[t] >> i) & 1 ? __builtin_fmaf(sc[t][i], kcol[t], -mref[t]) : -INFINITY;
+            }
+          }
+          h8 p[NT];
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) p[t][i] = (_Float16)__builtin_amdgcn_exp2f(e2[t][i]);
+            l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[t], l[t], 0, 0, 0);
+          }
+#pragma unroll
+          for (int bk = 0; bk < NB; bk++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+#pragma unroll
+              for (int t = 0; t < NT; t++) acc[t][2 * bk + hh] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[bk][hh], p[t], acc[t][2 * bk + hh], 0, 0, 0);
+            }
+          if (uniform(about[0] | about[1] | about[2] | about[3]) & NOT_FINITE) {  // scales of V that were left out, among the tokens that a column sees
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              uint32_t bad = 0;
+#pragma unroll
+              for (int n = 0; n < 8; n++)
+#pragma unroll
+                for (int bk = 0; bk < NB; bk++) {
+                  const uint32_t d = x.vs[n >> 2][g][bk >> 1][2 * (bk & 1) + ((n >> 1) & 1)] >> (16 * (n & 1));
+                  if ((d & 0x7FFFu) >= 0x7C00u && ((see[t] >> n) & 1)) bad |= 1u << bk;
+                }
+              bad |= __shfl_xor(bad, 16, 64);
+              bad |= __shfl_xor(bad, 32, 64);
+#pragma unroll
+              for (int bk = 0; bk < NB; bk++)
+                if ((bad >> bk) & 1) {
+                  const float n = __builtin_nanf("");
+                  acc[t][2 * bk] = f4{n, n, n, n};
+                  acc[t][2 * bk + 1] = f4{n, n, n, n};
+                }
+            }
+          }
+        }
+      };
+      int buf = 1;
+      bool some = false;  // a step to multiply
+      for (int step = t0 - SUB;;) {
+        const int next = step + SUB;
+        if (some) compute(buf, step);
+        if (next >= t1) break;
+        expand(buf ^ 1, next);
+        fetch();  // the step after it, also where there is none
+        __syncthreads();
+        step = next;
+        buf ^= 1;
+        some = true;
+        uint32_t all = 0;
+#pragma unroll
+        for (int i = 0; i < SUB; i++) {
+          const u32x4 x = *(const u32x4*)tiles[buf][i].about;
+          all |= x[0] | x[1] | x[2] | x[3];
+        }
+        if (uniform(all) & LARGE) {  // expand the step once more, with the item's scales turned down
+          turn = 0.0625f;
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            if (SCALED_K) kcol[t] *= 16.0f;
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) acc[t][i] *= turn;
+          }
+          start(step);
+          fetch();
+          __syncthreads();
+          step -= SUB;
+          buf ^= 1;
+          some = false;
+        }
+      }
+      __syncthreads();  // the buffers are the next part's
+    }
+    const float up = 1.0f / turn;
+    const int64_t slot = (begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w) * COLS;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const float sum = l[t][0];
+      const Column at = column(t);
+      if (at.row >= s.m) continue;
+      if (begins && ends) {
+        const float inv = sum == 0.0f ? 0.0f : up / sum;
+        T* dst = (T*)a.out.p + (int64_t)(s.r0 + at.row) * a.out.row + (int64_t)at.head * a.out.head + 4 * g;
+        const bool ovec = vec_rows(a.out, sizeof(T));
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+          T o[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[k] = E::put(acc[t][i][k] * inv);
+          if (ovec) {
+            *(u32x2*)(dst + 16 * i) = *(u32x2*)o;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) dst[16 * i + k] = o[k];
+          }
+        }
+      } else {
+        const int64_t c = slot + wave * 16 * NT + t * 16 + col;
+        if (g == 0) pc.ml[c] = float2{mref[t], sum};
+        if (sum == 0.0f) continue;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) *(f4*)(pc.acc + c * D + 16 * i + 4 * g) = acc[t][i] * up;
+      }
+    }
+  }
+}
+
 // Joins the pieces of an item that several waves computed, in their order: a workgroup
 // an item and `per` columns (more for every gridDim.y), its waves by column and by piece.
 template <int D, class E>
@@ -1265,6 +1728,8 @@ int compute_units() {
   return n[dev];
 }
 
+constexpr int kPromptWaves = 8;
+constexpr int kMergeWaves = 4096;
 constexpr int kLeast = 4;     // tiles a wave takes at least
 
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -1278,42 +1743,83 @@ size_t attn_bytes(int64_t items, int64_t workers, int cols, int hd) {
   return 256 + align256(sizeof(Begun) * items) + align256(sizeof(float2) * 2 * workers * cols) + sizeof(float) * 2 * workers * cols * hd;
 }
 
+// The parts of the workspace for `items` items, and `workers` workers of `cols` columns.
+Pieces pieces_in(void* ws, int64_t items, int64_t workers, int cols) {
+  char* p = (char*)ws;
+  Pieces pc;
+  pc.n_items = (int*)p;
+  p += 256;
+  pc.begun = (Begun*)p;
+  p += align256(sizeof(Begun) * items);
+  pc.ml = (float2*)p;
+  p += align256(sizeof(float2) * 2 * workers * cols);
+  pc.acc = (float*)p;
+  return pc;
+}
+
+template <int D, class E>
+hipError_t merge(hipStream_t st, const Kv4Attn& a, const Pieces& pc, int64_t items, int64_t workers, int cols, int64_t cap, int start) {
+  const int group = a.n_q / a.c.n_kv;
+  const Lines L{a.row_offsets, a.lengths, a.rows, a.c.n_kv, group, a.window, cols, cap, start, false};
+  // Waves a column: more where an item has many pieces, but not where there are columns enough
+  // to fill the card (8 items of 256 columns in 16 pieces: 60 -> 35 us with their attention).
+  const int64_t columns = std::min<int64_t>(cols, (int64_t)a.max_rows * group);
+  const int pieces = (int)(workers / items);
+  int share = pieces >= 16 ? 16 : pieces >= 4 ? 4 : 1;
+  while (share > 1 && items * columns * share > kMergeWaves) share /= 4;
+  const int per = share == 1 ? 4 : 1;
+  hipLaunchKernelGGL((k_kv4_merge<D, E>), dim3((unsigned)items, (unsigned)((columns + per - 1) / per)), dim3(share == 16 ? 1024 : 256), 0,
+                     st, a, L, pc, per);
+  return hipGetLastError();
+}
+
+int64_t attn_cap(const Kv4Attn& a) { return std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0); }
+
 template <int D, int NT, class E>
 hipError_t attn_tiles(hipStream_t st, const Kv4Attn& a) {
-  const int cols = 16 * NT, group = a.n_q / a.c.n_kv;
-  const int64_t cap = std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0);
+  const int cols = 16 * NT;
+  const int64_t cap = attn_cap(a), tiles = (cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
-  const int64_t tiles = (cap + kTile - 1) / kTile;
   const bool whole = tiles <= kLeast;
   const int64_t most = (int64_t)compute_units() * 4 * attn_waves(D, NT, Terms<E>::n);
   const int64_t want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
   const int workers = (int)((std::min(most, want) + 3) / 4 * 4), least = whole ? 1 : kLeast;
-  char* ws = (char*)a.ws;
-  Pieces pc;
-  pc.n_items = (int*)ws;
-  ws += 256;
-  pc.begun = (Begun*)ws;
-  ws += align256(sizeof(Begun) * items);
-  pc.ml = (float2*)ws;
-  ws += align256(sizeof(float2) * 2 * workers * cols);
-  pc.acc = (float*)ws;
+  const Pieces pc = pieces_in(a.ws, items, workers, cols);
   hipLaunchKernelGGL((k_kv4_attn<D, NT, attn_ring(D, NT, Terms<E>::n), E>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths,
                      a.page_table, a.c.base, pc, workers, least, whole);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || whole) return e;
-  const Lines L{a.row_offsets, a.lengths, a.rows, a.c.n_kv, group, a.window, cols, cap, false};
-  // items of many pieces have a workgroup a column, of very many a large one
-  const int pieces = (int)(workers / items), per = pieces >= 4 ? 1 : 4;
-  const int64_t columns = std::min<int64_t>(cols, (int64_t)a.max_rows * group);
-  hipLaunchKernelGGL((k_kv4_merge<D, E>), dim3((unsigned)items, (unsigned)((columns + per - 1) / per)), dim3(pieces >= 16 ? 1024 : 256), 0,
-                     st, a, L, pc, per);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || whole ? e : merge<D, E>(st, a, pc, items, workers, cols, cap, kStart);
+}
+
+template <class E>
+hipError_t attn_prompt(hipStream_t st, const Kv4Attn& a) {
+  constexpr int cols = 32 * kPromptWaves;
+  const int64_t cap = attn_cap(a), tiles = (cap + kTile - 1) / kTile;
+  const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
+  const int64_t most = (int64_t)compute_units() * (8 / kPromptWaves), want = (items * (tiles + kPromptStart) + kLeast - 1) / kLeast;
+  const int workers = (int)std::min(most, want);
+  const Pieces pc = pieces_in(a.ws, items, workers, cols);
+  hipLaunchKernelGGL((k_kv4_prompt<kPromptWaves, E>), dim3((unsigned)workers), dim3(64 * kPromptWaves), 0, st, a, a.row_offsets, a.lengths,
+                     a.page_table, a.c.base, pc, workers, kLeast);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : merge<128, E>(st, a, pc, items, workers, cols, cap, kPromptStart);
+}
+
+// Columns enough for the waves of a workgroup to share a tile's expansion: 64 a sequence, and a table of more
+// than 256 tokens.  32 heads, 8 kv heads, bf16, k_kv4_prompt against k_kv4_attn with NT = 2: one sequence of 64 rows
+// at 16384 tokens 52 and 63 us, of 512 rows at 2048 54 and 67, 16 sequences of 16 rows at 1024 40 and
+// 39; 64 of 8 rows (32 columns each) 81 and 52, one of 256 rows and tokens 28 and 27.
+bool many_columns(const Kv4Attn& a) {
+  const int64_t group = a.n_q / a.c.n_kv;
+  return a.max_rows * group >= 64 && a.rows * group >= (int64_t)64 * a.batch && attn_cap(a) > 256;
 }
 
 template <class E>
 hipError_t attn_type(hipStream_t st, const Kv4Attn& a) {
   const bool one = (int64_t)a.max_rows * (a.n_q / a.c.n_kv) <= 16;
   if (a.c.hd == 64) return one ? attn_tiles<64, 1, E>(st, a) : attn_tiles<64, 2, E>(st, a);
+  if constexpr (sizeof(typename E::T) == 2)
+    if (a.c.hd == 128 && many_columns(a)) return attn_prompt<E>(st, a);
   if (a.c.hd == 128) return one ? attn_tiles<128, 1, E>(st, a) : attn_tiles<128, 2, E>(st, a);
   return attn_tiles<256, 1, E>(st, a);
 }

@@ -11,9 +11,12 @@ with W = sum of w_j |v_j| of the row (w the exact probabilities),
 - f16 and bf16: each weight is rounded to fp16's 11 bits, half a step of which is up to 2^-11 of it
   (finfo.eps / 2), and its product with the block's scale again: 2 * 2^-11 = 2^-10 of W; weights below the
   smallest fp16 subnormal (2^-24 of 2^9) vanish or round: N * 2^-33 * max|v|;
+- bf16, many rows: keys are rounded to fp16 (2^-11 of each), which moves a score by up to 2^-11 * |q| . |k| * scale,
+  every weight by that factor and their sum again: 2^-10 * |q| . |k| * scale * W;
 - fp32: weights as two fp16 terms, 2^-22 * W, and fp32 sums over N tokens in at most N/8 dependent
   steps a lane: N * 2^-27 * W;
-- the output's own rounding: half a step, finfo.eps / 2 * |out|.
+- the output's own rounding: half a step, finfo.eps / 2 * |out|, and below the smallest normal number half of the steps there,
+  smallest_normal * eps / 2 (fp16: 2^-25, where -6.236e-7 is nearest to a number 2.8e-8 away).
 """
 import numpy as np
 import pytest
@@ -186,7 +189,10 @@ class Case:
         vmax = max([np.nanmax(np.abs(x)) for x in self.v if len(x)] + [0.0])
         rel = 2 * (D + 16) * 2.0 ** -24 * 10 * size
         rel = rel + (2.0 ** -10 if dtype != "f32" else 2.0 ** -22 + N * 2.0 ** -27)
+        if dtype == "bf16" and max(self.news) > 16:
+            rel = rel + 2.0 ** -10 * size
         tol = rel * mag + torch.finfo(TYPES[dtype]).eps / 2 * np.abs(want) * 1.01 + N * 2.0 ** -33 * vmax
+        tol = tol + torch.finfo(TYPES[dtype]).smallest_normal * torch.finfo(TYPES[dtype]).eps / 2
         far = np.abs(P.as_f64(got)[:R] - want[:R]) - tol[:R]
         assert np.all(np.isfinite(P.as_f64(got)[:R])), what
         assert far.max() <= 0, (what, far.max(), np.unravel_index(far.argmax(), far.shape))
@@ -218,6 +224,15 @@ SHAPES = [
     (4, 2, 64, 16, [33] * 70, [1] * 70, 0),      # more sequences than a wave has lanes
     (4, 2, 64, 16, [2500, 40], [1, 1], 1),       # a window of the token itself
     (4, 2, 128, 16, [3000, 10, 800], [4, 1, 2], 0),
+    # many columns a sequence, head dim 128: waves that share a tile's expansion (fp16, bf16)
+    (8, 2, 128, 16, [600, 530], [40, 33], 0),
+    (32, 8, 128, 16, [1000], [77], 100),
+    (6, 2, 128, 48, [1300, 0, 333], [90, 20, 64], 0),
+    (24, 1, 128, 64, [700, 100], [5, 3], 0),
+    (4, 2, 128, 16, [5, 700], [70, 3], 0),
+    (4, 2, 128, 16, [64, 300, 64], [0, 130, 0], 0),
+    (8, 8, 128, 16, [900, 31, 290], [64, 31, 100], 1),
+    (8, 1, 128, 32, [2000], [300], 0),
 ]
 
 
@@ -243,8 +258,9 @@ def test_attention(sess, shape, dtype):
 
 @pytest.mark.parametrize("how", ["padded", "heads_outside", "odd"])
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_attention_strides(sess, how, dtype):
-    c = Case(sess, 8, 2, 128, 16, [70, 200], [3, 20], layers=2)
+@pytest.mark.parametrize("lens,news", [([70, 200], [3, 20]), ([400, 300], [30, 20])])
+def test_attention_strides(sess, how, dtype, lens, news):
+    c = Case(sess, 8, 2, 128, 16, lens, news, layers=2)
     q = c.queries(dtype)
     out = _laid(torch.zeros_like(q), how)
     plan = c.plan()
@@ -258,15 +274,38 @@ def test_attention_strides(sess, how, dtype):
 
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("v_scale,k_scale,mul", [(1e-4, 1.0, 1.5), (300.0, 1.0, 1.5), (1.0, 20.0, 6.0), (1.0, 1e-3, 1e-3), (3000.0, 3.0, 1.0)])
-def test_attention_ranges(sess, dtype, v_scale, k_scale, mul):
+@pytest.mark.parametrize("news", [[1, 6], [100, 40]])
+def test_attention_ranges(sess, dtype, v_scale, k_scale, mul, news):
     """Tiny and large values, near-uniform and one-hot probabilities."""
-    print("ranges", dtype, v_scale, k_scale, mul, flush=True)
-    c = Case(sess, 4, 2, 128, 16, [900, 40], [1, 6], v_scale=v_scale, k_scale=k_scale)
+    print("ranges", dtype, v_scale, k_scale, mul, news, flush=True)
+    c = Case(sess, 4, 2, 128, 16, [900, 40], news, v_scale=v_scale, k_scale=k_scale)
     q = c.queries(dtype, mul=mul)
     out = torch.zeros_like(q).cuda()
     plan = c.plan()
-    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out, max_rows=6)
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out, max_rows=max(news))
     c.check(out, q, dtype, 0, 128 ** -0.5)
+    plan.close()
+    c.close()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("at", [3, 250, 699])
+def test_attention_past_fp16(sess, dtype, rows, at):
+    """Values (and keys, one token on) past fp16's range, whose scales are 2^13 and more, in the first, a middle or
+    the last tile; the scores stay small through the scale."""
+    print("past fp16", dtype, rows, at, flush=True)
+    c = Case(sess, 4, 2, 128, 16, [700], [rows])
+    rng = np.random.default_rng(at)
+    for t, mk, mv in ((at, 1.0, 1e5), (min(at + 1, 698), 1e5, 1.0)):
+        k, v = (torch.tensor(rng.standard_normal((1, 2, 128)) * m, dtype=torch.float32) for m in (mk, mv))
+        c.pool.append(0, k.cuda(), v.cuda(), _i32([c.table[0, t // 16] * 16 + t % 16]))
+        c.k[0][t], c.v[0][t] = P.quantised(P.as_f64(k))[0], P.quantised(P.as_f64(v))[0]
+    q = c.queries(dtype)
+    out = torch.zeros_like(q).cuda()
+    plan = c.plan()
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out, scale=1e-6)
+    c.check(out, q, dtype, 0, 1e-6)
     plan.close()
     c.close()
 
@@ -293,11 +332,11 @@ def test_fp32_is_fp32(sess, D, rows):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("rows", [2, 40])
-def test_what_is_not_seen_does_not_matter(sess, dtype, rows):
+@pytest.mark.parametrize("rows,n", [(2, 333), (40, 333), (100, 650)])
+def test_what_is_not_seen_does_not_matter(sess, dtype, rows, n):
     """NaN blocks behind a row's position, before its window, in free pages and behind the length
     change nothing, bit for bit; where a row does see one it is NaN in that block."""
-    D, page, n, window = 128, 16, 333, 64
+    D, page, window = 128, 16, 64
     c = Case(sess, 4, 2, D, page, [n, 50], [rows, 1])
     q = c.queries(dtype).cuda()
     plan = c.plan()
