@@ -1644,20 +1644,24 @@ __global__ void k_kv4_merge(Kv4Attn a, Lines L, Pieces pc, int per) {
   __shared__ float part[16][D];
   __shared__ float pl[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if ((int)blockIdx.x >= *pc.n_items) return;
-  const Begun it = pc.begun[blockIdx.x];
+  const int items = *pc.n_items;
+  const Begun it = pc.begun[blockIdx.x];  // (of an item that is not: whatever is there)
   const int n = it.pieces;
-  if (n == 0) return;
+  if ((int)blockIdx.x >= items || n == 0) return;
   const int64_t w0 = it.w;
-  const Seq s = sequence(L, it.b);
-  const int c0 = it.ct * L.cols, cols = min(L.cols, s.m * L.group - c0);
+  const int c0 = it.ct * L.cols;
+  const int32_t* ro = L.ro + it.b;
+  const int r0 = min(max(ro[0], 0), L.rows), m = max(min(max(ro[1], 0), L.rows) - r0, 0);
   const auto slot = [&](int i, int c) { return (i == 0 ? 2 * w0 + 1 : 2 * (w0 + i)) * L.cols + c; };
   const int share = (blockDim.x >> 6) / per, mine = wave % share;  // waves a column
-  for (int at = blockIdx.y * per; at < cols; at += gridDim.y * per) {  // the same for all waves
+  // The first columns' loads do not wait for the sequence's rows: behind the last one they are joined
+  // and not written.
+  const int at0 = blockIdx.y * per;
+  for (int at = at0; at < L.cols && (at == at0 || (c0 + at) / L.group < m); at += gridDim.y * per) {  // the same for all waves
     const int c = at + wave / share;
     float acc[V] = {}, l = 0.0f;
-    if (c < cols) {
-      float m = -INFINITY;
+    {
+      float top = -INFINITY;
       for (int i0 = mine; i0 == mine || i0 < n; i0 += 8 * share) {
         float2 x[8];
         float v[8][V];
@@ -1671,14 +1675,14 @@ __global__ void k_kv4_merge(Kv4Attn a, Lines L, Pieces pc, int per) {
         if (i0 == mine) {
           for (int i = lane; i < n; i += 64) {
             const float2 y = pc.ml[slot(i, c)];
-            if (y.y != 0.0f) m = fmaxf(m, y.x);
+            if (y.y != 0.0f) top = fmaxf(top, y.x);
           }
-          m = wave_max(m);
+          top = wave_max(top);
         }
 #pragma unroll
         for (int k = 0; k < 8; k++) {
           const bool some = i0 + k * share < n && x[k].y != 0.0f;
-          const float f = some ? __builtin_amdgcn_exp2f(x[k].x - m) : 0.0f;
+          const float f = some ? __builtin_amdgcn_exp2f(x[k].x - top) : 0.0f;
           l = __builtin_fmaf(f, some ? x[k].y : 0.0f, l);
 #pragma unroll
           for (int j = 0; j < V; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
@@ -1698,9 +1702,9 @@ __global__ void k_kv4_merge(Kv4Attn a, Lines L, Pieces pc, int per) {
         }
       __syncthreads();
     }
-    if (c < cols && mine == 0) {
-      const int cc = c0 + c, r = cc / L.group;
-      T* dst = (T*)a.out.p + (int64_t)(s.r0 + r) * a.out.row + ((int64_t)it.h * L.group + cc % L.group) * a.out.head + lane * V;
+    const int cc = c0 + c, r = cc / L.group;
+    if (r < m && mine == 0) {
+      T* dst = (T*)a.out.p + (int64_t)(r0 + r) * a.out.row + ((int64_t)it.h * L.group + cc % L.group) * a.out.head + lane * V;
 #pragma unroll
       for (int j = 0; j < V; j++) dst[j] = E::put(l == 0.0f ? 0.0f : acc[j] / l);
     }
