@@ -89,7 +89,10 @@ __device__ __forceinline__ float h2f(uint16_t h) { return (float)__builtin_bit_c
 // 16 do.  K: 8 neighbours of a block (blockIdx.y 0); V: columns 2i, 2i + 1 of a block pair,
 // that is 2 neighbours at four places, so that a thread holds whole halfwords.
 //
-// Few rows take one row a thread: 128 rows of 8 heads are then 4.2 us instead of 8.8.
+// Bound by memory and, for the codes, nearly so by vector instructions: 16411 bf16 rows of 8 heads of 128
+// (86 MB) are appended in 22 us, 3.9 TB/s, and read in 17, 5.0.
+// Few rows take one row a thread: 128 fp32 rows of 8 heads are then appended in 3.4 us (four
+// rows a thread: 5.9) and read in 3.3 (5.1); the 16411 rows above would be 27 and 27.
 //
 // Codes: x / d is the product with d's reciprocal, corrected once by its residual, and adding
 // 1.5 * 2^23 rounds it to the nearest integer, ties to even, and leaves that in the low bits.
@@ -457,7 +460,7 @@ __host__ __device__ inline bool vec_rows(const Rows& r, int size) {
 template <int D, class E>
 hipError_t rows_launch(hipStream_t st, bool append, const Kv4Layer& c, int rows, const Rows& k, const Rows& v,
                        const int32_t* slots) {
-  // a row a thread while that does not fill the chip twice over; else four, the first quad
+  // a row a thread while that does not fill the chip twice over (measured above); else four, the first quad
   // beginning up to 15 rows before the first row
   const bool few = (int64_t)rows * c.n_kv * (D / 8) * 2 < (int64_t)1 << 19;
   const int quads = few ? rows : (int)(((int64_t)rows + 15 + 15) / 16) * 4;
@@ -517,6 +520,15 @@ hipError_t rows_type(hipStream_t st, bool append, const Kv4Layer& c, int dtype, 
 // lengths are.  A wave writes the output of an item that lies in its part as a
 // whole; else (O, mref, l) of its piece, and k_kv4_merge joins the pieces in
 // order.
+//
+// NT = 1 where no sequence has more than 16 columns: 128 sequences of 128 to 4608 tokens, one fp16 row of 32
+// heads each (8 kv heads of 128, 351 MB) take 80 us, 4.4 TB/s, bound by memory (loads
+// alone: 65) and vector instructions together; with NT = 2 145.  Three of 20161 to 131072 tokens, bf16
+// (261 MB): 51 us, 5.1 TB/s, and 10 for the merge; 33 of 5 to 8192 with up to six fp32 rows of 16
+// heads (157 MB) 52 and 8, bound by the second product that each of two terms needs.
+// Where a table holds no more than kWhole tiles a wave does an item by itself: one sequence of 37 tokens 9 us,
+// without the 4 of a merge.  Parts of two tiles at least, where there is little work: 16 windows of 512
+// tokens, head dim 256, 16 us (four tiles: 20, one: 14), and 16 sequences of 200 tokens 14 (15, 17).
 constexpr int kTile = 32;
 constexpr int kStart = 6;  // what beginning an item costs, in tiles
 
@@ -526,7 +538,8 @@ template <class E> struct Terms { static constexpr int n = 1; static constexpr b
 template <> struct Terms<F32> { static constexpr int n = 2; static constexpr bool ONCE = true; };
 template <> struct Terms<BF16> { static constexpr int n = 1; static constexpr bool ONCE = false; };
 
-// Waves a SIMD: what the registers of a form allow.
+// Waves a SIMD: what the registers of a form allow.  (NT = 1 with two waves and rings of four tiles: 84 us for the 80
+// above, 55 for the 51, with a merge of fewer pieces that is as much shorter.)
 constexpr int attn_waves(int hd, int nt, int terms) { return hd == 256 ? 1 : nt == 1 ? 3 : 2; }
 
 // Tiles of a wave's ring: what 160 KB of LDS hold for that many waves.
@@ -1636,7 +1649,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
 }
 
 // Joins the pieces of an item that several waves computed, in their order: a workgroup
-// an item and `per` columns (more for every gridDim.y), its waves by column and by piece.
+// an item and `per` columns (more for every gridDim.y), its waves by column and by piece.  It waits for memory
+// four times, 4 us at the least; 55 MB of a prompt's pieces take 15.
 template <int D, class E>
 __global__ void k_kv4_merge(Kv4Attn a, Lines L, Pieces pc, int per) {
   constexpr int V = D / 64;  // dims a lane
@@ -1734,7 +1748,9 @@ int compute_units() {
 
 constexpr int kPromptWaves = 8;
 constexpr int kMergeWaves = 4096;
-constexpr int kLeast = 4;     // tiles a wave takes at least
+constexpr int kWhole = 4;        // tiles of an item that one wave does, without a merge
+constexpr int kLeast = 2;        // tiles a wave takes at least
+constexpr int kPromptLeast = 4;  // and a workgroup of k_kv4_prompt
 
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -1784,7 +1800,7 @@ hipError_t attn_tiles(hipStream_t st, const Kv4Attn& a) {
   const int cols = 16 * NT;
   const int64_t cap = attn_cap(a), tiles = (cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
-  const bool whole = tiles <= kLeast;
+  const bool whole = tiles <= kWhole;
   const int64_t most = (int64_t)compute_units() * 4 * attn_waves(D, NT, Terms<E>::n);
   const int64_t want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
   const int workers = (int)((std::min(most, want) + 3) / 4 * 4), least = whole ? 1 : kLeast;
@@ -1800,11 +1816,11 @@ hipError_t attn_prompt(hipStream_t st, const Kv4Attn& a) {
   constexpr int cols = 32 * kPromptWaves;
   const int64_t cap = attn_cap(a), tiles = (cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
-  const int64_t most = (int64_t)compute_units() * (8 / kPromptWaves), want = (items * (tiles + kPromptStart) + kLeast - 1) / kLeast;
+  const int64_t most = (int64_t)compute_units() * (8 / kPromptWaves), want = (items * (tiles + kPromptStart) + kPromptLeast - 1) / kPromptLeast;
   const int workers = (int)std::min(most, want);
   const Pieces pc = pieces_in(a.ws, items, workers, cols);
   hipLaunchKernelGGL((k_kv4_prompt<kPromptWaves, E>), dim3((unsigned)workers), dim3(64 * kPromptWaves), 0, st, a, a.row_offsets, a.lengths,
-                     a.page_table, a.c.base, pc, workers, kLeast);
+                     a.page_table, a.c.base, pc, workers, kPromptLeast);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess ? e : merge<128, E>(st, a, pc, items, workers, cols, cap, kPromptStart);
 }
