@@ -391,7 +391,7 @@ enum { RSTR_F32 = 0, RSTR_F16 = 1, RSTR_BF16 = 2 };
 /* A paged K/V cache in 4 bits: blocks of 32 consecutive elements of a head's row,
  * each an fp16 scale d and 32 codes that stand for d * (code - 8): 4.5 bits an
  * element.  head_dim 64, 128 or 256; page_size a multiple of 16;
- * physical_pages * page_size < 2^31.  All zeros when opened.  The layout inside
+ * physical_pages * page_size < 2^31, a page of all heads below 2 GB.  All zeros when opened.  The layout inside
  * a page is the library's own: rows go in and out through append and read. */
 int rstr_kv4_open(rstr_session* s, int32_t n_layers, int32_t n_kv, int32_t head_dim, int32_t page_size,
                   int32_t physical_pages, rstr_kv4** out);
@@ -424,7 +424,8 @@ int rstr_kv4_attn_close(rstr_kv4_attn* a);
  * (these included) in the pages page_table[b][0 .. pages_per_seq).  The row at
  * token p sees the tokens j <= p, and with window > 0 only j > p - window:
  * out = sum softmax(scale * q . k_j) v_j, in the type of q (f32: products and sums
- * in fp32 precision; f16, bf16: probabilities rounded to 11 bits).  A row that
+ * in fp32 precision; f16, bf16: probabilities, and their products with values, rounded to
+ * 11 bits; bf16 and many rows: keys too).  A row that
  * sees no token (length 0, more rows than tokens) is 0.  Tokens of a page id outside
  * the cache are not seen, nor are tokens behind the table's width.  Rows behind
  * row_offsets[batch] are left as they are; row_offsets must not decrease.
@@ -442,7 +443,8 @@ int rstr_kv4_attn_run(rstr_kv4_attn* a, int32_t layer, int32_t dtype, int32_t ba
  * pages_per_seq, the list lasts (one that needs no new page is served after it
  * has run out) and its rows fit `rows`; otherwise it keeps its length and has no rows.
  * Writes new_lengths[batch], row_offsets[batch+1] (of the rows served),
- * positions[rows] and slots[rows] (0 and -1 behind the last row; positions
+ * positions[rows] and slots[rows] (0 and -1 behind the last row, and -1 for a page id
+ * below 0 or whose slot does not fit in 31 bits; positions
  * include start_positions[batch] where given) and pages_taken[0], the length of the
  * list's part that is used up.  Outputs may not overlap inputs.  batch up to
  * RSTR_STEP_MAPS_BATCH. */

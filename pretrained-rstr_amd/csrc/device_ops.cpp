@@ -111,7 +111,8 @@ extern "C" int rstr_kv4_open(rstr_session* s, int32_t n_layers, int32_t n_kv, in
   if (!kv4_head_dim(head_dim)) return fail(s, RSTR_E_INVALID, "4-bit cache head dim must be 64, 128 or 256");
   if (page_size % 16) return fail(s, RSTR_E_INVALID, "4-bit cache page size must be a multiple of 16");
   if ((int64_t)page_size * physical_pages > 0x7FFFFFFF) return fail(s, RSTR_E_INVALID, "4-bit cache slots must fit in 31 bits");
-  if ((double)kv4_record_bytes(head_dim, page_size) * n_kv > 4e9) return fail(s, RSTR_E_INVALID, "4-bit cache pages must be smaller than 4 GB");
+  // offsets inside a page are 32 bits
+  if ((double)kv4_record_bytes(head_dim, page_size) * n_kv > 2e9) return fail(s, RSTR_E_INVALID, "4-bit cache pages must be smaller than 2 GB");
   std::unique_ptr<rstr_kv4> p(new (std::nothrow) rstr_kv4());
   if (!p) return fail(s, RSTR_E_OOM, "4-bit cache handle");
   p->s = s;
@@ -202,6 +203,7 @@ extern "C" int rstr_kv4_attn_open(rstr_kv4* p, int32_t n_q, int32_t max_batch, i
   *out = nullptr;
   if (n_q <= 0 || n_q % p->n_kv) return fail(s, RSTR_E_INVALID, "query heads must be a multiple of the cache's kv heads");
   if (max_batch <= 0 || max_rows <= 0) return fail(s, RSTR_E_INVALID, "attention plan extents must be positive");
+  if ((int64_t)max_rows * n_q > 0x7FFFF000) return fail(s, RSTR_E_INVALID, "attention plan has too many rows");
   std::unique_ptr<rstr_kv4_attn> a(new (std::nothrow) rstr_kv4_attn());
   if (!a) return fail(s, RSTR_E_OOM, "attention plan handle");
   OnDevice dev(s->device);
@@ -380,6 +382,10 @@ extern "C" int rstr_verify_run(rstr_verify* v, int32_t dtype, int32_t batch, int
     for (const auto& x2 : in)
       if (ranges_meet(x2.p, x2.n, accepted, n) || ranges_meet(x2.p, x2.n, tokens, r))
         return fail(s, RSTR_E_INVALID, "verification outputs overlap its inputs");
+    const uintptr_t x1 = rows_end(x, rows, 1, v->vocab, size);
+    if (ranges_meet((uintptr_t)logits, x1, (uintptr_t)accepted, (uintptr_t)accepted + n) ||
+        ranges_meet((uintptr_t)logits, x1, (uintptr_t)tokens, (uintptr_t)tokens + r))
+      return fail(s, RSTR_E_INVALID, "verification outputs overlap its inputs");
     if (ranges_meet(accepted, n, tokens, r)) return fail(s, RSTR_E_INVALID, "verification outputs overlap");
   }
   Verify a{batch, rows, v->vocab, logits, logits_row, row_offsets, drafts, draft_probs, probs_row, temperature,

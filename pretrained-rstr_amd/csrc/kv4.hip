@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "../../include/rstr_hip.h"
@@ -802,6 +803,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 
     // the columns' rows and what they see
     const int c0 = ct * COLS, p0 = s.len - s.m;
+    const auto first_seen = [&](int r) { return a.window > 0 ? max(max(p0 + r + 1, 0) - a.window, 0) : 0; };
     const int rf = c0 / group, rl = min(s.m - 1, (c0 + COLS - 1) / group);
     int hi[NT], lo[NT];
     int64_t qrow[NT], qhead[NT];
@@ -811,12 +813,12 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
       const int cc = c0 + t * 16 + col, r = cc / group;
       valid[t] = r < s.m;
       hi[t] = valid[t] ? max(p0 + r + 1, 0) : 0;
-      lo[t] = a.window > 0 ? max(p0 + r + 1 - a.window, 0) : 0;
+      lo[t] = first_seen(r);
       qrow[t] = s.r0 + r;
       qhead[t] = (int64_t)h * group + (cc - r * group);
     }
     const int hi_last = max(p0 + rl + 1, 0), hi_first = max(p0 + rf + 1, 0);
-    const int lo_first = a.window > 0 ? max(p0 + rf + 1 - a.window, 0) : 0, lo_last = a.window > 0 ? max(p0 + rl + 1 - a.window, 0) : 0;
+    const int lo_first = first_seen(rf), lo_last = first_seen(rl);
     int t0 = s.lo + (whole ? 0 : max(at - kStart, 0)), t1 = s.lo + (whole ? s.tiles : max(at + n - kStart, 0));
     t0 = max(t0, lo_first / kTile);
     t1 = min(t1, (hi_last + kTile - 1) / kTile);
@@ -831,7 +833,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
     for (int t = 0; t < NT; t++) {
 #pragma unroll
       for (int i = 0; i < 2 * NB; i++) acc[t][i] = f4{0, 0, 0, 0};
-      mref[t] = -1e30f;
+      mref[t] = -FLT_MAX;
       l[t] = f4{0, 0, 0, 0};
       elim[t] = TERMS == 1 ? 15 : 0;
       fs[t] = __builtin_amdgcn_ldexpf(1.0f, 15 - elim[t]);
@@ -1057,12 +1059,13 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
           bool big = false;
 #pragma unroll
           for (int t = 0; t < NT; t++) {
-            float m = -INFINITY;
+            float m = -INFINITY, over = e2[t][0];
             int e = exps[t];
             if (e > 15) e = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
               const bool ok = (see[t] >> i) & 1;
+              over = fmaxf(over, e2[t][i]);
               if (ok) m = fmaxf(m, sc[t][i] * kcol[t]);
               if (exps[t] > 15 && ok)
 #pragma unroll
@@ -1072,12 +1075,15 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
                 }
             }
             m = xor_max<32>(xor_max<16>(m));
+            over = xor_max<32>(xor_max<16>(over));
             e = max(e, elim[t]);
             e = max(e, __shfl_xor(e, 16, 64));
             e = max(e, __shfl_xor(e, 32, 64));
             if (e <= 15) { e |= e >> 1; e |= e >> 2; }
-            // a column that needs no change has none: it does not depend on its neighbours
-            const float now = m - mref[t] > 14.0f ? m - 10.0f : mref[t];
+            // A column that needs no change has none: it does not depend on its neighbours.  One that does
+            // takes differences of rounded scores, which stay below 14 however large the scores are.
+            const bool own = over > 14.0f;
+            const float now = own && m - mref[t] > 14.0f ? m - 10.0f : mref[t];
             const float keep = __builtin_amdgcn_exp2f(mref[t] - now);
             mref[t] = now;
             l[t] *= keep;
@@ -1088,7 +1094,8 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) acc[t][i] *= less;
 #pragma unroll
-            for (int i = 0; i < 8; i++) e2[t][i] = (see[t] >> i) & 1 ? __builtin_fmaf(sc[t][i], kcol[t], -mref[t]) : -INFINITY;
+            for (int i = 0; i < 8; i++)
+              e2[t][i] = !((see[t] >> i) & 1) ? -INFINITY : own ? sc[t][i] * kcol[t] - mref[t] : __builtin_fmaf(sc[t][i], kcol[t], -mref[t]);
           }
           scaled = __ballot(big) != 0;
         }
@@ -1281,14 +1288,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       const int row = cc / group;
       return Column{row, h * group + (cc - row * group)};
     };
+    const auto first_seen = [&](int row) { return a.window > 0 ? max(max(p0 + row + 1, 0) - a.window, 0) : 0; };
     int hi[NT], lo[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const int row = column(t).row;
       hi[t] = row < s.m ? max(p0 + row + 1, 0) : 0;
-      lo[t] = a.window > 0 ? max(p0 + row + 1 - a.window, 0) : 0;
+      lo[t] = first_seen(row);
     }
-    const auto first_seen = [&](int row) { return a.window > 0 ? max(p0 + row + 1 - a.window, 0) : 0; };
     const auto end_seen = [&](int row) { return max(p0 + row + 1, 0); };
     const int t0 = max(s.lo + max(line.at - kPromptStart, 0), first_seen(rf) / kTile);
     const int t1 = min(s.lo + max(line.at + line.n - kPromptStart, 0), (end_seen(rl) + kTile - 1) / kTile);
@@ -1304,7 +1311,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
 #pragma unroll
       for (int i = 0; i < 2 * NB; i++) acc[t][i] = f4{0, 0, 0, 0};
       l[t] = f4{0, 0, 0, 0};
-      mref[t] = -1e30f;
+      mref[t] = -FLT_MAX;
       kcol[t] = 0.0f;
     }
     if (t0 < t1) {
@@ -1525,19 +1532,24 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
 #pragma unroll
             for (int t = 0; t < NT; t++) {
               asm volatile("" : "+v"(see[t]));  // its bits are looked at here only
-              float m = -INFINITY;
+              float m = -INFINITY, over = e2[t][0];
 #pragma unroll
-              for (int i = 0; i < 8; i++)
+              for (int i = 0; i < 8; i++) {
+                over = fmaxf(over, e2[t][i]);
                 if ((see[t] >> i) & 1) m = fmaxf(m, sc[t][i] * kcol[t]);
+              }
               m = xor_max<32>(xor_max<16>(m));
-              const float now = m - mref[t] > 14.0f ? m - 10.0f : mref[t];
+              over = xor_max<32>(xor_max<16>(over));
+              const bool own = over > 14.0f;  // (as in k_kv4_attn)
+              const float now = own && m - mref[t] > 14.0f ? m - 10.0f : mref[t];
               const float keep = __builtin_amdgcn_exp2f(mref[t] - now);
               mref[t] = now;
               l[t] *= keep;
 #pragma unroll
               for (int i = 0; i < 2 * NB; i++) acc[t][i] *= keep;
 #pragma unroll
-              for (int i = 0; i < 8; i++) e2[t][i] = (see[t] >> i) & 1 ? __builtin_fmaf(sc[t][i], kcol[t], -mref[t]) : -INFINITY;
+              for (int i = 0; i < 8; i++)
+                e2[t][i] = !((see[t] >> i) & 1) ? -INFINITY : own ? sc[t][i] * kcol[t] - mref[t] : __builtin_fmaf(sc[t][i], kcol[t], -mref[t]);
             }
           }
           h8 p[NT];

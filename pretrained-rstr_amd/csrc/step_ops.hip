@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(kMapsThreads) k_step_maps(StepMaps a) {
       const int old = pages_of((uint32_t)have), pg = (int)((uint32_t)t / (uint32_t)a.page_size);
       const int page = pg < old ? a.page_table[(int64_t)b * a.pps + pg] : a.free_pages[page0[b] + (pg - old)];
       pos = t + (a.starts ? a.starts[b] : 0);
-      slot = page < 0 ? -1 : page * a.page_size + (t - pg * a.page_size);
+      const int64_t at = (int64_t)page * a.page_size + (t - pg * a.page_size);
+      slot = at < 0 || at > 0x7FFFFFFF ? -1 : (int)at;
     }
     a.positions[i] = pos;
     a.slots[i] = slot;

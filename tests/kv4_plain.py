@@ -83,6 +83,7 @@ def step_maps(page, lengths, counts, starts, free, table, rows):
             i = offs[-1] + t - n
             positions[i] = (starts[b] if starts is not None else 0) + t
             slots[i] = table[b, t // page] * page + t % page if table[b, t // page] >= 0 else -1
+            slots[i] = slots[i] if slots[i] < 2 ** 31 else -1
         offs.append(offs[-1] + m)
         new.append(n + m)
     return dict(table=table, new_lengths=new, offsets=offs, positions=positions, slots=slots, taken=[taken])

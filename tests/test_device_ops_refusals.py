@@ -78,7 +78,7 @@ def test_cache_open(dev):
     with hip.Session(0) as s:
         for args, match in (((0, 2, 128, 16, 4), "extents"), ((1, 0, 128, 16, 4), "extents"), ((1, 2, 128, 0, 4), "extents"),
                             ((1, 2, 128, 16, 0), "extents"), ((1, 2, 96, 16, 4), "head dim"), ((1, 2, 128, 24, 4), "multiple of 16"),
-                            ((1, 2, 128, 1 << 16, 1 << 15), "31 bits")):
+                            ((1, 2, 128, 1 << 16, 1 << 15), "31 bits"), ((1, 2, 64, 1 << 24, 1), "2 GB")):
             with pytest.raises(hip.RstrError, match=match) as e:
                 hip.Kv4Pool(s, *args)
             assert e.value.code == -1
@@ -105,6 +105,8 @@ def test_cache_open(dev):
             q = hip.Kv4Pool(s, 1, 2, 64, 16, 4)
             with pytest.raises(hip.RstrError, match="query heads"):
                 hip.Kv4Attention(q, n_q, 2, 5)
+            with pytest.raises(hip.RstrError, match="too many rows"):
+                hip.Kv4Attention(q, 64, 1, 1 << 26)
         with pytest.raises(hip.RstrError, match="vocabulary"):
             hip.Verifier(s, 1, 1, (1 << 24) + 1)
     assert dev.fake_blocks() == blocks
@@ -241,6 +243,11 @@ def test_verify(dev):
         refused(dev, hip.RstrError, "batch exceeds", lambda: run(row_offsets=ints(4), temperature=Dev((3,)), u_sample=Dev((3,)), accepted=ints(3)))
         refused(dev, hip.RstrError, "rows exceed", lambda: run(logits=Dev((6, 100)), drafts=ints(6), u_accept=Dev((6,)), tokens=ints(6)))
         refused(dev, hip.RstrError, "overlap", lambda: run(tokens=base["drafts"]))
+        for name in ("tokens", "accepted"):   # inside the logits' last row
+            x = Dev((5, 100))
+            inside = ints(5 if name == "tokens" else 2)
+            inside._keep, inside._shift = x._keep, 4 * 499
+            refused(dev, hip.RstrError, "overlap", lambda: run(logits=x, **{name: inside}))
         refused(dev, hip.RstrError, "aligned", lambda: run(logits=Dev((5, 100), shift=2)))
         for match, kw in (("shape", dict(logits=Dev((5, 99)))), ("last dimension", dict(logits=Dev((5, 100), strides=(200, 2)))),
                           ("must be float32", dict(draft_probs=Dev((5, 100), "float16"))), ("float32", dict(temperature=Dev((2,), "float16"))),

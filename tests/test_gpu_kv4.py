@@ -233,6 +233,10 @@ SHAPES = [
     (4, 2, 128, 16, [64, 300, 64], [0, 130, 0], 0),
     (8, 8, 128, 16, [900, 31, 290], [64, 31, 100], 1),
     (8, 1, 128, 32, [2000], [300], 0),
+    # the largest window there is, and rows before the first token
+    (2, 2, 128, 16, [5, 0, 3], [9, 4, 2], 2 ** 31 - 1),
+    (4, 2, 128, 16, [5, 700], [70, 3], 2 ** 31 - 1),
+    (4, 1, 256, 16, [30], [40], 2 ** 31 - 2),
 ]
 
 
@@ -306,6 +310,28 @@ def test_attention_past_fp16(sess, dtype, rows, at):
     plan = c.plan()
     plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out, scale=1e-6)
     c.check(out, q, dtype, 0, 1e-6)
+    plan.close()
+    c.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,D", [(1, 128), (40, 64), (70, 128), (3, 256)])
+def test_scores_far_below_zero(sess, dtype, rows, D):
+    """Scores from -1e34 down: the softmax is 1 at the largest, token 0, whose value is the output (rounded at
+    most twice to 11 bits and once to the output's type)."""
+    print("far below zero", dtype, rows, D, flush=True)
+    n = 300
+    c = Case(sess, 4, 2, D, 16, [n], [rows])
+    k = torch.arange(1, n + 1, dtype=torch.float32)[:, None, None].expand(n, 2, D).contiguous()
+    v = torch.tensor(c.rng.standard_normal((n, 2, D)), dtype=torch.float32)
+    c.pool.append(0, k.cuda(), v.cuda(), _i32(c.table[0, np.arange(n) // 16] * 16 + np.arange(n) % 16))
+    q = torch.full((rows, 4, D), -1e32).to(TYPES[dtype])
+    out = torch.zeros_like(q).cuda()
+    plan = c.plan()
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out)
+    want = np.repeat(P.quantised(P.as_f64(v[:1]))[0], 2, axis=0)
+    tol = (2.0 ** -10 if dtype != "f32" else 2.0 ** -21) + torch.finfo(TYPES[dtype]).eps / 2 * 1.01
+    assert (np.abs(P.as_f64(out) - want) <= tol * np.abs(want)).all()
     plan.close()
     c.close()
 

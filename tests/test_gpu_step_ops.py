@@ -58,6 +58,18 @@ def test_step_maps(sess, B, hi, new, page, free, slack):
         assert np.array_equal(got[name].cpu().numpy(), np.asarray(want[name]).reshape(got[name].shape)), name
 
 
+def test_step_maps_slots_past_31_bits(sess):
+    """Page ids whose slots do not fit are no slots: none wraps round to another page's."""
+    page, top = 48, 2 ** 31 - 1
+    table = np.array([[top, 3, 0, 0], [top // page, 0, 0, 0], [top // page + 1, 0, 0, 0], [-(2 ** 31), 0, 0, 0]])
+    lengths, counts, free = np.array([40, 20, 47, 5]), np.array([20, 30, 2, 3]), np.array([top, 2, 2 ** 28])
+    got = _maps(sess, page, lengths, counts, free, table, 60)
+    want = P.step_maps(page, lengths, counts, None, free, table, 60)
+    for name in want:
+        assert np.array_equal(got[name].cpu().numpy(), np.asarray(want[name]).reshape(got[name].shape)), name
+    assert -1 in want["slots"][:55] and max(want["slots"]) > 2 ** 31 - 100
+
+
 def test_step_maps_graph_and_loop(sess):
     """A captured call advances the tables step after step, its lengths fed back."""
     B, page, width = 40, 16, 30
