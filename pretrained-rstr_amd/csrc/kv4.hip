@@ -707,6 +707,12 @@ struct Line {
   }
 };
 
+// Is a lane of the own column among these?
+__device__ __forceinline__ bool of_column(uint64_t lanes) {
+  lanes |= lanes >> 32;
+  return ((lanes | lanes >> 16) >> (threadIdx.x & 15)) & 1;
+}
+
 template <int N>
 __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t* o) {
   if constexpr (N == 2) {
@@ -1047,25 +1053,25 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
           }
         }
         // does a score pass what mref allows, or a scale of V what fs does?
-        bool grow = false;
+        bool grow = false, passed[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
           float m = e2[t][0];
 #pragma unroll
           for (int i = 1; i < 8; i++) m = fmaxf(m, e2[t][i]);
-          grow |= m > 14.0f || exps[t] > elim[t];
+          passed[t] = m > 14.0f;
+          grow |= passed[t] || exps[t] > elim[t];
         }
         if (__ballot(grow)) {
           bool big = false;
 #pragma unroll
           for (int t = 0; t < NT; t++) {
-            float m = -INFINITY, over = e2[t][0];
+            float m = -INFINITY;
             int e = exps[t];
             if (e > 15) e = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
               const bool ok = (see[t] >> i) & 1;
-              over = fmaxf(over, e2[t][i]);
               if (ok) m = fmaxf(m, sc[t][i] * kcol[t]);
               if (exps[t] > 15 && ok)
 #pragma unroll
@@ -1075,14 +1081,13 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
                 }
             }
             m = xor_max<32>(xor_max<16>(m));
-            over = xor_max<32>(xor_max<16>(over));
             e = max(e, elim[t]);
             e = max(e, __shfl_xor(e, 16, 64));
             e = max(e, __shfl_xor(e, 32, 64));
             if (e <= 15) { e |= e >> 1; e |= e >> 2; }
             // A column that needs no change has none: it does not depend on its neighbours.  One that does
             // takes differences of rounded scores, which stay below 14 however large the scores are.
-            const bool own = over > 14.0f;
+            const bool own = of_column(__ballot(passed[t]));
             const float now = own && m - mref[t] > 14.0f ? m - 10.0f : mref[t];
             const float keep = __builtin_amdgcn_exp2f(mref[t] - now);
             mref[t] = now;
@@ -1095,7 +1100,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
             for (int i = 0; i < 2 * NB; i++) acc[t][i] *= less;
 #pragma unroll
             for (int i = 0; i < 8; i++)
-              e2[t][i] = !((see[t] >> i) & 1) ? -INFINITY : own ? sc[t][i] * kcol[t] - mref[t] : __builtin_fmaf(sc[t][i], kcol[t], -mref[t]);
+              if (own) e2[t][i] = (see[t] >> i) & 1 ? sc[t][i] * kcol[t] - mref[t] : -INFINITY;
           }
           scaled = __ballot(big) != 0;
         }
@@ -1501,7 +1506,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
           asm volatile("" ::: "memory");  // these loads run while the weights are computed
           uint32_t see[NT];
           float e2[NT][8];
-          bool grow = false;
+          bool grow = false, passed[NT];
 #pragma unroll
           for (int t = 0; t < NT; t++) {
             see[t] = 0xFF;
@@ -1526,21 +1531,19 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
             float m = e2[t][0];
 #pragma unroll
             for (int i = 1; i < 8; i++) m = fmaxf(m, e2[t][i]);
-            grow |= m > 14.0f;
+            passed[t] = m > 14.0f;
+            grow |= passed[t];
           }
           if (__ballot(grow)) {
 #pragma unroll
             for (int t = 0; t < NT; t++) {
               asm volatile("" : "+v"(see[t]));  // its bits are looked at here only
-              float m = -INFINITY, over = e2[t][0];
+              float m = -INFINITY;
 #pragma unroll
-              for (int i = 0; i < 8; i++) {
-                over = fmaxf(over, e2[t][i]);
+              for (int i = 0; i < 8; i++)
                 if ((see[t] >> i) & 1) m = fmaxf(m, sc[t][i] * kcol[t]);
-              }
               m = xor_max<32>(xor_max<16>(m));
-              over = xor_max<32>(xor_max<16>(over));
-              const bool own = over > 14.0f;  // (as in k_kv4_attn)
+              const bool own = of_column(__ballot(passed[t]));  // (as in k_kv4_attn)
               const float now = own && m - mref[t] > 14.0f ? m - 10.0f : mref[t];
               const float keep = __builtin_amdgcn_exp2f(mref[t] - now);
               mref[t] = now;
@@ -1549,7 +1552,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
               for (int i = 0; i < 2 * NB; i++) acc[t][i] *= keep;
 #pragma unroll
               for (int i = 0; i < 8; i++)
-                e2[t][i] = !((see[t] >> i) & 1) ? -INFINITY : own ? sc[t][i] * kcol[t] - mref[t] : __builtin_fmaf(sc[t][i], kcol[t], -mref[t]);
+                if (own) e2[t][i] = (see[t] >> i) & 1 ? sc[t][i] * kcol[t] - mref[t] : -INFINITY;
             }
           }
           h8 p[NT];
