@@ -572,30 +572,32 @@ __device__ __forceinline__ Seq sequence(const Lines& L, int b) {
   return s;
 }
 
-__device__ __forceinline__ int64_t shfl64(int64_t v, int lane) { return __shfl((long long)v, lane, 64); }
-__device__ __forceinline__ int64_t wave_sum_i64(int64_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor((long long)v, d, 64);
-  return v;
+// The value of one lane, the same for all.
+__device__ __forceinline__ int64_t lane64(int64_t v, int lane) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
 }
 __device__ __forceinline__ int wave_sum_i32(int v) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
   return v;
 }
+// Inclusive sums over the lanes, without the LDS crossbar: within rows of 16 lanes, then rows' last
+// lanes into the rows behind them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp_i64(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ int64_t wave_scan_i64(int64_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up((long long)v, d, 64);
-    if (lane >= d) v += o;
-  }
-  return v;
+  v += dpp_i64<0x111, 0xF>(v);
+  v += dpp_i64<0x112, 0xF>(v);
+  v += dpp_i64<0x114, 0xF>(v);
+  v += dpp_i64<0x118, 0xF>(v);
+  v += dpp_i64<0x142, 0xA>(v);
+  return v + dpp_i64<0x143, 0xC>(v);
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
-}
 
 // Pieces of items that several waves share: two a wave (the end of an item
 // that an earlier wave began, the beginning of one that later waves end).  The wave
@@ -621,7 +623,7 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 // 64 at a time, one a lane.
 struct Line {
   const Lines& L;
-  int batch, w, items;  // items: of the call
+  int batch, w;
   int64_t part, u, u_end;
   // the part that next() came to: its item, and n of the item's units from `at` on
   Seq s;
@@ -630,34 +632,38 @@ struct Line {
 
   __device__ __forceinline__ Line(const Lines& lines, int n_seqs, int worker, int workers, int least) : L(lines), batch(n_seqs), w(worker) {
     seqs = chunk_of(0);
-    int64_t mine = seqs.units;
-    items = L.n_kv * seqs.nct;
-    for (int i = 64; i < batch; i += 64) {
-      const Seq x = chunk_of(i);
-      mine += x.units;
-      items += L.n_kv * x.nct;
+    int64_t in = wave_scan_i64(seqs.units), total = lane64(in, 63);
+    if (batch > 64) {
+      int64_t mine = 0;
+      for (int i = 64; i < batch; i += 64) mine += chunk_of(i).units;
+      total += lane64(wave_scan_i64(mine), 63);
     }
-    items = wave_sum_i32(items);
-    const int64_t total = uniform64(wave_sum_i64(mine));
     part = quotient(total + workers - 1, workers);
     part = part > least ? part : least;
     u = (int64_t)w * part;
     u_end = min(u + part, total);
     if (u >= u_end) return;
     for (int64_t run = 0;;) {
-      const int64_t in = wave_scan_i64(seqs.units);
       const uint64_t over = __ballot(run + in > u);
       const int f = over ? __ffsll((unsigned long long)over) - 1 : 64;
-      item0 = uniform(item0 + wave_sum_i32((int)(threadIdx.x & 63) < f ? L.n_kv * seqs.nct : 0));
+      if (!L.whole && (f > 0)) item0 = uniform(item0 + wave_sum_i32((int)(threadIdx.x & 63) < f ? L.n_kv * seqs.nct : 0));
       if (over) {
-        first = uniform64(run + shfl64(in - seqs.units, f));
         at_seq = uniform(f);
+        first = run + lane64(in - seqs.units, at_seq);
         return;
       }
-      run += shfl64(in, 63);
+      run += lane64(in, 63);
       b0 += 64;
       seqs = chunk_of(b0);
+      in = wave_scan_i64(seqs.units);
     }
+  }
+
+  // Items of the call.
+  __device__ __forceinline__ int items() const {
+    int n = 0;
+    for (int i = 0; i < batch; i += 64) n += L.n_kv * chunk_of(i).nct;
+    return wave_sum_i32(n);
   }
 
   __device__ __forceinline__ bool next() {
@@ -790,7 +796,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), kStart, whole};
 
   Line line(L, a.batch, w, workers, least);
-  if (w == 0 && !whole && lane == 0) *pc.n_items = line.items;
+  if (w == 0 && !whole) *pc.n_items = line.items();
 
   typedef Ring<D> G;
   __shared__ __attribute__((aligned(16))) uint8_t rings[4][NS][G::TILE];
@@ -1266,7 +1272,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
   const int w = blockIdx.x, group = a.n_q / a.c.n_kv, ps = a.c.page_size;
   const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), kPromptStart, false};
   Line line(L, a.batch, w, workers, least);
-  if (w == 0 && threadIdx.x == 0) *pc.n_items = line.items;
+  if (w == 0 && wave == 0) *pc.n_items = line.items();
 
   const int64_t rec = kv4_record_bytes(D, ps);
   const uint32_t page_bytes = (uint32_t)(a.c.n_kv * rec);
