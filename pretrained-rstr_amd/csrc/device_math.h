@@ -195,4 +195,32 @@ __device__ __forceinline__ float group_max(float v) {
 }
 __device__ __forceinline__ float wave_max(float v) { return group_max<64>(v); }
 
+// Inclusive sums over the lanes, without the LDS crossbar: within rows of 16 lanes, then rows' last
+// lanes into the rows behind them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp_i64(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int64_t wave_scan_i64(int64_t v) {
+  v += dpp_i64<0x111, 0xF>(v);
+  v += dpp_i64<0x112, 0xF>(v);
+  v += dpp_i64<0x114, 0xF>(v);
+  v += dpp_i64<0x118, 0xF>(v);
+  v += dpp_i64<0x142, 0xA>(v);
+  return v + dpp_i64<0x143, 0xC>(v);
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
+  const auto add = [&](int64_t o) { v += __builtin_bit_cast(double, o); };
+  const auto bits = [&] { return __builtin_bit_cast(int64_t, v); };
+  add(dpp_i64<0x111, 0xF>(bits()));
+  add(dpp_i64<0x112, 0xF>(bits()));
+  add(dpp_i64<0x114, 0xF>(bits()));
+  add(dpp_i64<0x118, 0xF>(bits()));
+  add(dpp_i64<0x142, 0xA>(bits()));
+  add(dpp_i64<0x143, 0xC>(bits()));
+  return v;
+}
+
 }  // namespace rstr

@@ -23,11 +23,7 @@ constexpr int kMapsThreads = 512;
 // Inclusive sum over the workgroup's threads; `tmp` holds one value a wave.
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* tmp, int64_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
+  v = wave_scan_i64(v);
   if (lane == 63) tmp[wave] = v;
   __syncthreads();
   int64_t before = 0, all = 0;
@@ -467,6 +463,9 @@ template <class E>
 __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* __restrict__ stats, const SeqPick* __restrict__ picks,
                                                       const double* __restrict__ sums, int chunks) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // the first 64 chunks' sums (most vocabularies have no more), asked for beside the pick
+  const double* c = sums + (int64_t)b * chunks;
+  const double c0 = lane < chunks ? c[lane] : 0.0;
   SeqPick s = picks[b];
   if (s.row < 0) return;
   if (s.greedy >= 0) {
@@ -475,11 +474,9 @@ __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* _
   }
   __shared__ double wsum[kVT / 64], target, before;
   __shared__ int chosen, last, found;
-  const double* c = sums + (int64_t)b * chunks;
   bool plain = false;  // nothing is left of p - q: the token comes from p
   if (wave == 0) {
-    // the first 64 chunks' sums stay in registers: most vocabularies have no more
-    const double c0 = lane < chunks ? c[lane] : 0.0;
+    const double u = (double)a.u_sample[b];
     double total = c0;
     for (int i = lane + 64; i < chunks; i += 64) total += c[i];
     total = wave_sum64(total);
@@ -490,18 +487,13 @@ __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* _
       return st[i].sum > 0.0 ? st[i].sum * pow2(((double)st[i].top - s.top) * s.scale) : 0.0;
     };
     if (plain) total = s.z;
-    const double t = (double)a.u_sample[b] * total;
+    const double t = u * total;
     double run = 0.0, b4 = 0.0;
     int pickc = -1, lastc = 0;
     double lastb = 0.0;
     for (int i0 = 0; i0 < chunks && pickc < 0; i0 += 64) {
       const double w = i0 + lane < chunks ? mass(i0 + lane) : 0.0;
-      double in = w;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(in, d, 64);
-        if (lane >= d) in += o;
-      }
+      const double in = wave_scan_f64(w);
       const uint64_t over = __ballot(w > 0.0 && run + in > t), some = __ballot(w > 0.0);
       if (over) {
         const int f = __ffsll((unsigned long long)over) - 1;
@@ -535,12 +527,7 @@ __global__ void __launch_bounds__(kVT) k_verify_token(Verify a, const RowStat* _
     w[i] = v0 + i < v1 ? weight(s, x[i], s.from_probs ? q[i] : 0.0f, v0 + i) : 0.0;
     sum += w[i];
   }
-  double in = sum;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double o = __shfl_up(in, d, 64);
-    if (lane >= d) in += o;
-  }
+  const double in = wave_scan_f64(sum);
   if (lane == 63) wsum[wave] = in;
   __syncthreads();
   double run = before + (in - sum);
