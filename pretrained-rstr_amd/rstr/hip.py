@@ -822,7 +822,7 @@ class Kv4Attention:
             raise ValueError("q and out must have the same element type")
         width = page_table.shape[1]
         s.check(lib().rstr_kv4_attn_run(
-            self.h, layer, t, batch, rows, rows if max_rows is None else max_rows, window, hd ** -0.5 if scale is None else scale,
+            self.h, layer, t, batch, rows, rows if max_rows is None else max_rows, min(window, 0x7FFFFFFF), hd ** -0.5 if scale is None else scale,
             qp, qr, qh, _ints(s, row_offsets, "row_offsets", (batch + 1,)), _ints(s, page_table, "page_table", (batch, width)),
             width, _ints(s, lengths, "lengths", (batch,)), op, orow, oh, _stream(s, stream)))
 

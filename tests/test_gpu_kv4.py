@@ -237,6 +237,7 @@ SHAPES = [
     (2, 2, 128, 16, [5, 0, 3], [9, 4, 2], 2 ** 31 - 1),
     (4, 2, 128, 16, [5, 700], [70, 3], 2 ** 31 - 1),
     (4, 1, 256, 16, [30], [40], 2 ** 31 - 2),
+    (2, 2, 64, 16, [40], [3], 2 ** 32 + 5),
 ]
 
 
@@ -487,10 +488,11 @@ def test_long_context(sess):
     pool.close()
 
 
-def test_streams_and_graphs(sess):
+@pytest.mark.parametrize("lens,news", [([400, 90, 3], [2, 1, 1]), ([400, 300], [60, 40])])
+def test_streams_and_graphs(sess, lens, news):
     """Captured calls replay on changed inputs between eager calls; two plans run side by side on
     two streams; the session's own stream takes calls too."""
-    c = Case(sess, 8, 2, 128, 16, [400, 90, 3], [2, 1, 1])
+    c = Case(sess, 8, 2, 128, 16, lens, news)
     q = c.queries("f16").cuda()
     args = (_i32(c.offsets), _i32(c.table), _i32(c.lens))
     plans = [c.plan() for _ in range(3)]
