@@ -527,7 +527,7 @@ hipError_t rows_type(hipStream_t st, bool append, const Kv4Layer& c, int dtype, 
 // alone: 65) and vector instructions together; with NT = 2 145.  Three of 20161 to 131072 tokens, bf16
 // (261 MB): 51 us, 5.1 TB/s, and 10 for the merge; 33 of 5 to 8192 with up to six fp32 rows of 16
 // heads (157 MB) 52 and 8, bound by the second product that each of two terms needs.
-// Where a table holds no more than kWhole tiles a wave does an item by itself: one sequence of 37 tokens 9 us,
+// Where a table holds no more than kWhole tiles a wave does an item by itself: one sequence of 37 tokens 8.5 us,
 // without the 4 of a merge.  Parts of two tiles at least, where there is little work: 16 windows of 512
 // tokens, head dim 256, 16 us (four tiles: 20, one: 14), and 16 sequences of 200 tokens 14 (15, 17).
 constexpr int kTile = 32;
