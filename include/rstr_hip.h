@@ -428,7 +428,8 @@ int rstr_kv4_attn_close(rstr_kv4_attn* a);
  * 11 bits; bf16 and many rows: keys too).  A row that
  * sees no token (length 0, more rows than tokens) is 0.  Tokens of a page id outside
  * the cache are not seen, nor are tokens behind the table's width.  Rows behind
- * row_offsets[batch] are left as they are; row_offsets must not decrease.
+ * row_offsets[batch] are left as they are; where row_offsets decrease anywhere, nothing is
+ * written.
  * max_rows: the most rows a sequence of this call has (it chooses the tile; a sequence
  * with more is still computed). */
 int rstr_kv4_attn_run(rstr_kv4_attn* a, int32_t layer, int32_t dtype, int32_t batch, int32_t rows,

@@ -9,6 +9,7 @@
 #include "../../include/rstr_hip.h"
 #include "device_math.h"
 #include "kv4.h"
+#include "kv4_line.h"
 
 namespace rstr {
 
@@ -530,7 +531,6 @@ hipError_t rows_type(hipStream_t st, bool append, const Kv4Layer& c, int dtype, 
 // Where a table holds no more than kWhole tiles a wave does an item by itself: one sequence of 37 tokens 8.5 us,
 // without the 4 of a merge.  Parts of two tiles at least, where there is little work: 16 windows of 512
 // tokens, head dim 256, 16 us (four tiles: 20, one: 14), and 16 sequences of 200 tokens 14 (15, 17).
-constexpr int kTile = 32;
 constexpr int kStart = 6;  // what beginning an item costs, in tiles
 
 // Terms of a weight; ONCE: p * d is rounded once, from fp32.  bf16 results round to 8
@@ -545,32 +545,6 @@ constexpr int attn_waves(int hd, int nt, int terms) { return hd == 256 ? 1 : nt 
 
 // Tiles of a wave's ring: what 160 KB of LDS hold for that many waves.
 constexpr int attn_ring(int hd, int nt, int terms) { return attn_waves(hd, nt, terms) == 3 && hd == 128 ? 2 : 4; }
-
-// The sequences of a call, as every wave sees them.
-struct Lines {
-  const int32_t *ro, *lens;
-  int rows, n_kv, group, window, cols;  // cols: of a column tile
-  int64_t cap;                          // tokens that a page table row can hold
-  int start;                            // what beginning an item costs, in tiles
-  bool whole;                           // one unit an item
-  __device__ __forceinline__ int per_item(int tiles) const { return whole ? 1 : tiles + start; }
-};
-struct Seq {
-  int r0, m, len, lo, tiles, nct;
-  int64_t units;
-};
-__device__ __forceinline__ Seq sequence(const Lines& L, int b) {
-  Seq s;
-  s.r0 = min(max(L.ro[b], 0), L.rows);
-  s.m = max(min(max(L.ro[b + 1], 0), L.rows) - s.r0, 0);
-  s.len = (int)min((int64_t)max(L.lens[b], 0), L.cap);
-  const int64_t lo = L.window > 0 ? (int64_t)s.len - s.m + 1 - L.window : 0;
-  s.lo = lo > 0 ? (int)lo / kTile : 0;  // first tile
-  s.tiles = max((int)(((int64_t)s.len + kTile - 1) / kTile) - s.lo, 0);
-  s.nct = (int)(((int64_t)s.m * L.group + L.cols - 1) / L.cols);
-  s.units = (int64_t)L.n_kv * s.nct * L.per_item(s.tiles);
-  return s;
-}
 
 // The value of one lane, the same for all.
 __device__ __forceinline__ int64_t lane64(int64_t v, int lane) {
@@ -617,11 +591,18 @@ struct Line {
   __device__ __forceinline__ Line(const Lines& lines, int n_seqs, int worker, int workers, int least) : L(lines), batch(n_seqs), w(worker) {
     seqs = chunk_of(0);
     int64_t in = wave_scan_i64(seqs.units), total = lane64(in, 63);
+    ordered = seqs.ordered;
     if (batch > 64) {
       int64_t mine = 0;
-      for (int i = 64; i < batch; i += 64) mine += chunk_of(i).units;
+      for (int i = 64; i < batch; i += 64) {
+        const Seq x = chunk_of(i);
+        mine += x.units;
+        ordered = ordered && x.ordered;
+      }
       total += lane64(wave_scan_i64(mine), 63);
     }
+    ordered = __ballot(!ordered) == 0;
+    if (!ordered) total = 0;
     part = quotient(total + workers - 1, workers);
     part = part > least ? part : least;
     u = (int64_t)w * part;
@@ -645,6 +626,7 @@ struct Line {
 
   // Items of the call.
   __device__ __forceinline__ int items() const {
+    if (!ordered) return 0;
     int n = 0;
     for (int i = 0; i < batch; i += 64) n += L.n_kv * chunk_of(i).nct;
     return wave_sum_i32(n);
@@ -653,7 +635,7 @@ struct Line {
   __device__ __forceinline__ bool next() {
     while (u < u_end) {
       const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at_seq); };
-      s = Seq{of(seqs.r0), of(seqs.m), of(seqs.len), of(seqs.lo), of(seqs.tiles), of(seqs.nct), 0};
+      s = Seq{of(seqs.r0), of(seqs.m), of(seqs.len), of(seqs.lo), of(seqs.tiles), of(seqs.nct), true, 0};
       const int per_item = L.per_item(s.tiles);
       const int64_t units = (int64_t)L.n_kv * s.nct * per_item;
       if (u < first + units) {
@@ -687,6 +669,7 @@ struct Line {
 
  private:
   Seq seqs;
+  bool ordered;  // all sequences are
   int b0 = 0, at_seq = 0, item0 = 0;  // the sequence that unit u lies in (of seqs), its first item and unit
   int64_t first = 0;
   __device__ __forceinline__ Seq chunk_of(int from) const {
@@ -1759,10 +1742,6 @@ constexpr int kPromptLeast = 4;  // and a workgroup of k_kv4_prompt
 
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Items of a call, at most.
-int64_t attn_items(int n_q, int n_kv, int batch, int rows, int cols) {
-  return n_kv * ((int64_t)rows * (n_q / n_kv) / cols + std::min(batch, rows));
-}
 // Workspace: what up to `workers` waves leave of items that they share.
 size_t attn_bytes(int64_t items, int64_t workers, int cols, int hd) {
   return 256 + align256(sizeof(Begun) * items) + align256(sizeof(float2) * 2 * workers * cols) + sizeof(float) * 2 * workers * cols * hd;

@@ -1,0 +1,53 @@
+// kv4_line.h -- the line of work of attention over the 4-bit cache: the items that
+// the sequences of a call are and how many there can be.  Plain arithmetic, the same on
+// the device and on the host.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace rstr {
+
+constexpr int kTile = 32;
+
+__host__ __device__ inline int at_least(int v, int lo) { return v > lo ? v : lo; }
+__host__ __device__ inline int at_most(int v, int hi) { return v < hi ? v : hi; }
+
+// The sequences of a call, as every wave sees them.
+struct Lines {
+  const int32_t *ro, *lens;
+  int rows, n_kv, group, window, cols;  // cols: of a column tile
+  int64_t cap;                          // tokens that a page table row can hold
+  int start;                            // what beginning an item costs, in tiles
+  bool whole;                           // one unit an item
+  __host__ __device__ inline int per_item(int tiles) const { return whole ? 1 : tiles + start; }
+};
+struct Seq {
+  int r0, m, len, lo, tiles, nct;
+  bool ordered;  // its rows do not begin behind their end
+  int64_t units;
+};
+// Rows of sequences are apart where every sequence is ordered; a call in which one is not
+// has no items (what room they take follows from the rows all together).
+__host__ __device__ inline Seq sequence(const Lines& L, int b) {
+  Seq s;
+  const int begin = L.ro[b], end = L.ro[b + 1];
+  s.ordered = begin <= end;
+  s.r0 = at_most(at_least(begin, 0), L.rows);
+  s.m = at_least(at_most(at_least(end, 0), L.rows) - s.r0, 0);
+  s.len = at_least(L.lens[b], 0);
+  if (s.len > L.cap) s.len = (int)L.cap;
+  const int64_t lo = L.window > 0 ? (int64_t)s.len - s.m + 1 - L.window : 0;
+  s.lo = lo > 0 ? (int)lo / kTile : 0;  // first tile
+  s.tiles = at_least((int)(((int64_t)s.len + kTile - 1) / kTile) - s.lo, 0);
+  s.nct = (int)(((int64_t)s.m * L.group + L.cols - 1) / L.cols);
+  s.units = (int64_t)L.n_kv * s.nct * L.per_item(s.tiles);
+  return s;
+}
+
+// Items of a call whose sequences are ordered, at most: column tiles that are full, and one a
+// sequence that is not.
+__host__ __device__ inline int64_t attn_items(int n_q, int n_kv, int batch, int rows, int cols) {
+  return n_kv * ((int64_t)rows * (n_q / n_kv) / cols + at_most(batch, rows));
+}
+
+}  // namespace rstr

@@ -1,0 +1,66 @@
+// The items that attention over the 4-bit cache makes of a call's row offsets, whatever these
+// hold: their numbers stay inside the room that the host counts for them.
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+
+#include "../../pretrained-rstr_amd/csrc/kv4_line.h"
+
+using namespace rstr;
+
+static int checks = 0;
+
+// The items of a call, numbered as the kernels number them.  Returns whether it has any.
+static bool call(const std::vector<int32_t>& ro, int rows, int n_q, int n_kv, int cols) {
+  const int batch = (int)ro.size() - 1;
+  std::vector<int32_t> lens(batch, 100);
+  const Lines L{ro.data(), lens.data(), rows, n_kv, n_q / n_kv, 0, cols, 1000, 6, false};
+  int64_t items = 0, taken = 0;
+  bool ordered = true;
+  for (int b = 0; b < batch; b++) {
+    const Seq s = sequence(L, b);
+    ordered = ordered && s.ordered;
+    items += (int64_t)n_kv * s.nct;
+    taken += s.m;
+    if (s.r0 < 0 || s.m < 0 || s.r0 + s.m > rows) { printf("rows %d + %d of %d\n", s.r0, s.m, rows); exit(1); }
+  }
+  checks++;
+  if (!ordered) return false;
+  const int64_t room = attn_items(n_q, n_kv, batch, rows, cols);
+  if (items > room || taken > rows) {
+    printf("batch %d rows %d heads %d/%d cols %d: %lld items in room for %lld, %lld rows\n", batch, rows, n_q, n_kv, cols,
+           (long long)items, (long long)room, (long long)taken);
+    exit(1);
+  }
+  return true;
+}
+
+int main() {
+  srand(1);
+  const int heads[][2] = {{1, 1}, {32, 8}, {8, 8}, {24, 1}, {4, 1}};
+  for (const auto& h : heads)
+    for (int cols : {16, 32, 256}) {
+      for (int rows : {1, 2, 33, 4096}) {
+        for (int batch : {1, 2, 3, 64, 65, 200, 4096}) {
+          std::vector<int32_t> ro(batch + 1), even(batch + 1);
+          for (int b = 0; b <= batch; b++) ro[b] = b % 2 ? rows : 0;  // over and over the same rows
+          if (call(ro, rows, h[0], h[1], cols) != (batch == 1)) { printf("offsets that decrease were taken\n"); return 1; }
+          for (int b = 0; b <= batch; b++) even[b] = (int32_t)((int64_t)rows * b / batch);
+          if (!call(even, rows, h[0], h[1], cols)) { printf("ordered offsets were refused\n"); return 1; }
+          for (int i = 0; i < 20; i++) {
+            // an ordered line, beginning before the array and ending behind it, with one place disturbed
+            int64_t at = rand() % 5 - 2;
+            for (int b = 0; b <= batch; b++) {
+              ro[b] = at > 0x7FFFFFFF ? 0x7FFFFFFF : (int32_t)at;
+              at += i % 4 == 0 ? rand() % 3 : i % 4 == 1 ? rand() % (2 * rows + 1) : i % 4 == 2 ? (rand() % 8 == 0) * rows : (int64_t)rand() * 2;
+            }
+            if (!call(ro, rows, h[0], h[1], cols)) { printf("ordered offsets were refused\n"); return 1; }
+            ro[rand() % (batch + 1)] = rand() % 2 ? -(int32_t)0x7FFFFFFF - 1 : rand() % (rows + 1);
+            call(ro, rows, h[0], h[1], cols);
+          }
+        }
+      }
+    }
+  printf("ok %d\n", checks);
+  return 0;
+}

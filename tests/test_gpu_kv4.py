@@ -530,3 +530,28 @@ def test_streams_and_graphs(sess, lens, news):
     for p in plans:
         p.close()
     c.close()
+
+
+@pytest.mark.parametrize("dtype,D,n_q,each", [("f32", 64, 4, 1), ("f16", 128, 8, 5), ("bf16", 128, 8, 20), ("bf16", 256, 4, 2)])
+@pytest.mark.parametrize("B", [2, 64, 70, 200])
+def test_offsets_that_decrease(sess, dtype, D, n_q, each, B):
+    """Where row offsets decrease, nothing is written: their sequences would have the same rows, and more items than the
+    workspace has room for.  The plan serves the next call."""
+    print("decreasing offsets", dtype, D, B, flush=True)
+    c = Case(sess, n_q, 2 if n_q > 4 else 1, D, 16, [140 + i % 50 for i in range(B)], [each] * B, width=20)
+    q = c.queries(dtype).cuda()
+    R = B * each
+    plan = c.plan()
+    over_and_over = [R if b % 2 else 0 for b in range(B + 1)]
+    one_back, last_back = c.offsets.copy(), c.offsets.copy()
+    one_back[B // 2 + 1] = one_back[B // 2] - 1
+    last_back[B] = 0
+    for bad in (over_and_over, one_back, last_back, [2 ** 31 - 1] + c.offsets[1:].tolist()):
+        out = torch.full_like(q, 7.0)
+        plan.run(0, q, _i32(bad), _i32(c.table), _i32(c.lens), out, max_rows=each)
+        torch.cuda.synchronize()
+        assert bool((out == 7.0).all())
+        plan.run(0, q, _i32(c.offsets), _i32(c.table), _i32(c.lens), out, max_rows=each)
+        c.check(out, q, dtype, 0, D ** -0.5)
+    plan.close()
+    c.close()
