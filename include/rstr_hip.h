@@ -425,7 +425,8 @@ int rstr_kv4_attn_close(rstr_kv4_attn* a);
  * token p sees the tokens j <= p, and with window > 0 only j > p - window:
  * out = sum softmax(scale * q . k_j) v_j, in the type of q (f32: products and sums
  * in fp32 precision; f16, bf16: probabilities, and their products with values, rounded to
- * 11 bits; bf16 and many rows: keys too).  A row that
+ * 11 bits; bf16 and many rows: keys too; a product of a probability and a value is off
+ * by 2^-32 where that is more).  A row that
  * sees no token (length 0, more rows than tokens) is 0.  Tokens of a page id outside
  * the cache are not seen, nor are tokens behind the table's width.  Rows behind
  * row_offsets[batch] are left as they are; where row_offsets decrease anywhere, nothing is

@@ -513,9 +513,10 @@ hipError_t rows_type(hipStream_t st, bool append, const Kv4Layer& c, int dtype, 
 // when a score passes it by 2^4, so the exchange between lanes that the
 // maximum needs, and the rescaling of O and l, happen a few times a segment; p
 // carries a factor 2^10, so small weights keep their bits: fp16's subnormals
-// begin 2^24 below the largest.  Scales of V of 2 and more are brought below 2 by a
-// power of two that follows the largest one seen (and with two terms, small
-// ones are brought up).
+// begin 2^24 below the largest.  With two terms, a power of two that follows the largest
+// scale of V seen so far, up to 2, brings small products up.  Scales of 2 and more are taken
+// with 2^-15 of themselves, and the rest of their part, 2^15 - 1 times as much, is added by products of their
+// own, so that scales beside them keep their bits.
 //
 // The tiles of all (sequence, kv head, column tile) items form one line of units
 // that is cut into equal parts, one a wave: the load is even whatever the
@@ -804,9 +805,8 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 
     f4 acc[NT][2 * NB];
     float mref[NT], kcol[NT], fs[NT];
-    f4 l[NT];             // ONCE: the lane's own part of the sum of p in the first; else the sum, in all four
-    int elim[NT];         // exponents of the V scales seen so far are no larger; fs = 2^(15 - elim)
-    bool scaled = false;  // some column's fs is below 1
+    f4 l[NT];      // ONCE: the lane's own part of the sum of p in the first; else the sum, in all four
+    int elim[NT];  // two terms: exponents of the V scales below 2 seen so far are no larger; fs = 2^(15 - elim)
     h8 q[NT][TERMS][NB];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
       for (int i = 0; i < 2 * NB; i++) acc[t][i] = f4{0, 0, 0, 0};
       mref[t] = -FLT_MAX;
       l[t] = f4{0, 0, 0, 0};
-      elim[t] = TERMS == 1 ? 15 : 0;
+      elim[t] = 0;
       fs[t] = __builtin_amdgcn_ldexpf(1.0f, 15 - elim[t]);
     }
     if (t0 < t1) {
@@ -986,8 +986,8 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 #pragma unroll
           for (int i = 0; i < 8; i++) e2[t][i] = __builtin_fmaf(sc[t][i], kcol[t], -mref[t]);
         // the largest exponent of a V scale, from above: of all bits together (exponents
-        // to 15 have no bit that 15 has not), and exactly where that is more than 15
-        const auto exponent = [](uint32_t o) { return (int)(((o | (o >> 16)) >> 10) & 31); };
+        // to 15 have no bit that 15 has not; 15 where there are larger ones)
+        const auto exponent = [](uint32_t o) { return min((int)(((o | (o >> 16)) >> 10) & 31), 15); };
         uint32_t ors = 0;
 #pragma unroll
         for (int j = 0; j < 2; j++)
@@ -1033,31 +1033,16 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 #pragma unroll
           for (int i = 1; i < 8; i++) m = fmaxf(m, e2[t][i]);
           passed[t] = m > 14.0f;
-          grow |= passed[t] || exps[t] > elim[t];
+          grow |= passed[t] || (TERMS == 2 && exps[t] > elim[t]);
         }
         if (__ballot(grow)) {
-          bool big = false;
 #pragma unroll
           for (int t = 0; t < NT; t++) {
             float m = -INFINITY;
-            int e = exps[t];
-            if (e > 15) e = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const bool ok = (see[t] >> i) & 1;
-              if (ok) m = fmaxf(m, sc[t][i] * kcol[t]);
-              if (exps[t] > 15 && ok)
-#pragma unroll
-                for (int bk = 0; bk < NB; bk++) {
-                  const int k = (int)((xv.s[i >> 2][2 * bk + ((i >> 1) & 1)] >> (16 * (i & 1) + 10)) & 31);
-                  if (k < 31) e = max(e, k);
-                }
-            }
+            for (int i = 0; i < 8; i++)
+              if ((see[t] >> i) & 1) m = fmaxf(m, sc[t][i] * kcol[t]);
             m = xor_max<32>(xor_max<16>(m));
-            e = max(e, elim[t]);
-            e = max(e, __shfl_xor(e, 16, 64));
-            e = max(e, __shfl_xor(e, 32, 64));
-            if (e <= 15) { e |= e >> 1; e |= e >> 2; }
             // A column that needs no change has none: it does not depend on its neighbours.  One that does
             // takes differences of rounded scores, which stay below 14 however large the scores are.
             const bool own = of_column(__ballot(passed[t]));
@@ -1065,17 +1050,36 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
             const float keep = __builtin_amdgcn_exp2f(mref[t] - now);
             mref[t] = now;
             l[t] *= keep;
-            const float less = __builtin_amdgcn_ldexpf(keep, elim[t] - e);
-            elim[t] = e;
-            fs[t] = __builtin_amdgcn_ldexpf(1.0f, 15 - e);
-            big |= e > 15;
+            float less = keep;
+            if constexpr (TERMS == 2) {
+              int e = max(exps[t], elim[t]);
+              e = max(e, __shfl_xor(e, 16, 64));
+              e = max(e, __shfl_xor(e, 32, 64));
+              e |= e >> 1;
+              e |= e >> 2;
+              less = __builtin_amdgcn_ldexpf(keep, elim[t] - e);
+              elim[t] = e;
+              fs[t] = __builtin_amdgcn_ldexpf(1.0f, 15 - e);
+            }
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) acc[t][i] *= less;
 #pragma unroll
             for (int i = 0; i < 8; i++)
               if (own) e2[t][i] = (see[t] >> i) & 1 ? sc[t][i] * kcol[t] - mref[t] : -INFINITY;
           }
-          scaled = __ballot(big) != 0;
+        }
+        // scales of 2 and more (finite), and what makes 2^-15 of them
+        const auto large = [](uint32_t d) { return (d & 0x7FFFu) >= 0x4000u && (d & 0x7FFFu) < 0x7C00u; };
+        constexpr uint32_t kLess = 15u << 10;
+        const bool some_large = __ballot((ors & 0x40004000u) != 0) != 0;
+        if (some_large) {
+          asm volatile("");  // stays a branch
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++)
+#pragma unroll
+              for (int k = 0; k < 2; k++) xv.s[j][i] -= large(xv.s[j][i] >> (16 * k)) ? kLess << (16 * k) : 0u;
         }
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -1083,32 +1087,17 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 #pragma unroll
           for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(e2[t][i]);
           h2 ph[2][2];
-          uint32_t vs[2][2 * NB];  // scales of V, below 2 by fs, where there are such
           if constexpr (ONCE) {
             l[t][0] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            if (TERMS == 2 || scaled) {
-              if constexpr (TERMS == 1) asm volatile("");  // stays a branch
+            if constexpr (TERMS == 2)
 #pragma unroll
               for (int i = 0; i < 8; i++) p[i] *= fs[t];
-            }
           } else {
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
               for (int i = 0; i < 2; i++) ph[j][i] = h2{(_Float16)p[4 * j + 2 * i], (_Float16)p[4 * j + 2 * i + 1]};
             l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pack8(ph[0][0], ph[0][1], ph[1][0], ph[1][1]), l[t], 0, 0, 0);
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-              for (int i = 0; i < 2 * NB; i++) vs[j][i] = xv.s[j][i];
-            if (scaled) {
-              asm volatile("");  // stays a branch
-              const h2 f = {(_Float16)fs[t], (_Float16)fs[t]};
-#pragma unroll
-              for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int i = 0; i < 2 * NB; i++) vs[j][i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, vs[j][i]) * f);
-            }
           }
 #pragma unroll
           for (int bk = 0; bk < NB; bk++) {
@@ -1131,7 +1120,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
               for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                  y[j][i] = ph[j][i] * __builtin_bit_cast(h2, vs[j][2 * bk + i]);
+                  y[j][i] = ph[j][i] * __builtin_bit_cast(h2, xv.s[j][2 * bk + i]);
                   if constexpr (NT > 1) {
                     const uint32_t m = see[t] >> (4 * j + 2 * i);
                     const uint32_t pair = (m & 1 ? 0xFFFFu : 0) | (m & 2 ? 0xFFFF0000u : 0);
@@ -1150,6 +1139,34 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
               if constexpr (TERMS == 2) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pd[1], o, 0, 0, 0);
             }
           }
+          if (some_large) {  // the rest of their part; scales and codes come from the ring once more, as there are no registers for both
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int bk = 0; bk < NB; bk++) {
+              h8 pd[TERMS];
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const uint32_t s = *(const uint16_t*)(at + vs_at + (i >> 2) * D + 8 * bk + 2 * (i & 3));
+                float y = ONCE ? p[i] : (float)ph[i >> 2][(i >> 1) & 1][i & 1];
+                y = large(s) ? y * half_of(s - kLess, 0) : 0.0f;
+                if constexpr (TERMS == 2) asm("" : "+v"(y));
+                const _Float16 top = (_Float16)y;
+                pd[0][i] = top;
+                if constexpr (TERMS == 2) pd[1][i] = (_Float16)(y - (float)top);
+              }
+              const uint8_t* c = at + v_at + (bk < 4 ? 0 : 256) + ((bk >> 1) & 1) * 8;
+#pragma unroll
+              for (int hh = 0; hh < 2; hh++) {
+                const int pr = (bk & 1) * 2 + hh;
+                const auto pair = [&](int j, int k) { return code_pair(magic, *(const uint32_t*)(c + j * 8 * D + 4 * k), pr); };
+                const h8 vq = pack8(pair(0, 0), pair(0, 1), pair(1, 0), pair(1, 1));
+                f4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pd[0], f4{0, 0, 0, 0}, 0, 0, 0);
+                if constexpr (TERMS == 2) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pd[1], d, 0, 0, 0);
+                acc[t][2 * bk + hh] += 32767.0f * d;
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
         }
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the slot is free
       }
@@ -1159,7 +1176,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
     // O on the scale of l
 #pragma unroll
     for (int t = 0; t < NT; t++)
-      if (TERMS == 2 || scaled)
+      if constexpr (TERMS == 2)
 #pragma unroll
         for (int i = 0; i < 2 * NB; i++)
 #pragma unroll
@@ -1213,8 +1230,9 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
 // for its sequence, its pages, queries and codes, one after the other.  Four waves a workgroup, two of
 // those a CU: 87 us.  One wave of a SIMD expanding while the other multiplies: 84.
 //
-// Scales of 2^13 and more would pass fp16's range in V (c - 8): the first step that brings one
-// turns the part's scales down by 2^4 for good.  A NaN scale of V is expanded as 0, which
+// Scales of 2^13 and more would pass fp16's range times c - 8: those blocks are expanded with 2^-4 of their
+// scale, and the missing 15 / 16 of their part are added by products of their own, so that scales beside them
+// keep their bits.  A NaN scale of V is expanded as 0, which
 // spares the columns that do not see its token, and written into O of those that do.
 constexpr int kPromptStart = 8;  // what beginning an item costs, in tiles
 
@@ -1229,11 +1247,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
   const Magic magic;
   struct Tile {
     h8 k[2][NB][64], v[NB][2][64];
-    u32x2 ks[2][4][NB];       // K scales of four tokens: half, token group, block
+    u32x2 ks[2][4][NB];       // K scales of four tokens: half, token group, block (SCALED_K: where the half has large ones)
     u32x4 vs[2][4][NB / 2];   // V scales: half, token group, two blocks
     uint32_t about[4];        // what each of the four waves that expanded it found
   };
-  enum { LARGE = 1, NOT_FINITE = 2, GONE = 4 };
+  enum { LARGE_K = 1, LARGE_V = 2, NOT_FINITE = 4, GONE = 8 };
   __shared__ Tile tiles[2][SUB];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int w = blockIdx.x, group = a.n_q / a.c.n_kv, ps = a.c.page_size;
@@ -1283,7 +1301,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
     f4 acc[NT][2 * NB], l[NT];
     float mref[NT], kcol[NT];
     h8 q[NT][NB];
-    float turn = 1.0f;  // of the item's scales
 #pragma unroll
     for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -1329,6 +1346,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
         vs = *(const u32x4*)(p + (R::vsbase(ps) + so + R::s(vt, 2 * vp)));
         look();
       };
+      // fp16 scales of 2^13 and more (finite), and what makes a sixteenth of them
+      const auto large = [](uint32_t d) { return (d & 0x7FFFu) >= 0x7000u && (d & 0x7FFFu) < 0x7C00u; };
+      constexpr uint32_t kSixteenth = 4u << 10;
       // its expansion into buffer i
       const auto expand = [&](int i, int step) {
         Tile& x = tiles[i][sub];
@@ -1353,28 +1373,29 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
         uint32_t about = there ? 0 : GONE;
         if (__ballot(max(e[0], e[1]) >= 0x7000)) {  // 2^13 and more, or not finite: hardly ever
           asm volatile("");
-          bool large = false, odd = false;
+          bool large_k = false, large_v = false, odd = false;
 #pragma unroll
           for (int n = 0; n < 8; n++) {
-            const uint32_t d = (vd[n >> 1] >> (16 * (n & 1))) & 0x7FFFu;
-            odd |= d >= 0x7C00u;
-            large |= d >= 0x7000u && d < 0x7C00u;
-            if (d >= 0x7C00u) vd[n >> 1] &= n & 1 ? 0xFFFFu : 0xFFFF0000u;
+            const uint32_t d = vd[n >> 1] >> (16 * (n & 1));
+            odd |= (d & 0x7FFFu) >= 0x7C00u;
+            if ((d & 0x7FFFu) >= 0x7C00u) vd[n >> 1] &= n & 1 ? 0xFFFFu : 0xFFFF0000u;
+            if (large(d)) {
+              large_v = true;
+              vd[n >> 1] -= kSixteenth << (16 * (n & 1));
+            }
           }
           if constexpr (SCALED_K)
 #pragma unroll
-            for (int n = 0; n < 2; n++) large |= (kd[n] & 0x7FFFu) >= 0x7000u && (kd[n] & 0x7FFFu) < 0x7C00u;
-          about |= (__ballot(large) && turn == 1.0f ? LARGE : 0) | (__ballot(odd) ? NOT_FINITE : 0);
+            for (int n = 0; n < 2; n++) {
+              if (kg == 0) ((uint16_t*)&x.ks[j][ktok >> 2][kb + n])[ktok & 3] = kd[n];
+              if (large(kd[n])) {
+                large_k = true;
+                kd[n] -= kSixteenth;
+              }
+            }
+          about |= (__ballot(large_k) ? LARGE_K : 0) | (__ballot(large_v) ? LARGE_V : 0) | (__ballot(odd) ? NOT_FINITE : 0);
         }
         if (lane == 0) x.about[wave & 3] = about;
-        if (turn != 1.0f) {
-          const h2 down = {(_Float16)turn, (_Float16)turn};
-#pragma unroll
-          for (int n = 0; n < 4; n++) vd[n] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, vd[n]) * down);
-          if constexpr (SCALED_K)
-#pragma unroll
-            for (int n = 0; n < 2; n++) kd[n] = __builtin_bit_cast(uint16_t, (_Float16)(__builtin_bit_cast(_Float16, kd[n]) * down[0]));
-        }
 #pragma unroll
         for (int n = 0; n < 2; n++) {
           h2 p[4];
@@ -1432,6 +1453,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
           const int tok0 = (step + i) * kTile;
           if (step + i >= t1 || tok0 >= w_hi || tok0 + kTile <= w_lo) continue;
           const u32x4 about = *(const u32x4*)x.about;
+          const uint32_t found = uniform(about[0] | about[1] | about[2] | about[3]);
           const uint32_t lost = uniform((about[0] & GONE) / GONE | (about[2] & GONE) / GONE << 1);
           const bool edge = lost || tok0 < w_lo_last || tok0 + kTile > w_hi_first;
           float sc[NT][8];
@@ -1477,6 +1499,23 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
 #pragma unroll
             for (int hh = 0; hh < 2; hh++) v[bk][hh] = x.v[bk][hh][lane];
           asm volatile("" ::: "memory");  // these loads run while the weights are computed
+          if (SCALED_K && (found & LARGE_K)) {
+            asm volatile("");
+#pragma unroll
+            for (int bk = 0; bk < NB; bk++)
+#pragma unroll
+              for (int i = 0; i < 2; i++) {
+                if (!(uniform(about[2 * i]) & LARGE_K)) continue;  // no scales were left for the half
+                const u32x2 ks = x.ks[i][g][bk];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                  const f4 part = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[i][bk][lane], q[t][bk], f4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                  for (int n = 0; n < 4; n++)
+                    if (large(ks[n >> 1] >> (16 * (n & 1)))) sc[t][4 * i + n] = __builtin_fmaf(15.0f, part[n], sc[t][4 * i + n]);
+                }
+              }
+          }
           uint32_t see[NT];
           float e2[NT][8];
           bool grow = false, passed[NT];
@@ -1542,67 +1581,63 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
 #pragma unroll
               for (int t = 0; t < NT; t++) acc[t][2 * bk + hh] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[bk][hh], p[t], acc[t][2 * bk + hh], 0, 0, 0);
             }
-          if (uniform(about[0] | about[1] | about[2] | about[3]) & NOT_FINITE) {  // scales of V that were left out, among the tokens that a column sees
+          if (found & (LARGE_V | NOT_FINITE)) {
+            asm volatile("");
+            if (found & LARGE_V) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-              uint32_t bad = 0;
+              for (int bk = 0; bk < NB; bk++) {
+                h8 pl[NT];
 #pragma unroll
-              for (int n = 0; n < 8; n++)
+                for (int n = 0; n < 8; n++) {
+                  const bool here = large(x.vs[n >> 2][g][bk >> 1][2 * (bk & 1) + ((n >> 1) & 1)] >> (16 * (n & 1)));
 #pragma unroll
-                for (int bk = 0; bk < NB; bk++) {
-                  const uint32_t d = x.vs[n >> 2][g][bk >> 1][2 * (bk & 1) + ((n >> 1) & 1)] >> (16 * (n & 1));
-                  if ((d & 0x7FFFu) >= 0x7C00u && ((see[t] >> n) & 1)) bad |= 1u << bk;
+                  for (int t = 0; t < NT; t++) pl[t][n] = here ? p[t][n] : (_Float16)0.0f;
                 }
-              bad |= __shfl_xor(bad, 16, 64);
-              bad |= __shfl_xor(bad, 32, 64);
 #pragma unroll
-              for (int bk = 0; bk < NB; bk++)
-                if ((bad >> bk) & 1) {
-                  const float n = __builtin_nanf("");
-                  acc[t][2 * bk] = f4{n, n, n, n};
-                  acc[t][2 * bk + 1] = f4{n, n, n, n};
-                }
+                for (int hh = 0; hh < 2; hh++)
+#pragma unroll
+                  for (int t = 0; t < NT; t++)
+                    acc[t][2 * bk + hh] += 15.0f * __builtin_amdgcn_mfma_f32_16x16x32_f16(x.v[bk][hh][lane], pl[t], f4{0, 0, 0, 0}, 0, 0, 0);
+              }
+            }
+            if (found & NOT_FINITE) {  // scales of V that were left out, among the tokens that a column sees
+#pragma unroll
+              for (int t = 0; t < NT; t++) {
+                uint32_t bad = 0;
+#pragma unroll
+                for (int n = 0; n < 8; n++)
+#pragma unroll
+                  for (int bk = 0; bk < NB; bk++) {
+                    const uint32_t d = x.vs[n >> 2][g][bk >> 1][2 * (bk & 1) + ((n >> 1) & 1)] >> (16 * (n & 1));
+                    if ((d & 0x7FFFu) >= 0x7C00u && ((see[t] >> n) & 1)) bad |= 1u << bk;
+                  }
+                bad |= __shfl_xor(bad, 16, 64);
+                bad |= __shfl_xor(bad, 32, 64);
+#pragma unroll
+                for (int bk = 0; bk < NB; bk++)
+                  if ((bad >> bk) & 1) {
+                    const float n = __builtin_nanf("");
+                    acc[t][2 * bk] = f4{n, n, n, n};
+                    acc[t][2 * bk + 1] = f4{n, n, n, n};
+                  }
+              }
             }
           }
         }
       };
       int buf = 1;
-      bool some = false;  // a step to multiply
       for (int step = t0 - SUB;;) {
         const int next = step + SUB;
-        if (some) compute(buf, step);
+        if (step >= t0) compute(buf, step);
         if (next >= t1) break;
         expand(buf ^ 1, next);
         fetch();  // the step after it, also where there is none
         __syncthreads();
         step = next;
         buf ^= 1;
-        some = true;
-        uint32_t all = 0;
-#pragma unroll
-        for (int i = 0; i < SUB; i++) {
-          const u32x4 x = *(const u32x4*)tiles[buf][i].about;
-          all |= x[0] | x[1] | x[2] | x[3];
-        }
-        if (uniform(all) & LARGE) {  // expand the step once more, with the item's scales turned down
-          turn = 0.0625f;
-#pragma unroll
-          for (int t = 0; t < NT; t++) {
-            if (SCALED_K) kcol[t] *= 16.0f;
-#pragma unroll
-            for (int i = 0; i < 2 * NB; i++) acc[t][i] *= turn;
-          }
-          start(step);
-          fetch();
-          __syncthreads();
-          step -= SUB;
-          buf ^= 1;
-          some = false;
-        }
       }
       __syncthreads();  // the buffers are the next part's
     }
-    const float up = 1.0f / turn;
     const int64_t slot = (begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w) * COLS;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -1610,7 +1645,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       const Column at = column(t);
       if (at.row >= s.m) continue;
       if (begins && ends) {
-        const float inv = sum == 0.0f ? 0.0f : up / sum;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         T* dst = (T*)a.out.p + (int64_t)(s.r0 + at.row) * a.out.row + (int64_t)at.head * a.out.head + 4 * g;
         const bool ovec = vec_rows(a.out, sizeof(T));
 #pragma unroll
@@ -1630,7 +1665,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
         if (g == 0) pc.ml[c] = float2{mref[t], sum};
         if (sum == 0.0f) continue;
 #pragma unroll
-        for (int i = 0; i < 2 * NB; i++) *(f4*)(pc.acc + c * D + 16 * i + 4 * g) = acc[t][i] * up;
+        for (int i = 0; i < 2 * NB; i++) *(f4*)(pc.acc + c * D + 16 * i + 4 * g) = acc[t][i];
       }
     }
   }

@@ -555,3 +555,69 @@ def test_offsets_that_decrease(sess, dtype, D, n_q, each, B):
         c.check(out, q, dtype, 0, D ** -0.5)
     plan.close()
     c.close()
+
+
+def _attention_by_position(q, k, v, length, window, scale):
+    """The last rows q [m][n_q][D] of a sequence of `length` tokens, of which k, v [tokens][n_kv][D] are
+    held: out, sum of w|v|, the largest |scale| |q| . |k| of a row's keys that weigh anything, and its least weights: sum of
+    min(w, 2^-33) |v|."""
+    m, n_q, D = q.shape
+    out, mag, size, low = (np.zeros(s) for s in ((m, n_q, D), (m, n_q, D), (m, n_q, 1), (m, n_q, D)))
+    for r in range(m):
+        p = length - m + r
+        j = np.arange(max(0, p - window + 1) if window else 0, min(p + 1, len(k)))
+        if not j.size:
+            continue
+        for h in range(n_q):
+            kk, vv = k[j, h // (n_q // k.shape[1])], v[j, h // (n_q // k.shape[1])]
+            s = kk @ q[r, h] * scale
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            out[r, h], mag[r, h], low[r, h] = w @ vv, w @ np.abs(vv), np.minimum(w, 2.0 ** -33) @ np.abs(vv)
+            size[r, h] = np.max((np.abs(kk) @ np.abs(q[r, h]))[w > 2.0 ** -60]) * abs(scale)
+    return out, mag, size, low
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("what,small", [("key", 1e-5), ("key", 1.0), ("block", 2e-4), ("block", 2e-3), ("token", 2e-4), ("token", 2e-2), ("all", 1.0)])
+def test_values_of_very_different_size(sess, dtype, rows, D, what, small):
+    """One token's keys, one block of its values, or all its values past fp16's range (scales of 2^13 and more) beside
+    values of `small` size, which keep their bits: a product of a weight and a value is off by its own
+    rounding, or by 2^-32 where that is more (a weight is 2^10 at the largest score, a product of it with a block's
+    scale then a multiple of 2^-24 or rounded to one, and a code at most 8 of those: 8 * 2^-25 / 2^10).
+    "token": the large values are those of a token that weighs nothing.  Few tokens, so that the first rows' roundings
+    do not average out; a table of 320 tokens, which many rows of head dim 128 share the expansion of."""
+    print("different size", dtype, rows, D, what, small, flush=True)
+    n, scale = 40, 1e-6 if what == "key" else D ** -0.5
+    c = Case(sess, 4, 2, D, 16, [n], [rows], width=20, v_scale=small)
+    q = c.queries(dtype)
+    q[..., 0] = 8.0
+    rng = np.random.default_rng(D)
+    first = torch.tensor(rng.standard_normal((2, 1, 2, D)) * np.array([1.0, small]).reshape(2, 1, 1, 1), dtype=torch.float32)
+    k, v = first[0], first[1]
+    if what == "key":
+        k *= 1e5
+    elif what == "block":
+        v[..., 32:64] *= 1e5 / small
+    else:
+        v *= 1e5 / small
+    if what == "token":
+        k[..., 0] = -4000.0   # a score of -2000 and less
+    c.pool.append(0, k.cuda(), v.cuda(), _i32([c.table[0, 0] * 16]))
+    c.k[0][0], c.v[0][0] = P.quantised(P.as_f64(k))[0], P.quantised(P.as_f64(v))[0]
+    out = torch.zeros_like(q).cuda()
+    plan = c.plan()
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out, scale=scale)
+    want, mag, size, low = _attention_by_position(P.as_f64(q), c.k[0], c.v[0], n, 0, scale)
+    rel = 2 * (D + 16) * 2.0 ** -24 * 10 * size + (2.0 ** -10 if dtype != "f32" else 2.0 ** -22 + n * 2.0 ** -27)
+    if dtype == "bf16" and rows > 16:
+        rel = rel + 2.0 ** -10 * size
+    eps = torch.finfo(TYPES[dtype]).eps
+    tol = rel * mag + eps / 2 * np.abs(want) * 1.01 + low + n * 2.0 ** -32 + torch.finfo(TYPES[dtype]).smallest_normal * eps / 2
+    fits = np.abs(want) < torch.finfo(TYPES[dtype]).max * (1 - 2.0 ** -9)   # fp16 does not hold the first rows' largest
+    far = np.where(fits, np.abs(P.as_f64(out) - want) - tol, -1.0) / (np.abs(want) + 1e-30)
+    assert far.max() <= 0, (far.max(), np.unravel_index(far.argmax(), far.shape))
+    plan.close()
+    c.close()
