@@ -428,7 +428,8 @@ int rstr_kv4_attn_close(rstr_kv4_attn* a);
  * 11 bits; bf16 and many rows: keys too; a product of a probability and a value is off
  * by 2^-32 where that is more).  A row that
  * sees no token (length 0, more rows than tokens) is 0.  Tokens of a page id outside
- * the cache are not seen, nor are tokens behind the table's width.  Rows behind
+ * the cache are not seen, nor are tokens behind the table's width or from 2^31 - 64 on (the
+ * positions of a longer sequence's rows follow from its length all the same).  Rows behind
  * row_offsets[batch] are left as they are; where row_offsets decrease anywhere, nothing is
  * written.
  * max_rows: the most rows a sequence of this call has (it chooses the tile; a sequence

@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int w = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
   const int group = a.n_q / a.c.n_kv, ps = a.c.page_size;
-  const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), kStart, whole};
+  const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, (int)min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), kStart, whole};
 
   Line line(L, a.batch, w, workers, least);
   if (w == 0 && !whole) *pc.n_items = line.items();
@@ -782,7 +782,8 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
     if (begins && !whole && lane == 0) pc.begun[line.item] = Begun{b, h, ct, w, line.pieces};
 
     // the columns' rows and what they see
-    const int c0 = ct * COLS, p0 = s.len - s.m;
+    const int c0 = ct * COLS, p0 = s.len - s.m, held = L.held(s.len);
+    const auto end_seen = [&](int r) { return min(max(p0 + r + 1, 0), held); };
     const auto first_seen = [&](int r) { return a.window > 0 ? max(max(p0 + r + 1, 0) - a.window, 0) : 0; };
     const int rf = c0 / group, rl = min(s.m - 1, (c0 + COLS - 1) / group);
     int hi[NT], lo[NT];
@@ -792,12 +793,12 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
     for (int t = 0; t < NT; t++) {
       const int cc = c0 + t * 16 + col, r = cc / group;
       valid[t] = r < s.m;
-      hi[t] = valid[t] ? max(p0 + r + 1, 0) : 0;
+      hi[t] = valid[t] ? end_seen(r) : 0;
       lo[t] = first_seen(r);
       qrow[t] = s.r0 + r;
       qhead[t] = (int64_t)h * group + (cc - r * group);
     }
-    const int hi_last = max(p0 + rl + 1, 0), hi_first = max(p0 + rf + 1, 0);
+    const int hi_last = end_seen(rl), hi_first = end_seen(rf);
     const int lo_first = first_seen(rf), lo_last = first_seen(rl);
     int t0 = s.lo + (whole ? 0 : max(at - kStart, 0)), t1 = s.lo + (whole ? s.tiles : max(at + n - kStart, 0));
     t0 = max(t0, lo_first / kTile);
@@ -822,7 +823,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
       // for a page that is not there, from page 0, so that the count of loads in
       // flight is known.  Page ids are read one tile ahead of their loads.
       const TablePtr row = (TablePtr)(table + (int64_t)b * a.pps);
-      const int n_pages = (int)(((int64_t)s.len + ps - 1) / ps);
+      const int n_pages = (int)(((int64_t)held + ps - 1) / ps);
       int pg = t0 * kTile / ps, off = t0 * kTile - pg * ps, slot = 0;
       const uint8_t* head = base + (int64_t)h * rec;
       const uint32_t page_bytes = (uint32_t)(a.c.n_kv * rec);
@@ -1255,7 +1256,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
   __shared__ Tile tiles[2][SUB];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int w = blockIdx.x, group = a.n_q / a.c.n_kv, ps = a.c.page_size;
-  const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), kPromptStart, false};
+  const Lines L{ro, lens, a.rows, a.c.n_kv, group, a.window, COLS, (int)min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0), kPromptStart, false};
   Line line(L, a.batch, w, workers, least);
   if (w == 0 && wave == 0) *pc.n_items = line.items();
 
@@ -1268,7 +1269,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
 
   while (line.next()) {
     const Seq& s = line.s;
-    const int h = line.h, c0 = line.ct * COLS, p0 = s.len - s.m;
+    const int h = line.h, c0 = line.ct * COLS, p0 = s.len - s.m, held = L.held(s.len);
     const bool begins = line.begins, ends = line.ends;
     if (begins && threadIdx.x == 0) pc.begun[line.item] = Begun{line.b, h, line.ct, w, line.pieces};
     const auto row_of = [&](int c) { return min(s.m - 1, c / group); };
@@ -1285,14 +1286,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
       return Column{row, h * group + (cc - row * group)};
     };
     const auto first_seen = [&](int row) { return a.window > 0 ? max(max(p0 + row + 1, 0) - a.window, 0) : 0; };
+    const auto end_seen = [&](int row) { return min(max(p0 + row + 1, 0), held); };
     int hi[NT], lo[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const int row = column(t).row;
-      hi[t] = row < s.m ? max(p0 + row + 1, 0) : 0;
+      hi[t] = row < s.m ? end_seen(row) : 0;
       lo[t] = first_seen(row);
     }
-    const auto end_seen = [&](int row) { return max(p0 + row + 1, 0); };
     const int t0 = max(s.lo + max(line.at - kPromptStart, 0), first_seen(rf) / kTile);
     const int t1 = min(s.lo + max(line.at + line.n - kPromptStart, 0), (end_seen(rl) + kTile - 1) / kTile);
     const bool any = cw < s.m * group;  // the wave has columns
@@ -1311,7 +1312,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
     }
     if (t0 < t1) {
       const TablePtr rowp = (TablePtr)(table + (int64_t)line.b * a.pps);
-      const int n_pages = (int)(((int64_t)s.len + ps - 1) / ps);
+      const int n_pages = (int)(((int64_t)held + ps - 1) / ps);
       const uint8_t* head = base + (int64_t)h * rec;
       // the wave's 16 tokens of a step: page and token in it, and the id, read a step ahead of its use
       int pg, off, id, id_off;
@@ -1355,13 +1356,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
         const int tok = (step + sub) * kTile + 16 * j;  // of the wave's first
         uint16_t kd[2] = {ks[0], ks[1]};
         uint32_t vd[4] = {vs[0], vs[1], vs[2], vs[3]};
-        if (!there || tok + 16 > s.len) {  // scales of no token are 0
+        if (!there || tok + 16 > held) {  // scales of no token are 0
 #pragma unroll
-          for (int n = 0; n < 2; n++) kd[n] = there && tok + ktok < s.len ? kd[n] : 0;
+          for (int n = 0; n < 2; n++) kd[n] = there && tok + ktok < held ? kd[n] : 0;
 #pragma unroll
           for (int n = 0; n < 4; n++) {
             const int at = tok + 4 * vt + 2 * (n & 1);
-            vd[n] &= there ? (at + 1 < s.len ? 0xFFFFFFFFu : at < s.len ? 0xFFFFu : 0u) : 0u;
+            vd[n] &= there ? (at + 1 < held ? 0xFFFFFFFFu : at < held ? 0xFFFFu : 0u) : 0u;
           }
         }
         if (vc == 0) x.vs[j][vt][vp] = u32x4{vd[0], vd[1], vd[2], vd[3]};
@@ -1797,7 +1798,7 @@ Pieces pieces_in(void* ws, int64_t items, int64_t workers, int cols) {
 }
 
 template <int D, class E>
-hipError_t merge(hipStream_t st, const Kv4Attn& a, const Pieces& pc, int64_t items, int64_t workers, int cols, int64_t cap, int start) {
+hipError_t merge(hipStream_t st, const Kv4Attn& a, const Pieces& pc, int64_t items, int64_t workers, int cols, int cap, int start) {
   const int group = a.n_q / a.c.n_kv;
   const Lines L{a.row_offsets, a.lengths, a.rows, a.c.n_kv, group, a.window, cols, cap, start, false};
   // Waves a column: more where an item has many pieces, but not where there are columns enough
@@ -1812,12 +1813,13 @@ hipError_t merge(hipStream_t st, const Kv4Attn& a, const Pieces& pc, int64_t ite
   return hipGetLastError();
 }
 
-int64_t attn_cap(const Kv4Attn& a) { return std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0); }
+int attn_cap(const Kv4Attn& a) { return (int)std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0); }
 
 template <int D, int NT, class E>
 hipError_t attn_tiles(hipStream_t st, const Kv4Attn& a) {
   const int cols = 16 * NT;
-  const int64_t cap = attn_cap(a), tiles = (cap + kTile - 1) / kTile;
+  const int cap = attn_cap(a);
+  const int64_t tiles = ((int64_t)cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
   const bool whole = tiles <= kWhole;
   const int64_t most = (int64_t)compute_units() * 4 * attn_waves(D, NT, Terms<E>::n);
@@ -1833,7 +1835,8 @@ hipError_t attn_tiles(hipStream_t st, const Kv4Attn& a) {
 template <class E>
 hipError_t attn_prompt(hipStream_t st, const Kv4Attn& a) {
   constexpr int cols = 32 * kPromptWaves;
-  const int64_t cap = attn_cap(a), tiles = (cap + kTile - 1) / kTile;
+  const int cap = attn_cap(a);
+  const int64_t tiles = ((int64_t)cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
   const int64_t most = (int64_t)compute_units() * (8 / kPromptWaves), want = (items * (tiles + kPromptStart) + kPromptLeast - 1) / kPromptLeast;
   const int workers = (int)std::min(most, want);

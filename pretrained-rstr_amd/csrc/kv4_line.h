@@ -16,10 +16,12 @@ __host__ __device__ inline int at_most(int v, int hi) { return v < hi ? v : hi; 
 struct Lines {
   const int32_t *ro, *lens;
   int rows, n_kv, group, window, cols;  // cols: of a column tile
-  int64_t cap;                          // tokens that a page table row can hold
+  int cap;                              // tokens that a page table row can hold
   int start;                            // what beginning an item costs, in tiles
   bool whole;                           // one unit an item
   __host__ __device__ inline int per_item(int tiles) const { return whole ? 1 : tiles + start; }
+  // tokens that are there of a sequence of `len`: its length gives its rows' positions, the table its end
+  __host__ __device__ inline int held(int len) const { return at_most(len, cap); }
 };
 struct Seq {
   int r0, m, len, lo, tiles, nct;
@@ -35,10 +37,9 @@ __host__ __device__ inline Seq sequence(const Lines& L, int b) {
   s.r0 = at_most(at_least(begin, 0), L.rows);
   s.m = at_least(at_most(at_least(end, 0), L.rows) - s.r0, 0);
   s.len = at_least(L.lens[b], 0);
-  if (s.len > L.cap) s.len = (int)L.cap;
   const int64_t lo = L.window > 0 ? (int64_t)s.len - s.m + 1 - L.window : 0;
   s.lo = lo > 0 ? (int)lo / kTile : 0;  // first tile
-  s.tiles = at_least((int)(((int64_t)s.len + kTile - 1) / kTile) - s.lo, 0);
+  s.tiles = at_least((int)(((int64_t)L.held(s.len) + kTile - 1) / kTile) - s.lo, 0);
   s.nct = (int)(((int64_t)s.m * L.group + L.cols - 1) / L.cols);
   s.units = (int64_t)L.n_kv * s.nct * L.per_item(s.tiles);
   return s;

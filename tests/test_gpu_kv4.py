@@ -621,3 +621,30 @@ def test_values_of_very_different_size(sess, dtype, rows, D, what, small):
     assert far.max() <= 0, (far.max(), np.unravel_index(far.argmax(), far.shape))
     plan.close()
     c.close()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,D,held,length,window", [
+    (1, 64, 64, 100, 50), (1, 64, 64, 100, 0), (3, 128, 64, 65, 0), (3, 128, 64, 66, 20), (2, 256, 320, 400, 100), (9, 64, 320, 324, 40),
+    (1, 128, 64, 200, 50), (40, 128, 320, 345, 0), (70, 128, 320, 380, 100), (60, 128, 320, 1000, 30), (3, 128, 320, 2 ** 31 - 1, 2 ** 31 - 30),
+    (50, 128, 320, 2 ** 31 - 1, 2 ** 31 - 30), (2, 64, 320, 2 ** 31 - 1, 0),
+])
+def test_lengths_beyond_the_table(sess, dtype, rows, D, held, length, window):
+    """A row's position follows from the sequence's length, also where the table ends before it: the tokens
+    behind the table's width are not seen, and nothing else changes."""
+    print("beyond the table", dtype, rows, D, held, length, window, flush=True)
+    c = Case(sess, 4, 2, D, 16, [held], [rows])
+    q = c.queries(dtype)
+    out = torch.full_like(q, 7.0).cuda()
+    plan = c.plan()
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32([length]), out, window=window)
+    want, mag, size, _ = _attention_by_position(P.as_f64(q), c.k[0], c.v[0], length, window, D ** -0.5)
+    rel = 2 * (D + 16) * 2.0 ** -24 * 10 * size + (2.0 ** -10 if dtype != "f32" else 2.0 ** -22 + held * 2.0 ** -27)
+    if dtype == "bf16" and rows > 16:
+        rel = rel + 2.0 ** -10 * size
+    eps = torch.finfo(TYPES[dtype]).eps
+    tol = rel * mag + eps / 2 * np.abs(want) * 1.01 + held * 2.0 ** -33 * np.abs(c.v[0]).max() + torch.finfo(TYPES[dtype]).smallest_normal * eps / 2
+    far = np.abs(P.as_f64(out) - want) - tol
+    assert far.max() <= 0, (far.max(), np.unravel_index(far.argmax(), far.shape))
+    plan.close()
+    c.close()
