@@ -571,12 +571,9 @@ struct Pieces {
   float* acc;   // [2 * workers][cols][D]
 };
 
-// a / b of numbers below 2^53 (units of work), in an eighth of the instructions that 64-bit division is.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  const int64_t q = (int64_t)((double)a * __builtin_amdgcn_rcp((double)b));
-  const int64_t r = a - q * b;
-  return r < 0 ? q - 1 : r >= b ? q + 1 : q;
-}
+// a / b of numbers of units without the loop that 64-bit division is.  (The reciprocal instruction
+// gives an estimate, good to about 2^-23.)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return quotient_from(a, b, __builtin_amdgcn_rcp((double)b)); }
 
 // The parts of items that a wave (or a workgroup) works on, in their order.  A wave holds the sequences
 // 64 at a time, one a lane.

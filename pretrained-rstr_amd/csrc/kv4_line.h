@@ -12,6 +12,16 @@ constexpr int kTile = 32;
 __host__ __device__ inline int at_least(int v, int lo) { return v > lo ? v : lo; }
 __host__ __device__ inline int at_most(int v, int hi) { return v < hi ? v : hi; }
 
+// a / b for 0 <= a < 2^52 and b > 0, from an estimate r of 1 / b within 2^-20 of it: two Newton steps
+// leave it within 2^-52 of itself and a step of its rounding, so that a * r is off by less than 1 where the quotient is below 2^50.
+__host__ __device__ inline int64_t quotient_from(int64_t a, int64_t b, double r) {
+  const double d = (double)b;
+  r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  const int64_t q = (int64_t)((double)a * r), rest = a - q * b;
+  return rest < 0 ? q - 1 : rest >= b ? q + 1 : q;
+}
+
 // The sequences of a call, as every wave sees them.
 struct Lines {
   const int32_t *ro, *lens;

@@ -1,5 +1,6 @@
 // The items that attention over the 4-bit cache makes of a call's row offsets, whatever these
-// hold: their numbers stay inside the room that the host counts for them.
+// hold: their numbers stay inside the room that the host counts for them.  And the division that cuts
+// them into parts.
 #include <cstdio>
 #include <cstdlib>
 #include <vector>
@@ -35,8 +36,26 @@ static bool call(const std::vector<int32_t>& ro, int rows, int n_q, int n_kv, in
   return true;
 }
 
+// Quotients up to 2^49 from reciprocals as far off as an estimate may be.
+static void quotients() {
+  const auto random = [](int bits) { return (int64_t)((((uint64_t)rand() << 31 | (uint64_t)rand()) << 2 | (rand() & 3)) >> (64 - bits)); };
+  for (int i = 0; i < 2000000; i++) {
+    const int bits = 1 + rand() % 49, of = rand() % (52 - bits);
+    const int64_t b = 1 + random(of + 1) % ((int64_t)1 << of), q = random(bits);
+    const int64_t least = q * b, a = i % 3 == 0 ? least : i % 3 == 1 ? least + b - 1 : least + random(50) % b;
+    const double off = (rand() % 2001 - 1000) / 1000.0 * 0x1p-22;
+    const int64_t got = quotient_from(a, b, 1.0 / (double)b * (1.0 + off));
+    checks++;
+    if (got != a / b) {
+      printf("%lld / %lld: %lld, not %lld\n", (long long)a, (long long)b, (long long)got, (long long)(a / b));
+      exit(1);
+    }
+  }
+}
+
 int main() {
   srand(1);
+  quotients();
   const int heads[][2] = {{1, 1}, {32, 8}, {8, 8}, {24, 1}, {4, 1}};
   for (const auto& h : heads)
     for (int cols : {16, 32, 256}) {
