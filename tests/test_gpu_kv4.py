@@ -648,3 +648,76 @@ def test_lengths_beyond_the_table(sess, dtype, rows, D, held, length, window):
     assert far.max() <= 0, (far.max(), np.unravel_index(far.argmax(), far.shape))
     plan.close()
     c.close()
+
+
+# ---- append and read in prompt quantity -----------------------------------------------------
+def _quantised_all(x):
+    """P.quantised, all blocks at once."""
+    w = np.asarray(x, np.float64).reshape(-1, 32)
+    finite = np.isfinite(w).all(1)
+    w = np.where(finite[:, None], w, 0.0)
+    m = w[np.arange(len(w)), np.abs(w).argmax(1)]
+    d = np.clip(m / -8.0, -65504.0, 65504.0).astype(np.float16).astype(np.float64)[:, None]
+    o = np.where(d == 0, 0.0, d * np.clip(np.rint(w / np.where(d == 0, 1.0, d)), -8, 7))
+    return np.where(finite[:, None], o, np.nan).reshape(np.shape(x))
+
+
+def _prompt_slots(rng, rows, room, order):
+    """Slots of `rows` rows: as consecutive pages' tokens from a place inside a group of four or
+    of sixteen, in any order, or with rows that have none, the first among them."""
+    if order == "aligned":
+        return np.arange(32, 32 + rows)
+    if order == "run":
+        return np.arange(21, 21 + rows)
+    if order == "backwards":
+        return np.arange(rows)[::-1] + 7
+    if order == "permuted":
+        return rng.permutation(room)[:rows]
+    if order == "groups":  # whole groups of four tokens, in any order
+        return (rng.permutation(room // 4)[:, None] * 4 + np.arange(4)).reshape(-1)[:rows]
+    slots = np.arange(rows) + 2
+    slots[rng.random(rows) < 0.1] = -1
+    slots[rng.random(rows) < 0.05] = room + 3
+    slots[0] = -1 if order == "none_first" else room if order == "outside_first" else 2 ** 31 - 1
+    return slots
+
+
+@pytest.mark.parametrize("D,heads,page,rows", [(64, 8, 16, 4099), (128, 8, 48, 2066), (256, 1, 32, 8193)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("order,how", [("aligned", "plain"), ("run", "padded"), ("backwards", "odd"), ("permuted", "plain"), ("groups", "heads_outside"),
+                                       ("none_first", "odd"), ("outside_first", "plain"), ("largest_first", "heads_outside")])
+def test_append_read_prompts(sess, D, heads, page, rows, dtype, order, how):
+    """Rows enough for four a thread, bit for bit."""
+    print("append prompt", D, heads, page, rows, dtype, order, how, flush=True)
+    rng = np.random.default_rng([D, len(order)])
+    pages = -(-(rows + 40) // page) + 2
+    room = pages * page
+    pool = hip.Kv4Pool(sess, 2, heads, D, page, pages)
+    k = torch.tensor(_hard_rows(rng, rows, heads, D)).to(TYPES[dtype])
+    v = torch.tensor(_hard_rows(rng, rows, heads, D) * 1.5).to(TYPES[dtype])
+    slots = _prompt_slots(rng, rows, room, order)
+    pool.append(1, _laid(k, how), _laid(v, how), _i32(slots))
+    there = (slots >= 0) & (slots < room)
+    free = np.setdiff1d(np.arange(room), slots[there])
+    # as they were appended; then any order, some twice, with those that were never written
+    mixed = np.concatenate([slots, free, slots[:rows // 3]])
+    for listed in (slots, rng.permutation(mixed)):
+        ko = _laid(torch.full((len(listed), heads, D), 9.0, dtype=TYPES[dtype]), how)
+        vo = _laid(torch.full((len(listed), heads, D), 9.0, dtype=TYPES[dtype]), how)
+        pool.read(1, _i32(listed), ko, vo)
+        for x, o in ((k, ko), (v, vo)):
+            held = np.zeros((room + 1, heads, D))
+            held[slots[there]] = _quantised_all(P.as_f64(x))[there]
+            want = held[np.where((listed >= 0) & (listed < room), listed, room)]
+            want = torch.tensor(want).to(torch.float32).to(TYPES[dtype])
+            got = o.cpu()
+            same = (got == want) | (got.isnan() & want.isnan())
+            assert bool(same.all()), (torch.nonzero(~same)[:4], got[~same][:4], want[~same][:4])
+    pool.read(0, _i32(slots), ko[:rows], vo[:rows])  # the other layer is untouched
+    assert not ko[:rows].any() and not vo[:rows].any()
+    pool.close()
+
+
+def test_all_blocks_at_once():
+    x = _hard_rows(np.random.default_rng(2), 24, 2, 64)
+    assert np.array_equal(_quantised_all(x), P.quantised(x), equal_nan=True)
