@@ -721,3 +721,58 @@ def test_append_read_prompts(sess, D, heads, page, rows, dtype, order, how):
 def test_all_blocks_at_once():
     x = _hard_rows(np.random.default_rng(2), 24, 2, 64)
     assert np.array_equal(_quantised_all(x), P.quantised(x), equal_nan=True)
+
+
+# ---- attention of many sequences --------------------------------------------------------------
+def _lines(rng, B, most, rows, gaps):
+    """Ragged lengths and rows of B sequences; those of `gaps` have no rows."""
+    lens = rng.integers(0, most, B)
+    news = rng.integers(1, rows + 1, B)
+    news[gaps] = 0
+    lens[[1, B - 1]], news[[1, B - 1]] = [most, most - 1], rows
+    return lens.tolist(), news.tolist()
+
+
+@pytest.mark.parametrize("B,gaps,rows,n_q,n_kv,D", [
+    (65, [63, 64], 1, 8, 2, 128), (65, [0], 1, 4, 1, 256), (128, [63, 64, 126], 1, 8, 2, 64), (128, [], 1, 32, 8, 128),
+    (200, list(range(60, 140)), 1, 8, 2, 128), (200, list(range(64, 128)), 1, 4, 2, 64),
+    (65, [63], 6, 16, 2, 128), (130, [64, 127, 128], 5, 16, 2, 64), (200, list(range(64, 199)), 6, 8, 2, 128), (129, [0, 2, 64], 3, 4, 1, 256),
+])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_of_many_sequences(sess, B, gaps, rows, n_q, n_kv, D, dtype):
+    """More sequences than a wave has lanes, and tables of many tiles: items of every 64 sequences are
+    cut and joined."""
+    print("many sequences", B, rows, n_q, n_kv, D, dtype, flush=True)
+    rng = np.random.default_rng([B, rows, D])
+    lens, news = _lines(rng, B, 420, rows, gaps)
+    c = Case(sess, n_q, n_kv, D, 16, lens, news)
+    q = c.queries(dtype, behind=2)
+    plan = c.plan(behind=2)
+    for window in (0, 90):
+        out = torch.full_like(q, 7.0).cuda()
+        plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(lens), out, max_rows=max(news), window=window)
+        c.check(out, q, dtype, window, D ** -0.5)
+        assert bool((out[int(c.offsets[-1]):] == 7.0).all())
+    plan.close()
+    c.close()
+
+
+@pytest.mark.parametrize("B,gaps", [(66, [0]), (70, [63, 64]), (140, list(range(64, 131)))])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attention_of_many_prompts(sess, B, gaps, dtype):
+    """The same where waves share a tile's expansion: 64 columns a sequence and more, on average too."""
+    print("many prompts", B, dtype, flush=True)
+    rng = np.random.default_rng(B)
+    lens, news = _lines(rng, B, 330, 20, gaps)
+    news = [m + (28 if m and B == 140 else 8 if m else 0) for m in news]
+    assert sum(news) * 4 >= 64 * B and max(news) * 4 >= 64
+    c = Case(sess, 8, 2, 128, 16, lens, news)
+    q = c.queries(dtype, behind=2)
+    plan = c.plan(behind=2)
+    for window in (0, 90):
+        out = torch.full_like(q, 7.0).cuda()
+        plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(lens), out, max_rows=max(news), window=window)
+        c.check(out, q, dtype, window, 128 ** -0.5)
+        assert bool((out[int(c.offsets[-1]):] == 7.0).all())
+    plan.close()
+    c.close()
