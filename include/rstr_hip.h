@@ -409,7 +409,8 @@ int64_t rstr_kv4_bytes(const rstr_kv4* p);
 int rstr_kv4_append(rstr_kv4* p, int32_t layer, int32_t rows, int32_t dtype, const void* k, int64_t k_row,
                     int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int32_t* slots, void* stream);
 /* The values that slots[rows] hold, rounded once to the output's type, as rows
- * k, v; zeros for a slot outside the cache.  A slot may be listed twice. */
+ * k, v; zeros for a slot outside the cache.  A slot may be listed twice.  Keys and
+ * values may lie in one array, not in the same elements. */
 int rstr_kv4_read(rstr_kv4* p, int32_t layer, int32_t rows, int32_t dtype, const int32_t* slots, void* k,
                   int64_t k_row, int64_t k_head, void* v, int64_t v_row, int64_t v_head, void* stream);
 
@@ -433,7 +434,7 @@ int rstr_kv4_attn_close(rstr_kv4_attn* a);
  * row_offsets[batch] are left as they are; where row_offsets decrease anywhere, nothing is
  * written.
  * max_rows: the most rows a sequence of this call has (it chooses the tile; a sequence
- * with more is still computed). */
+ * with more is still computed).  out overlaps no input. */
 int rstr_kv4_attn_run(rstr_kv4_attn* a, int32_t layer, int32_t dtype, int32_t batch, int32_t rows,
                       int32_t max_rows, int32_t window, float scale, const void* q, int64_t q_row, int64_t q_head,
                       const int32_t* row_offsets, const int32_t* page_table, int32_t pages_per_seq,
@@ -475,7 +476,8 @@ int rstr_verify_close(rstr_verify* v);
  * the largest), are greedy: the draft is accepted if it is the first largest
  * logit, which is the token otherwise.  Drafts outside the vocabulary are refused.  accepted[b] is the number
  * of drafts accepted; tokens[rows] are those drafts, then the token, then -1.
- * Random numbers lie in [0, 1).  Rows behind row_offsets[batch] are left as they are. */
+ * Random numbers lie in [0, 1).  Rows behind row_offsets[batch] are left as they are.
+ * Outputs overlap no input. */
 int rstr_verify_run(rstr_verify* v, int32_t dtype, int32_t batch, int32_t rows, const void* logits,
                     int64_t logits_row, const int32_t* row_offsets, const int32_t* drafts, const float* draft_probs,
                     int64_t probs_row, const float* temperature, const float* u_accept, const float* u_sample,

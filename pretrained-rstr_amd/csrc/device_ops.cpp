@@ -73,6 +73,18 @@ bool ranges_meet(const void* a, size_t an, const void* b, size_t bn) {
   return ranges_meet((uintptr_t)a, (uintptr_t)a + an, (uintptr_t)b, (uintptr_t)b + bn);
 }
 
+// Do two arrays of one shape share an element?  Where their ranges meet they do not if, on the same
+// strides, one lies in the gaps of the other: between its rows or its heads.
+bool share(const Rows& a, const Rows& b, int64_t rows, int64_t heads, int64_t hd, int size) {
+  if (!ranges_meet((uintptr_t)a.p, rows_end(a, rows, heads, hd, size), (uintptr_t)b.p, rows_end(b, rows, heads, hd, size))) return false;
+  const uintptr_t bytes = a.p < b.p ? (uintptr_t)b.p - (uintptr_t)a.p : (uintptr_t)a.p - (uintptr_t)b.p;
+  if (a.row != b.row || a.head != b.head || bytes % size) return true;
+  const int64_t d = (int64_t)(bytes / size);
+  const auto between = [&](int64_t stride, int64_t span) { return stride > 0 && d % stride >= span && d % stride + span <= stride; };
+  return !(between(a.row, (heads - 1) * a.head + hd) || between(a.head, (rows - 1) * a.row + hd) ||
+           (a.head > 0 && a.row % a.head == 0 && between(a.head, hd)) || (a.row > 0 && a.head % a.row == 0 && between(a.row, hd)));
+}
+
 int check_rows(rstr_session* s, const char* what, const Rows& r, int size) {
   if (!r.p) return fail(s, RSTR_E_INVALID, std::string("null ") + what + " rows");
   if (!aligned(r.p, size)) return fail(s, RSTR_E_INVALID, std::string(what) + " rows are not aligned to their elements");
@@ -190,6 +202,11 @@ extern "C" int rstr_kv4_read(rstr_kv4* p, int32_t layer, int32_t rows, int32_t d
   if (rows == 0) return RSTR_OK;
   if (!apart(kr, rows, p->n_kv, p->hd) || !apart(vr, rows, p->n_kv, p->hd))
     return fail(s, RSTR_E_INVALID, "output rows share elements");
+  const int size = elem_size(dtype);
+  if (share(kr, vr, rows, p->n_kv, p->hd, size)) return fail(s, RSTR_E_INVALID, "output keys and values share elements");
+  for (const Rows& o : {kr, vr})
+    if (ranges_meet((uintptr_t)slots, (uintptr_t)(slots + rows), (uintptr_t)o.p, rows_end(o, rows, p->n_kv, p->hd, size)))
+      return fail(s, RSTR_E_INVALID, "output rows overlap the slots");
   OnDevice dev(s->device);
   HIPCHK(s, dev.e);
   HIPCHK(s, launch_kv4_read(on_stream(s, stream), layer_of(p, layer), dtype, rows, slots, kr, vr));
@@ -257,6 +274,10 @@ extern "C" int rstr_kv4_attn_run(rstr_kv4_attn* a, int32_t layer, int32_t dtype,
   if (!apart(o, rows, a->n_q, p->hd)) return fail(s, RSTR_E_INVALID, "output rows share elements");
   if (ranges_meet((uintptr_t)q, rows_end(qr, rows, a->n_q, p->hd, size), (uintptr_t)out, rows_end(o, rows, a->n_q, p->hd, size)))
     return fail(s, RSTR_E_INVALID, "output overlaps the queries");
+  const struct { const int32_t* p; int64_t n; } ints[] = {{row_offsets, batch + (int64_t)1}, {page_table, (int64_t)batch * pages_per_seq}, {lengths, batch}};
+  for (const auto& x : ints)
+    if (ranges_meet((uintptr_t)x.p, (uintptr_t)(x.p + x.n), (uintptr_t)out, rows_end(o, rows, a->n_q, p->hd, size)))
+      return fail(s, RSTR_E_INVALID, "output overlaps the sequences' tables");
   Kv4Attn k{};
   k.c = layer_of(p, layer);
   k.n_q = a->n_q;
@@ -382,10 +403,12 @@ extern "C" int rstr_verify_run(rstr_verify* v, int32_t dtype, int32_t batch, int
     for (const auto& x2 : in)
       if (ranges_meet(x2.p, x2.n, accepted, n) || ranges_meet(x2.p, x2.n, tokens, r))
         return fail(s, RSTR_E_INVALID, "verification outputs overlap its inputs");
-    const uintptr_t x1 = rows_end(x, rows, 1, v->vocab, size);
-    if (ranges_meet((uintptr_t)logits, x1, (uintptr_t)accepted, (uintptr_t)accepted + n) ||
-        ranges_meet((uintptr_t)logits, x1, (uintptr_t)tokens, (uintptr_t)tokens + r))
-      return fail(s, RSTR_E_INVALID, "verification outputs overlap its inputs");
+    const Rows probs{(void*)draft_probs, probs_row, 0};
+    const struct { uintptr_t a, b; } wide[] = {{(uintptr_t)logits, rows_end(x, rows, 1, v->vocab, size)},
+                                               {(uintptr_t)draft_probs, draft_probs ? rows_end(probs, rows, 1, v->vocab, 4) : 0}};
+    for (const auto& y : wide)
+      if (ranges_meet(y.a, y.b, (uintptr_t)accepted, (uintptr_t)accepted + n) || ranges_meet(y.a, y.b, (uintptr_t)tokens, (uintptr_t)tokens + r))
+        return fail(s, RSTR_E_INVALID, "verification outputs overlap its inputs");
     if (ranges_meet(accepted, n, tokens, r)) return fail(s, RSTR_E_INVALID, "verification outputs overlap");
   }
   Verify a{batch, rows, v->vocab, logits, logits_row, row_offsets, drafts, draft_probs, probs_row, temperature,

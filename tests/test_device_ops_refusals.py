@@ -254,3 +254,50 @@ def test_verify(dev):
                           ("shape", dict(u_sample=Dev((5,)))), ("int32", dict(drafts=Dev((5,), "int64"))),
                           ("session's GPU", dict(logits=Dev((5, 100), device=1)))):
             refused(dev, ValueError, match, lambda: run(**kw))
+
+
+def inside(x, other, at):
+    """The array x over the memory of another, from byte `at` on."""
+    x._keep, x._shift = other._keep, at
+    return x
+
+
+def test_reads_into_shared_memory(dev):
+    with hip.Session(0) as s:
+        p = hip.Kv4Pool(s, 1, 2, 128, 16, 4)
+        sl = ints(3)
+        one = Dev((3, 2, 2, 128))
+        read = lambda at, strides: p.read(0, sl, inside(Dev((3, 2, 128), strides=strides), one, 0), inside(Dev((3, 2, 128), strides=strides), one, 4 * at))  # noqa: E731
+        read(256, (512, 128, 1))     # [rows][k, v][heads][head_dim]
+        read(128, (512, 256, 1))     # [rows][heads][k, v][head_dim]
+        read(384, (128, 768, 1))     # [heads][k, v][rows][head_dim]
+        read(128, (256, 768, 1))     # [heads][rows][k, v][head_dim]
+        read(768, (256, 128, 1))     # one behind the other
+        read(384 * 2, (128, 384, 1))
+        for at, strides in ((0, (256, 128, 1)), (128, (512, 128, 1)), (255, (512, 128, 1)), (127, (512, 256, 1)), (256, (256, 128, 1)),
+                            (257, (512, 128, 1)), (383, (128, 768, 1)), (64, (512, 256, 1)), (640, (256, 128, 1))):
+            refused(dev, hip.RstrError, "share elements", lambda: read(at, strides))
+        k, v = Dev((3, 2, 128)), Dev((3, 2, 128))
+        refused(dev, hip.RstrError, "overlap the slots", lambda: p.read(0, inside(ints(3), k, 4 * 767), k, v))
+        refused(dev, hip.RstrError, "overlap the slots", lambda: p.read(0, inside(ints(3), v, 0), k, v))
+        p.read(0, inside(ints(3), v, 4 * 768), k, v)
+
+
+def test_outputs_inside_tables_and_probabilities(dev):
+    with hip.Session(0) as s:
+        p = hip.Kv4Pool(s, 2, 2, 128, 16, 4)
+        plan = hip.Kv4Attention(p, 4, 2, 5)
+        out = Dev((5, 4, 128))
+        for which, a in enumerate((ints(3), ints((2, 7)), ints(2))):
+            tables = [ints(3), ints((2, 7)), ints(2)]
+            tables[which] = inside(a, out, 4 * (5 * 4 * 128 - 1))
+            refused(dev, hip.RstrError, "overlaps the sequences' tables", lambda: plan.run(0, Dev((5, 4, 128)), *tables, out))
+            tables[which] = inside(a, out, 4 * 5 * 4 * 128)
+            plan.run(0, Dev((5, 4, 128)), *tables, out)
+        v = hip.Verifier(s, 2, 5, 100)
+        base = dict(logits=Dev((5, 100)), row_offsets=ints(3), drafts=ints(5), temperature=Dev((2,)), u_accept=Dev((5,)), u_sample=Dev((2,)),
+                    accepted=ints(2), tokens=ints(5))
+        for name, n in (("tokens", 5), ("accepted", 2)):
+            probs = Dev((5, 100))
+            refused(dev, hip.RstrError, "overlap", lambda: v.run(**{**base, name: inside(ints(n), probs, 4 * 499)}, draft_probs=probs))
+            v.run(**{**base, name: inside(ints(n), probs, 4 * 500)}, draft_probs=probs)
