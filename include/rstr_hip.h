@@ -415,7 +415,8 @@ int rstr_kv4_read(rstr_kv4* p, int32_t layer, int32_t rows, int32_t dtype, const
                   int64_t k_row, int64_t k_head, void* v, int64_t v_row, int64_t v_head, void* stream);
 
 /* A plan for attention of up to max_batch sequences and max_rows query rows of
- * n_q heads: the call's workspace.  One plan serves one call at a time: calls
+ * n_q heads: the call's workspace.  n_kv * (max_rows * (n_q / n_kv) / 16 + the
+ * smaller of max_rows and max_batch) < 2^24.  One plan serves one call at a time: calls
  * (and graphs that hold them) that may run at once need a plan each. */
 int rstr_kv4_attn_open(rstr_kv4* p, int32_t n_q, int32_t max_batch, int32_t max_rows, rstr_kv4_attn** out);
 /* Waits for the device. */
@@ -459,7 +460,7 @@ int rstr_step_maps(rstr_session* s, int32_t page_size, int32_t batch, int32_t pa
                    int32_t* row_offsets, int32_t* positions, int32_t* slots, int32_t* pages_taken, void* stream);
 
 /* Workspace for the verification of up to max_batch sequences and max_rows rows
- * over a vocabulary (up to RSTR_VERIFY_VOCAB).  One call at a time, as with
+ * (below 2^24 of each) over a vocabulary (up to RSTR_VERIFY_VOCAB).  One call at a time, as with
  * attention plans. */
 #define RSTR_VERIFY_VOCAB (1 << 24)
 int rstr_verify_open(rstr_session* s, int32_t max_batch, int32_t max_rows, int32_t vocab, rstr_verify** out);

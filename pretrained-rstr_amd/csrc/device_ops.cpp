@@ -10,6 +10,7 @@
 #include <string>
 
 #include "kv4.h"
+#include "kv4_line.h"
 #include "session.h"
 
 using namespace rstr;
@@ -97,6 +98,8 @@ int check_ints(rstr_session* s, const char* what, const int32_t* p) {
   if (!aligned(p, 4)) return fail(s, RSTR_E_INVALID, std::string(what) + " not aligned to its elements");
   return RSTR_OK;
 }
+
+constexpr int64_t kGridGroups = 1 << 24;  // workgroups of 256 threads that a grid cannot hold any more
 
 #define TRY(expr)                \
   do {                           \
@@ -220,7 +223,8 @@ extern "C" int rstr_kv4_attn_open(rstr_kv4* p, int32_t n_q, int32_t max_batch, i
   *out = nullptr;
   if (n_q <= 0 || n_q % p->n_kv) return fail(s, RSTR_E_INVALID, "query heads must be a multiple of the cache's kv heads");
   if (max_batch <= 0 || max_rows <= 0) return fail(s, RSTR_E_INVALID, "attention plan extents must be positive");
-  if ((int64_t)max_rows * n_q > 0x7FFFF000) return fail(s, RSTR_E_INVALID, "attention plan has too many rows");
+  // a workgroup of up to 256 threads an item joins its pieces, and a grid holds fewer than 2^32 threads
+  if ((int64_t)max_rows * n_q > 0x7FFFF000 || attn_items(n_q, p->n_kv, max_batch, max_rows, 16) >= kGridGroups) return fail(s, RSTR_E_INVALID, "attention plan has too many rows");
   std::unique_ptr<rstr_kv4_attn> a(new (std::nothrow) rstr_kv4_attn());
   if (!a) return fail(s, RSTR_E_OOM, "attention plan handle");
   OnDevice dev(s->device);
@@ -350,6 +354,7 @@ extern "C" int rstr_verify_open(rstr_session* s, int32_t max_batch, int32_t max_
   if (!out) return fail(s, RSTR_E_INVALID, "null output pointer");
   *out = nullptr;
   if (max_batch <= 0 || max_rows <= 0 || vocab <= 0) return fail(s, RSTR_E_INVALID, "verification extents must be positive");
+  if (max_batch >= kGridGroups || max_rows >= kGridGroups) return fail(s, RSTR_E_INVALID, "verification has too many rows");
   if (vocab > RSTR_VERIFY_VOCAB) return fail(s, RSTR_E_INVALID, "vocabulary is too large for verification");
   std::unique_ptr<rstr_verify> v(new (std::nothrow) rstr_verify());
   if (!v) return fail(s, RSTR_E_OOM, "verification handle");

@@ -301,3 +301,21 @@ def test_outputs_inside_tables_and_probabilities(dev):
             probs = Dev((5, 100))
             refused(dev, hip.RstrError, "overlap", lambda: v.run(**{**base, name: inside(ints(n), probs, 4 * 499)}, draft_probs=probs))
             v.run(**{**base, name: inside(ints(n), probs, 4 * 500)}, draft_probs=probs)
+
+
+def test_plans_past_a_grid(dev):
+    """Rows or sequences of which a launch cannot have a workgroup each."""
+    blocks = dev.fake_blocks()
+    with hip.Session(0) as s:
+        p = hip.Kv4Pool(s, 1, 8, 64, 16, 4)
+        for n_q, batch, rows in ((8, 1 << 22, 1 << 22), (32, 1, (1 << 26) - 1024), (8, 1, 1 << 25)):
+            with pytest.raises(hip.RstrError, match="too many rows"):
+                hip.Kv4Attention(p, n_q, batch, rows)
+        hip.Kv4Attention(p, 8, 1 << 20, 1 << 20).close()
+        hip.Kv4Attention(p, 32, 1 << 20, 1 << 17).close()
+        for batch, rows in ((1, 1 << 24), (1 << 24, 1), (1, 2 ** 31 - 1)):
+            with pytest.raises(hip.RstrError, match="too many rows"):
+                hip.Verifier(s, batch, rows, 2)
+        hip.Verifier(s, 1 << 23, 1 << 23, 2).close()
+        p.close()
+    assert dev.fake_blocks() == blocks
