@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <type_traits>
 
@@ -1760,11 +1761,13 @@ hipError_t launch_kv4_read(hipStream_t st, const Kv4Layer& c, int dtype, int row
 namespace {
 
 int compute_units() {
-  static int n[64] = {};
-  int dev = 0;
+  static std::atomic<int> known[64];  // calls may come from several threads
+  int dev = 0, n = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (n[dev] == 0 && (hipDeviceGetAttribute(&n[dev], hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n[dev] <= 0)) n[dev] = 256;
-  return n[dev];
+  if ((n = known[dev].load(std::memory_order_relaxed)) != 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 constexpr int kPromptWaves = 8;
