@@ -541,12 +541,8 @@ template <class E> struct Terms { static constexpr int n = 1; static constexpr b
 template <> struct Terms<F32> { static constexpr int n = 2; static constexpr bool ONCE = true; };
 template <> struct Terms<BF16> { static constexpr int n = 1; static constexpr bool ONCE = false; };
 
-// Waves a SIMD: what the registers of a form allow.  (NT = 1 with two waves and rings of four tiles: 84 us for the 80
-// above, 55 for the 51, with a merge of fewer pieces that is as much shorter.)
-constexpr int attn_waves(int hd, int nt, int terms) { return hd == 256 ? 1 : nt == 1 ? 3 : 2; }
-
 // Tiles of a wave's ring: what 160 KB of LDS hold for that many waves.
-constexpr int attn_ring(int hd, int nt, int terms) { return attn_waves(hd, nt, terms) == 3 && hd == 128 ? 2 : 4; }
+constexpr int attn_ring(int hd, int nt) { return attn_waves(hd, nt) == 3 && hd == 128 ? 2 : 4; }
 
 // The value of one lane, the same for all.
 __device__ __forceinline__ int64_t lane64(int64_t v, int lane) {
@@ -748,7 +744,7 @@ __device__ __forceinline__ void wait_loads() {
 }
 
 template <int D, int NT, int NS, class E>
-__global__ void __launch_bounds__(256, attn_waves(D, NT, Terms<E>::n))
+__global__ void __launch_bounds__(256, attn_waves(D, NT))
     k_kv4_attn(Kv4Attn a, const int32_t* __restrict__ ro, const int32_t* __restrict__ lens, const int32_t* __restrict__ table,
                const uint8_t* __restrict__ base, Pieces pc, int workers, int least, bool whole) {
   typedef Rec<D> R;
@@ -1770,18 +1766,12 @@ int compute_units() {
   return n;
 }
 
-constexpr int kPromptWaves = 8;
 constexpr int kMergeWaves = 4096;
 constexpr int kWhole = 4;        // tiles of an item that one wave does, without a merge
 constexpr int kLeast = 2;        // tiles a wave takes at least
 constexpr int kPromptLeast = 4;  // and a workgroup of k_kv4_prompt
 
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
-
-// Workspace: what up to `workers` waves leave of items that they share.
-size_t attn_bytes(int64_t items, int64_t workers, int cols, int hd) {
-  return 256 + align256(sizeof(Begun) * items) + align256(sizeof(float2) * 2 * workers * cols) + sizeof(float) * 2 * workers * cols * hd;
-}
 
 // The parts of the workspace for `items` items, and `workers` workers of `cols` columns.
 Pieces pieces_in(void* ws, int64_t items, int64_t workers, int cols) {
@@ -1822,11 +1812,11 @@ hipError_t attn_tiles(hipStream_t st, const Kv4Attn& a) {
   const int64_t tiles = ((int64_t)cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
   const bool whole = tiles <= kWhole;
-  const int64_t most = (int64_t)compute_units() * 4 * attn_waves(D, NT, Terms<E>::n);
+  const int64_t most = attn_workers(D, NT, compute_units());
   const int64_t want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
   const int workers = (int)((std::min(most, want) + 3) / 4 * 4), least = whole ? 1 : kLeast;
   const Pieces pc = pieces_in(a.ws, items, workers, cols);
-  hipLaunchKernelGGL((k_kv4_attn<D, NT, attn_ring(D, NT, Terms<E>::n), E>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths,
+  hipLaunchKernelGGL((k_kv4_attn<D, NT, attn_ring(D, NT), E>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths,
                      a.page_table, a.c.base, pc, workers, least, whole);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess || whole ? e : merge<D, E>(st, a, pc, items, workers, cols, cap, kStart);
@@ -1838,7 +1828,7 @@ hipError_t attn_prompt(hipStream_t st, const Kv4Attn& a) {
   const int cap = attn_cap(a);
   const int64_t tiles = ((int64_t)cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
-  const int64_t most = (int64_t)compute_units() * (8 / kPromptWaves), want = (items * (tiles + kPromptStart) + kPromptLeast - 1) / kPromptLeast;
+  const int64_t most = prompt_workers(compute_units()), want = (items * (tiles + kPromptStart) + kPromptLeast - 1) / kPromptLeast;
   const int workers = (int)std::min(most, want);
   const Pieces pc = pieces_in(a.ws, items, workers, cols);
   hipLaunchKernelGGL((k_kv4_prompt<kPromptWaves, E>), dim3((unsigned)workers), dim3(64 * kPromptWaves), 0, st, a, a.row_offsets, a.lengths,
@@ -1853,12 +1843,12 @@ hipError_t attn_prompt(hipStream_t st, const Kv4Attn& a) {
 // 39; 64 of 8 rows (32 columns each) 81 and 52, one of 256 rows and tokens 28 and 27.
 bool many_columns(const Kv4Attn& a) {
   const int64_t group = a.n_q / a.c.n_kv;
-  return a.max_rows * group >= 64 && a.rows * group >= (int64_t)64 * a.batch && attn_cap(a) > 256;
+  return a.max_rows * group >= kManyColumns && a.rows * group >= (int64_t)kManyColumns * a.batch && attn_cap(a) > 256;
 }
 
 template <class E>
 hipError_t attn_type(hipStream_t st, const Kv4Attn& a) {
-  const bool one = (int64_t)a.max_rows * (a.n_q / a.c.n_kv) <= 16;
+  const bool one = (int64_t)a.max_rows * (a.n_q / a.c.n_kv) <= kOneTile;
   if (a.c.hd == 64) return one ? attn_tiles<64, 1, E>(st, a) : attn_tiles<64, 2, E>(st, a);
   if constexpr (sizeof(typename E::T) == 2)
     if (a.c.hd == 128 && many_columns(a)) return attn_prompt<E>(st, a);
@@ -1869,7 +1859,8 @@ hipError_t attn_type(hipStream_t st, const Kv4Attn& a) {
 }  // namespace
 
 size_t kv4_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows) {
-  return attn_bytes(attn_items(n_q, n_kv, batch, rows, 16), (int64_t)compute_units() * 4 * 3, hd == 256 ? 16 : 32, hd);
+  const int64_t columns = piece_columns(hd, (int64_t)rows * (n_q / n_kv), compute_units());
+  return 256 + align256(sizeof(Begun) * attn_items(n_q, n_kv, batch, rows, 16)) + align256(sizeof(float2) * columns) + sizeof(float) * columns * hd;
 }
 
 hipError_t launch_kv4_attn(hipStream_t st, int dtype, const Kv4Attn& a) {

@@ -61,4 +61,30 @@ __host__ __device__ inline int64_t attn_items(int n_q, int n_kv, int batch, int 
   return n_kv * ((int64_t)rows * (n_q / n_kv) / cols + at_most(batch, rows));
 }
 
+// Waves a SIMD that the registers of a form leave room for (head dim 64, one tile of columns, fp16 and bf16: four would
+// fit; not tried).  (NT = 1 with two waves and rings of four tiles: 84 us for 128 sequences of one fp16 row, 80 with
+// three, and 55 for 51 of three long ones, with a merge of fewer pieces that is as much shorter.)
+constexpr int attn_waves(int hd, int nt) { return hd == 256 ? 1 : nt == 1 ? 3 : 2; }
+constexpr int kPromptWaves = 8;   // of a workgroup that shares a tile's expansion, 32 columns each
+constexpr int kOneTile = 16;      // columns a sequence up to which items have one tile of columns, above it two
+constexpr int kManyColumns = 64;  // columns a sequence from which waves may share a tile's expansion
+
+// Workers of a call, at most: waves of a form, workgroups of a prompt.
+inline int64_t attn_workers(int hd, int nt, int compute_units) { return (int64_t)compute_units * 4 * attn_waves(hd, nt); }
+inline int64_t prompt_workers(int compute_units) { return (int64_t)compute_units * (8 / kPromptWaves); }
+
+// Columns of the pieces, two a worker, that calls of up to `columns` query columns of a kv head leave, at most.
+inline int64_t piece_columns(int hd, int64_t columns, int compute_units) {
+  int64_t n = attn_workers(hd, 1, compute_units) * 16;
+  if (hd != 256 && columns > kOneTile) {
+    const int64_t two = attn_workers(hd, 2, compute_units) * 32;
+    n = n > two ? n : two;
+  }
+  if (hd == 128 && columns >= kManyColumns) {
+    const int64_t prompt = prompt_workers(compute_units) * 32 * kPromptWaves;
+    n = n > prompt ? n : prompt;
+  }
+  return 2 * n;
+}
+
 }  // namespace rstr

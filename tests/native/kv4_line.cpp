@@ -1,6 +1,6 @@
 // The items that attention over the 4-bit cache makes of a call's row offsets, whatever these
 // hold: their numbers stay inside the room that the host counts for them.  And the division that cuts
-// them into parts.
+// them into parts, and the room for the pieces of those.
 #include <cstdio>
 #include <cstdlib>
 #include <vector>
@@ -53,9 +53,31 @@ static void quotients() {
   }
 }
 
+// The room for pieces covers every form that a call within a plan may take, and is no more than the
+// largest of them.
+static void pieces() {
+  for (int cu : {1, 64, 256, 304})
+    for (int hd : {64, 128, 256})
+      for (int64_t plan : {1, 4, 16, 17, 63, 64, 65, 100000}) {
+        const int64_t room = piece_columns(hd, plan, cu);
+        int64_t used = 0;
+        for (int64_t call = 1; call <= plan; call += plan > 200 ? 997 : 1) {  // columns of its longest sequence
+          const auto form = [&](int64_t workers, int cols) {
+            checks++;
+            if (2 * workers * cols > used) used = 2 * workers * cols;
+          };
+          if (hd == 256 || call <= kOneTile) form(attn_workers(hd, 1, cu), 16);
+          else form(attn_workers(hd, 2, cu), 32);
+          if (hd == 128 && call >= kManyColumns) form(prompt_workers(cu), 32 * kPromptWaves);
+        }
+        if (used != room) { printf("head dim %d, %lld columns: %lld for %lld\n", hd, (long long)plan, (long long)room, (long long)used); exit(1); }
+      }
+}
+
 int main() {
   srand(1);
   quotients();
+  pieces();
   const int heads[][2] = {{1, 1}, {32, 8}, {8, 8}, {24, 1}, {4, 1}};
   for (const auto& h : heads)
     for (int cols : {16, 32, 256}) {

@@ -776,3 +776,19 @@ def test_attention_of_many_prompts(sess, B, gaps, dtype):
         assert bool((out[int(c.offsets[-1]):] == 7.0).all())
     plan.close()
     c.close()
+
+
+@pytest.mark.parametrize("D,rows,columns", [(64, 1, 12 * 16), (64, 40, 8 * 32), (128, 1, 12 * 16), (128, 5, 8 * 32), (128, 600, 256), (256, 1, 4 * 16), (256, 600, 4 * 16)])
+def test_plans_take_what_their_calls_can_use(sess, D, rows, columns):
+    """Device memory of a plan: two pieces of `columns` columns of the largest form that its rows can take, for
+    each compute unit, each D + 2 numbers of 4 bytes; 20 bytes an item; and what allocations are rounded up by."""
+    units = torch.cuda.get_device_properties(0).multi_processor_count
+    pool = hip.Kv4Pool(sess, 1, 2, D, 16, 4)
+    plans, free = [], torch.cuda.mem_get_info()[0]
+    for _ in range(8):
+        plans.append(hip.Kv4Attention(pool, 8, 2, rows))
+    items = 2 * (rows * 4 // 16 + 2)
+    assert (free - torch.cuda.mem_get_info()[0]) / 8 <= 2 * columns * units * (D + 2) * 4 + 20 * items + 2 ** 21
+    for p in plans:
+        p.close()
+    pool.close()
