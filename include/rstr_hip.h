@@ -445,7 +445,7 @@ int rstr_kv4_attn_run(rstr_kv4_attn* a, int32_t layer, int32_t dtype, int32_t ba
  * counts[b] more.  New pages come from free_pages[0 .. n_free) in order, sequence
  * by sequence; pages already in page_table[batch][pages_per_seq] are kept and the
  * new ones written behind them.  A sequence is served if its tokens fit
- * pages_per_seq, the list lasts (one that needs no new page is served after it
+ * pages_per_seq and 31 bits, the list lasts (one that needs no new page is served after it
  * has run out) and its rows fit `rows`; otherwise it keeps its length and has no rows.
  * Writes new_lengths[batch], row_offsets[batch+1] (of the rows served),
  * positions[rows] and slots[rows] (0 and -1 behind the last row, and -1 for a page id

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kMapsThreads) k_step_maps(StepMaps a) {
   __shared__ int64_t smax[2];
   const int tid = threadIdx.x, per = (a.batch + kMapsThreads - 1) / kMapsThreads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-  const int64_t cap = (int64_t)a.pps * a.page_size;
+  const int64_t cap = min((int64_t)a.pps * a.page_size, (int64_t)0x7FFFFFFF);
   const auto pages_of = [&](uint32_t n) {
     const uint32_t p = n / (uint32_t)a.page_size;
     return (int)(p + (n != p * (uint32_t)a.page_size ? 1 : 0));

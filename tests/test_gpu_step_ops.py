@@ -341,3 +341,16 @@ def test_the_step_as_a_whole(sess):
     ver.close()
     plan.close()
     pool.close()
+
+
+def test_step_maps_lengths_past_31_bits(sess):
+    """Pages so large that a table holds more tokens than a length can say: a sequence whose new length does not fit 31 bits
+    is refused, one that just fits is served."""
+    page, top = 2 ** 30, 2 ** 31 - 1
+    lengths, counts = np.array([top, top - 4, top - 4, 5]), np.array([1, 5, 4, top])
+    table = np.array([[3, 4, 5, 6], [0, 1, 2, 3], [0, 1, 2, 3], [0, 1, 2, 3]])
+    got = {k: v.cpu().tolist() for k, v in _maps(sess, page, lengths, counts, np.array([7, 8]), table, 6).items()}
+    assert got["new_lengths"] == [top, top - 4, top, 5] and got["offsets"] == [0, 0, 0, 4, 4]
+    assert got["positions"] == [top - 4, top - 3, top - 2, top - 1, 0, 0]
+    assert got["slots"] == [top - 4, top - 3, top - 2, top - 1, -1, -1]
+    assert got["taken"] == [0] and got["table"] == table.tolist()
