@@ -355,8 +355,8 @@ class Session:
         """The tables of a step on the GPU (rstr_step_maps): int32 device arrays; ``page_table``
         [batch][width] and everything behind it are written.  The length of ``slots``
         bounds the step's rows, that of ``free_pages`` its new pages."""
-        batch, (rows,) = len(lengths), slots.shape
-        width, n_free = page_table.shape[1], len(free_pages)
+        batch, (rows,) = lengths.shape[0], slots.shape
+        width, n_free = page_table.shape[1], free_pages.shape[0]
         self.check(lib().rstr_step_maps(
             self.h, page_size, batch, width, rows, _ints(self, lengths, "lengths", (batch,)),
             _ints(self, counts, "counts", (batch,)), None if starts is None else _ints(self, starts, "starts", (batch,)),
@@ -780,14 +780,14 @@ class Kv4Pool:
     def append(self, layer: int, k, v, slots, stream=None):
         """Quantises rows k, v [rows][n_kv][head_dim] into ``slots`` [rows] (rstr_kv4_append);
         rows whose slot is negative are skipped."""
-        rows = len(slots)
+        rows = slots.shape[0]
         t, k, v = self._kv(k, v, rows)
         self.sess.check(lib().rstr_kv4_append(self.h, layer, rows, t, *k, *v, _ints(self.sess, slots, "slots", (rows,)),
                                               _stream(self.sess, stream)))
 
     def read(self, layer: int, slots, k, v, stream=None):
         """Writes the values that ``slots`` hold into rows k, v (rstr_kv4_read)."""
-        rows = len(slots)
+        rows = slots.shape[0]
         t, k, v = self._kv(k, v, rows)
         self.sess.check(lib().rstr_kv4_read(self.h, layer, rows, t, _ints(self.sess, slots, "slots", (rows,)), *k, *v,
                                             _stream(self.sess, stream)))
@@ -815,7 +815,7 @@ class Kv4Attention:
         """q, out [rows][n_q][head_dim] of one type; int32 row_offsets [batch+1], page_table
         [batch][width], lengths [batch].  ``max_rows``: the most rows of one sequence (default: all rows)."""
         s, hd = self.sess, self.pool.head_dim
-        batch, rows = len(lengths), q.shape[0]
+        batch, rows = lengths.shape[0], q.shape[0]
         qp, t, qr, qh = _rows(s, q, "q", self.n_q, hd)
         op, ot, orow, oh = _rows(s, out, "out", self.n_q, hd, rows)
         if t != ot:
@@ -849,7 +849,7 @@ class Verifier:
         u_accept [rows], u_sample [batch], draft_probs [rows][vocab]; writes int32 accepted [batch] and
         tokens [rows]."""
         s = self.sess
-        batch, rows = len(row_offsets) - 1, len(drafts)
+        batch, rows = row_offsets.shape[0] - 1, drafts.shape[0]
         lp, t, lr = _matrix(s, logits, "logits", rows, self.vocab)
         pp, pr = None, 0
         if draft_probs is not None:

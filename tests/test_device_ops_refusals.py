@@ -319,3 +319,28 @@ def test_plans_past_a_grid(dev):
         hip.Verifier(s, 1 << 23, 1 << 23, 2).close()
         p.close()
     assert dev.fake_blocks() == blocks
+
+
+class Bare:
+    """An array with nothing but what the operators ask of one."""
+
+    def __init__(self, x):
+        self.data_ptr, self.shape, self.stride, self.dtype, self.device = x.data_ptr, x.shape, x.stride, x.dtype, x.device
+
+
+def test_arrays_without_a_length(dev):
+    """data_ptr(), shape, stride(), dtype and device are enough."""
+    with hip.Session(0) as s:
+        keep = [Dev((2, 2, 128)), Dev((2, 2, 128)), ints(2), Dev((2, 4, 128)), Dev((2, 4, 128)), ints(3), ints((2, 5)), ints(2), ints(2), ints(2), ints(1),
+                ints(6), Dev((2, 100)), Dev((2,)), Dev((2,)), Dev((2,)), ints(2), ints(2)]
+        k, v, slots, q, out, offs, table, lens, more, pos, one, free, logits, T, ua, us, acc, tok = [Bare(x) for x in keep]
+        n = dev.fake_launches()
+        p = hip.Kv4Pool(s, 1, 2, 128, 16, 4)
+        p.append(0, k, v, slots)
+        p.read(0, slots, k, v)
+        hip.Kv4Attention(p, 4, 2, 2).run(0, q, offs, table, lens, out)
+        s.step_maps(16, lens, more, free, table, acc, offs, pos, slots, one)
+        hip.Verifier(s, 2, 2, 100).run(logits, offs, slots, T, ua, us, acc, tok)
+        view = hip.DeviceView(keep[12].data_ptr(), (2, 100), "float32", 0, None)
+        hip.Verifier(s, 2, 2, 100).run(view, offs, slots, T, ua, us, acc, tok)
+        assert dev.fake_launches() == n + 6
