@@ -534,6 +534,8 @@ hipError_t rows_type(hipStream_t st, bool append, const Kv4Layer& c, int dtype, 
 // without the 4 of a merge.  Parts of two tiles at least, where there is little work: 16 windows of 512
 // tokens, head dim 256, 16 us (four tiles: 20, one: 14), and 16 sequences of 200 tokens 14 (15, 17).
 constexpr int kStart = 6;  // what beginning an item costs, in tiles
+// Queries are brought down by no more, so that what brings their scores up again stays finite: the largest are 2^8 then.
+constexpr int kLargestPower = 120;
 
 // Terms of a weight; ONCE: p * d is rounded once, from fp32.  bf16 results round to 8
 // bits anyway, so there p is rounded to fp16 and multiplied by pairs.
@@ -904,7 +906,7 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT))
           for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[bk][i]));
         }
         big = xor_max<32>(xor_max<16>(big));
-        const int e = __builtin_amdgcn_frexp_expf(big);
+        const int e = min(__builtin_amdgcn_frexp_expf(big), kLargestPower);
         kcol[t] = __builtin_amdgcn_ldexpf(a.scale * 1.4426950408889634f, e);
 #pragma unroll
         for (int bk = 0; bk < NB; bk++)
@@ -1431,7 +1433,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
           for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[bk][i]));
         }
         big = xor_max<32>(xor_max<16>(big));
-        const int e = __builtin_amdgcn_frexp_expf(big);
+        const int e = min(__builtin_amdgcn_frexp_expf(big), kLargestPower);
         kcol[t] = __builtin_amdgcn_ldexpf(a.scale * 1.4426950408889634f, e);
 #pragma unroll
         for (int bk = 0; bk < NB; bk++)

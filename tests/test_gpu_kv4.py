@@ -787,3 +787,25 @@ def test_plans_take_what_their_calls_can_use(sess, D, rows, columns):
     for p in plans:
         p.close()
     pool.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,D", [(1, 128), (40, 64), (70, 128), (3, 256)])
+def test_the_largest_queries(sess, dtype, rows, D):
+    """Queries next to the type's largest value on small keys: the scores that matter are finite.  The softmax is 1 at the
+    largest, token 0 (the others' are at least 1e34 below), whose value is the output."""
+    print("largest queries", dtype, rows, D, flush=True)
+    n = 300
+    c = Case(sess, 4, 2, D, 16, [n], [rows])
+    k = (torch.arange(1, n + 1, dtype=torch.float32) * 1e-3)[:, None, None].expand(n, 2, D).contiguous()
+    v = torch.tensor(c.rng.standard_normal((n, 2, D)), dtype=torch.float32)
+    c.pool.append(0, k.cuda(), v.cuda(), _i32(c.table[0, np.arange(n) // 16] * 16 + np.arange(n) % 16))
+    q = torch.full((rows, 4, D), -3e38).to(TYPES[dtype])
+    out = torch.zeros_like(q).cuda()
+    plan = c.plan()
+    plan.run(0, q.cuda(), _i32(c.offsets), _i32(c.table), _i32(c.lens), out, scale=1.0)
+    want = np.repeat(P.quantised(P.as_f64(v[:1]))[0], 2, axis=0)
+    tol = (2.0 ** -10 if dtype != "f32" else 2.0 ** -21) + torch.finfo(TYPES[dtype]).eps / 2 * 1.01
+    assert (np.abs(P.as_f64(out) - want) <= tol * np.abs(want)).all()
+    plan.close()
+    c.close()
