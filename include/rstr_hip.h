@@ -427,8 +427,8 @@ int rstr_kv4_attn_close(rstr_kv4_attn* a);
  * token p sees the tokens j <= p, and with window > 0 only j > p - window:
  * out = sum softmax(scale * q . k_j) v_j, in the type of q (f32: products and sums
  * in fp32 precision; f16, bf16: probabilities, and their products with values, rounded to
- * 11 bits; bf16 and many rows: keys too; a product of a probability and a value is off
- * by 2^-32 where that is more).  A row that
+ * 11 bits; bf16 and many rows: keys too; a query's elements are off by 2^-24 of its largest, and
+ * a product of a probability and a value by 2^-32, where these are more).  A row that
  * sees no token (length 0, more rows than tokens) is 0.  Tokens of a page id outside
  * the cache are not seen, nor are tokens behind the table's width or from 2^31 - 64 on (the
  * positions of a longer sequence's rows follow from its length all the same).  Rows behind
@@ -468,7 +468,8 @@ int rstr_verify_open(rstr_session* s, int32_t max_batch, int32_t max_rows, int32
 int rstr_verify_close(rstr_verify* v);
 /* Sequence b has the rows [row_offsets[b], row_offsets[b+1]): row i's logits are
  * the target's after i drafted tokens, drafts[i] is the token drafted there (not read at the
- * last row).  With p = softmax(logits / temperature[b]) in 64 bits and q the row's
+ * last row).  With p = softmax(logits / temperature[b]) in 64 bits (its exponentials to 3e-13 of
+ * themselves) and q the row's
  * draft_probs [rows][vocab] (NULL: the draft was certain, q = 1 at it), draft i is
  * accepted while u_accept[i] * q(draft) < p(draft).  At the first one refused a token is
  * drawn from max(p - q, 0) (from p where that is 0 everywhere), after the last from p: the first
@@ -477,7 +478,7 @@ int rstr_verify_close(rstr_verify* v);
  * the largest), are greedy: the draft is accepted if it is the first largest
  * logit, which is the token otherwise.  Drafts outside the vocabulary are refused.  accepted[b] is the number
  * of drafts accepted; tokens[rows] are those drafts, then the token, then -1.
- * Random numbers lie in [0, 1).  Rows behind row_offsets[batch] are left as they are.
+ * Random numbers lie in [0, 1), row_offsets do not decrease.  Rows behind row_offsets[batch] are left as they are.
  * Outputs overlap no input. */
 int rstr_verify_run(rstr_verify* v, int32_t dtype, int32_t batch, int32_t rows, const void* logits,
                     int64_t logits_row, const int32_t* row_offsets, const int32_t* drafts, const float* draft_probs,

@@ -526,13 +526,14 @@ hipError_t rows_type(hipStream_t st, bool append, const Kv4Layer& c, int dtype, 
 // order.
 //
 // NT = 1 where no sequence has more than 16 columns: 128 sequences of 128 to 4608 tokens, one fp16 row of 32
-// heads each (8 kv heads of 128, 351 MB) take 80 us, 4.4 TB/s, bound by memory (loads
-// alone: 65) and vector instructions together; with NT = 2 145.  Three of 20161 to 131072 tokens, bf16
-// (261 MB): 51 us, 5.1 TB/s, and 10 for the merge; 33 of 5 to 8192 with up to six fp32 rows of 16
-// heads (157 MB) 52 and 8, bound by the second product that each of two terms needs.
-// Where a table holds no more than kWhole tiles a wave does an item by itself: one sequence of 37 tokens 8.5 us,
+// heads each (8 kv heads of 128, 351 MB) take 80 us, 4.4 TB/s, bound by memory (362 MB are read; loads
+// alone: 65) and vector instructions (busy 63 % of the time) together; the whole call 88, with NT = 2 137.  Three of 20161
+// to 131072 tokens, bf16 (261 MB): 51 us, 5.1 TB/s, memory, and 11 for the merge; 33 of 5 to 8192 with up to six fp32
+// rows of 16 heads (157 MB) 52 and 8: vector instructions are busy 58 %, as every weight and its rest need a product each,
+// and memory gives 3.4 TB/s, so neither alone is the bound: waves wait to issue a third of the time, for memory a fifth.
+// Where a table holds no more than kWhole tiles a wave does an item by itself: one sequence of 37 tokens 8.1 us,
 // without the 4 of a merge.  Parts of two tiles at least, where there is little work: 16 windows of 512
-// tokens, head dim 256, 16 us (four tiles: 20, one: 14), and 16 sequences of 200 tokens 14 (15, 17).
+// tokens, head dim 256, 15 us (four tiles: 20, one: 14), and 16 sequences of 200 tokens 14 (15, 17).
 constexpr int kStart = 6;  // what beginning an item costs, in tiles
 // Queries are brought down by no more, so that what brings their scores up again stays finite: the largest are 2^8 then.
 constexpr int kLargestPower = 120;
@@ -1221,8 +1222,9 @@ __global__ void __launch_bounds__(256, attn_waves(D, NT))
 // tile on the expansion; here it is a quarter of 200.  Parts, pieces and the merge are
 // those of k_kv4_attn with a workgroup in the place of a wave.
 //
-// 512 rows of 32 heads at 4096 tokens (8 kv heads, bf16): 80 us (k_kv4_attn: 112), a fifth of
-// the matrix rate.  A step of 64 tokens takes 3.3 us, of which matrix
+// 512 rows of 32 heads at 4096 tokens (8 kv heads, bf16), and 77 at 77: 81 us, 15 for the merge (the whole call back to back
+// 90; k_kv4_attn 107), a third of the matrix rate.  Waits bind it: matrix instructions are busy 16 % of the time, vector
+// instructions 35 %.  A step of 64 tokens takes 3.3 us, of which matrix
 // instructions are 0.9 and vector instructions 1.7; before its first one a part waits 10 us
 // for its sequence, its pages, queries and codes, one after the other.  Four waves a workgroup, two of
 // those a CU: 87 us.  One wave of a SIMD expanding while the other multiplies: 84.
@@ -1670,7 +1672,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2)
 
 // Joins the pieces of an item that several waves computed, in their order: a workgroup
 // an item and `per` columns (more for every gridDim.y), its waves by column and by piece.  It waits for memory
-// four times, 4 us at the least; 55 MB of a prompt's pieces take 15.
+// four times, 4 us at the least; 38 MB of a prompt's pieces take 15.
 template <int D, class E>
 __global__ void k_kv4_merge(Kv4Attn a, Lines L, Pieces pc, int per) {
   constexpr int V = D / 64;  // dims a lane
@@ -1841,8 +1843,9 @@ hipError_t attn_prompt(hipStream_t st, const Kv4Attn& a) {
 
 // Columns enough for the waves of a workgroup to share a tile's expansion: 64 a sequence, and a table of more
 // than 256 tokens.  32 heads, 8 kv heads, bf16, k_kv4_prompt against k_kv4_attn with NT = 2: one sequence of 64 rows
-// at 16384 tokens 52 and 63 us, of 512 rows at 2048 54 and 67, 16 sequences of 16 rows at 1024 40 and
-// 39; 64 of 8 rows (32 columns each) 81 and 52, one of 256 rows and tokens 28 and 27.
+// at 16384 tokens 59 and 70 us, of 512 rows at 2048 61 and 71 (fp16 66 and 81); at the border the other form is the faster
+// one for short tables, 16 sequences of 16 rows at 1024 45 and 41.  Not taken: 64 sequences of 8 rows (32 columns
+// each) 92 and 62, one of 256 rows and tokens 31 and 27.  (Calls back to back, with their merges.)
 bool many_columns(const Kv4Attn& a) {
   const int64_t group = a.n_q / a.c.n_kv;
   return a.max_rows * group >= kManyColumns && a.rows * group >= (int64_t)kManyColumns * a.batch && attn_cap(a) > 256;
