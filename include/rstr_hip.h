@@ -427,7 +427,7 @@ int rstr_kv4_attn_close(rstr_kv4_attn* a);
  * token p sees the tokens j <= p, and with window > 0 only j > p - window:
  * out = sum softmax(scale * q . k_j) v_j, in the type of q (f32: products and sums
  * in fp32 precision; f16, bf16: probabilities, and their products with values, rounded to
- * 11 bits; bf16 and many rows: keys too; a query's elements are off by 2^-24 of its largest, and
+ * 11 bits; bf16 and many rows: keys too; a query's elements are off by 2^-23 of its largest, and
  * a product of a probability and a value by 2^-32, where these are more).  A row that
  * sees no token (length 0, more rows than tokens) is 0.  Tokens of a page id outside
  * the cache are not seen, nor are tokens behind the table's width or from 2^31 - 64 on (the
@@ -435,7 +435,8 @@ int rstr_kv4_attn_close(rstr_kv4_attn* a);
  * row_offsets[batch] are left as they are; where row_offsets decrease anywhere, nothing is
  * written.
  * max_rows: the most rows a sequence of this call has (it chooses the tile; a sequence
- * with more is still computed).  out overlaps no input. */
+ * with more is still computed).  A call takes one form for all its sequences, so a prompt
+ * beside many single rows is faster as two calls.  out overlaps no input. */
 int rstr_kv4_attn_run(rstr_kv4_attn* a, int32_t layer, int32_t dtype, int32_t batch, int32_t rows,
                       int32_t max_rows, int32_t window, float scale, const void* q, int64_t q_row, int64_t q_head,
                       const int32_t* row_offsets, const int32_t* page_table, int32_t pages_per_seq,
