@@ -36,6 +36,9 @@ typedef struct rstr_transfer rstr_transfer;
 typedef struct rstr_kv4 rstr_kv4;
 typedef struct rstr_kv4_attn rstr_kv4_attn;
 typedef struct rstr_verify rstr_verify;
+typedef struct rstr_pool_attn rstr_pool_attn;
+typedef struct rstr_bounds rstr_bounds;
+typedef struct rstr_select rstr_select;
 
 /* Descriptor flags of src/pretrained/arch/{gemma3,qwen3,llama}.clj plus the HF
  * hyper-parameters read by decoder.clj:31-56 (load-hf). */
@@ -485,6 +488,86 @@ int rstr_verify_run(rstr_verify* v, int32_t dtype, int32_t batch, int32_t rows, 
                     int64_t logits_row, const int32_t* row_offsets, const int32_t* drafts, const float* draft_probs,
                     int64_t probs_row, const float* temperature, const float* u_accept, const float* u_sample,
                     int32_t* accepted, int32_t* tokens, void* stream);
+
+/* ---- operators on device arrays over the page pool ------------------------------
+ * The fp16 pages of an rstr_pool, read and written on a caller's stream: appends
+ * with the position rotation on the way, attention of one or several new tokens
+ * per sequence, and attention over those blocks of a context that a cheap score selects.  Rules of the
+ * operators above; a block is a page.  Work of the session's own calls on the same pages is on its stream: the
+ * caller orders the two.  A pool with open plans or bounds does not close (RSTR_E_STATE). */
+
+/* Device address of one slab (0: keys, 1: values) of a layer, fp16 [page][page_size][n_kv][head_dim], valid
+ * until the pool is closed. */
+int rstr_pool_device(rstr_pool* p, int32_t slab, int32_t layer, void** out);
+/* Appends rows k, v [rows][n_kv][head_dim] to one layer at slots[rows] (page * page_size + offset; a row
+ * whose slot is negative or outside the pool is skipped), and writes the queries that belong to them.
+ * Heads of q and k are, in this order: with gains (fp32 [head_dim], NULL: none) x / sqrt(mean x^2 + eps) * (gain_offset +
+ * gain); with rotary_dim > 0 (a multiple of 16, up to head_dim) turned at positions[row], pairs (i, i + rotary_dim/2) by the angle
+ * position * frequencies[i] (fp64 [rotary_dim/2], radians a position; the product, its sine and its cosine are computed in 64 bits
+ * and these rounded to fp32; angles past 2^32 give NaN); elements behind rotary_dim stay.  k and v are rounded to fp16 (past its range:
+ * infinity), q_out [rows][n_q][head_dim] to the type of q; n_q = 0: no queries.  q_out is q itself or
+ * overlaps no input; views of one array with all heads a row are apart where their heads are.  Rows do not lie in the
+ * layer's pages.  Slots of one call are distinct: of two rows for one slot either may stay, element by element. */
+int rstr_pool_rope_append(rstr_pool* p, int32_t layer, int32_t rows, int32_t dtype, const void* k, int64_t k_row,
+                          int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int32_t n_q, const void* q,
+                          int64_t q_row, int64_t q_head, void* q_out, int64_t q_out_row, int64_t q_out_head,
+                          const float* q_gain, const float* k_gain, float eps, float gain_offset, int32_t rotary_dim,
+                          const double* frequencies, const int32_t* positions, const int32_t* slots, void* stream);
+
+/* A plan for attention of up to max_batch sequences and max_rows query rows of n_q heads: the call's
+ * workspace.  n_kv * (max_rows * (n_q / n_kv) / 16 + the smaller of max_rows and max_batch), and rows * n_kv, < 2^24.
+ * One plan serves one call at a time: calls (and graphs that hold them) that may run at once need a plan each. */
+int rstr_pool_attn_open(rstr_pool* p, int32_t n_q, int32_t max_batch, int32_t max_rows, rstr_pool_attn** out);
+/* Waits for the device. */
+int rstr_pool_attn_close(rstr_pool_attn* a);
+/* Attention over one layer; sequences, rows, positions, window and what is not seen are those of rstr_kv4_attn_run:
+ * out = sum softmax(scale * q . k_j) v_j over the tokens j <= p that the row at token p sees, in the type of q (f32:
+ * products and sums in fp32 precision; f16, bf16: probabilities rounded to 11 bits; a query's elements are off by 2^-39 of
+ * its largest where that is more).  A row that sees no token is 0, and so is one whose scores are all -infinity.  What is
+ * in a token that a row does not see, NaN and infinities among it, does not reach it.  (An infinite value whose weight is below
+ * 2^-23 of the row's largest may give NaN.)
+ * blocks NULL: all blocks.  Else int32 [rows][n_kv][blocks_per_row]: a row of a query and kv head sees only the tokens of
+ * the blocks (indices into the sequence's page table row) that it lists, in any order.  Of the list of a row at token p the
+ * first p / page_size + 1 entries (as many as the table is wide, at most) count; an entry that is negative or outside the table is none, one that is
+ * listed twice counts twice.  max_rows: the most rows a sequence of this call has (it chooses the tile; a sequence with
+ * more is still computed). */
+int rstr_pool_attn_run(rstr_pool_attn* a, int32_t layer, int32_t dtype, int32_t batch, int32_t rows, int32_t max_rows,
+                       int32_t window, float scale, const void* q, int64_t q_row, int64_t q_head,
+                       const int32_t* row_offsets, const int32_t* page_table, int32_t pages_per_seq,
+                       const int32_t* lengths, const int32_t* blocks, int32_t blocks_per_row, void* out, int64_t out_row,
+                       int64_t out_head, void* stream);
+
+/* The bounds of a pool's blocks: for every layer, page, kv head and channel the least and the greatest element of
+ * the page's keys, fp16 [page][n_kv][2][head_dim] a layer.  Zeros when opened.  They follow the pages only where
+ * they are updated: after appends, and after pages were written in any other way. */
+int rstr_bounds_open(rstr_pool* p, rstr_bounds** out);
+/* Waits for the device.  RSTR_E_STATE while selections are open on it. */
+int rstr_bounds_close(rstr_bounds* b);
+/* Device address of a layer's bounds, valid until they are closed. */
+int rstr_bounds_device(rstr_bounds* b, int32_t layer, void** out);
+/* Bounds of the blocks in which the call's rows lie, from the keys that are there: of a sequence's tokens only (a page's
+ * places behind the length do not count).  Sequences as in rstr_pool_attn_run; `rows` is the most that row_offsets
+ * reach (rows behind it are not looked at), rows * n_kv < 2^26.  A NaN among a channel's keys is both of its bounds.  A page that
+ * several sequences share is full, or has the same length in all of them. */
+int rstr_bounds_update(rstr_bounds* b, int32_t layer, int32_t batch, int32_t rows, const int32_t* row_offsets,
+                       const int32_t* page_table, int32_t pages_per_seq, const int32_t* lengths, void* stream);
+
+/* Workspace for selections of up to max_batch sequences and max_rows query rows of n_q heads over page tables of up
+ * to max_pages.  max_rows * n_kv < 2^24, and times the 64s of max_pages < 2^26.  One call at a time, as with attention plans. */
+int rstr_select_open(rstr_bounds* b, int32_t n_q, int32_t max_batch, int32_t max_rows, int32_t max_pages, rstr_select** out);
+/* Waits for the device. */
+int rstr_select_close(rstr_select* a);
+/* The blocks that each row and kv head reads: blocks[rows][n_kv][blocks_per_row], ascending, -1 behind the last.  A
+ * row at token p has the blocks 0 .. p / page_size (of its table).  Where they fit, all are listed; else the `first` first
+ * ones, the `last` last ones (one at least: the row's own), and of those between them the ones of the highest score, of equal
+ * ones the first.  A block's score is the most that a key inside its bounds can give: the largest over the group's
+ * query heads of sum_d max(q_d lo_d, q_d hi_d), in 64 bits; a sum that is no number counts as infinity, a block whose
+ * page is outside the pool as -infinity.  A row without a position (more rows than tokens) lists none.  Rows behind row_offsets[batch] are
+ * left as they are; where row_offsets decrease anywhere, nothing is written.  The list overlaps no input. */
+int rstr_select_run(rstr_select* a, int32_t layer, int32_t dtype, int32_t batch, int32_t rows, const void* q, int64_t q_row,
+                    int64_t q_head, const int32_t* row_offsets, const int32_t* page_table, int32_t pages_per_seq,
+                    const int32_t* lengths, int32_t blocks_per_row, int32_t first, int32_t last, int32_t* blocks,
+                    void* stream);
 
 #ifdef __cplusplus
 }

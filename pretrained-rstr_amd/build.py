@@ -14,7 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "lib", "librstr_hip.so")
 
-HIP_SOURCES = ["kernels.hip", "kv4.hip", "step_ops.hip", "rstr_hip.cpp", "device_ops.cpp"]
+HIP_SOURCES = ["kernels.hip", "kv4.hip", "step_ops.hip", "pool_attn.hip", "pool_rows.hip", "rstr_hip.cpp", "device_ops.cpp",
+               "pool_ops.cpp"]
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
                "-ffp-contract=off", "-Wno-unused-value",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

@@ -200,6 +200,35 @@ __device__ __forceinline__ bool of_column(uint64_t lanes) {
   return ((lanes | lanes >> 16) >> (threadIdx.x & 15)) & 1;
 }
 
+// ---- the rows of a call ------------------------------------------------------------------
+// The sequence that a row belongs to, found by all lanes of a wave together: offsets are read 64 at a time.
+// Where they decrease anywhere no row belongs to one.
+struct RowOf {
+  int b, p;  // -1: none; the row's position (negative: it sees nothing)
+  int first;  // the sequence's first row
+  __device__ __forceinline__ RowOf(const int32_t* ro, const int32_t* lens, int batch, int rows, int row) {
+    int n = 0;
+    bool ordered = true;
+    for (int i0 = 0; i0 < batch; i0 += 64) {
+      const int i = i0 + (int)(threadIdx.x & 63);
+      const int at = ro[min(i, batch)], next = ro[min(i + 1, batch)];
+      n += __popcll(__ballot(i < batch && at <= row));
+      ordered = ordered && at <= next;
+    }
+    b = n - 1;
+    p = first = 0;
+    if (__ballot(!ordered)) b = -1;
+    if (b < 0) return;
+    const int end = min(ro[b + 1], rows);
+    if (row >= end) {
+      b = -1;
+      return;
+    }
+    first = max(ro[b], 0);
+    p = max(lens[b], 0) - (end - row);
+  }
+};
+
 // ---- host side ----------------------------------------------------------------------
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 

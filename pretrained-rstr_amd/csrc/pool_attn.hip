@@ -1,0 +1,702 @@
+// pool_attn.hip -- attention of ragged query rows over the fp16 page pool, over all tokens or over the blocks
+// that a list names.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+
+#include "../../include/rstr_hip.h"
+#include "attn_line.h"
+#include "device_math.h"
+#include "pool_ops.h"
+
+namespace rstr {
+
+namespace {
+
+// One wave works on 16 * NT columns (a query row of one head of the kv head's group is a column) of one sequence
+// and kv head, over tiles of 32 tokens, and needs neither LDS nor a barrier:
+//
+//   S^T = K Q^T     K is the A operand of 16x16x32 products as it lies in the pages: lane (c, g) loads 16 bytes
+//                   of token c at dims 32 s + 8 g.
+//   O^T += V^T P^T  a lane's S^T values are tokens 4g .. 4g + 3 of two halves of 16 of one column, which is what
+//                   the B operand P^T wants from that lane.  The A operand wants eight tokens of one dim of V where
+//                   a page holds eight dims of one token: the lane loads the same dims, 8 c .. 8 c + 7, of its eight
+//                   tokens and pairs their halves, one byte permutation an operand register.  Product j so has the
+//                   dims 8 c + j as its rows; 16 lanes read a whole row of a token.
+//
+// Queries are brought to [2^14, 2^15) of their row's largest element by a power of two and taken as one fp16 term
+// (f16, bf16: no bit of an element above 2^-28 of the largest is lost) or two (fp32).  Weights are
+// p = 2^((S - m) k + 10) with S the raw products, k the scale and that power of two: differences are taken before
+// the scale, so scores of any size give finite weights.  m follows the column's maximum when a score passes it by 2^4, so the exchange between
+// lanes and the rescaling of O are rare; p is below 2^14, and the factor 2^10 keeps small weights' bits: fp16's
+// subnormals begin 2^24 below the largest.  p is one fp16 term (f16, bf16) or two (fp32).  S, m, l and O are fp32.
+//
+// The tiles of all (sequence, kv head, column tile) items form one line of units that is cut into equal parts, one
+// a wave, as in kv4_line.h; with a list of blocks every row and kv head is an item, and all have as many parts.
+constexpr int kStart = 4;  // what beginning an item costs, in tiles
+
+template <class E> struct Terms { static constexpr int n = 1; };
+template <> struct Terms<F32> { static constexpr int n = 2; };
+
+// The first of two fp16 terms of x, short of it by 2^-12 to 2^-10 of x: the rest has the sign of x and is never 0 (but for an x
+// near fp16's smallest numbers), so that products of both terms with an infinity are that infinity.  The rest is rounded to 11
+// bits: 1.25 * 2^-21 of x.
+__device__ __forceinline__ _Float16 first_term(float x) {
+  return (_Float16)__builtin_amdgcn_cvt_pkrtz(x * (1.0f - 0x1p-12f), 0.0f)[0];
+}
+
+constexpr int pool_waves(int hd, int nt) { return hd == 256 ? 1 : 2; }
+
+// What the parts of an item leave: (m, l, k) and O of each column.
+struct PoolPieces {
+  int* n_items;
+  Begun* begun;  // [items]
+  f4* ml;        // [pieces][cols]
+  float* acc;    // [pieces][cols][D]
+};
+
+// A part of a column tile's work.
+struct Part {
+  int b, h, r0, m, p0, c0;  // sequence, kv head, first row, rows, position of the first, first column
+  int t0, t1;               // tiles
+  bool whole;               // of the item: its output is written, not a piece
+  int64_t piece;
+  const int32_t* list;      // the row's blocks, or null
+  int entries;              // pages (blocks) of it
+};
+
+template <int D>
+struct Dims {
+  static constexpr int KS = D / 32, JT = D / 16, VW = D / 32;  // products of a score, of a tile of O; dwords of a token a lane
+  static constexpr int PIECE = D / 16 < 8 ? D / 16 : 8;        // neighbouring dims a lane loads
+  // dim of row r of product j
+  static __device__ __forceinline__ constexpr int dim(int j, int r) { return j / PIECE * 128 + PIECE * r + j % PIECE; }
+};
+
+template <bool STREAM, class V>
+__device__ __forceinline__ V load_page(const void* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load((const V*)p);
+  else return *(const V*)p;
+}
+
+template <int D, int NT, class E, bool LISTED>
+__global__ void __launch_bounds__(256, pool_waves(D, NT))
+    k_pool_attn(PoolAttn a, const int32_t* __restrict__ ro, const int32_t* __restrict__ lens, const int32_t* __restrict__ table,
+                PoolPieces pc, int workers, int least, bool whole, int parts) {
+  typedef Dims<D> G;
+  typedef typename E::T T;
+  constexpr int KS = G::KS, JT = G::JT, VW = G::VW, COLS = 16 * NT, TERMS = Terms<E>::n;
+  constexpr bool STREAM = NT == 1 && !LISTED;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int w = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int n_kv = a.c.n_kv, group = a.n_q / n_kv, ps = a.c.page_size;
+  const int cap = (int)min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0);
+  const int64_t row_bytes = (int64_t)n_kv * D * 2;
+  const uint32_t step_e = kTile / ps, step_off = kTile - step_e * ps;
+
+  const auto work = [&](const Part& s) {
+    const auto end_seen = [&](int r) { return min(max(s.p0 + r + 1, 0), cap); };
+    const auto first_seen = [&](int r) { return a.window > 0 ? max(max(s.p0 + r + 1, 0) - a.window, 0) : 0; };
+    const int rf = min(s.m - 1, s.c0 / group), rl = min(s.m - 1, (s.c0 + COLS - 1) / group);
+    int hi[NT], lo[NT];
+    int64_t qrow[NT], qhead[NT];
+    bool valid[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int cc = s.c0 + t * 16 + col, r = cc / group;
+      valid[t] = r < s.m;
+      hi[t] = valid[t] ? end_seen(r) : 0;
+      lo[t] = first_seen(r);
+      qrow[t] = s.r0 + r;
+      qhead[t] = (int64_t)s.h * group + (cc - r * group);
+    }
+    const int hi_last = end_seen(rl), hi_first = end_seen(rf), lo_first = first_seen(rf), lo_last = first_seen(rl);
+    int t0 = s.t0, t1 = s.t1;
+    if constexpr (!LISTED) {
+      t0 = max(t0, lo_first / kTile);
+      t1 = min(t1, (hi_last + kTile - 1) / kTile);
+    }
+
+    f4 acc[NT][JT];
+    float mref[NT], l[NT], kcol[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+      for (int j = 0; j < JT; j++) acc[t][j] = f4{0, 0, 0, 0};
+      mref[t] = -FLT_MAX;
+      l[t] = kcol[t] = 0.0f;
+    }
+    if (t0 < t1) {
+      // pages of 64 entries from e0 on, one a lane; -1: not there
+      const int32_t* row = table + (int64_t)s.b * a.pps;
+      int e0 = 0, page = -1, block = 0;
+      const auto look = [&](int from) {
+        e0 = from;
+        const int e = from + lane;
+        int id = -1;
+        if (LISTED) {
+          block = e < s.entries ? s.list[e] : -1;
+          if ((uint32_t)block < (uint32_t)a.pps) id = row[block];
+          else block = 0;
+        } else if (e < s.entries) {
+          id = row[e];
+        }
+        page = (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
+      };
+      // entry and place of the lane's token of each half, and of the tile's first and last token
+      int ent[2], off[2], e_first = (int)((uint32_t)t0 * kTile / (uint32_t)ps), o_first = t0 * kTile - e_first * ps;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const uint32_t at = (uint32_t)t0 * kTile + 16 * j + col;
+        ent[j] = (int)(at / (uint32_t)ps);
+        off[j] = (int)(at - (uint32_t)ent[j] * ps);
+      }
+      look(e_first);
+      int slot_k[2], slot_v[2], tok_v[2];  // slots of the lane's tokens (-1: none), position of its first token of V
+      const auto slots = [&](int tile) {
+        if (uniform((int)((uint32_t)o_first + kTile - 1) / ps + e_first - e0) >= 64) look(e_first);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int at = (ent[j] - e0) & 63, id = __shfl(page, at, 64);
+          slot_k[j] = id < 0 ? -1 : id * ps + off[j];
+          slot_v[j] = __shfl(slot_k[j], 4 * g, 64);
+          if (LISTED) {
+            const int tok = __shfl(block, at, 64) * ps + off[j];
+            tok_v[j] = __shfl(tok, 4 * g, 64);
+          } else {
+            tok_v[j] = tile * kTile + 16 * j + 4 * g;
+          }
+          ent[j] += step_e;
+          off[j] += step_off;
+          if (off[j] >= ps) off[j] -= ps, ent[j]++;
+        }
+        e_first += step_e;
+        o_first += step_off;
+        if (o_first >= ps) o_first -= ps, e_first++;
+      };
+      const uint8_t* kbase = (const uint8_t*)a.c.k + (int64_t)s.h * D * 2 + 16 * g;
+      const uint8_t* vbase = (const uint8_t*)a.c.v + (int64_t)s.h * D * 2 + 2 * G::PIECE * col;
+      h8 kr[2][KS];
+      uint32_t vr[2][4][VW];
+      const auto load_k = [&] {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const uint8_t* p = kbase + (uint64_t)(uint32_t)max(slot_k[j], 0) * (uint64_t)row_bytes;
+#pragma unroll
+          for (int i = 0; i < KS; i++) kr[j][i] = __builtin_bit_cast(h8, load_page<STREAM, u32x4>(p + 64 * i));
+        }
+      };
+      const auto load_v = [&] {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const uint8_t* p = vbase + (uint64_t)(uint32_t)max(slot_v[j], 0) * (uint64_t)row_bytes;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if constexpr (VW == 2) {
+              const u32x2 x = load_page<STREAM, u32x2>(p + i * row_bytes);
+              vr[j][i][0] = x[0];
+              vr[j][i][1] = x[1];
+            } else {
+#pragma unroll
+              for (int u = 0; u < VW / 4; u++) {
+                const u32x4 x = load_page<STREAM, u32x4>(p + i * row_bytes + 256 * u);
+#pragma unroll
+                for (int k = 0; k < 4; k++) vr[j][i][4 * u + k] = x[k];
+              }
+            }
+          }
+        }
+      };
+      slots(t0);
+      load_k();
+      load_v();
+
+      h8 q[NT][TERMS][KS];
+      const bool vec = vec_rows(a.q, sizeof(T));
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float x[KS][8], big = 0.0f;
+#pragma unroll
+        for (int s2 = 0; s2 < KS; s2++) {
+          if (valid[t]) {
+            const T* src = (const T*)a.q.p + qrow[t] * a.q.row + qhead[t] * a.q.head + s2 * 32 + g * 8;
+            if (vec) load8<E, true>(src, x[s2]); else load8<E, false>(src, x[s2]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[s2][i] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[s2][i]));
+        }
+        big = xor_max<32>(xor_max<16>(big));
+        // (a largest of 0 or infinity has the exponent 0; the sign of the scale goes into the queries)
+        const int e = __builtin_amdgcn_frexp_expf(big) - 15;
+        kcol[t] = fminf(__builtin_amdgcn_ldexpf(fabsf(a.scale) * 1.4426950408889634f, e), FLT_MAX);
+#pragma unroll
+        for (int s2 = 0; s2 < KS; s2++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            float y = __builtin_amdgcn_ldexpf(x[s2][i], -e);
+            if (a.scale < 0.0f) y = -y;
+            if constexpr (TERMS == 2) {
+              q[t][0][s2][i] = first_term(y);
+              q[t][1][s2][i] = (_Float16)(y - (float)q[t][0][s2][i]);
+            } else {
+              q[t][0][s2][i] = (_Float16)y;
+            }
+          }
+      }
+
+      for (int tile = t0; tile < t1; tile++) {
+        const int sv[2] = {slot_v[0], slot_v[1]}, tv[2] = {tok_v[0], tok_v[1]}, sk[2] = {slot_k[0], slot_k[1]};
+        float sc[NT][8];
+        {
+          f4 d[NT][2];
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) d[t][j] = f4{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+              for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int u = 0; u < TERMS; u++) d[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[j][i], q[t][u][i], d[t][j], 0, 0, 0);
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) sc[t][i] = d[t][i >> 2][i & 3];
+        }
+        const bool more = tile + 1 < t1;
+        if (more) {
+          slots(tile + 1);
+          load_k();
+        }
+        // tokens that are not there, or that not all columns see
+        const int tok0 = tile * kTile;
+        bool edge;
+        if (LISTED) {
+          const bool odd = sv[0] < 0 || sv[1] < 0 || max(tv[0], tv[1]) + 4 > hi_first || min(tv[0], tv[1]) < lo_last;
+          edge = __ballot(odd) != 0;
+        } else {
+          edge = tok0 < lo_last || tok0 + kTile > hi_first || __ballot(sv[0] < 0 || sv[1] < 0) != 0;
+        }
+        uint32_t see[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) see[t] = 0xFF;
+        bool redo = false;  // values of V that are no numbers, of tokens that only some columns see
+        if (edge) {
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            see[t] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const int tok = tv[i >> 2] + (i & 3);
+              if (sv[i >> 2] >= 0 && tok >= lo[t] && tok < hi[t]) see[t] |= 1u << i;
+            }
+          }
+          // 0 times an infinity or a NaN: V of tokens that no column sees becomes 0
+          uint32_t odd = 0;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int tok = tv[i >> 2] + (i & 3);
+            const bool some = sv[i >> 2] >= 0 && tok >= lo_first && tok < hi_last, all = tok >= lo_last && tok < hi_first;
+#pragma unroll
+            for (int k = 0; k < VW; k++) {
+              uint32_t& x = vr[i >> 2][i & 3][k];
+              if (!some) x = 0;
+              else if (!all) odd |= ((x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u) ? 1u : 0u;
+            }
+          }
+          redo = !LISTED && __ballot(odd != 0) != 0;
+        }
+        float e2[NT][8];
+        bool grow = false;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            e2[t][i] = __builtin_fmaf(sc[t][i] - mref[t], kcol[t], 10.0f);
+            if (edge && !((see[t] >> i) & 1)) e2[t][i] = -INFINITY;
+            grow |= e2[t][i] > 14.0f;
+          }
+        if (__ballot(grow)) {
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            float m = -INFINITY;
+            bool passed = false;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              if ((see[t] >> i) & 1) m = fmaxf(m, sc[t][i]);
+              passed |= e2[t][i] > 14.0f;
+            }
+            m = xor_max<32>(xor_max<16>(m));
+            // a column that needs no change has none: it does not depend on its neighbours
+            const bool own = of_column(__ballot(passed));
+            const float now = own ? fmaxf(m, mref[t]) : mref[t];
+            const float keep = own ? __builtin_amdgcn_exp2f((mref[t] - now) * kcol[t]) : 1.0f;
+            mref[t] = now;
+            l[t] *= keep;
+#pragma unroll
+            for (int j = 0; j < JT; j++) acc[t][j] *= keep;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              if (own) e2[t][i] = (see[t] >> i) & 1 ? __builtin_fmaf(sc[t][i] - now, kcol[t], 10.0f) : -INFINITY;
+          }
+        }
+        float p[NT][8];
+        h8 ph[NT][TERMS];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            p[t][i] = __builtin_amdgcn_exp2f(e2[t][i]);
+            if constexpr (TERMS == 2) {
+              ph[t][0][i] = first_term(p[t][i]);
+              ph[t][1][i] = (_Float16)(p[t][i] - (float)ph[t][0][i]);
+            } else {
+              ph[t][0][i] = (_Float16)p[t][i];
+            }
+          }
+          l[t] += ((p[t][0] + p[t][1]) + (p[t][2] + p[t][3])) + ((p[t][4] + p[t][5]) + (p[t][6] + p[t][7]));
+        }
+        if (!LISTED && redo) {  // their part is added by itself, to the columns that see them
+          asm volatile("");
+#pragma unroll 1
+          for (int n = 0; n < kTile; n++) {
+            const int tok = tok0 + n;
+            const bool all = tok >= lo_last && tok < hi_first, some = tok >= lo_first && tok < hi_last;
+            if (all || !some) continue;
+            const int half = n >> 4, i = n & 3;
+            const int slot = __shfl(sk[half], n & 15, 64);
+            if (slot < 0) continue;
+            const _Float16* v = (const _Float16*)a.c.v + ((int64_t)slot * n_kv + s.h) * D;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              float mine = 0.0f;
+#pragma unroll
+              for (int k = 0; k < 8; k++) mine = k == 4 * half + i ? p[t][k] : mine;
+              mine = __shfl(mine, (((n >> 2) & 3) << 4) + col, 64);
+              const bool sees = tok >= lo[t] && tok < hi[t];
+#pragma unroll
+              for (int j = 0; j < JT; j++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                  if (sees) acc[t][j][k] = __builtin_fmaf(mine, (float)v[G::dim(j, 4 * g + k)], acc[t][j][k]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int tok = tv[i >> 2] + (i & 3);
+            if (!(tok >= lo_last && tok < hi_first))
+#pragma unroll
+              for (int k = 0; k < VW; k++) vr[i >> 2][i & 3][k] = 0;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < JT; j++) {
+          const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+          u32x4 o;
+#pragma unroll
+          for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_perm(vr[i >> 1][2 * (i & 1) + 1][j >> 1], vr[i >> 1][2 * (i & 1)][j >> 1], sel);
+          const h8 v = __builtin_bit_cast(h8, o);
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int u = 0; u < TERMS; u++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t][u], acc[t][j], 0, 0, 0);
+        }
+        if (more) load_v();
+      }
+    }
+
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const float sum = xor_add<32>(xor_add<16>(l[t]));
+      if (!valid[t]) continue;
+      if (s.whole) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* dst = (T*)a.out.p + qrow[t] * a.out.row + qhead[t] * a.out.head;
+        const bool ovec = vec_rows(a.out, sizeof(T));
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < JT; j += 4) {
+            T* to = dst + G::dim(j, 4 * g + i);
+            T o[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] = E::put(acc[t][j + k][i] * inv);
+            if (ovec) {
+              if constexpr (sizeof(T) == 4) *(u32x4*)to = *(u32x4*)o;
+              else *(u32x2*)to = *(u32x2*)o;
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; k++) to[k] = o[k];
+            }
+          }
+      } else {
+        const int64_t c = s.piece * COLS + t * 16 + col;
+        if (g == 0) pc.ml[c] = f4{mref[t], sum, kcol[t], 0.0f};
+        if (sum == 0.0f) continue;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < JT; j += 4) *(f4*)(pc.acc + c * D + G::dim(j, 4 * g + i)) = f4{acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]};
+      }
+    }
+  };
+
+  if constexpr (LISTED) {
+    const int ncts = (group + COLS - 1) / COLS;
+    const int item = w / parts, part = w - item * parts;
+    const int row = item / (n_kv * ncts), rest = item - row * (n_kv * ncts);
+    if (row >= a.rows) return;
+    const RowOf of(ro, lens, a.batch, a.rows, row);
+    if (of.b < 0) return;
+    Part s;
+    s.b = of.b;
+    s.h = rest / ncts;
+    s.c0 = (rest - s.h * ncts) * COLS;
+    s.r0 = row;
+    s.m = 1;
+    s.p0 = of.p;
+    s.list = a.blocks + ((int64_t)row * n_kv + s.h) * a.top;
+    s.entries = of.p < 0 ? 0 : min(min(a.top, a.pps), of.p / ps + 1);
+    const int tiles = (int)(((int64_t)s.entries * ps + kTile - 1) / kTile);
+    s.t0 = part * least;
+    s.t1 = min(s.t0 + least, tiles);
+    s.whole = whole;
+    s.piece = w;
+    work(s);
+  } else {
+    const Lines L{ro, lens, a.rows, n_kv, group, a.window, COLS, cap, kStart, whole};
+    Line line(L, a.batch, w, workers, least);
+    if (w == 0 && !whole) *pc.n_items = line.items();
+    while (line.next()) {
+      const Seq& x = line.s;
+      if (line.begins && !whole && lane == 0) pc.begun[line.item] = Begun{line.b, line.h, line.ct, w, line.pieces};
+      Part s;
+      s.b = line.b;
+      s.h = line.h;
+      s.r0 = x.r0;
+      s.m = x.m;
+      s.p0 = x.len - x.m;
+      s.c0 = line.ct * COLS;
+      s.t0 = x.lo + (whole ? 0 : max(line.at - kStart, 0));
+      s.t1 = x.lo + (whole ? x.tiles : max(line.at + line.n - kStart, 0));
+      s.whole = line.begins && line.ends;
+      s.piece = line.begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w;
+      s.list = nullptr;
+      s.entries = (int)(((int64_t)L.held(x.len) + ps - 1) / ps);
+      work(s);
+    }
+  }
+}
+
+// Joins the pieces of an item, in their order: a workgroup an item and `per` columns (more for every gridDim.y),
+// its waves by column and by piece.
+template <int D, class E, bool LISTED>
+__global__ void k_pool_merge(PoolAttn a, Lines L, PoolPieces pc, int per, int parts) {
+  constexpr int V = D / 64;  // dims a lane
+  typedef typename E::T T;
+  __shared__ float part[16][D];
+  __shared__ float pl[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int n, c0, r0, m, h;
+  int64_t first, rest;  // the first piece, and what the ones behind it are counted from
+  if constexpr (LISTED) {
+    const int ncts = (L.group + L.cols - 1) / L.cols, item = blockIdx.x, row = item / (L.n_kv * ncts), hc = item - row * (L.n_kv * ncts);
+    const RowOf of(L.ro, L.lens, a.batch, a.rows, row);
+    if (of.b < 0) return;
+    n = parts;
+    h = hc / ncts;
+    c0 = (hc - h * ncts) * L.cols;
+    r0 = row;
+    m = 1;
+    first = rest = (int64_t)item * parts;
+  } else {
+    const int items = *pc.n_items;
+    const Begun it = pc.begun[blockIdx.x];  // (of an item that is not: whatever is there)
+    n = it.pieces;
+    if ((int)blockIdx.x >= items || n == 0) return;
+    h = it.h;
+    c0 = it.ct * L.cols;
+    const int32_t* ro = L.ro + it.b;
+    r0 = min(max(ro[0], 0), L.rows);
+    m = max(min(max(ro[1], 0), L.rows) - r0, 0);
+    first = 2 * (int64_t)it.w + 1;
+    rest = 2 * (int64_t)it.w;
+  }
+  const auto slot = [&](int i, int c) { return (i == 0 ? first : LISTED ? rest + i : rest + 2 * i) * L.cols + c; };
+  const int share = (blockDim.x >> 6) / per, mine = wave % share;  // waves a column
+  const int at0 = blockIdx.y * per;
+  for (int at = at0; at < L.cols && (c0 + at) / L.group < m; at += gridDim.y * per) {  // the same for all waves
+    const int c = at + wave / share;
+    float acc[V] = {}, l = 0.0f, top = -FLT_MAX;
+    for (int i = lane; i < n; i += 64) {
+      const f4 y = pc.ml[slot(i, c)];
+      if (y[1] != 0.0f) top = fmaxf(top, y[0]);
+    }
+    top = wave_max(top);
+    for (int i0 = mine; i0 < n; i0 += 8 * share) {
+      f4 x[8];
+      float v[8][V];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {  // all loads before the first use
+        const int64_t p = slot(min(i0 + k * share, n - 1), c);
+        x[k] = pc.ml[p];
+#pragma unroll
+        for (int j = 0; j < V; j++) v[k][j] = pc.acc[p * D + lane * V + j];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const bool some = i0 + k * share < n && x[k][1] != 0.0f;
+        const float f = some ? __builtin_amdgcn_exp2f((x[k][0] - top) * x[k][2]) : 0.0f;
+        l = __builtin_fmaf(f, some ? x[k][1] : 0.0f, l);
+#pragma unroll
+        for (int j = 0; j < V; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
+      }
+    }
+    if (share > 1) {
+#pragma unroll
+      for (int j = 0; j < V; j++) part[wave][lane * V + j] = acc[j];
+      if (lane == 0) pl[wave] = l;
+      __syncthreads();
+      if (mine == 0)
+        for (int k = 1; k < share; k++) {
+#pragma unroll
+          for (int j = 0; j < V; j++) acc[j] += part[wave + k][lane * V + j];
+          l += pl[wave + k];
+        }
+      __syncthreads();
+    }
+    const int cc = c0 + c, r = cc / L.group;
+    if (r < m && mine == 0) {
+      T* dst = (T*)a.out.p + (int64_t)(r0 + r) * a.out.row + ((int64_t)h * L.group + cc % L.group) * a.out.head + lane * V;
+#pragma unroll
+      for (int j = 0; j < V; j++) dst[j] = E::put(l == 0.0f ? 0.0f : acc[j] / l);
+    }
+  }
+}
+
+// ---- launches ------------------------------------------------------------------------
+constexpr int kMergeWaves = 4096;
+constexpr int kWhole = 4;  // tiles of an item that one wave does, without a merge
+constexpr int kLeast = 2;  // tiles a wave takes at least
+constexpr int kOneTile = 16;  // columns a sequence up to which items have one tile of columns, above it two
+
+int64_t most_workers(int hd, int nt) { return (int64_t)compute_units() * 4 * pool_waves(hd, nt); }
+
+PoolPieces pool_pieces(void* ws, int64_t items, int64_t pieces, int cols) {
+  char* p = (char*)ws;
+  PoolPieces pc;
+  pc.n_items = (int*)p;
+  p += 256;
+  pc.begun = (Begun*)p;
+  p += align256(sizeof(Begun) * items);
+  pc.ml = (f4*)p;
+  p += align256(sizeof(f4) * pieces * cols);
+  pc.acc = (float*)p;
+  return pc;
+}
+
+// Parts that each item of a list of blocks is cut into, and the tiles of a part.
+struct Cut {
+  int64_t items;
+  int parts, tiles;
+};
+Cut listed_cut(int n_q, int n_kv, int hd, int rows, int64_t tiles) {
+  const int group = n_q / n_kv, ncts = (group + 15) / 16;
+  Cut c;
+  c.items = (int64_t)rows * n_kv * ncts;
+  int64_t parts = most_workers(hd, 1) / c.items;
+  parts = std::min(parts, (tiles + kLeast - 1) / kLeast);
+  if (tiles <= kWhole || parts < 1) parts = 1;
+  c.tiles = (int)((tiles + parts - 1) / parts);
+  c.parts = (int)((tiles + c.tiles - 1) / c.tiles);
+  return c;
+}
+
+template <int D, class E, bool LISTED>
+hipError_t merge(hipStream_t st, const PoolAttn& a, const PoolPieces& pc, int64_t items, int64_t pieces, int cols, int parts) {
+  const int group = a.n_q / a.c.n_kv;
+  const int cap = (int)std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0);
+  const Lines L{a.row_offsets, a.lengths, a.rows, a.c.n_kv, group, a.window, cols, cap, kStart, false};
+  // Waves a column: more where an item has many pieces, but not where there are columns enough to fill the card.
+  const int64_t columns = std::min<int64_t>(cols, LISTED ? group : (int64_t)a.max_rows * group);
+  const int each = (int)(pieces / items);
+  int share = each >= 16 ? 16 : each >= 4 ? 4 : 1;
+  while (share > 1 && items * columns * share > kMergeWaves) share /= 4;
+  const int per = share == 1 ? 4 : 1;
+  hipLaunchKernelGGL((k_pool_merge<D, E, LISTED>), dim3((unsigned)items, (unsigned)((columns + per - 1) / per)), dim3(share == 16 ? 1024 : 256),
+                     0, st, a, L, pc, per, parts);
+  return hipGetLastError();
+}
+
+template <int D, int NT, class E>
+hipError_t attn_tiles(hipStream_t st, const PoolAttn& a) {
+  const int cols = 16 * NT;
+  const int64_t cap = std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0), tiles = (cap + kTile - 1) / kTile;
+  const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
+  const bool whole = tiles <= kWhole;
+  const int64_t most = most_workers(D, NT), want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
+  const int64_t workers = whole ? (items + 3) / 4 * 4 : (std::min(most, want) + 3) / 4 * 4;
+  const PoolPieces pc = pool_pieces(a.ws, items, 2 * workers, cols);
+  hipLaunchKernelGGL((k_pool_attn<D, NT, E, false>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths, a.page_table,
+                     pc, (int)workers, whole ? 1 : kLeast, whole, 0);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || whole ? e : merge<D, E, false>(st, a, pc, items, workers, cols, 0);
+}
+
+template <int D, class E>
+hipError_t attn_listed(hipStream_t st, const PoolAttn& a) {
+  const int64_t entries = std::min<int64_t>(a.top, a.pps), tiles = (entries * a.c.page_size + kTile - 1) / kTile;
+  const Cut c = listed_cut(a.n_q, a.c.n_kv, D, a.rows, tiles);
+  const int64_t workers = (c.items * c.parts + 3) / 4 * 4;
+  const PoolPieces pc = pool_pieces(a.ws, 0, workers, 16);
+  hipLaunchKernelGGL((k_pool_attn<D, 1, E, true>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths, a.page_table,
+                     pc, (int)workers, c.tiles, c.parts == 1, c.parts);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || c.parts == 1 ? e : merge<D, E, true>(st, a, pc, c.items, c.items * c.parts, 16, c.parts);
+}
+
+template <int D, class E>
+hipError_t attn_dim(hipStream_t st, const PoolAttn& a) {
+  if (a.blocks) return attn_listed<D, E>(st, a);
+  if constexpr (D != 256)
+    if ((int64_t)a.max_rows * (a.n_q / a.c.n_kv) > kOneTile) return attn_tiles<D, 2, E>(st, a);
+  return attn_tiles<D, 1, E>(st, a);
+}
+
+template <class E>
+hipError_t attn_type(hipStream_t st, const PoolAttn& a) {
+  if (a.c.hd == 64) return attn_dim<64, E>(st, a);
+  if (a.c.hd == 128) return attn_dim<128, E>(st, a);
+  return attn_dim<256, E>(st, a);
+}
+
+}  // namespace
+
+// A grid holds fewer than 2^32 threads: of a merge with 256 an item (those with more have few items), and of a wave
+// an item of a list.
+bool pool_attn_fits(int n_q, int n_kv, int batch, int rows) {
+  const int64_t items = std::max(attn_items(n_q, n_kv, batch, rows, 16), (int64_t)rows * n_kv * ((n_q / n_kv + 15) / 16));
+  return (int64_t)rows * n_q <= 0x7FFFF000 && items < (1 << 24);
+}
+
+size_t pool_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows) {
+  // a call has at most two pieces a worker, of 32 columns at most; a list's parts are no more than the workers
+  const int64_t columns = 2 * std::max(most_workers(hd, 1) * 16, most_workers(hd, 2) * 32) + 64;
+  return 256 + align256(sizeof(Begun) * attn_items(n_q, n_kv, batch, rows, 16)) + align256(sizeof(f4) * columns) + sizeof(float) * columns * hd;
+}
+
+hipError_t launch_pool_attn(hipStream_t st, int dtype, const PoolAttn& a) {
+  if (a.rows == 0 || a.batch == 0) return hipSuccess;
+  if (dtype == RSTR_F32) return attn_type<F32>(st, a);
+  if (dtype == RSTR_F16) return attn_type<F16>(st, a);
+  return attn_type<BF16>(st, a);
+}
+
+}  // namespace rstr

@@ -24,6 +24,7 @@
 
 #include "device_math.h"
 #include "kernels.h"
+#include "pool_ops.h"
 #include "session.h"
 
 using namespace rstr;
@@ -172,6 +173,8 @@ struct rstr_pool {
   void* attn_host = nullptr;
   size_t attn_dev_bytes = 0, attn_host_bytes = 0;
   bool attn_busy = false;  // a call uses them
+  int held = 0;            // open handles that read the pool on streams of their own
+  bool shared = false;     // work on it may be queued on any stream
 };
 // What a pool keeps for the isolated attention between calls: a device block, and
 // pinned staging of arrays up to kAttnStage.  Calls with larger partials, and calls
@@ -762,7 +765,9 @@ extern "C" int rstr_pool_open(rstr_model* m, int32_t page_size, int32_t physical
 extern "C" int rstr_pool_close(rstr_pool* p) {
   if (!p) return RSTR_OK;
   if (p->open_transfers > 0) return fail(p->m->s, RSTR_E_STATE, "pool has chunk transfers in flight");
+  if (p->held > 0) return fail(p->m->s, RSTR_E_STATE, "pool has open attention plans or block bounds");
   hipSetDevice(p->m->s->device);
+  if (p->shared) (void)hipDeviceSynchronize();
   {
     std::lock_guard<std::mutex> lock(g_pools_mu);
     g_pools.erase(std::remove(g_pools.begin(), g_pools.end(), p), g_pools.end());
@@ -782,6 +787,15 @@ extern "C" int rstr_pool_close(rstr_pool* p) {
   delete p;
   return RSTR_OK;
 }
+
+// What the operators on device arrays see of a pool (pool_ops.h).
+PoolView rstr::pool_view(const rstr_pool* p, int layer) {
+  const rstr_model_desc& d = p->m->d;
+  return PoolView{p->m->s, d.n_layers,
+                  PoolLayer{p->slabs[layer], p->slabs[d.n_layers + layer], d.n_kv, d.head_dim, p->page_size, p->physical_pages}};
+}
+void rstr::pool_hold(rstr_pool* p, int by) { p->held += by; }
+void rstr::pool_shared(rstr_pool* p) { p->shared = true; }
 
 // ---------------------------------------------------------------------------
 // durable chunk transfer

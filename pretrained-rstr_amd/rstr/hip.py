@@ -46,6 +46,8 @@ EXPORTS = (
     "rstr_kv4_open", "rstr_kv4_close", "rstr_kv4_bytes", "rstr_kv4_append", "rstr_kv4_read",
     "rstr_kv4_attn_open", "rstr_kv4_attn_close", "rstr_kv4_attn_run",
     "rstr_step_maps", "rstr_verify_open", "rstr_verify_close", "rstr_verify_run",
+    "rstr_pool_device", "rstr_pool_rope_append", "rstr_pool_attn_open", "rstr_pool_attn_close", "rstr_pool_attn_run",
+    "rstr_bounds_open", "rstr_bounds_close", "rstr_bounds_device", "rstr_bounds_update", "rstr_select_open", "rstr_select_close", "rstr_select_run",
 )
 
 
@@ -160,6 +162,18 @@ def lib():
             "rstr_verify_open": (i32, [P, i32, i32, i32, C.POINTER(P)]),
             "rstr_verify_close": (i32, [P]),
             "rstr_verify_run": (i32, [P, i32, i32, i32, P, i64, P, P, P, i64, P, P, P, P, P, P]),
+            "rstr_pool_device": (i32, [P, i32, i32, C.POINTER(P)]),
+            "rstr_pool_rope_append": (i32, [P, i32, i32, i32, P, i64, i64, P, i64, i64, i32, P, i64, i64, P, i64, i64, P, P, f32, f32, i32, P, P, P, P]),
+            "rstr_pool_attn_open": (i32, [P, i32, i32, i32, C.POINTER(P)]),
+            "rstr_pool_attn_close": (i32, [P]),
+            "rstr_pool_attn_run": (i32, [P, i32, i32, i32, i32, i32, i32, f32, P, i64, i64, P, P, i32, P, P, i32, P, i64, i64, P]),
+            "rstr_bounds_open": (i32, [P, C.POINTER(P)]),
+            "rstr_bounds_close": (i32, [P]),
+            "rstr_bounds_device": (i32, [P, i32, C.POINTER(P)]),
+            "rstr_bounds_update": (i32, [P, i32, i32, i32, P, P, i32, P, P]),
+            "rstr_select_open": (i32, [P, i32, i32, i32, i32, C.POINTER(P)]),
+            "rstr_select_close": (i32, [P]),
+            "rstr_select_run": (i32, [P, i32, i32, i32, i32, P, i64, i64, P, P, i32, P, i32, i32, i32, P, P]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -330,8 +344,9 @@ class Session:
 
     def close(self):
         if self.h:
-            order = {"Decoder": 0, "Prefill": 0, "Kv4Attention": 0, "Verifier": 0, "Pool": 1, "Kv4Pool": 1, "Model": 2}
-            for obj in sorted(self.children, key=lambda o: order.get(type(o).__name__, 3)):
+            order = {"Decoder": 0, "Prefill": 0, "Kv4Attention": 0, "Verifier": 0, "PagedAttention": 0, "BlockSelect": 0,
+                     "BlockBounds": 1, "Pool": 2, "Kv4Pool": 2, "Model": 3}
+            for obj in sorted(self.children, key=lambda o: order.get(type(o).__name__, 4)):
                 obj.close()
             self.children = []
             lib().rstr_session_close(self.h)
@@ -497,6 +512,51 @@ class Pool:
         self.sess.check(lib().rstr_append_run(self.h, layer, slots.size, _p(k_rows), _p(v_rows),
                                               _p(slots)))
 
+    def pages_device(self, slab: int, layer: int) -> DeviceView:
+        """One slab (0: keys, 1: values) of a layer where it is, on the GPU (rstr_pool_device):
+        float16 [pages][page_size][n_kv][head_dim]."""
+        c, p = self.model.cfg, C.c_void_p()
+        self.sess.check(lib().rstr_pool_device(self.h, slab, layer, C.byref(p)))
+        return DeviceView(p.value, (self.physical_pages, self.page_size, c["n_kv"], c["head_dim"]), "float16", self.sess.device, self)
+
+    def rope_append(self, layer: int, k, v, slots, positions=None, frequencies=None, q=None, q_out=None, q_gain=None, k_gain=None,
+                    eps: float = 1e-6, gain_offset: float = 0.0, stream=None):
+        """Appends device rows k, v [rows][n_kv][head_dim] to ``slots`` [rows], and writes q [rows][n_q][head_dim] to
+        ``q_out`` (``q`` itself, by default), with heads of q and k normalised where a float32 gain [head_dim] is
+        given and turned by ``positions`` [rows] times the float64 ``frequencies`` [rotary_dim / 2] (None: not
+        turned) (rstr_pool_rope_append).  Rows whose slot is negative are not appended."""
+        s, c = self.sess, self.model.cfg
+        rows, hd = slots.shape[0], c["head_dim"]
+        kp, kt, kr, kh = _rows(s, k, "k", c["n_kv"], hd, rows)
+        vp, vt, vr, vh = _rows(s, v, "v", c["n_kv"], hd, rows)
+        n_q, qs, os = 0, (None, 0, 0), (None, 0, 0)
+        if q is not None:
+            n_q = q.shape[1]
+            qp, qt, qr, qh = _rows(s, q, "q", n_q, hd, rows)
+            qs = os = qp, qr, qh
+            if q_out is not None:
+                op, ot, orow, oh = _rows(s, q_out, "q_out", n_q, hd, rows)
+                os = op, orow, oh
+                if ot != qt:
+                    raise ValueError("q and q_out must have the same element type")
+            if qt != kt:
+                raise ValueError("q, k and v must have the same element type")
+        elif q_out is not None:
+            raise ValueError("q_out is given without q")
+        if kt != vt:
+            raise ValueError("k and v must have the same element type")
+        rot, fp, pp = 0, None, None
+        if frequencies is not None:
+            if positions is None:
+                raise ValueError("frequencies are given without positions")
+            half = frequencies.shape[0]
+            rot, fp = 2 * half, _flat(s, frequencies, "frequencies", (half,), "float64", "float64")
+            pp = _ints(s, positions, "positions", (rows,))
+        s.check(lib().rstr_pool_rope_append(
+            self.h, layer, rows, kt, kp, kr, kh, vp, vr, vh, n_q, *qs, *os,
+            None if q_gain is None else _floats(s, q_gain, "q_gain", (hd,)), None if k_gain is None else _floats(s, k_gain, "k_gain", (hd,)),
+            eps, gain_offset, rot, fp, pp, _ints(s, slots, "slots", (rows,)), _stream(s, stream)))
+
     def chunk_elements(self, token_count: int) -> int:
         """Payload elements of a durable chunk of ``token_count`` tokens."""
         c = self.model.cfg
@@ -574,7 +634,7 @@ class Pool:
         return a.value, b.value
 
     def close(self):
-        """Frees the slabs; refused (RstrError) while chunk transfers are in flight."""
+        """Frees the slabs; refused (RstrError) while chunk transfers are in flight, or plans or bounds open."""
         if self.h:
             self.sess.check(lib().rstr_pool_close(self.h))
             self.h = None
@@ -865,6 +925,107 @@ class Verifier:
     def close(self):
         if self.h:
             self.sess.check(lib().rstr_verify_close(self.h))
+            self.h = None
+            _left(self)
+
+
+class PagedAttention:
+    """Attention over a :class:`Pool` from device arrays (rstr_pool_attn_run) and its workspace: one
+    call at a time, so programs and graphs that run side by side have one each."""
+
+    def __init__(self, pool: Pool, n_q: int, max_batch: int, max_rows: int):
+        self.pool, self.sess, self.n_q, self.max_batch, self.max_rows = pool, pool.sess, n_q, max_batch, max_rows
+        h = C.c_void_p()
+        self.sess.check(lib().rstr_pool_attn_open(pool.h, n_q, max_batch, max_rows, C.byref(h)))
+        self.h = h
+        self.sess._adopt(self)
+
+    def run(self, layer: int, q, row_offsets, page_table, lengths, out, max_rows: int | None = None, window: int = 0,
+            scale: float | None = None, blocks=None, stream=None):
+        """q, out [rows][n_q][head_dim] of one type; int32 row_offsets [batch+1], page_table
+        [batch][width], lengths [batch].  ``max_rows``: the most rows of one sequence (default: all rows).
+        ``blocks``: int32 [rows][n_kv][count], the blocks of the table that each row and kv head sees (None: all)."""
+        s, c = self.sess, self.pool.model.cfg
+        hd = c["head_dim"]
+        batch, rows = lengths.shape[0], q.shape[0]
+        qp, t, qr, qh = _rows(s, q, "q", self.n_q, hd)
+        op, ot, orow, oh = _rows(s, out, "out", self.n_q, hd, rows)
+        if t != ot:
+            raise ValueError("q and out must have the same element type")
+        width, bp, count = page_table.shape[1], None, 0
+        if blocks is not None:
+            count = blocks.shape[2]
+            bp = _ints(s, blocks, "blocks", (rows, c["n_kv"], count))
+        s.check(lib().rstr_pool_attn_run(
+            self.h, layer, t, batch, rows, rows if max_rows is None else max_rows, min(window, 0x7FFFFFFF), hd ** -0.5 if scale is None else scale,
+            qp, qr, qh, _ints(s, row_offsets, "row_offsets", (batch + 1,)), _ints(s, page_table, "page_table", (batch, width)),
+            width, _ints(s, lengths, "lengths", (batch,)), bp, count, op, orow, oh, _stream(s, stream)))
+
+    def close(self):
+        if self.h:
+            self.sess.check(lib().rstr_pool_attn_close(self.h))
+            self.h = None
+            _left(self)
+
+
+class BlockBounds:
+    """The least and the greatest key element of every channel of a :class:`Pool`'s pages (rstr_bounds_open)."""
+
+    def __init__(self, pool: Pool):
+        self.pool, self.sess = pool, pool.sess
+        h = C.c_void_p()
+        self.sess.check(lib().rstr_bounds_open(pool.h, C.byref(h)))
+        self.h = h
+        self.sess._adopt(self)
+
+    def update(self, layer: int, row_offsets, page_table, lengths, rows: int, stream=None):
+        """Bounds of the pages in which the new rows of a step lie, ``rows`` of them at most, from the keys that are
+        there (rstr_bounds_update)."""
+        s, batch, width = self.sess, lengths.shape[0], page_table.shape[1]
+        s.check(lib().rstr_bounds_update(
+            self.h, layer, batch, rows, _ints(s, row_offsets, "row_offsets", (batch + 1,)),
+            _ints(s, page_table, "page_table", (batch, width)), width, _ints(s, lengths, "lengths", (batch,)), _stream(s, stream)))
+
+    def device(self, layer: int) -> DeviceView:
+        """A layer's bounds where they are, on the GPU: float16 [pages][n_kv][2][head_dim]."""
+        c, p = self.pool.model.cfg, C.c_void_p()
+        self.sess.check(lib().rstr_bounds_device(self.h, layer, C.byref(p)))
+        return DeviceView(p.value, (self.pool.physical_pages, c["n_kv"], 2, c["head_dim"]), "float16", self.sess.device, self)
+
+    def close(self):
+        """Refused (RstrError) while selections are open."""
+        if self.h:
+            self.sess.check(lib().rstr_bounds_close(self.h))
+            self.h = None
+            _left(self)
+
+
+class BlockSelect:
+    """Selection of the blocks that a query reads, by the bounds of their keys (rstr_select_run), and its workspace:
+    one call at a time."""
+
+    def __init__(self, bounds: BlockBounds, n_q: int, max_batch: int, max_rows: int, max_pages: int):
+        self.bounds, self.sess, self.n_q = bounds, bounds.sess, n_q
+        self.max_batch, self.max_rows, self.max_pages = max_batch, max_rows, max_pages
+        h = C.c_void_p()
+        self.sess.check(lib().rstr_select_open(bounds.h, n_q, max_batch, max_rows, max_pages, C.byref(h)))
+        self.h = h
+        self.sess._adopt(self)
+
+    def run(self, layer: int, q, row_offsets, page_table, lengths, blocks, first: int = 1, last: int = 1, stream=None):
+        """Writes int32 ``blocks`` [rows][n_kv][count]: for q [rows][n_q][head_dim], the blocks of highest score, the
+        ``first`` first and the ``last`` last ones always among them; ascending, -1 behind the last."""
+        s, c = self.sess, self.bounds.pool.model.cfg
+        batch, rows, width, count = lengths.shape[0], q.shape[0], page_table.shape[1], blocks.shape[2]
+        qp, t, qr, qh = _rows(s, q, "q", self.n_q, c["head_dim"])
+        s.check(lib().rstr_select_run(
+            self.h, layer, t, batch, rows, qp, qr, qh, _ints(s, row_offsets, "row_offsets", (batch + 1,)),
+            _ints(s, page_table, "page_table", (batch, width)), width, _ints(s, lengths, "lengths", (batch,)), count, first, last,
+            _ints(s, blocks, "blocks", (rows, c["n_kv"], count)), _stream(s, stream)))
+
+    def close(self):
+        if self.h:
+            self.sess.check(lib().rstr_select_close(self.h))
             self.h = None
             _left(self)
 
