@@ -172,25 +172,42 @@ def _open_session():
     return _session
 
 
-class _Held(dict):
-    """A case's inputs, with the handles that a serving program keeps; closed with the object."""
+class _Handles(list):
+    """The handles that a serving program keeps, in the order of opening; closed once neither a state nor what a pass returned
+    (the pool's own pages, the bounds) needs them."""
 
     def __del__(self):
-        for name in ("select", "plan", "bounds", "pool", "model"):
-            if name in self:
-                self.pop(name).close()
+        while self:
+            self.pop().close()
+
+
+class _Lent:
+    """Memory of a handle as a tensor takes it, which keeps the handles open."""
+
+    def __init__(self, view, handles):
+        self.__cuda_array_interface__, self._handles = view.__cuda_array_interface__, handles
+
+
+def _lent(s, view):
+    return torch.as_tensor(_Lent(view, s["handles"]), device="cuda")
+
+
+def _opened(s, name, handle):
+    s["handles"].append(handle)
+    s[name] = handle
 
 
 def _open_pool(s, case, pages):
-    """The pool of one layer of a model with these heads, and its pages as tensors."""
+    """The pool of one layer of a model with these heads."""
     hip = _hip()
+    s["handles"] = _Handles()
     cfg = dict(n_layers=1, d_model=256, d_ff=256, n_q=case["n_kv"], n_kv=case["n_kv"], head_dim=case["hd"], vocab=256, weight_bits=4,
                gain_offset=0, qk_norm=0, sandwich=0, ffn_geglu=0, rope_dual=0, global_pattern=0, sliding_window=0,
                embed_scale_sqrt_d=0, eps=1e-6, attn_scale=case["hd"] ** -0.5, rope_global=1e4, rope_local=1e4)
     if case["n_kv"] * case["hd"] % 128:
         cfg["n_q"] *= 2
-    s["model"] = hip.Model(_open_session(), cfg, seed=1)
-    s["pool"] = hip.Pool(s["model"], case["page"], pages)
+    _opened(s, "model", hip.Model(_open_session(), cfg, seed=1))
+    _opened(s, "pool", hip.Pool(s["model"], case["page"], pages))
 
 
 def _paged(need, pages, rng):
@@ -224,14 +241,14 @@ def _prepare_rope(case, seed, g, rng):
     qkv[:, :, hd // 2:: 17] *= 4.0  # a few channels of larger values, as queries and keys have them
     qkv = qkv.to(dt)  # as a projection of all heads leaves them
     rot = case["rot"]
-    s = _Held(case=case, q=qkv[:, :n_q], k=qkv[:, n_q:n_q + n_kv], v=qkv[:, n_q + n_kv:], slots=_dev(slots), positions=_dev(positions),
+    s = dict(case=case, q=qkv[:, :n_q], k=qkv[:, n_q:n_q + n_kv], v=qkv[:, n_q + n_kv:], slots=_dev(slots), positions=_dev(positions),
               frequencies=_dev(case["theta"] ** (-np.arange(0, rot, 2) / rot), torch.float64), q_gain=None, k_gain=None, eps=1e-6,
               q_out=torch.empty(rows, n_q, hd, dtype=dt, device="cuda"))
     if case["norm"]:
         s["q_gain"], s["k_gain"] = (1.0 + 0.2 * torch.randn(hd, generator=g, device="cuda") for _ in "qk")
     if own:
         _open_pool(s, case, pages)
-        s["pages"] = [torch.as_tensor(s["pool"].pages_device(slab, 0), device="cuda") for slab in (0, 1)]
+        s["pages"] = [_lent(s, s["pool"].pages_device(slab, 0)) for slab in (0, 1)]
     else:
         s["pages"] = [torch.zeros(pages, page, n_kv, hd, dtype=torch.float16, device="cuda") for _ in "kv"]
     return s
@@ -255,7 +272,7 @@ def _prepare_attend(case, seed, g, rng):
     v = torch.randn(total, n_kv, hd, generator=g, device="cuda") * 0.7
     q = torch.randn(rows, n_q, hd, generator=g, device="cuda") * 0.7
     q += 0.6 * about[_dev(rng.integers(0, 16, rows), torch.int64)].repeat_interleave(n_q // n_kv, 1)
-    s = _Held(case=case, lengths=_dev(lens), offsets=_dev(offs), table=_dev(table), most=int(news.max()), scale=hd ** -0.5,
+    s = dict(case=case, lengths=_dev(lens), offsets=_dev(offs), table=_dev(table), most=int(news.max()), scale=hd ** -0.5,
               batch=batch, q=q.to(DTYPES[case["dtype"]]))
     s["out"] = torch.empty_like(s["q"])
     k, v = k.half(), v.half()
@@ -265,12 +282,12 @@ def _prepare_attend(case, seed, g, rng):
         hip = _hip()
         _open_pool(s, case, pages)
         s["pool"].rope_append(0, k, v, slots)  # the keys as they are
-        s["plan"] = hip.PagedAttention(s["pool"], n_q, batch, rows)
+        _opened(s, "plan", hip.PagedAttention(s["pool"], n_q, batch, rows))
         if case["kind"] == "sparse":
-            s["bounds"] = hip.BlockBounds(s["pool"])
-            s["select"] = hip.BlockSelect(s["bounds"], n_q, batch, rows, table.shape[1])
+            _opened(s, "bounds", hip.BlockBounds(s["pool"]))
+            _opened(s, "select", hip.BlockSelect(s["bounds"], n_q, batch, rows, table.shape[1]))
             s["bounds"].update(0, _dev(np.concatenate([[0], np.cumsum(lens)])), s["table"], s["lengths"], total)
-            s["limits"] = torch.as_tensor(s["bounds"].device(0), device="cuda")
+            s["limits"] = _lent(s, s["bounds"].device(0))
     else:
         s["pages"] = [torch.zeros(pages * page, n_kv, hd, dtype=torch.float16, device="cuda") for _ in "kv"]
         for to, x in zip(s["pages"], (k, v)):
