@@ -679,13 +679,6 @@ hipError_t attn_type(hipStream_t st, const PoolAttn& a) {
 
 }  // namespace
 
-// A grid holds fewer than 2^32 threads: of a merge with 256 an item (those with more have few items), and of a wave
-// an item of a list.
-bool pool_attn_fits(int n_q, int n_kv, int batch, int rows) {
-  const int64_t items = std::max(attn_items(n_q, n_kv, batch, rows, 16), (int64_t)rows * n_kv * ((n_q / n_kv + 15) / 16));
-  return (int64_t)rows * n_q <= 0x7FFFF000 && items < (1 << 24);
-}
-
 size_t pool_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows) {
   // a call has at most two pieces a worker, of 32 columns at most; a list's parts are no more than the workers
   const int64_t columns = 2 * std::max(most_workers(hd, 1) * 16, most_workers(hd, 2) * 32) + 64;

@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "kv4.h"
+#include "kv4_line.h"
 
 struct rstr_pool;
 struct rstr_session;
@@ -49,10 +50,14 @@ struct PoolAttn {
   const int32_t* blocks;  // [rows][n_kv][top], or null: all blocks
   void* ws;
 };
-// Bytes of workspace that every call of up to `rows` query rows and `batch` sequences can need, and whether a
-// grid holds them.
+// Bytes of workspace that every call of up to `rows` query rows and `batch` sequences can need.
 size_t pool_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows);
-bool pool_attn_fits(int n_q, int n_kv, int batch, int rows);
+// A grid holds fewer than 2^32 threads: of a merge with 256 an item (those with more have few items), and of a wave
+// an item of a list.
+inline bool pool_attn_fits(int n_q, int n_kv, int batch, int rows) {
+  const int64_t dense = attn_items(n_q, n_kv, batch, rows, 16), listed = (int64_t)rows * n_kv * ((n_q / n_kv + 15) / 16);
+  return (int64_t)rows * n_q <= 0x7FFFF000 && dense < (1 << 24) && listed < (1 << 24);
+}
 hipError_t launch_pool_attn(hipStream_t st, int dtype, const PoolAttn& a);
 
 // Bounds of one layer's blocks: fp16 [page][n_kv][2][hd], the least and the greatest key element of a channel.
@@ -74,7 +79,10 @@ struct BlockSelect {
   void* ws;
   int ws_blocks;  // blocks a row and kv head that the workspace has room for
 };
-bool select_fits(int n_kv, int rows, int blocks);  // grids hold it
+constexpr int kScoreBlocks = 64;  // blocks that a wave scores
+inline bool select_fits(int n_kv, int rows, int blocks) {  // grids hold it
+  return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * ((blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26);
+}
 size_t select_workspace(int n_q, int n_kv, int hd, int rows, int blocks);
 hipError_t launch_block_select(hipStream_t st, int dtype, const BlockSelect& a);
 

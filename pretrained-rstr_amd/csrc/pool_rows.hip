@@ -206,7 +206,6 @@ __global__ void __launch_bounds__(256) k_bounds_update(BoundsUpdate a) {
 // fp16 or bf16 lose nothing: which of two blocks is taken is part of the result.
 // 1. k_block_scores: the scores, as integers of the same order (a NaN counts as +infinity).
 // 2. k_block_pick: the border, found by eight bits of it at a time, and the list in ascending order.
-constexpr int kScoreBlocks = 64;  // blocks a wave
 
 __device__ __forceinline__ uint64_t order_of(double s) {
   if (s != s) s = INFINITY;
@@ -395,11 +394,6 @@ hipError_t launch_bounds_update(hipStream_t st, const BoundsUpdate& a) {
   else if (a.c.hd == 128) hipLaunchKernelGGL(k_bounds_update<128>, dim3(grid), dim3(256), 0, st, a);
   else hipLaunchKernelGGL(k_bounds_update<256>, dim3(grid), dim3(256), 0, st, a);
   return hipGetLastError();
-}
-
-bool select_fits(int n_kv, int rows, int blocks) {
-  return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * ((blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26) &&
-         (double)rows * n_kv * blocks < 1e14;
 }
 
 size_t select_workspace(int n_q, int n_kv, int hd, int rows, int blocks) {

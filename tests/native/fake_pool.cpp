@@ -1,0 +1,48 @@
+// A pool without a GPU for the operators over it: beside fake_device.cpp, which counts the launches.
+#include <hip/hip_runtime.h>
+
+#include <cstdlib>
+
+#include "../../pretrained-rstr_amd/csrc/pool_ops.h"
+#include "../../pretrained-rstr_amd/csrc/session.h"
+
+struct rstr_model {
+  rstr_session* s;
+  rstr_model_desc d;
+};
+struct rstr_pool {
+  rstr_model* m;
+  int page_size, pages, held;
+  char* slab[8];
+};
+
+// one launch of the counting device
+static hipError_t launched(hipStream_t st) { return rstr::launch_step_maps(st, rstr::StepMaps{}); }
+
+rstr::PoolView rstr::pool_view(const rstr_pool* p, int layer) {
+  const rstr_model_desc& d = p->m->d;
+  return PoolView{p->m->s, d.n_layers, PoolLayer{(uint16_t*)p->slab[layer], (uint16_t*)p->slab[d.n_layers + layer], d.n_kv, d.head_dim, p->page_size, p->pages}};
+}
+void rstr::pool_hold(rstr_pool* p, int by) { p->held += by; }
+void rstr::pool_shared(rstr_pool*) {}
+hipError_t rstr::launch_rope_append(hipStream_t st, int, const RopeAppend&) { return launched(st); }
+size_t rstr::pool_attn_workspace(int, int, int, int, int) { return 64; }
+hipError_t rstr::launch_pool_attn(hipStream_t st, int, const PoolAttn&) { return launched(st); }
+hipError_t rstr::launch_bounds_update(hipStream_t st, const BoundsUpdate&) { return launched(st); }
+size_t rstr::select_workspace(int, int, int, int, int) { return 64; }
+hipError_t rstr::launch_block_select(hipStream_t st, int, const BlockSelect&) { return launched(st); }
+
+extern "C" {
+int rstr_model_bind_synthetic(rstr_session* s, const rstr_model_desc* d, uint64_t, rstr_model** out) { return *out = new rstr_model{s, *d}, 0; }
+int rstr_model_close(rstr_model* m) { return delete m, 0; }
+int rstr_pool_open(rstr_model* m, int32_t page_size, int32_t pages, rstr_pool** out) {
+  *out = new rstr_pool{m, page_size, pages, 0, {}};
+  for (int i = 0; i < 2 * m->d.n_layers; i++) (*out)->slab[i] = (char*)malloc((size_t)page_size * pages * m->d.n_kv * m->d.head_dim * 2);
+  return 0;
+}
+int rstr_pool_close(rstr_pool* p) {
+  if (p->held) return rstr::fail(p->m->s, RSTR_E_STATE, "pool has open attention plans or block bounds");
+  for (char* x : p->slab) free(x);
+  return delete p, 0;
+}
+}
