@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "../../include/rstr_hip.h"
 #include "attn_line.h"
@@ -48,6 +49,12 @@ __device__ __forceinline__ _Float16 first_term(float x) {
 
 constexpr int pool_waves(int hd, int nt) { return hd == 256 ? 1 : 2; }
 
+// What raw scores of queries that were brought down by 2^e are multiplied with: finite and not 0, so that it leaves the
+// difference of two equal scores 0 and that of a score and -infinity -infinity.
+__device__ __forceinline__ float score_scale(float scale, int e) {
+  return fmaxf(fminf(__builtin_amdgcn_ldexpf(fabsf(scale) * 1.4426950408889634f, e), FLT_MAX), FLT_MIN);
+}
+
 // What the parts of an item leave: (m, l, k) and O of each column.
 struct PoolPieces {
   int* n_items;
@@ -73,6 +80,13 @@ struct Dims {
   // dim of row r of product j
   static __device__ __forceinline__ constexpr int dim(int j, int r) { return j / PIECE * 128 + PIECE * r + j % PIECE; }
 };
+
+// s_waitcnt vmcnt(0) alone: loads into LDS are not waited for by a barrier.
+__device__ __forceinline__ void wait_vmem() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  asm volatile("" ::: "memory");
+}
 
 template <bool STREAM, class V>
 __device__ __forceinline__ V load_page(const void* p) {
@@ -232,7 +246,7 @@ __global__ void __launch_bounds__(256, pool_waves(D, NT))
         big = xor_max<32>(xor_max<16>(big));
         // (a largest of 0 or infinity has the exponent 0; the sign of the scale goes into the queries)
         const int e = __builtin_amdgcn_frexp_expf(big) - 15;
-        kcol[t] = fminf(__builtin_amdgcn_ldexpf(fabsf(a.scale) * 1.4426950408889634f, e), FLT_MAX);
+        kcol[t] = score_scale(a.scale, e);
 #pragma unroll
         for (int s2 = 0; s2 < KS; s2++)
 #pragma unroll
@@ -495,6 +509,415 @@ __global__ void __launch_bounds__(256, pool_waves(D, NT))
   }
 }
 
+// ---- prompts -----------------------------------------------------------------------------
+// Many columns a sequence: the waves of a workgroup take 32 columns each, two tiles of 16, of one sequence and kv head and
+// share its keys and values, which go straight from the pages into LDS, 64 tokens at a time and one step ahead.
+// The products are those of k_pool_attn.  K's operand is 16 bytes of a row; the operand of V, eight tokens of one dim, comes from two
+// transposing reads of four tokens x 16 dims.  A row of a token is swizzled in LDS by its number, 16 bytes at a time, so that 16 tokens' same
+// dims lie in different banks; the loads into LDS write 1 KB in the lanes' order, so a lane asks for the piece that
+// belongs to its place.
+constexpr int kPromptStart = 8;  // what beginning an item costs, in tiles
+constexpr int kStep = 64;        // tokens at a time
+constexpr int prompt_waves(int hd, int terms) { return hd == 256 || (hd == 128 && terms == 2) ? 4 : 8; }  // (registers of one wave a SIMD, or of two)
+
+typedef short sv4 __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(4))) int32_t* TablePtr;  // read-only for the kernel: scalar loads
+typedef __attribute__((address_space(3))) uint8_t* LdsPtr;
+#define RSTR_LDS(p) ((__attribute__((address_space(3))) void*)(p))
+
+__device__ __forceinline__ u32x2 read_transposed(LdsPtr at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sv4*)at));
+}
+template <int D, class E>
+__global__ void __launch_bounds__(64 * prompt_waves(D, Terms<E>::n), prompt_waves(D, Terms<E>::n) / 4)
+    k_pool_prompt(PoolAttn a, const int32_t* __restrict__ ro, const int32_t* __restrict__ lens, const int32_t* __restrict__ table, PoolPieces pc,
+                  int workers, int least) {
+  typedef typename E::T T;
+  constexpr int NT = 2, TERMS = Terms<E>::n, WAVES = prompt_waves(D, TERMS), COLS = 32 * WAVES;
+  constexpr int ROW = 2 * D, KS = D / 32, JT = D / 16, TB = kStep / 16;  // bytes of a token; products of a score, of O; 16s of tokens
+  constexpr int MINE = kStep / WAVES, GROUPS = MINE / 4, LOADS = MINE * ROW / 1024;  // tokens that a wave loads, fours of them, instructions
+  constexpr int BUF = kStep * ROW;                             // bytes of K or V of a step
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][BUF];  // buffer, K or V
+  __shared__ uint32_t gone_at[2][WAVES], odd_at[2][WAVES];     // fours of tokens whose page is not there; values left out
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  // neighbours on the line of work share keys and values: they go to the same chip (workgroups are dealt to the
+  // eight of them in turn)
+  const int w = uniform((int)(workers % 8 == 0 ? (blockIdx.x % 8) * (workers / 8) + blockIdx.x / 8 : blockIdx.x));
+  const int n_kv = a.c.n_kv, group = a.n_q / n_kv, ps = a.c.page_size;
+  const int cap = (int)min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0);
+  const int64_t row_bytes = (int64_t)n_kv * ROW;
+  const Lines L{ro, lens, a.rows, n_kv, group, a.window, COLS, cap, kPromptStart, false};
+  Line line(L, a.batch, w, workers, least);
+  if (w == 0 && wave == 0) *pc.n_items = line.items();
+
+  // places in LDS
+  const auto swizzle = [](int token) { return D == 64 ? (token >> 1) & 7 : token & 15; };
+  const LdsPtr lds0 = (LdsPtr)RSTR_LDS(&lds[0][0][0]);
+  LdsPtr k_at[KS], v_at[JT];
+#pragma unroll
+  for (int i = 0; i < KS; i++) k_at[i] = lds0 + col * ROW + (((4 * i + g) ^ swizzle(col)) << 4);
+#pragma unroll
+  for (int j = 0; j < JT; j++) {
+    const int token = 4 * g + (col >> 2);
+    v_at[j] = lds0 + BUF + token * ROW + (((2 * j + ((col & 3) >> 1)) ^ swizzle(token)) << 4) + (col & 1) * 8;
+  }
+  // the piece of a token that a lane's load asks for
+  const auto piece_of = [&](int n, int& token) {  // instruction n of the wave's
+    const int byte = n * 1024 + lane * 16;
+    token = byte / ROW;
+    return (((byte % ROW) >> 4) ^ swizzle(wave * MINE + token)) << 4;
+  };
+
+  while (line.next()) {
+    const Seq& s = line.s;
+    const int b = line.b, h = line.h, c0 = line.ct * COLS, p0 = s.len - s.m, held = L.held(s.len);
+    const bool begins = line.begins, ends = line.ends;
+    if (begins && threadIdx.x == 0) pc.begun[line.item] = Begun{b, h, line.ct, w, line.pieces};
+    const auto row_of = [&](int c) { return min(s.m - 1, c / group); };
+    const auto first_seen = [&](int row) { return a.window > 0 ? max(max(p0 + row + 1, 0) - a.window, 0) : 0; };
+    const auto end_seen = [&](int row) { return min(max(p0 + row + 1, 0), cap); };
+    const int rf = row_of(c0), rl = row_of(c0 + COLS - 1);
+    const int cw = c0 + wave * 32;
+    // a column's row and head; found anew where they are needed, as keeping them costs registers of the loop
+    struct Column {
+      int row, head;
+    };
+    const auto column = [&](int t) {
+      int cc = cw + t * 16 + col;
+      asm("" : "+v"(cc));
+      const int row = cc / group;
+      return Column{row, h * group + (cc - row * group)};
+    };
+    const bool any = cw < s.m * group;
+    const int wf = row_of(cw), wl = row_of(cw + 31);  // the wave's rows
+    const int t0 = max(s.lo + max(line.at - kPromptStart, 0), first_seen(rf) / kTile);
+    const int t1 = min(s.lo + max(line.at + line.n - kPromptStart, 0), (end_seen(rl) + kTile - 1) / kTile);
+    const int part_end = t1 * kTile;
+    const int g_lo = first_seen(rf), g_hi = min(end_seen(rl), part_end), g_lo_last = first_seen(rl), g_hi_first = min(end_seen(rf), part_end);
+    const int w_lo = first_seen(wf), w_hi = any ? min(end_seen(wl), part_end) : 0, w_lo_last = first_seen(wl), w_hi_first = min(end_seen(wf), part_end);
+
+    f4 acc[NT][JT];
+    float mref[NT], l[NT], kcol[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+      for (int j = 0; j < JT; j++) acc[t][j] = f4{0, 0, 0, 0};
+      mref[t] = -FLT_MAX;
+      l[t] = kcol[t] = 0.0f;
+    }
+    if (t0 < t1) {
+      const TablePtr rowp = (TablePtr)(table + (int64_t)b * a.pps);
+      const int n_pages = (int)(((int64_t)held + ps - 1) / ps);
+      const int step_e = kStep / ps, step_off = kStep - step_e * ps;
+      // page and place in it of the wave's fours of tokens, and the page's id, read a step ahead of its use
+      int pg[GROUPS], off[GROUPS], id[GROUPS], id_off[GROUPS];
+#pragma unroll
+      for (int n = 0; n < GROUPS; n++) {
+        const int tok = t0 * kTile + wave * MINE + 4 * n;
+        pg[n] = tok / ps;
+        off[n] = tok - pg[n] * ps;
+      }
+      const auto look = [&] {
+#pragma unroll
+        for (int n = 0; n < GROUPS; n++) {
+          const int v = rowp[min(pg[n], n_pages - 1)];
+          id[n] = pg[n] < n_pages ? v : -1;
+          id_off[n] = off[n];
+          pg[n] += step_e;
+          off[n] += step_off;
+          if (off[n] >= ps) off[n] -= ps, pg[n]++;
+        }
+      };
+      const uint8_t* kbase = (const uint8_t*)a.c.k + (int64_t)h * ROW;
+      const uint8_t* vbase = (const uint8_t*)a.c.v + (int64_t)h * ROW;
+      const auto issue = [&](int buf) {
+        int64_t at[GROUPS];
+        uint32_t gone = 0;
+#pragma unroll
+        for (int n = 0; n < GROUPS; n++) {
+          const bool ok = (uint32_t)id[n] < (uint32_t)a.c.pages;
+          if (!ok) gone |= 1u << n;
+          at[n] = ((int64_t)(ok ? id[n] : 0) * ps + id_off[n]) * row_bytes;
+        }
+        if (lane == 0) gone_at[buf][wave] = gone, odd_at[buf][wave] = 0;
+#pragma unroll
+        for (int n = 0; n < LOADS; n++) {
+          int token;
+          const int piece = piece_of(n, token);
+          int64_t from = at[0];
+#pragma unroll
+          for (int j = 1; j < GROUPS; j++) from = (D == 64 ? token >> 2 : n * 1024 / ROW / 4) == j ? at[j] : from;
+          const int64_t byte = from + (int64_t)(token & 3) * row_bytes + piece;
+#pragma unroll
+          for (int kv = 0; kv < 2; kv++)
+            __builtin_amdgcn_global_load_lds((const void*)((kv ? vbase : kbase) + byte), RSTR_LDS(&lds[buf][kv][wave * MINE * ROW + n * 1024]), 16, 0, 0);
+        }
+        look();
+      };
+      look();
+      issue(0);
+
+      h8 q[NT][TERMS][KS];
+      int hi[NT], lo[NT];
+      const bool vec = vec_rows(a.q, sizeof(T));
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const Column c = column(t);
+        const bool valid = c.row < s.m;
+        hi[t] = valid ? min(end_seen(c.row), part_end) : 0;
+        lo[t] = first_seen(c.row);
+        float x[KS][8], big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+          if (valid) {
+            const T* src = (const T*)a.q.p + (int64_t)(s.r0 + c.row) * a.q.row + (int64_t)c.head * a.q.head + i * 32 + g * 8;
+            if (vec) load8<E, true>(src, x[i]); else load8<E, false>(src, x[i]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[i][k] = 0.0f;
+          }
+#pragma unroll
+          for (int k = 0; k < 8; k++) big = fmaxf(big, fabsf(x[i][k]));
+        }
+        big = xor_max<32>(xor_max<16>(big));
+        const int e = __builtin_amdgcn_frexp_expf(big) - 15;
+        kcol[t] = score_scale(a.scale, e);
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            float y = __builtin_amdgcn_ldexpf(x[i][k], -e);
+            if (a.scale < 0.0f) y = -y;
+            if constexpr (TERMS == 2) {
+              q[t][0][i][k] = first_term(y);
+              q[t][1][i][k] = (_Float16)(y - (float)q[t][0][i][k]);
+            } else {
+              q[t][0][i][k] = (_Float16)y;
+            }
+          }
+      }
+
+      // A weight of 0 times an infinity or a NaN: of values whose token some column of the workgroup does not see, those that are no
+      // numbers become 0 where they were loaded; odd_at says that there were some of tokens that others see.
+      const auto partly = [&](int tok) { return tok >= g_lo && tok < g_hi && !(tok >= g_lo_last && tok < g_hi_first); };
+      const auto mend = [&](int buf, int tok0) {
+        uint32_t odd = 0;
+        const uint32_t gone = gone_at[buf][wave];
+#pragma unroll
+        for (int n = 0; n < LOADS; n++) {
+          const int token = (n * 1024 + lane * 16) / ROW, tok = tok0 + wave * MINE + token;
+          const bool there = !((gone >> (token >> 2)) & 1);
+          __attribute__((address_space(3))) u32x4* at = (__attribute__((address_space(3))) u32x4*)(lds0 + (buf * 2 + 1) * BUF + wave * MINE * ROW + n * 1024 + lane * 16);
+          u32x4 x = *at;
+          uint32_t bad = 0;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t halves = ((((x[i] & 0x7C007C00u) + 0x04000400u) >> 15) & 0x10001u) * 0xFFFFu;  // exponents of all ones
+            x[i] &= ~halves;
+            bad |= halves;
+          }
+          const bool all = there && tok >= g_lo_last && tok < g_hi_first;
+          if (bad != 0 && !all) {
+            *at = x;
+            if (there && partly(tok)) odd = 1;
+          }
+        }
+        if (__ballot(odd != 0) && lane == 0) odd_at[buf][wave] = 1;
+      };
+
+      // one step: tokens [tok0, tok0 + 64) from buffer `buf`; edge: some column does not see some of them
+      const auto compute = [&](bool edge, int buf, int tok0) {
+        const int base = buf * (2 * BUF);
+        f4 sc[NT][TB];
+#pragma unroll
+        for (int tb = 0; tb < TB; tb++) {
+#pragma unroll
+          for (int t = 0; t < NT; t++) sc[t][tb] = f4{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < KS; i++) {
+            const h8 k = __builtin_bit_cast(h8, *(__attribute__((address_space(3))) u32x4*)(k_at[i] + base + tb * 16 * ROW));
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int u = 0; u < TERMS; u++) sc[t][tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[t][u][i], sc[t][tb], 0, 0, 0);
+          }
+        }
+        if (edge) {
+          // bits of the lane's tokens (bit 4 tb + i is token 16 tb + 4 g + i of the step)
+          const auto below = [&](int end) {
+            uint32_t o = 0;
+#pragma unroll
+            for (int tb = 0; tb < TB; tb++) o |= ((1u << min(max(end - tok0 - 16 * tb - 4 * g, 0), 4)) - 1u) << (4 * tb);
+            return o;
+          };
+          uint32_t here = ~0u;
+#pragma unroll
+          for (int tb = 0; tb < TB; tb++) {
+            const int n = 16 * tb + 4 * g;
+            if ((gone_at[buf][n / MINE] >> (n % MINE / 4)) & 1) here &= ~(15u << (4 * tb));
+          }
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            const uint32_t see = below(hi[t]) & ~below(lo[t]) & here;
+#pragma unroll
+            for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) sc[t][tb][i] = (see >> (4 * tb + i)) & 1 ? sc[t][tb][i] : -INFINITY;
+          }
+        }
+        float m[NT];
+        bool passed[NT], grow = false;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          m[t] = -INFINITY;
+#pragma unroll
+          for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) m[t] = __builtin_elementwise_maximum(m[t], sc[t][tb][i]);  // (a NaN is in the column's sums anyhow)
+          passed[t] = __builtin_fmaf(m[t] - mref[t], kcol[t], 10.0f) > 14.0f;
+          grow |= passed[t];
+        }
+        if (__ballot(grow)) {
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            // a column that needs no change has none: it does not depend on its neighbours
+            const bool own = of_column(__ballot(passed[t]));
+            const float top = xor_max<32>(xor_max<16>(m[t])), now = own ? fmaxf(top, mref[t]) : mref[t];
+            const float keep = own ? __builtin_amdgcn_exp2f((mref[t] - now) * kcol[t]) : 1.0f;
+            mref[t] = now;
+            l[t] *= keep;
+#pragma unroll
+            for (int j = 0; j < JT; j++) acc[t][j] *= keep;
+          }
+        }
+        h8 ph[NT][TB / 2][TERMS];
+#pragma unroll
+        for (int u = 0; u < TB / 2; u++)
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][2 * u + (i >> 2)][i & 3] - mref[t], kcol[t], 10.0f));
+              if constexpr (TERMS == 2) {
+                ph[t][u][0][i] = first_term(p[i]);
+                ph[t][u][1][i] = (_Float16)(p[i] - (float)ph[t][u][0][i]);
+              } else {
+                ph[t][u][0][i] = (_Float16)p[i];
+              }
+            }
+            if constexpr (TERMS == 2) {
+              l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; i++) l[t] = __builtin_amdgcn_fdot2(h2{ph[t][u][0][2 * i], ph[t][u][0][2 * i + 1]}, h2{(_Float16)1.0f, (_Float16)1.0f}, l[t], false);
+            }
+          }
+#pragma unroll
+        for (int u = 0; u < TB / 2; u++)
+#pragma unroll
+          for (int j = 0; j < JT; j++) {
+            u32x4 o;
+#pragma unroll
+            for (int b2 = 0; b2 < 2; b2++) {
+              const u32x2 x = read_transposed(v_at[j] + base + (32 * u + 16 * b2) * ROW);
+              o[2 * b2] = x[0];
+              o[2 * b2 + 1] = x[1];
+            }
+            const h8 v = __builtin_bit_cast(h8, o);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int x = 0; x < TERMS; x++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t][u][x], acc[t][j], 0, 0, 0);
+          }
+        uint32_t odd = 0;
+        if (edge)
+#pragma unroll
+          for (int i = 0; i < WAVES; i++) odd |= odd_at[buf][i];
+        if (uniform(odd)) {  // values that mend() left out, for the columns that see them
+          const TablePtr pages = (TablePtr)(table + (int64_t)b * a.pps);
+#pragma unroll 1
+          for (int n = 0; n < kStep; n++) {
+            const int tok = tok0 + n;
+            if (!uniform(odd_at[buf][n / MINE]) || !partly(tok)) continue;
+            const int e = tok / ps, id = pages[e];
+            if ((uint32_t)id >= (uint32_t)a.c.pages) continue;
+            const uint16_t* v = a.c.v + (((int64_t)id * ps + (tok - e * ps)) * n_kv + h) * D + 4 * g;
+            const int reg = 4 * (n >> 4) + (n & 3);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              float mine = 0.0f;
+#pragma unroll
+              for (int k = 0; k < 4 * TB; k++) {
+                float p = (float)ph[t][k >> 3][0][k & 7];
+                if constexpr (TERMS == 2) p += (float)ph[t][k >> 3][1][k & 7];
+                mine = k == reg ? p : mine;
+              }
+              mine = __shfl(mine, ((n >> 2) & 3) * 16 + col, 64);
+              const bool sees = tok >= lo[t] && tok < hi[t];
+#pragma unroll
+              for (int j = 0; j < JT; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                  const uint16_t x = v[16 * j + i];
+                  if (sees && (x & 0x7C00u) == 0x7C00u) acc[t][j][i] = __builtin_fmaf(mine, (float)__builtin_bit_cast(_Float16, x), acc[t][j][i]);
+                }
+            }
+          }
+        }
+      };
+
+      int buf = 0;
+      for (int tok0 = t0 * kTile; tok0 < part_end; tok0 += kStep) {
+        wait_vmem();
+        if (tok0 < g_lo_last || tok0 + kStep > g_hi_first || uniform(gone_at[buf][wave]) != 0) mend(buf, tok0);
+        __syncthreads();  // this step's tokens are there, and the other buffer is free
+        if (tok0 + kStep < part_end) issue(buf ^ 1);
+        if (tok0 < w_hi && tok0 + kStep > w_lo) {
+          uint32_t gone = 0;
+#pragma unroll
+          for (int i = 0; i < WAVES; i++) gone |= gone_at[buf][i];
+          compute(tok0 < w_lo_last || tok0 + kStep > w_hi_first || uniform(gone) != 0, buf, tok0);
+        }
+        buf ^= 1;
+      }
+      __syncthreads();  // the buffers are the next part's
+    }
+
+    const int64_t piece = (begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w) * COLS;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const float sum = xor_add<32>(xor_add<16>(l[t]));
+      const Column at = column(t);
+      if (at.row >= s.m) continue;
+      if (begins && ends) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* dst = (T*)a.out.p + (int64_t)(s.r0 + at.row) * a.out.row + (int64_t)at.head * a.out.head + 4 * g;
+        const bool ovec = vec_rows(a.out, sizeof(T));
+#pragma unroll
+        for (int j = 0; j < JT; j++) {
+          T o[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[k] = E::put(acc[t][j][k] * inv);
+          if (ovec) {
+            if constexpr (sizeof(T) == 4) *(u32x4*)(dst + 16 * j) = *(u32x4*)o;
+            else *(u32x2*)(dst + 16 * j) = *(u32x2*)o;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) dst[16 * j + k] = o[k];
+          }
+        }
+      } else {
+        const int64_t c = piece + wave * 32 + t * 16 + col;
+        if (g == 0) pc.ml[c] = f4{mref[t], sum, kcol[t], 0.0f};
+        if (sum == 0.0f) continue;
+#pragma unroll
+        for (int j = 0; j < JT; j++) *(f4*)(pc.acc + c * D + 16 * j + 4 * g) = acc[t][j];
+      }
+    }
+  }
+}
+
 // Joins the pieces of an item, in their order: a workgroup an item and `per` columns (more for every gridDim.y),
 // its waves by column and by piece.
 template <int D, class E, bool LISTED>
@@ -585,6 +1008,8 @@ __global__ void k_pool_merge(PoolAttn a, Lines L, PoolPieces pc, int per, int pa
 constexpr int kMergeWaves = 4096;
 constexpr int kWhole = 4;  // tiles of an item that one wave does, without a merge
 constexpr int kLeast = 2;  // tiles a wave takes at least
+constexpr int kPromptLeast = 8;  // and a workgroup of k_pool_prompt
+constexpr int kManyColumns = 64;  // columns a sequence from which waves share tiles
 constexpr int kOneTile = 16;  // columns a sequence up to which items have one tile of columns, above it two
 
 int64_t most_workers(int hd, int nt) { return (int64_t)compute_units() * 4 * pool_waves(hd, nt); }
@@ -651,6 +1076,20 @@ hipError_t attn_tiles(hipStream_t st, const PoolAttn& a) {
 }
 
 template <int D, class E>
+hipError_t attn_prompt(hipStream_t st, const PoolAttn& a) {
+  constexpr int waves = prompt_waves(D, Terms<E>::n), cols = 32 * waves;
+  const int64_t cap = std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0), tiles = (cap + kTile - 1) / kTile;
+  const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
+  const int64_t most = compute_units(), want = (items * (tiles + kPromptStart) + kPromptLeast - 1) / kPromptLeast;
+  const int workers = (int)std::min(most, want);
+  const PoolPieces pc = pool_pieces(a.ws, items, 2 * workers, cols);
+  hipLaunchKernelGGL((k_pool_prompt<D, E>), dim3((unsigned)workers), dim3(64 * waves), 0, st, a, a.row_offsets, a.lengths, a.page_table, pc, workers,
+                     kPromptLeast);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : merge<D, E, false>(st, a, pc, items, workers, cols, 0);
+}
+
+template <int D, class E>
 hipError_t attn_listed(hipStream_t st, const PoolAttn& a) {
   const int64_t entries = std::min<int64_t>(a.top, a.pps), tiles = (entries * a.c.page_size + kTile - 1) / kTile;
   const Cut c = listed_cut(a.n_q, a.c.n_kv, D, a.rows, tiles);
@@ -662,9 +1101,15 @@ hipError_t attn_listed(hipStream_t st, const PoolAttn& a) {
   return e != hipSuccess || c.parts == 1 ? e : merge<D, E, true>(st, a, pc, c.items, c.items * c.parts, 16, c.parts);
 }
 
+bool many_columns(const PoolAttn& a) {
+  const int64_t group = a.n_q / a.c.n_kv;
+  return a.max_rows * group >= kManyColumns && a.rows * group >= (int64_t)kManyColumns * a.batch;
+}
+
 template <int D, class E>
 hipError_t attn_dim(hipStream_t st, const PoolAttn& a) {
   if (a.blocks) return attn_listed<D, E>(st, a);
+  if (many_columns(a)) return attn_prompt<D, E>(st, a);
   if constexpr (D != 256)
     if ((int64_t)a.max_rows * (a.n_q / a.c.n_kv) > kOneTile) return attn_tiles<D, 2, E>(st, a);
   return attn_tiles<D, 1, E>(st, a);
@@ -681,7 +1126,8 @@ hipError_t attn_type(hipStream_t st, const PoolAttn& a) {
 
 size_t pool_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows) {
   // a call has at most two pieces a worker, of 32 columns at most; a list's parts are no more than the workers
-  const int64_t columns = 2 * std::max(most_workers(hd, 1) * 16, most_workers(hd, 2) * 32) + 64;
+  const int64_t prompt = (int64_t)compute_units() * 32 * prompt_waves(hd, 1);
+  const int64_t columns = 2 * std::max(std::max(most_workers(hd, 1) * 16, most_workers(hd, 2) * 32), prompt) + 64;
   return 256 + align256(sizeof(Begun) * attn_items(n_q, n_kv, batch, rows, 16)) + align256(sizeof(f4) * columns) + sizeof(float) * columns * hd;
 }
 

@@ -18,7 +18,8 @@ the tokens it sees:
   twice), the sum with the constant: 5 * 2^-24 of no more than 2 S; in all e = S * ((32 + 2 D / 32) * 2^-23 + 1.25 * 2^-21 + D * 2^-39 + 10 * 2^-24).
   A weight is off by e, their sum too: 2 e W;
 - the exponential: 2^-22 of the weight, twice: 2^-21 W;
-- f16 and bf16: a weight is rounded to fp16: 2^-11 W; weights below fp16's normal numbers are off by half a
+- f16 and bf16: a weight is rounded to fp16: 2^-11 W, and where many rows share tiles the weights' sum is that of the rounded ones: off by
+  2^-11 of itself at most, so the quotient by as much again, 2^-10 W in all; weights below fp16's normal numbers are off by half a
   step there, 2^-25, where the largest weight is at least 2^6 (the reference lags by 2^4 at most: 2^10 / 2^4): N * 2^-31 * max|v|.
   fp32: two terms as above, 1.25 * 2^-21 W, and N * 2^-31 * 2^-11 max|v|;
 - the sums over tokens: 32 terms and N / 32 products, and up to 64 pieces: (32 + N / 32 + 64) * 2^-23 W, the sum of the weights likewise;
@@ -221,10 +222,10 @@ def test_rope_append_numbers_at_the_ends(sess):
 
 
 # ---- attention ---------------------------------------------------------------------------
-def _attn_tol(dtype, D, out, mag, size, seen, vmax):
+def _attn_tol(dtype, D, out, mag, size, seen, vmax, prompt=False):
     wide = dtype == torch.float32
     e = size * ((32 + 2 * D / 32) * 2.0 ** -23 + 1.25 * 2.0 ** -21 + D * 2.0 ** -39 + 10 * 2.0 ** -24)
-    rel = 2 * e + 2.0 ** -21 + (1.25 * 2.0 ** -21 if wide else 2.0 ** -11) + 2 * (96 + seen / 32) * 2.0 ** -23 + 2.0 ** -23
+    rel = 2 * e + 2.0 ** -21 + (1.25 * 2.0 ** -21 if wide else 2.0 ** -10 if prompt else 2.0 ** -11) + 2 * (96 + seen / 32) * 2.0 ** -23 + 2.0 ** -23
     lost = seen * 2.0 ** -31 * vmax * (2.0 ** -11 if wide else 1.0)
     return 1.01 * (np.nan_to_num(mag, nan=0.0, posinf=0.0) * np.nan_to_num(rel, nan=0.0, posinf=0.0) + lost) + 1.01 * _own(dtype, np.nan_to_num(out, nan=0.0, posinf=0.0, neginf=0.0))
 
@@ -278,7 +279,7 @@ def test_attention(sess, n_q, n_kv, D, page, dtype, window, form):
         _attend(x, q.cuda(), table, lengths, offsets, out, n_q, max_rows=max(news), window=window, scale=scale)
         want, mag, size, seen, mine = P.attention(P.as_f64(q), P.as_f64(k), P.as_f64(v), table, lengths, offsets, window, scale)
         assert bool((out[rows:] == 5.0).all())  # rows of no sequence
-        tol = _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()))
+        tol = _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=True)
         _near(out[:rows], want[:rows], tol[:rows])
         again = torch.full_like(out, 5.0)  # max_rows chooses the tile only
         _attend(x, q.cuda(), table, lengths, offsets, again, n_q, window=window, scale=scale)
@@ -303,7 +304,7 @@ def test_attention_long(sess, dtype, lengths, news, width_extra):
         _attend(x, q.cuda(), table, lengths, offsets, out, n_q, max_rows=max(news))
         sel = np.unique(np.concatenate([np.arange(min(rows, 3)), rng.integers(0, rows, 12), [rows - 1]]))  # the plain form of some rows
         want, mag, size, seen, _ = _some_rows(P.as_f64(q), k, v, table, lengths, offsets, sel, D ** -0.5)
-        _near(out.cpu()[sel], want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max())))
+        _near(out.cpu()[sel], want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=max(news) > 1))
 
 
 def _some_rows(q, k, v, table, lengths, offsets, sel, scale, **kw):
@@ -368,7 +369,7 @@ def test_attention_what_is_not_seen(sess, dtype, D):
                 _attend(x, q.cuda(), table, lengths, offsets, out, n_q, max_rows=most, window=window)
                 want, mag, size, seen, _ = P.attention(P.as_f64(q), P.as_f64(k), P.as_f64(v), table, lengths, offsets, window, D ** -0.5)
                 vmax = float(v[v.isfinite()].abs().max())
-                _near(out, want, _attn_tol(dt, D, want, mag, size, seen, vmax))
+                _near(out, want, _attn_tol(dt, D, want, mag, size, seen, vmax, prompt=most > 1))
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
@@ -716,7 +717,7 @@ def test_steps_of_a_server(sess, dtype, stream):
             assert np.array_equal(blocks.cpu().numpy(), P.select(q, lim, t, n, o, page, top, 1, 1))
             for out, lst in ((dense, None), (sparse, blocks.tolist())):
                 want, mag, size, seen, _ = P.attention(q, k, v, t, n, o, 0, D ** -0.5, lst)
-                _near(out, want, _attn_tol(dt, D, want, mag, size, seen, vmax))
+                _near(out, want, _attn_tol(dt, D, want, mag, size, seen, vmax, prompt=lst is None and max(counts) > 1))
 
 
 def test_a_captured_step(sess):
