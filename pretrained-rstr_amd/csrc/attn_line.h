@@ -204,28 +204,30 @@ __device__ __forceinline__ bool of_column(uint64_t lanes) {
 // The sequence that a row belongs to, found by all lanes of a wave together: offsets are read 64 at a time.
 // Where they decrease anywhere no row belongs to one.
 struct RowOf {
-  int b, p;  // -1: none; the row's position (negative: it sees nothing)
+  int b, p;   // -1: none; the row's position (negative: it sees nothing)
   int first;  // the sequence's first row
   __device__ __forceinline__ RowOf(const int32_t* ro, const int32_t* lens, int batch, int rows, int row) {
-    int n = 0;
+    const int lane = threadIdx.x & 63;
     bool ordered = true;
-    for (int i0 = 0; i0 < batch; i0 += 64) {
-      const int i = i0 + (int)(threadIdx.x & 63);
-      const int at = ro[min(i, batch)], next = ro[min(i + 1, batch)];
-      n += __popcll(__ballot(i < batch && at <= row));
+    int begin = 0, end = 0, len = 0;
+    b = -1;
+    for (int i0 = 0; i0 < batch; i0 += 64) {  // all that is needed of a sequence in one wait
+      const int i = i0 + lane;
+      const int at = ro[min(i, batch)], next = ro[min(i + 1, batch)], n = lens[min(i, batch - 1)];
+      const uint64_t below = __ballot(i < batch && at <= row);
       ordered = ordered && at <= next;
+      if (below) {
+        const int f = 63 - __clzll((long long)below);
+        b = i0 + f;
+        begin = __builtin_amdgcn_readlane(at, f);
+        end = __builtin_amdgcn_readlane(next, f);
+        len = __builtin_amdgcn_readlane(n, f);
+      }
     }
-    b = n - 1;
-    p = first = 0;
-    if (__ballot(!ordered)) b = -1;
-    if (b < 0) return;
-    const int end = min(ro[b + 1], rows);
-    if (row >= end) {
-      b = -1;
-      return;
-    }
-    first = max(ro[b], 0);
-    p = max(lens[b], 0) - (end - row);
+    end = min(end, rows);
+    if (__ballot(!ordered) || row >= end) b = -1;
+    first = max(begin, 0);
+    p = max(len, 0) - (end - row);
   }
 };
 

@@ -94,16 +94,20 @@ __device__ __forceinline__ V load_page(const void* p) {
   else return *(const V*)p;
 }
 
-template <int D, int NT, class E, bool LISTED>
-__global__ void __launch_bounds__(256, pool_waves(D, NT))
+// LW > 0: a list of blocks; LW waves of a workgroup share a row's list and join their parts in LDS.
+constexpr int listed_threads(int lw) { return lw > 1 ? 64 * lw : 256; }
+template <int D, int NT, class E, int LW>
+__global__ void __launch_bounds__(listed_threads(LW), pool_waves(D, NT))
     k_pool_attn(PoolAttn a, const int32_t* __restrict__ ro, const int32_t* __restrict__ lens, const int32_t* __restrict__ table,
                 PoolPieces pc, int workers, int least, bool whole, int parts) {
   typedef Dims<D> G;
   typedef typename E::T T;
   constexpr int KS = G::KS, JT = G::JT, VW = G::VW, COLS = 16 * NT, TERMS = Terms<E>::n;
-  constexpr bool STREAM = NT == 1 && !LISTED;
+  constexpr bool LISTED = LW > 0, STREAM = NT == 1 && !LISTED;
+  __shared__ f4 join_ml[LW > 1 ? LW : 1][LW > 1 ? COLS : 1];
+  __shared__ __attribute__((aligned(16))) float join_acc[LW > 1 ? LW : 1][LW > 1 ? COLS : 1][LW > 1 ? D : 4];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int w = uniform(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int wave = uniform(threadIdx.x >> 6), w = uniform(blockIdx.x * (LW > 1 ? LW : 4) + wave);
   const int n_kv = a.c.n_kv, group = a.n_q / n_kv, ps = a.c.page_size;
   const int cap = (int)min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0);
   const int64_t row_bytes = (int64_t)n_kv * D * 2;
@@ -426,6 +430,57 @@ __global__ void __launch_bounds__(256, pool_waves(D, NT))
       }
     }
 
+    if constexpr (LW > 1) {
+      const float sum = xor_add<32>(xor_add<16>(l[0]));
+      if (g == 0) join_ml[wave][col] = f4{mref[0], sum, kcol[0], 0.0f};
+      if (valid[0] && sum != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < JT; j += 4)
+            *(f4*)&join_acc[wave][col][G::dim(j, 4 * g + i)] = f4{acc[0][j][i], acc[0][j + 1][i], acc[0][j + 2][i], acc[0][j + 3][i]};
+      }
+      __syncthreads();
+      const int columns = min(COLS, group - s.c0);
+      for (int at = threadIdx.x; at < columns * (D / 4); at += 64 * LW) {
+        const int c = at / (D / 4), d = at % (D / 4) * 4;
+        float top = -FLT_MAX, all = 0.0f, k = FLT_MIN;
+        f4 ml[LW], o = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < LW; i++) {
+          ml[i] = join_ml[i][c];
+          if (ml[i][1] != 0.0f) top = fmaxf(top, ml[i][0]), k = ml[i][2];
+        }
+#pragma unroll
+        for (int i = 0; i < LW; i++) {
+          if (ml[i][1] == 0.0f) continue;
+          const float f = __builtin_amdgcn_exp2f((ml[i][0] - top) * ml[i][2]);
+          const f4 x = *(const f4*)&join_acc[i][c][d];
+          all = __builtin_fmaf(f, ml[i][1], all);
+#pragma unroll
+          for (int j = 0; j < 4; j++) o[j] = __builtin_fmaf(f, x[j], o[j]);
+        }
+        if (s.whole) {
+          const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+          T* to = (T*)a.out.p + (int64_t)s.r0 * a.out.row + ((int64_t)s.h * group + s.c0 + c) * a.out.head + d;
+          T y[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) y[j] = E::put(o[j] * inv);
+          if (vec_rows(a.out, sizeof(T))) {
+            if constexpr (sizeof(T) == 4) *(u32x4*)to = *(u32x4*)y;
+            else *(u32x2*)to = *(u32x2*)y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) to[j] = y[j];
+          }
+        } else {
+          const int64_t p = s.piece * COLS + c;
+          if (d == 0) pc.ml[p] = f4{top, all, k, 0.0f};
+          *(f4*)(pc.acc + p * D + d) = o;
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const float sum = xor_add<32>(xor_add<16>(l[t]));
@@ -464,7 +519,8 @@ __global__ void __launch_bounds__(256, pool_waves(D, NT))
 
   if constexpr (LISTED) {
     const int ncts = (group + COLS - 1) / COLS;
-    const int item = w / parts, part = w - item * parts;
+    // a wave of its own, or a workgroup: its item and part of it
+    const int unit = LW > 1 ? (int)blockIdx.x : w, item = unit / parts, part = unit - item * parts;
     const int row = item / (n_kv * ncts), rest = item - row * (n_kv * ncts);
     if (row >= a.rows) return;
     const RowOf of(ro, lens, a.batch, a.rows, row);
@@ -479,10 +535,10 @@ __global__ void __launch_bounds__(256, pool_waves(D, NT))
     s.list = a.blocks + ((int64_t)row * n_kv + s.h) * a.top;
     s.entries = of.p < 0 ? 0 : min(min(a.top, a.pps), of.p / ps + 1);
     const int tiles = (int)(((int64_t)s.entries * ps + kTile - 1) / kTile);
-    s.t0 = part * least;
+    s.t0 = (LW > 1 ? part * LW + wave : part) * least;
     s.t1 = min(s.t0 + least, tiles);
     s.whole = whole;
-    s.piece = w;
+    s.piece = unit;
     work(s);
   } else {
     const Lines L{ro, lens, a.rows, n_kv, group, a.window, COLS, cap, kStart, whole};
@@ -743,6 +799,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(D, Terms<E>::n), prompt_wave
           }
         }
         if (edge) {
+          asm volatile("");  // stays a branch
           // bits of the lane's tokens (bit 4 tb + i is token 16 tb + 4 g + i of the step)
           const auto below = [&](int end) {
             uint32_t o = 0;
@@ -812,6 +869,8 @@ __global__ void __launch_bounds__(64 * prompt_waves(D, Terms<E>::n), prompt_wave
 #pragma unroll
               for (int i = 0; i < 4; i++) l[t] = __builtin_amdgcn_fdot2(h2{ph[t][u][0][2 * i], ph[t][u][0][2 * i + 1]}, h2{(_Float16)1.0f, (_Float16)1.0f}, l[t], false);
             }
+#pragma unroll
+            for (int x = 0; x < TERMS; x++) asm("" : "+v"(ph[t][u][x]));  // packed from here on, also for what hardly ever needs them singly
           }
 #pragma unroll
         for (int u = 0; u < TB / 2; u++)
@@ -1027,20 +1086,24 @@ PoolPieces pool_pieces(void* ws, int64_t items, int64_t pieces, int cols) {
   return pc;
 }
 
-// Parts that each item of a list of blocks is cut into, and the tiles of a part.
+// How the items of lists of blocks are shared out: waves an item, workgroups an item, tiles a wave.
 struct Cut {
   int64_t items;
-  int parts, tiles;
+  int waves, parts, tiles;
 };
+constexpr int listed_waves(int hd) { return hd == 256 ? 4 : 8; }
+// A wave an item where these fill the card, and where a list is short; else a workgroup an item, and where a wave would have more than
+// kListedTiles tiles several.
+constexpr int kListedTiles = 16;
 Cut listed_cut(int n_q, int n_kv, int hd, int rows, int64_t tiles) {
   const int group = n_q / n_kv, ncts = (group + 15) / 16;
-  Cut c;
-  c.items = (int64_t)rows * n_kv * ncts;
-  int64_t parts = most_workers(hd, 1) / c.items;
-  parts = std::min(parts, (tiles + kLeast - 1) / kLeast);
-  if (tiles <= kWhole || parts < 1) parts = 1;
-  c.tiles = (int)((tiles + parts - 1) / parts);
-  c.parts = (int)((tiles + c.tiles - 1) / c.tiles);
+  Cut c{(int64_t)rows * n_kv * ncts, 1, 1, (int)tiles};
+  if (tiles <= kLeast || c.items >= most_workers(hd, 1)) return c;
+  c.waves = listed_waves(hd);
+  const int64_t room = std::max<int64_t>(1, most_workers(hd, 1) / (c.items * c.waves));
+  const int64_t parts = std::min(room, (tiles + (int64_t)c.waves * kListedTiles - 1) / (c.waves * kListedTiles));
+  c.tiles = (int)((tiles + parts * c.waves - 1) / (parts * c.waves));
+  c.parts = (int)((tiles + (int64_t)c.tiles * c.waves - 1) / ((int64_t)c.tiles * c.waves));
   return c;
 }
 
@@ -1069,7 +1132,7 @@ hipError_t attn_tiles(hipStream_t st, const PoolAttn& a) {
   const int64_t most = most_workers(D, NT), want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
   const int64_t workers = whole ? (items + 3) / 4 * 4 : (std::min(most, want) + 3) / 4 * 4;
   const PoolPieces pc = pool_pieces(a.ws, items, 2 * workers, cols);
-  hipLaunchKernelGGL((k_pool_attn<D, NT, E, false>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths, a.page_table,
+  hipLaunchKernelGGL((k_pool_attn<D, NT, E, 0>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths, a.page_table,
                      pc, (int)workers, whole ? 1 : kLeast, whole, 0);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess || whole ? e : merge<D, E, false>(st, a, pc, items, workers, cols, 0);
@@ -1093,10 +1156,11 @@ template <int D, class E>
 hipError_t attn_listed(hipStream_t st, const PoolAttn& a) {
   const int64_t entries = std::min<int64_t>(a.top, a.pps), tiles = (entries * a.c.page_size + kTile - 1) / kTile;
   const Cut c = listed_cut(a.n_q, a.c.n_kv, D, a.rows, tiles);
-  const int64_t workers = (c.items * c.parts + 3) / 4 * 4;
-  const PoolPieces pc = pool_pieces(a.ws, 0, workers, 16);
-  hipLaunchKernelGGL((k_pool_attn<D, 1, E, true>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths, a.page_table,
-                     pc, (int)workers, c.tiles, c.parts == 1, c.parts);
+  const int64_t groups = c.waves > 1 ? c.items * c.parts : (c.items + 3) / 4;
+  const PoolPieces pc = pool_pieces(a.ws, 0, c.items * c.parts, 16);
+  auto f = c.waves > 1 ? k_pool_attn<D, 1, E, listed_waves(D)> : k_pool_attn<D, 1, E, 1>;
+  hipLaunchKernelGGL(f, dim3((unsigned)groups), dim3(64 * (c.waves > 1 ? c.waves : 4)), 0, st, a, a.row_offsets, a.lengths, a.page_table,
+                     pc, (int)groups, c.tiles, c.parts == 1, c.parts);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess || c.parts == 1 ? e : merge<D, E, true>(st, a, pc, c.items, c.items * c.parts, 16, c.parts);
 }

@@ -79,7 +79,7 @@ struct BlockSelect {
   void* ws;
   int ws_blocks;  // blocks a row and kv head that the workspace has room for
 };
-constexpr int kScoreBlocks = 64;  // blocks that a wave scores
+constexpr int kScoreBlocks = 32;  // blocks that a wave scores
 inline bool select_fits(int n_kv, int rows, int blocks) {  // grids hold it
   return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * ((blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26);
 }

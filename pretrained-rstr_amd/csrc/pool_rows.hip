@@ -201,18 +201,10 @@ __global__ void __launch_bounds__(256) k_bounds_update(BoundsUpdate a) {
 }
 
 // ---- selection of blocks -----------------------------------------------------------------
-// A row's score of a block is the most that a product of one of the group's queries with a key of the block could
+// A row's score of a block is the most that a product of one of the group's queries with a key inside the block's bounds can
 // be: s_j = max over the heads g of sum_d max(q_gd lo_jd, q_gd hi_jd).  Sums are in 64 bits, where products of fp16 with
 // fp16 or bf16 lose nothing: which of two blocks is taken is part of the result.
-// 1. k_block_scores: the scores, as integers of the same order (a NaN counts as +infinity).
-// 2. k_block_pick: the border, found by eight bits of it at a time, and the list in ascending order.
-
-__device__ __forceinline__ uint64_t order_of(double s) {
-  if (s != s) s = INFINITY;
-  s += 0.0;  // -0 is 0
-  const uint64_t u = __builtin_bit_cast(uint64_t, s);
-  return u >> 63 ? ~u : u | 1ull << 63;
-}
+// 1. k_block_scores: twice the scores.  2. k_block_pick: the border between what is taken and what is not, and the list in ascending order.
 
 // The blocks that a row's list is chosen from: those from `first` on up to, not with, the last ones.
 struct Choice {
@@ -224,55 +216,339 @@ struct Choice {
   }
 };
 
+// Sum over aligned groups of N lanes (8, 16 or 32) of HG values at once: a lane ends with the sum of value lane % HG
+// (the first steps halve the values that a lane holds instead of adding all of them).
+template <int N, int HG>
+__device__ __forceinline__ double scatter_sum(double (&v)[HG]) {
+  const int lane = threadIdx.x & 63;
+  double x = v[0];
+  if constexpr (HG == 4) {
+    const bool odd = lane & 1;
+    double keep[2], give[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      keep[i] = odd ? v[2 * i + 1] : v[2 * i];
+      give[i] = odd ? v[2 * i] : v[2 * i + 1];
+      keep[i] += dpp_f64<0xB1>(give[i]);
+    }
+    const bool high = lane & 2;
+    x = (high ? keep[1] : keep[0]) + dpp_f64<0x4E>(high ? keep[0] : keep[1]);
+  } else if constexpr (HG == 2) {
+    const bool odd = lane & 1;
+    x = (odd ? v[1] : v[0]) + dpp_f64<0xB1>(odd ? v[0] : v[1]);
+    x += dpp_f64<0x4E>(x);
+  } else {
+    x += dpp_f64<0xB1>(x);
+    x += dpp_f64<0x4E>(x);
+  }
+  // within rows of 16 lanes, the lanes of one residue modulo 4 (rotations keep it)
+  if constexpr (N == 8) {
+    x += __shfl_xor(x, 4, 64);
+  } else {
+    x += dpp_f64<0x124>(x);
+    x += dpp_f64<0x128>(x);
+    if constexpr (N == 32) x += __shfl_xor(x, 16, 64);
+  }
+  return x;
+}
+
+// By the definition: where something is not finite.
 template <int D, class E>
-__global__ void __launch_bounds__(256) k_block_scores(BlockSelect a, uint64_t* __restrict__ keys, int chunks) {
+__device__ __attribute__((noinline)) double odd_score(const typename E::T* q, int64_t head, int group, const _Float16* bound) {
+  double best = -INFINITY;
+  for (int g = 0; g < group; g++) {
+    double s = 0.0;
+    for (int d = 0; d < D; d++) {
+      const double x = (double)E::get(q[g * head + d]) * (double)(float)bound[d], y = (double)E::get(q[g * head + d]) * (double)(float)bound[D + d];
+      s += x > y || x != x ? x : y;
+    }
+    if (s != s) return INFINITY;
+    best = s > best ? s : best;
+  }
+  return 2.0 * best;
+}
+
+// A wave scores kScoreBlocks blocks for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers twice the
+// larger of q lo and q hi is q (lo + hi) + |q| |hi - lo|, so a bound is converted once for all heads, and a product costs two
+// multiply-adds; where a sum is not finite the block is scored by the definition.
+template <int D, int HG, class E>
+__global__ void __launch_bounds__(256) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks) {
   typedef typename E::T T;
-  constexpr int CH = D / 8, PER = 64 / CH;  // lanes of a block, blocks at a time
+  constexpr int CH = D / 8, PER = 64 / CH, STEPS = kScoreBlocks / PER, AHEAD = 4;
   const int lane = threadIdx.x & 63, c = lane % CH;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int chunk = uniform((int)(unit % chunks));
   const int64_t rh = unit / chunks;
-  const int row = uniform((int)(rh / a.n_kv)), h = uniform((int)(rh % a.n_kv));
+  const int chunk = uniform((int)(unit - rh * chunks));
+  const int row = uniform((int)(rh / a.n_kv)), h = uniform((int)(rh - (int64_t)row * a.n_kv));
   if (row >= a.rows) return;
+  const int group = a.n_q / a.n_kv;
+  const T* q0 = (const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)h * group * a.q.head;
+  const bool vec = vec_rows(a.q, sizeof(T));
+  float qf[HG][8];
+  const auto queries = [&](int g0) {  // behind the last head: that head again
+#pragma unroll
+    for (int i = 0; i < HG; i++) {
+      const T* p = q0 + (int64_t)min(g0 + i, group - 1) * a.q.head + 8 * c;
+      if (vec) load8<E, true>(p, qf[i]); else load8<E, false>(p, qf[i]);
+    }
+  };
+  queries(0);
   const RowOf of(a.row_offsets, a.lengths, a.batch, a.rows, row);
   if (of.b < 0 || of.p < 0) return;
   const Choice ch(a, of.p);
-  const int group = a.n_q / a.n_kv;
-  const int j0 = chunk * kScoreBlocks, j1 = min(j0 + kScoreBlocks, ch.n);
-  uint64_t* out = keys + rh * a.ws_blocks;
-  for (int j = j0 + lane / CH; j - lane / CH < j1; j += PER) {
-    const int jj = min(j, j1 - 1);
-    const int page = a.page_table[(int64_t)of.b * a.pps + ch.lo + jj];
-    const bool there = (uint32_t)page < (uint32_t)a.pages;
-    const _Float16* src = (const _Float16*)a.bounds + ((int64_t)(there ? page : 0) * a.n_kv + h) * 2 * D + 8 * c;
-    float lo[8], hi[8];
-    load8<F16, true>(src, lo);
-    load8<F16, true>(src + D, hi);
-    double best = -INFINITY;
-    bool nan = false;
-    for (int g = 0; g < group; g++) {
-      float q[8];
-      load8<E, false>((const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)(h * group + g) * a.q.head + 8 * c, q);
-      double s = 0.0;
+  const int j0 = chunk * kScoreBlocks, n = min(kScoreBlocks, ch.n - j0);
+  if (n <= 0) return;
+  double* out = scores + rh * a.ws_blocks + j0;
+  const int page = lane < n ? a.page_table[(int64_t)of.b * a.pps + ch.lo + j0 + lane] : -1;
+  const int64_t head = (int64_t)2 * D;
+  const _Float16* base = (const _Float16*)a.bounds + h * head + 8 * c;
+  const auto bound_of = [&](int step, int& id) {
+    id = __shfl(page, step * PER + lane / CH, 64);
+    if ((uint32_t)id >= (uint32_t)a.pages) id = -1;
+    return base + (int64_t)max(id, 0) * a.n_kv * head;
+  };
+  for (int g0 = 0; g0 < group; g0 += HG) {
+    if (g0) queries(g0);
+    double q[HG][8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const double x = (double)q[i] * (double)lo[i], y = (double)q[i] * (double)hi[i];
-        s += x > y || x != x ? x : y;
+    for (int i = 0; i < HG; i++)
+#pragma unroll
+      for (int k = 0; k < 8; k++) q[i][k] = (double)qf[i][k];
+#pragma unroll 1
+    for (int s0 = 0; s0 * PER < n; s0 += AHEAD) {
+      u32x4 lo[AHEAD], hi[AHEAD];
+      int id[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) {
+        const _Float16* p = bound_of(min(s0 + i, STEPS - 1), id[i]);
+        lo[i] = *(const u32x4*)p;
+        hi[i] = *(const u32x4*)(p + D);
       }
 #pragma unroll
-      for (int d = 1; d < CH; d <<= 1) s += __shfl_xor(s, d, 64);
-      nan = nan || s != s;
-      best = s > best ? s : best;
+      for (int i = 0; i < AHEAD; i++) {
+        double s[HG];
+#pragma unroll
+        for (int g = 0; g < HG; g++) s[g] = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const uint32_t wl = lo[i][k >> 1], wh = hi[i][k >> 1];
+          const double x = (double)(float)__builtin_bit_cast(h2, wl)[k & 1], y = (double)(float)__builtin_bit_cast(h2, wh)[k & 1];
+          const double sum = y + x, wide = __builtin_fabs(y - x);
+#pragma unroll
+          for (int g = 0; g < HG; g++) s[g] = __builtin_fma(__builtin_fabs(q[g][k]), wide, __builtin_fma(q[g][k], sum, s[g]));
+        }
+        double x = scatter_sum<CH, HG>(s);
+        bool odd = !(__builtin_fabs(x) < INFINITY);
+        if constexpr (HG >= 2) {
+          const double o = dpp_f64<0xB1>(x);
+          odd = odd || !(__builtin_fabs(o) < INFINITY);
+          x = o > x ? o : x;
+        }
+        if constexpr (HG == 4) {
+          const double o = dpp_f64<0x4E>(x);
+          x = o > x ? o : x;
+          odd = odd || __builtin_amdgcn_update_dpp(0, (int)odd, 0x4E, 0xF, 0xF, true);
+        }
+        const int j = (s0 + i) * PER + lane / CH;
+        if (c == 0 && s0 + i < STEPS && j < n) {
+          if (g0) x = out[j] > x ? out[j] : x;  // (an odd block's score is the same in all rounds)
+          if (odd) x = odd_score<D, E>(q0, a.q.head, group, base + (int64_t)max(id[i], 0) * a.n_kv * head);
+          out[j] = id[i] < 0 ? -INFINITY : x;
+        }
+      }
     }
-    if (c == 0 && j < j1) out[j] = order_of(there ? (nan ? INFINITY : best) : -INFINITY);
   }
 }
 
-// The list of one row and kv head.
+// ---- the list of one row and kv head ----
+// Inclusive sum over the workgroup's threads; `tmp` holds one value a wave.
 template <int THREADS>
-__global__ void __launch_bounds__(THREADS) k_block_pick(BlockSelect a, const uint64_t* __restrict__ keys) {
-  __shared__ int hist[256], wsum[THREADS / 64], chosen[2];
+__device__ __forceinline__ int block_sum(int v, int* tmp, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int in = (int)wave_scan_i64(v);
+  __syncthreads();
+  if (lane == 63) tmp[wave] = in;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; w++) {
+    const int x = tmp[w];
+    if (w < wave) in += x;
+    total += x;
+  }
+  return in;
+}
+__device__ __forceinline__ uint64_t order_of(double s) {  // integers of the same order
+  const uint64_t u = __builtin_bit_cast(uint64_t, s + 0.0);  // -0 is 0
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+constexpr int kBuckets = 2048, kFew = 256;
+
+// The n candidates lie in registers, KPT neighbours a thread.  Their scores' range is cut into equal buckets, and what is in the
+// bucket that the border falls into is ranked by counting; where that is too much (many alike, or a few far from the rest) the border is found by
+// eight bits of the scores' integers at a time.
+template <int THREADS, int KPT>
+__global__ void __launch_bounds__(THREADS) k_block_pick(BlockSelect a, const double* __restrict__ scores) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ int hist[kBuckets], tmp[WAVES], chosen[2], few_n;
+  __shared__ double ends[2][WAVES];
+  __shared__ uint64_t few[kFew];
+  __shared__ int few_at[kFew];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t rh = blockIdx.x;
+  const int row = (int)(rh / a.n_kv);
+  // scores, asked for before the row's candidates are known (in the workspace wherever they end)
+  const double* from = scores + rh * a.ws_blocks;
+  double s[KPT];
+#pragma unroll
+  for (int i = 0; i < KPT; i++) s[i] = a.pps > a.top ? from[min(tid * KPT + i, a.ws_blocks - 1)] : 0.0;
+  const RowOf of(a.row_offsets, a.lengths, a.batch, a.rows, row);
+  if (of.b < 0) return;
+  int32_t* out = a.blocks + rh * a.top;
+  const Choice ch(a, of.p);
+  if (of.p < 0 || ch.n == 0) {
+    for (int i = tid; i < a.top; i += THREADS) out[i] = of.p >= 0 && i <= ch.cur ? i : -1;
+    return;
+  }
+  const int take = a.top - a.first - a.last;  // of the candidates
+  for (int i = tid; i < a.first; i += THREADS) out[i] = i;
+  for (int i = tid; i < a.last; i += THREADS) out[a.top - a.last + i] = ch.cur + 1 - a.last + i;
+  if (take == 0) return;
+  // the range of the finite ones
+  double lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < KPT; i++) {
+    const bool fin = tid * KPT + i < ch.n && __builtin_fabs(s[i]) < INFINITY;
+    lo = fin && s[i] < lo ? s[i] : lo;
+    hi = fin && s[i] > hi ? s[i] : hi;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    lo = __builtin_fmin(lo, __shfl_xor(lo, d, 64));
+    hi = __builtin_fmax(hi, __shfl_xor(hi, d, 64));
+  }
+  if (lane == 0) ends[0][wave] = lo, ends[1][wave] = hi;
+  for (int i = tid; i < kBuckets; i += THREADS) hist[i] = 0;
+  if (tid == 0) few_n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) {
+    lo = __builtin_fmin(lo, ends[0][w]);
+    hi = __builtin_fmax(hi, ends[1][w]);
+  }
+  // a bucket's number does not decrease with the score
+  const double per = (double)(kBuckets - 2) / (hi - lo);  // (all alike: infinite or none, and one bucket)
+  const auto bucket = [&](double x) {
+    if (x == INFINITY) return kBuckets - 1;
+    if (x == -INFINITY) return 0;
+    const double at = (x - lo) * per;
+    return at >= 0.0 ? (at < (double)(kBuckets - 3) ? 1 + (int)at : kBuckets - 2) : 1;
+  };
+  int in[KPT];
+#pragma unroll
+  for (int i = 0; i < KPT; i++) {
+    in[i] = tid * KPT + i < ch.n ? bucket(s[i]) : -1;
+    if (in[i] >= 0) atomicAdd(&hist[in[i]], 1);
+  }
+  __syncthreads();
+  // from the highest bucket down: where the count reaches `take`
+  constexpr int BPT = kBuckets / THREADS;
+  int mine[BPT], sum = 0, total;
+#pragma unroll
+  for (int i = 0; i < BPT; i++) sum += mine[i] = hist[kBuckets - 1 - tid * BPT - i];
+  int run = block_sum<THREADS>(sum, tmp, total) - sum;
+#pragma unroll
+  for (int i = 0; i < BPT; i++) {
+    if (run < take && run + mine[i] >= take) {
+      chosen[0] = kBuckets - 1 - tid * BPT - i;
+      chosen[1] = take - run;
+    }
+    run += mine[i];
+  }
+  __syncthreads();
+  const int border_bucket = chosen[0], left = chosen[1], inside = hist[border_bucket];
+  // of the border's bucket: keys above `border` are taken, and of those equal to it the first `equal`
+  uint64_t border = 0;
+  int equal = 0;
+  if (inside == left) {
+    // all of it: border 0
+  } else if (inside <= kFew) {
+#pragma unroll
+    for (int i = 0; i < KPT; i++)
+      if (in[i] == border_bucket) {
+        const int at = atomicAdd(&few_n, 1);
+        few[at] = order_of(s[i]);
+        few_at[at] = tid * KPT + i;
+      }
+    __syncthreads();
+    for (int i = tid; i < inside; i += THREADS) {  // its rank; the one of rank left - 1 is the last that is taken
+      const uint64_t k = few[i];
+      const int at = few_at[i];
+      int above = 0, same_before = 0;
+      for (int o = 0; o < inside; o++) {
+        above += few[o] > k;
+        same_before += few[o] == k && few_at[o] < at;
+      }
+      if (above + same_before == left - 1) chosen[0] = i, chosen[1] = same_before + 1;
+    }
+    __syncthreads();
+    border = few[chosen[0]];
+    equal = chosen[1];
+  } else {
+    int want = left, shift = 56;
+    for (;; shift -= 8) {
+      __syncthreads();
+      for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < KPT; i++) {
+        const uint64_t k = order_of(s[i]);
+        if (in[i] == border_bucket && (shift == 56 || ((k ^ border) >> (shift + 8)) == 0)) atomicAdd(&hist[(k >> shift) & 255], 1);
+      }
+      __syncthreads();
+      const int here = tid < 256 ? hist[255 - tid] : 0;
+      const int before = block_sum<THREADS>(here, tmp, total) - here;
+      if (before < want && before + here >= want) chosen[0] = 255 - tid, chosen[1] = want - before;
+      __syncthreads();
+      border |= (uint64_t)chosen[0] << shift;
+      want = chosen[1];
+      if (shift == 0) break;
+    }
+    equal = want;
+  }
+  // the list, in the blocks' order: a thread's candidates are neighbours
+  int ties = 0, sure = 0;
+  uint32_t tie = 0, taken = 0;
+#pragma unroll
+  for (int i = 0; i < KPT; i++) {
+    bool t = in[i] > border_bucket, e = false;
+    if (in[i] == border_bucket) {
+      const uint64_t k = order_of(s[i]);
+      t = inside == left || k > border;
+      e = !t && k == border;
+    }
+    taken |= t ? 1u << i : 0u;
+    tie |= e ? 1u << i : 0u;
+    sure += t;
+    ties += e;
+  }
+  int tie_rank = block_sum<THREADS>(ties, tmp, total) - ties;
+  const int ties_taken = min(max(equal - tie_rank, 0), ties);
+  int at = block_sum<THREADS>(sure + ties_taken, tmp, total) - sure - ties_taken;
+#pragma unroll
+  for (int i = 0; i < KPT; i++) {
+    bool t = (taken >> i) & 1;
+    if ((tie >> i) & 1) t = tie_rank++ < equal;
+    if (t) out[a.first + at++] = ch.lo + tid * KPT + i;
+  }
+}
+
+// Any number of candidates: the border by eight bits at a time, from the workspace.
+__global__ void __launch_bounds__(1024) k_block_pick_many(BlockSelect a, const double* __restrict__ scores) {
+  constexpr int THREADS = 1024;
+  __shared__ int hist[256], tmp[THREADS / 64], chosen[2];
+  const int tid = threadIdx.x;
   const int64_t rh = blockIdx.x;
   const int row = (int)(rh / a.n_kv);
   const RowOf of(a.row_offsets, a.lengths, a.batch, a.rows, row);
@@ -283,91 +559,60 @@ __global__ void __launch_bounds__(THREADS) k_block_pick(BlockSelect a, const uin
     for (int i = tid; i < a.top; i += THREADS) out[i] = of.p >= 0 && i <= ch.cur ? i : -1;
     return;
   }
-  const uint64_t* key = keys + rh * a.ws_blocks;
-  const int take = a.top - a.first - a.last;  // of the candidates
+  const double* s = scores + rh * a.ws_blocks;
+  const int take = a.top - a.first - a.last;
   for (int i = tid; i < a.first; i += THREADS) out[i] = i;
   for (int i = tid; i < a.last; i += THREADS) out[a.top - a.last + i] = ch.cur + 1 - a.last + i;
   if (take == 0) return;
-  // the border: keys above it are taken, and of those equal to it the first `left`
   uint64_t border = 0;
-  int left = take, shift = 56;
-  for (;; shift -= 8) {
+  int want = take, total;
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    __syncthreads();
     for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
     __syncthreads();
     for (int j = tid; j < ch.n; j += THREADS) {
-      const uint64_t k = key[j];
+      const uint64_t k = order_of(s[j]);
       if (shift == 56 || ((k ^ border) >> (shift + 8)) == 0) atomicAdd(&hist[(k >> shift) & 255], 1);
     }
     __syncthreads();
-    if (wave == 0) {  // from the highest digit down: where the count reaches `left`
-      int mine[4], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 4; i++) sum += mine[i] = hist[255 - 4 * lane - i];
-      int in = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(in, d, 64);
-        if (lane >= d) in += o;
-      }
-      int run = in - sum;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (run < left && run + mine[i] >= left) {
-          chosen[0] = 255 - 4 * lane - i;
-          chosen[1] = left - run;
-        }
-        run += mine[i];
-      }
-    }
+    const int here = tid < 256 ? hist[255 - tid] : 0;
+    const int before = block_sum<THREADS>(here, tmp, total) - here;
+    if (before < want && before + here >= want) chosen[0] = 255 - tid, chosen[1] = want - before;
     __syncthreads();
     border |= (uint64_t)chosen[0] << shift;
-    left = chosen[1];
-    const bool all = hist[chosen[0]] == left;  // the whole bucket is taken
-    __syncthreads();
-    if (shift == 0 || all) break;
+    want = chosen[1];
   }
-  // with the whole bucket taken the low bits of the border are 0 and no key counts as equal to it
-  const uint64_t high = border >> shift;
-  const bool whole = shift > 0;
-  int before = 0, equal = 0;
+  int at = a.first, ties = 0;
   for (int j0 = 0; j0 < ch.n; j0 += THREADS) {
     const int j = j0 + tid;
-    const uint64_t k = j < ch.n ? key[j] >> shift : 0;
-    const bool same = !whole && j < ch.n && k == high;
-    const bool above = j < ch.n && (whole ? k >= high : k > high);
-    const uint64_t sb = __ballot(same), ab = __ballot(above);
-    const uint64_t below = (1ull << lane) - 1;
-    if (lane == 0) wsum[wave] = __popcll(ab) << 16 | __popcll(sb);
-    __syncthreads();
-    int a_before = before, s_before = equal, a_all = 0, s_all = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; w++) {
-      if (w < wave) {
-        a_before += wsum[w] >> 16;
-        s_before += wsum[w] & 0xFFFF;
-      }
-      a_all += wsum[w] >> 16;
-      s_all += wsum[w] & 0xFFFF;
-    }
-    const int s_rank = s_before + __popcll(sb & below), a_rank = a_before + __popcll(ab & below);
-    if (above || (same && s_rank < left)) out[a.first + a_rank + min(s_rank, left)] = ch.lo + j;
-    before += a_all;
-    equal += s_all;
-    __syncthreads();
+    const uint64_t k = j < ch.n ? order_of(s[j]) : 0;
+    const bool same = j < ch.n && k == border;
+    int all;
+    const int rank = ties + block_sum<THREADS>(same, tmp, all) - same;
+    ties += all;
+    const bool t = j < ch.n && (k > border || (same && rank < want));
+    const int place = at + block_sum<THREADS>(t, tmp, all) - t;
+    at += all;
+    if (t) out[place] = ch.lo + j;
   }
 }
 
 template <int D, class E>
 hipError_t select_dim(hipStream_t st, const BlockSelect& a) {
-  uint64_t* keys = (uint64_t*)a.ws;
-  const int chunks = (a.pps + kScoreBlocks - 1) / kScoreBlocks;
+  double* scores = (double*)a.ws;
+  const int group = a.n_q / a.n_kv, chunks = (a.pps + kScoreBlocks - 1) / kScoreBlocks;
   const int64_t rh = (int64_t)a.rows * a.n_kv, units = rh * chunks;
   if (a.pps > a.top) {
-    hipLaunchKernelGGL((k_block_scores<D, E>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, keys, chunks);
+    auto f = group == 1 ? k_block_scores<D, 1, E> : group == 2 ? k_block_scores<D, 2, E> : k_block_scores<D, 4, E>;
+    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, chunks);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(k_block_pick<256>, dim3((unsigned)rh), dim3(256), 0, st, a, keys);
+  const dim3 grid((unsigned)rh);
+  if (a.pps <= 256 * 4) hipLaunchKernelGGL((k_block_pick<256, 4>), grid, dim3(256), 0, st, a, scores);
+  else if (a.pps <= 1024 * 4) hipLaunchKernelGGL((k_block_pick<1024, 4>), grid, dim3(1024), 0, st, a, scores);
+  else if (a.pps <= 1024 * 16) hipLaunchKernelGGL((k_block_pick<1024, 16>), grid, dim3(1024), 0, st, a, scores);
+  else hipLaunchKernelGGL(k_block_pick_many, grid, dim3(1024), 0, st, a, scores);
   return hipGetLastError();
 }
 template <class E>
@@ -398,7 +643,7 @@ hipError_t launch_bounds_update(hipStream_t st, const BoundsUpdate& a) {
 
 size_t select_workspace(int n_q, int n_kv, int hd, int rows, int blocks) {
   (void)n_q, (void)hd;
-  return (size_t)rows * n_kv * blocks * sizeof(uint64_t);
+  return (size_t)rows * n_kv * blocks * sizeof(double);
 }
 
 hipError_t launch_block_select(hipStream_t st, int dtype, const BlockSelect& a) {
