@@ -1094,7 +1094,7 @@ struct Cut {
 constexpr int listed_waves(int hd) { return hd == 256 ? 4 : 8; }
 // A wave an item where these fill the card, and where a list is short; else a workgroup an item, and where a wave would have more than
 // kListedTiles tiles several.
-constexpr int kListedTiles = 16;
+constexpr int kListedTiles = 2;
 Cut listed_cut(int n_q, int n_kv, int hd, int rows, int64_t tiles) {
   const int group = n_q / n_kv, ncts = (group + 15) / 16;
   Cut c{(int64_t)rows * n_kv * ncts, 1, 1, (int)tiles};

@@ -372,7 +372,8 @@ extern "C" int rstr_select_run(rstr_select* a, int32_t layer, int32_t dtype, int
     if (ranges_meet(x.p, x.n, blocks, n)) return fail(s, RSTR_E_INVALID, "blocks overlap the sequences' tables");
   if (ints_meet(blocks, (int64_t)n, qr, rows, a->n_q, v.c.hd, size)) return fail(s, RSTR_E_INVALID, "blocks overlap the queries");
   BlockSelect k{a->b->base + layer * a->b->layer_elems, v.c.n_kv, v.c.hd, v.c.page_size, v.c.pages, a->n_q, batch, rows, pages_per_seq,
-                blocks_per_row, first, last, qr, row_offsets, page_table, lengths, blocks, a->ws, a->blocks};
+                blocks_per_row, first, last, qr, row_offsets, page_table, lengths, blocks, a->ws,
+                select_stride(a->blocks)};
   OnDevice dev(s->device);
   HIPCHK(s, dev.e);
   HIPCHK(s, launch_block_select(on_stream(s, stream), dtype, k));

@@ -268,13 +268,13 @@ __device__ __attribute__((noinline)) double odd_score(const typename E::T* q, in
   return 2.0 * best;
 }
 
-// A wave scores kScoreBlocks blocks for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers twice the
-// larger of q lo and q hi is q (lo + hi) + |q| |hi - lo|, so a bound is converted once for all heads, and a product costs two
-// multiply-adds; where a sum is not finite the block is scored by the definition.
+// A wave scores `per` blocks, up to 64, for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers
+// twice the larger of q lo and q hi is q (lo + hi) + |q| |hi - lo|, so a bound is converted once for all heads, and a product costs
+// two multiply-adds; where a sum is not finite the block is scored by the definition.
 template <int D, int HG, class E>
-__global__ void __launch_bounds__(256) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks) {
+__global__ void __launch_bounds__(256, HG == 4 ? 3 : 4) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks, int per) {
   typedef typename E::T T;
-  constexpr int CH = D / 8, PER = 64 / CH, STEPS = kScoreBlocks / PER, AHEAD = 4;
+  constexpr int CH = D / 8, PER = 64 / CH;  // lanes of a block, blocks at a time
   const int lane = threadIdx.x & 63, c = lane % CH;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t rh = unit / chunks;
@@ -284,78 +284,79 @@ __global__ void __launch_bounds__(256) k_block_scores(BlockSelect a, double* __r
   const int group = a.n_q / a.n_kv;
   const T* q0 = (const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)h * group * a.q.head;
   const bool vec = vec_rows(a.q, sizeof(T));
-  float qf[HG][8];
+  double q[HG][8];
   const auto queries = [&](int g0) {  // behind the last head: that head again
 #pragma unroll
     for (int i = 0; i < HG; i++) {
       const T* p = q0 + (int64_t)min(g0 + i, group - 1) * a.q.head + 8 * c;
-      if (vec) load8<E, true>(p, qf[i]); else load8<E, false>(p, qf[i]);
+      float x[8];
+      if (vec) load8<E, true>(p, x); else load8<E, false>(p, x);
+#pragma unroll
+      for (int k = 0; k < 8; k++) q[i][k] = (double)x[k];
     }
   };
   queries(0);
   const RowOf of(a.row_offsets, a.lengths, a.batch, a.rows, row);
   if (of.b < 0 || of.p < 0) return;
   const Choice ch(a, of.p);
-  const int j0 = chunk * kScoreBlocks, n = min(kScoreBlocks, ch.n - j0);
+  const int j0 = chunk * per, n = min(per, ch.n - j0);
   if (n <= 0) return;
   double* out = scores + rh * a.ws_blocks + j0;
   const int page = lane < n ? a.page_table[(int64_t)of.b * a.pps + ch.lo + j0 + lane] : -1;
   const int64_t head = (int64_t)2 * D;
   const _Float16* base = (const _Float16*)a.bounds + h * head + 8 * c;
-  const auto bound_of = [&](int step, int& id) {
-    id = __shfl(page, step * PER + lane / CH, 64);
-    if ((uint32_t)id >= (uint32_t)a.pages) id = -1;
-    return base + (int64_t)max(id, 0) * a.n_kv * head;
+  const auto bound_of = [&](int step) {
+    const int id = __shfl(page, min(step * PER + lane / CH, 63), 64);
+    return base + (int64_t)((uint32_t)id < (uint32_t)a.pages ? id : 0) * a.n_kv * head;
   };
   for (int g0 = 0; g0 < group; g0 += HG) {
     if (g0) queries(g0);
-    double q[HG][8];
+    u32x4 lo[2], hi[2];
+    const auto load = [&](int i, int step) {
+      const _Float16* p = bound_of(step);
+      lo[i] = *(const u32x4*)p;
+      hi[i] = *(const u32x4*)(p + D);
+    };
+    const auto score = [&](int i, int step) {
+      double s[HG];
 #pragma unroll
-    for (int i = 0; i < HG; i++)
+      for (int g = 0; g < HG; g++) s[g] = 0.0;
 #pragma unroll
-      for (int k = 0; k < 8; k++) q[i][k] = (double)qf[i][k];
+      for (int k = 0; k < 8; k++) {
+        const uint32_t wl = lo[i][k >> 1], wh = hi[i][k >> 1];
+        const double x = (double)(float)__builtin_bit_cast(h2, wl)[k & 1], y = (double)(float)__builtin_bit_cast(h2, wh)[k & 1];
+        const double sum = y + x, wide = __builtin_fabs(y - x);
+#pragma unroll
+        for (int g = 0; g < HG; g++) s[g] = __builtin_fma(__builtin_fabs(q[g][k]), wide, __builtin_fma(q[g][k], sum, s[g]));
+      }
+      double x = scatter_sum<CH, HG>(s);
+      int odd = !(__builtin_fabs(x) < INFINITY);
+      if constexpr (HG >= 2) {
+        odd |= __builtin_amdgcn_update_dpp(0, odd, 0xB1, 0xF, 0xF, true);
+        const double o = dpp_f64<0xB1>(x);
+        x = o > x ? o : x;
+      }
+      if constexpr (HG == 4) {
+        odd |= __builtin_amdgcn_update_dpp(0, odd, 0x4E, 0xF, 0xF, true);
+        const double o = dpp_f64<0x4E>(x);
+        x = o > x ? o : x;
+      }
+      const int j = step * PER + lane / CH, id = __shfl(page, min(j, 63), 64);
+      if (c == 0 && j < n) {
+        const bool there = (uint32_t)id < (uint32_t)a.pages;
+        if (g0) x = out[j] > x ? out[j] : x;  // (an odd block's score is the same in all rounds)
+        if (odd) x = odd_score<D, E>(q0, a.q.head, group, base + (int64_t)(there ? id : 0) * a.n_kv * head);
+        out[j] = there ? x : -INFINITY;
+      }
+    };
+    load(0, 0);
+    load(1, 1);
 #pragma unroll 1
-    for (int s0 = 0; s0 * PER < n; s0 += AHEAD) {
-      u32x4 lo[AHEAD], hi[AHEAD];
-      int id[AHEAD];
-#pragma unroll
-      for (int i = 0; i < AHEAD; i++) {
-        const _Float16* p = bound_of(min(s0 + i, STEPS - 1), id[i]);
-        lo[i] = *(const u32x4*)p;
-        hi[i] = *(const u32x4*)(p + D);
-      }
-#pragma unroll
-      for (int i = 0; i < AHEAD; i++) {
-        double s[HG];
-#pragma unroll
-        for (int g = 0; g < HG; g++) s[g] = 0.0;
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const uint32_t wl = lo[i][k >> 1], wh = hi[i][k >> 1];
-          const double x = (double)(float)__builtin_bit_cast(h2, wl)[k & 1], y = (double)(float)__builtin_bit_cast(h2, wh)[k & 1];
-          const double sum = y + x, wide = __builtin_fabs(y - x);
-#pragma unroll
-          for (int g = 0; g < HG; g++) s[g] = __builtin_fma(__builtin_fabs(q[g][k]), wide, __builtin_fma(q[g][k], sum, s[g]));
-        }
-        double x = scatter_sum<CH, HG>(s);
-        bool odd = !(__builtin_fabs(x) < INFINITY);
-        if constexpr (HG >= 2) {
-          const double o = dpp_f64<0xB1>(x);
-          odd = odd || !(__builtin_fabs(o) < INFINITY);
-          x = o > x ? o : x;
-        }
-        if constexpr (HG == 4) {
-          const double o = dpp_f64<0x4E>(x);
-          x = o > x ? o : x;
-          odd = odd || __builtin_amdgcn_update_dpp(0, (int)odd, 0x4E, 0xF, 0xF, true);
-        }
-        const int j = (s0 + i) * PER + lane / CH;
-        if (c == 0 && s0 + i < STEPS && j < n) {
-          if (g0) x = out[j] > x ? out[j] : x;  // (an odd block's score is the same in all rounds)
-          if (odd) x = odd_score<D, E>(q0, a.q.head, group, base + (int64_t)max(id[i], 0) * a.n_kv * head);
-          out[j] = id[i] < 0 ? -INFINITY : x;
-        }
-      }
+    for (int step = 0; step * PER < n; step += 2) {  // (loads behind the last block are of a page that is there)
+      score(0, step);
+      load(0, step + 2);
+      score(1, step + 1);
+      load(1, step + 3);
     }
   }
 }
@@ -392,17 +393,17 @@ template <int THREADS, int KPT>
 __global__ void __launch_bounds__(THREADS) k_block_pick(BlockSelect a, const double* __restrict__ scores) {
   constexpr int WAVES = THREADS / 64;
   __shared__ int hist[kBuckets], tmp[WAVES], chosen[2], few_n;
-  __shared__ double ends[2][WAVES];
+  __shared__ float ends[2][WAVES];
   __shared__ uint64_t few[kFew];
   __shared__ int few_at[kFew];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t rh = blockIdx.x;
   const int row = (int)(rh / a.n_kv);
   // scores, asked for before the row's candidates are known (in the workspace wherever they end)
-  const double* from = scores + rh * a.ws_blocks;
+  const double* from = scores + rh * a.ws_blocks + min(tid * KPT, a.ws_blocks - KPT);
   double s[KPT];
 #pragma unroll
-  for (int i = 0; i < KPT; i++) s[i] = a.pps > a.top ? from[min(tid * KPT + i, a.ws_blocks - 1)] : 0.0;
+  for (int i = 0; i < KPT / 2; i++) ((u32x4*)s)[i] = a.pps > a.top ? ((const u32x4*)from)[i] : u32x4{0, 0, 0, 0};
   const RowOf of(a.row_offsets, a.lengths, a.batch, a.rows, row);
   if (of.b < 0) return;
   int32_t* out = a.blocks + rh * a.top;
@@ -415,35 +416,34 @@ __global__ void __launch_bounds__(THREADS) k_block_pick(BlockSelect a, const dou
   for (int i = tid; i < a.first; i += THREADS) out[i] = i;
   for (int i = tid; i < a.last; i += THREADS) out[a.top - a.last + i] = ch.cur + 1 - a.last + i;
   if (take == 0) return;
-  // the range of the finite ones
-  double lo = INFINITY, hi = -INFINITY;
+  // the range of the finite ones, in fp32 (rounding keeps the order)
+  float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
   for (int i = 0; i < KPT; i++) {
-    const bool fin = tid * KPT + i < ch.n && __builtin_fabs(s[i]) < INFINITY;
-    lo = fin && s[i] < lo ? s[i] : lo;
-    hi = fin && s[i] > hi ? s[i] : hi;
+    const float x = (float)s[i];
+    const bool fin = tid * KPT + i < ch.n && fabsf(x) < INFINITY;
+    lo = fin ? fminf(lo, x) : lo;
+    hi = fin ? fmaxf(hi, x) : hi;
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    lo = __builtin_fmin(lo, __shfl_xor(lo, d, 64));
-    hi = __builtin_fmax(hi, __shfl_xor(hi, d, 64));
-  }
+  lo = -wave_max(-lo);
+  hi = wave_max(hi);
   if (lane == 0) ends[0][wave] = lo, ends[1][wave] = hi;
   for (int i = tid; i < kBuckets; i += THREADS) hist[i] = 0;
   if (tid == 0) few_n = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; w++) {
-    lo = __builtin_fmin(lo, ends[0][w]);
-    hi = __builtin_fmax(hi, ends[1][w]);
+    lo = fminf(lo, ends[0][w]);
+    hi = fmaxf(hi, ends[1][w]);
   }
   // a bucket's number does not decrease with the score
-  const double per = (double)(kBuckets - 2) / (hi - lo);  // (all alike: infinite or none, and one bucket)
-  const auto bucket = [&](double x) {
+  const float per = (float)(kBuckets - 2) / (hi - lo);  // (all alike: infinite or none, and one bucket)
+  const auto bucket = [&](double score) {
+    const float x = (float)score;
     if (x == INFINITY) return kBuckets - 1;
     if (x == -INFINITY) return 0;
-    const double at = (x - lo) * per;
-    return at >= 0.0 ? (at < (double)(kBuckets - 3) ? 1 + (int)at : kBuckets - 2) : 1;
+    const float at = (x - lo) * per;
+    return at >= 0.0f ? (at < (float)(kBuckets - 3) ? 1 + (int)at : kBuckets - 2) : 1;
   };
   int in[KPT];
 #pragma unroll
@@ -600,11 +600,15 @@ __global__ void __launch_bounds__(1024) k_block_pick_many(BlockSelect a, const d
 template <int D, class E>
 hipError_t select_dim(hipStream_t st, const BlockSelect& a) {
   double* scores = (double*)a.ws;
-  const int group = a.n_q / a.n_kv, chunks = (a.pps + kScoreBlocks - 1) / kScoreBlocks;
-  const int64_t rh = (int64_t)a.rows * a.n_kv, units = rh * chunks;
+  const int group = a.n_q / a.n_kv;
+  const int64_t rh = (int64_t)a.rows * a.n_kv;
+  // 64 blocks a wave where that leaves the card full, else 32
+  const int per = rh * ((a.pps + 63) / 64) >= 16 * (int64_t)compute_units() ? 64 : kScoreBlocks;
+  const int chunks = (a.pps + per - 1) / per;
+  const int64_t units = rh * chunks;
   if (a.pps > a.top) {
     auto f = group == 1 ? k_block_scores<D, 1, E> : group == 2 ? k_block_scores<D, 2, E> : k_block_scores<D, 4, E>;
-    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, chunks);
+    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, chunks, per);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -643,7 +647,7 @@ hipError_t launch_bounds_update(hipStream_t st, const BoundsUpdate& a) {
 
 size_t select_workspace(int n_q, int n_kv, int hd, int rows, int blocks) {
   (void)n_q, (void)hd;
-  return (size_t)rows * n_kv * blocks * sizeof(double);
+  return (size_t)rows * n_kv * select_stride(blocks) * sizeof(double);
 }
 
 hipError_t launch_block_select(hipStream_t st, int dtype, const BlockSelect& a) {
