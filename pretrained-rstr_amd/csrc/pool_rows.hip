@@ -254,10 +254,11 @@ __device__ __forceinline__ double scatter_sum(double (&v)[HG]) {
 
 // By the definition: where something is not finite.
 template <int D, class E>
-__device__ __attribute__((noinline)) double odd_score(const typename E::T* q, int64_t head, int group, const _Float16* bound) {
+__device__ double odd_score(const typename E::T* q, int64_t head, int group, const _Float16* bound) {
   double best = -INFINITY;
   for (int g = 0; g < group; g++) {
     double s = 0.0;
+#pragma unroll 1
     for (int d = 0; d < D; d++) {
       const double x = (double)E::get(q[g * head + d]) * (double)(float)bound[d], y = (double)E::get(q[g * head + d]) * (double)(float)bound[D + d];
       s += x > y || x != x ? x : y;
@@ -272,9 +273,9 @@ __device__ __attribute__((noinline)) double odd_score(const typename E::T* q, in
 // twice the larger of q lo and q hi is q (lo + hi) + |q| |hi - lo|, so a bound is converted once for all heads, and a product costs
 // two multiply-adds; where a sum is not finite the block is scored by the definition.
 template <int D, int HG, class E>
-__global__ void __launch_bounds__(256, HG == 4 ? 3 : 4) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks, int per) {
+__global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks, int per) {
   typedef typename E::T T;
-  constexpr int CH = D / 8, PER = 64 / CH;  // lanes of a block, blocks at a time
+  constexpr int CH = D / 8, PER = 64 / CH, AHEAD = 4;  // lanes of a block, blocks at a time, steps in flight
   const int lane = threadIdx.x & 63, c = lane % CH;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t rh = unit / chunks;
@@ -284,15 +285,12 @@ __global__ void __launch_bounds__(256, HG == 4 ? 3 : 4) k_block_scores(BlockSele
   const int group = a.n_q / a.n_kv;
   const T* q0 = (const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)h * group * a.q.head;
   const bool vec = vec_rows(a.q, sizeof(T));
-  double q[HG][8];
+  float q[HG][8];
   const auto queries = [&](int g0) {  // behind the last head: that head again
 #pragma unroll
     for (int i = 0; i < HG; i++) {
       const T* p = q0 + (int64_t)min(g0 + i, group - 1) * a.q.head + 8 * c;
-      float x[8];
-      if (vec) load8<E, true>(p, x); else load8<E, false>(p, x);
-#pragma unroll
-      for (int k = 0; k < 8; k++) q[i][k] = (double)x[k];
+      if (vec) load8<E, true>(p, q[i]); else load8<E, false>(p, q[i]);
     }
   };
   queries(0);
@@ -309,9 +307,10 @@ __global__ void __launch_bounds__(256, HG == 4 ? 3 : 4) k_block_scores(BlockSele
     const int id = __shfl(page, min(step * PER + lane / CH, 63), 64);
     return base + (int64_t)((uint32_t)id < (uint32_t)a.pages ? id : 0) * a.n_kv * head;
   };
+  uint32_t odds = 0;  // steps whose block has no finite score
   for (int g0 = 0; g0 < group; g0 += HG) {
     if (g0) queries(g0);
-    u32x4 lo[2], hi[2];
+    u32x4 lo[AHEAD], hi[AHEAD];
     const auto load = [&](int i, int step) {
       const _Float16* p = bound_of(step);
       lo[i] = *(const u32x4*)p;
@@ -327,7 +326,10 @@ __global__ void __launch_bounds__(256, HG == 4 ? 3 : 4) k_block_scores(BlockSele
         const double x = (double)(float)__builtin_bit_cast(h2, wl)[k & 1], y = (double)(float)__builtin_bit_cast(h2, wh)[k & 1];
         const double sum = y + x, wide = __builtin_fabs(y - x);
 #pragma unroll
-        for (int g = 0; g < HG; g++) s[g] = __builtin_fma(__builtin_fabs(q[g][k]), wide, __builtin_fma(q[g][k], sum, s[g]));
+        for (int g = 0; g < HG; g++) {
+          const double y2 = (double)q[g][k];  // (kept in 32 bits: more waves a SIMD)
+          s[g] = __builtin_fma(__builtin_fabs(y2), wide, __builtin_fma(y2, sum, s[g]));
+        }
       }
       double x = scatter_sum<CH, HG>(s);
       int odd = !(__builtin_fabs(x) < INFINITY);
@@ -344,20 +346,31 @@ __global__ void __launch_bounds__(256, HG == 4 ? 3 : 4) k_block_scores(BlockSele
       const int j = step * PER + lane / CH, id = __shfl(page, min(j, 63), 64);
       if (c == 0 && j < n) {
         const bool there = (uint32_t)id < (uint32_t)a.pages;
-        if (g0) x = out[j] > x ? out[j] : x;  // (an odd block's score is the same in all rounds)
-        if (odd) x = odd_score<D, E>(q0, a.q.head, group, base + (int64_t)(there ? id : 0) * a.n_kv * head);
+        if (g0) x = out[j] > x ? out[j] : x;
+        if (odd) odds |= 1u << step;
         out[j] = there ? x : -INFINITY;
       }
     };
-    load(0, 0);
-    load(1, 1);
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) load(i, i);
 #pragma unroll 1
-    for (int step = 0; step * PER < n; step += 2) {  // (loads behind the last block are of a page that is there)
-      score(0, step);
-      load(0, step + 2);
-      score(1, step + 1);
-      load(1, step + 3);
-    }
+    for (int step = 0; step * PER < n; step += AHEAD)  // (loads behind the last block are of a page that is there)
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) {
+        // queries are converted anew for every step: hoisted they would take twice the registers
+#pragma unroll
+        for (int g = 0; g < HG; g++)
+#pragma unroll
+          for (int k = 0; k < 8; k++) asm("" : "+v"(q[g][k]));
+        score(i, step + i);
+        load(i, step + i + AHEAD);
+      }
+  }
+  while (odds) {
+    const int step = __ffs(odds) - 1, j = step * PER + lane / CH;
+    odds &= odds - 1;
+    const int id = a.page_table[(int64_t)of.b * a.pps + ch.lo + j0 + j];
+    if ((uint32_t)id < (uint32_t)a.pages) out[j] = odd_score<D, E>(q0, a.q.head, group, base + (int64_t)id * a.n_kv * head);
   }
 }
 
