@@ -285,12 +285,15 @@ __global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* 
   const int group = a.n_q / a.n_kv;
   const T* q0 = (const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)h * group * a.q.head;
   const bool vec = vec_rows(a.q, sizeof(T));
-  float q[HG][8];
+  double q[HG][8];
   const auto queries = [&](int g0) {  // behind the last head: that head again
 #pragma unroll
     for (int i = 0; i < HG; i++) {
       const T* p = q0 + (int64_t)min(g0 + i, group - 1) * a.q.head + 8 * c;
-      if (vec) load8<E, true>(p, q[i]); else load8<E, false>(p, q[i]);
+      float x[8];
+      if (vec) load8<E, true>(p, x); else load8<E, false>(p, x);
+#pragma unroll
+      for (int k = 0; k < 8; k++) q[i][k] = (double)x[k];
     }
   };
   queries(0);
@@ -326,10 +329,7 @@ __global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* 
         const double x = (double)(float)__builtin_bit_cast(h2, wl)[k & 1], y = (double)(float)__builtin_bit_cast(h2, wh)[k & 1];
         const double sum = y + x, wide = __builtin_fabs(y - x);
 #pragma unroll
-        for (int g = 0; g < HG; g++) {
-          const double y2 = (double)q[g][k];  // (kept in 32 bits: more waves a SIMD)
-          s[g] = __builtin_fma(__builtin_fabs(y2), wide, __builtin_fma(y2, sum, s[g]));
-        }
+        for (int g = 0; g < HG; g++) s[g] = __builtin_fma(__builtin_fabs(q[g][k]), wide, __builtin_fma(q[g][k], sum, s[g]));
       }
       double x = scatter_sum<CH, HG>(s);
       int odd = !(__builtin_fabs(x) < INFINITY);
@@ -357,11 +357,6 @@ __global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* 
     for (int step = 0; step * PER < n; step += AHEAD)  // (loads behind the last block are of a page that is there)
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
-        // queries are converted anew for every step: hoisted they would take twice the registers
-#pragma unroll
-        for (int g = 0; g < HG; g++)
-#pragma unroll
-          for (int k = 0; k < 8; k++) asm("" : "+v"(q[g][k]));
         score(i, step + i);
         load(i, step + i + AHEAD);
       }
