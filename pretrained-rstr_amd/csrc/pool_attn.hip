@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D, NT))
 }
 
 // ---- prompts -----------------------------------------------------------------------------
-// Many columns a sequence: the waves of a workgroup take 32 columns each, two tiles of 16, of one sequence and kv head and
+// Many columns a sequence: the waves of a workgroup take one or two tiles of 16 columns each of one sequence and kv head and
 // share its keys and values, which go straight from the pages into LDS, 64 tokens at a time and one step ahead.
 // The products are those of k_pool_attn.  K's operand is 16 bytes of a row; the operand of V, eight tokens of one dim, comes from two
 // transposing reads of four tokens x 16 dims.  A row of a token is swizzled in LDS by its number, 16 bytes at a time, so that 16 tokens' same
@@ -574,7 +574,10 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D, NT))
 // belongs to its place.
 constexpr int kPromptStart = 8;  // what beginning an item costs, in tiles
 constexpr int kStep = 64;        // tokens at a time
-constexpr int prompt_waves(int hd, int terms) { return hd == 256 || (hd == 128 && terms == 2) ? 4 : 8; }  // (registers of one wave a SIMD, or of two)
+constexpr int kShareWaves = 8;  // two a SIMD, with half its registers each
+// Tiles of 16 columns a wave: what these registers hold.  Four waves of two tiles instead: 167 us for 98 at D = 256, 556 for 449 in fp32
+// at D = 128 (1900 rows at 5000 tokens, 4 and 32 heads).
+constexpr int prompt_tiles(int hd, int terms) { return hd * terms >= 256 ? 1 : 2; }
 
 typedef short sv4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t* TablePtr;  // read-only for the kernel: scalar loads
@@ -585,11 +588,11 @@ __device__ __forceinline__ u32x2 read_transposed(LdsPtr at) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sv4*)at));
 }
 template <int D, class E>
-__global__ void __launch_bounds__(64 * prompt_waves(D, Terms<E>::n), prompt_waves(D, Terms<E>::n) / 4)
+__global__ void __launch_bounds__(64 * kShareWaves, kShareWaves / 4)
     k_pool_prompt(PoolAttn a, const int32_t* __restrict__ ro, const int32_t* __restrict__ lens, const int32_t* __restrict__ table, PoolPieces pc,
                   int workers, int least) {
   typedef typename E::T T;
-  constexpr int NT = 2, TERMS = Terms<E>::n, WAVES = prompt_waves(D, TERMS), COLS = 32 * WAVES;
+  constexpr int NT = prompt_tiles(D, Terms<E>::n), TERMS = Terms<E>::n, WAVES = kShareWaves, COLS = 16 * NT * WAVES;
   constexpr int ROW = 2 * D, KS = D / 32, JT = D / 16, TB = kStep / 16;  // bytes of a token; products of a score, of O; 16s of tokens
   constexpr int MINE = kStep / WAVES, GROUPS = MINE / 4, LOADS = MINE * ROW / 1024;  // tokens that a wave loads, fours of them, instructions
   constexpr int BUF = kStep * ROW;                             // bytes of K or V of a step
@@ -633,7 +636,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(D, Terms<E>::n), prompt_wave
     const auto first_seen = [&](int row) { return a.window > 0 ? max(max(p0 + row + 1, 0) - a.window, 0) : 0; };
     const auto end_seen = [&](int row) { return min(max(p0 + row + 1, 0), cap); };
     const int rf = row_of(c0), rl = row_of(c0 + COLS - 1);
-    const int cw = c0 + wave * 32;
+    const int cw = c0 + wave * 16 * NT;
     // a column's row and head; found anew where they are needed, as keeping them costs registers of the loop
     struct Column {
       int row, head;
@@ -645,7 +648,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(D, Terms<E>::n), prompt_wave
       return Column{row, h * group + (cc - row * group)};
     };
     const bool any = cw < s.m * group;
-    const int wf = row_of(cw), wl = row_of(cw + 31);  // the wave's rows
+    const int wf = row_of(cw), wl = row_of(cw + 16 * NT - 1);  // the wave's rows
     const int t0 = max(s.lo + max(line.at - kPromptStart, 0), first_seen(rf) / kTile);
     const int t1 = min(s.lo + max(line.at + line.n - kPromptStart, 0), (end_seen(rl) + kTile - 1) / kTile);
     const int part_end = t1 * kTile;
@@ -967,7 +970,7 @@ __global__ void __launch_bounds__(64 * prompt_waves(D, Terms<E>::n), prompt_wave
           }
         }
       } else {
-        const int64_t c = piece + wave * 32 + t * 16 + col;
+        const int64_t c = piece + (wave * NT + t) * 16 + col;
         if (g == 0) pc.ml[c] = f4{mref[t], sum, kcol[t], 0.0f};
         if (sum == 0.0f) continue;
 #pragma unroll
@@ -977,89 +980,146 @@ __global__ void __launch_bounds__(64 * prompt_waves(D, Terms<E>::n), prompt_wave
   }
 }
 
-// Joins the pieces of an item, in their order: a workgroup an item and `per` columns (more for every gridDim.y),
-// its waves by column and by piece.
+// An item whose pieces are joined: where they are, and where the result goes.
+template <bool LISTED>
+struct Joined {
+  int n, c0, r0, m, h;
+  int64_t first, rest;  // the first piece, and what the ones behind it are counted from
+  __device__ bool find(const PoolAttn& a, const Lines& L, const PoolPieces& pc, int item, int parts) {
+    if constexpr (LISTED) {
+      const int ncts = (L.group + L.cols - 1) / L.cols, row = item / (L.n_kv * ncts), hc = item - row * (L.n_kv * ncts);
+      const RowOf of(L.ro, L.lens, a.batch, a.rows, row);
+      if (of.b < 0) return false;
+      n = parts;
+      h = hc / ncts;
+      c0 = (hc - h * ncts) * L.cols;
+      r0 = row;
+      m = 1;
+      first = rest = (int64_t)item * parts;
+    } else {
+      const int items = *pc.n_items;
+      const Begun it = pc.begun[item];  // (of an item that is not: whatever is there)
+      n = it.pieces;
+      if (item >= items || n == 0) return false;
+      h = it.h;
+      c0 = it.ct * L.cols;
+      const int32_t* ro = L.ro + it.b;
+      r0 = min(max(ro[0], 0), L.rows);
+      m = max(min(max(ro[1], 0), L.rows) - r0, 0);
+      first = 2 * (int64_t)it.w + 1;
+      rest = 2 * (int64_t)it.w;
+    }
+    return true;
+  }
+  __device__ int64_t slot(const Lines& L, int i, int c) const { return (i == 0 ? first : LISTED ? rest + i : rest + 2 * i) * L.cols + c; }
+  __device__ int64_t out_at(const PoolAttn& a, const Lines& L, int c) const {
+    const int cc = c0 + c, r = cc / L.group;
+    return (int64_t)(r0 + r) * a.out.row + ((int64_t)h * L.group + (cc - r * L.group)) * a.out.head;
+  }
+};
+
+// Joins the pieces of an item, in their order: a workgroup a column, its waves by piece.
 template <int D, class E, bool LISTED>
-__global__ void k_pool_merge(PoolAttn a, Lines L, PoolPieces pc, int per, int parts) {
+__global__ void k_pool_merge(PoolAttn a, Lines L, PoolPieces pc, int parts) {
   constexpr int V = D / 64;  // dims a lane
   typedef typename E::T T;
   __shared__ float part[16][D];
   __shared__ float pl[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int n, c0, r0, m, h;
-  int64_t first, rest;  // the first piece, and what the ones behind it are counted from
-  if constexpr (LISTED) {
-    const int ncts = (L.group + L.cols - 1) / L.cols, item = blockIdx.x, row = item / (L.n_kv * ncts), hc = item - row * (L.n_kv * ncts);
-    const RowOf of(L.ro, L.lens, a.batch, a.rows, row);
-    if (of.b < 0) return;
-    n = parts;
-    h = hc / ncts;
-    c0 = (hc - h * ncts) * L.cols;
-    r0 = row;
-    m = 1;
-    first = rest = (int64_t)item * parts;
-  } else {
-    const int items = *pc.n_items;
-    const Begun it = pc.begun[blockIdx.x];  // (of an item that is not: whatever is there)
-    n = it.pieces;
-    if ((int)blockIdx.x >= items || n == 0) return;
-    h = it.h;
-    c0 = it.ct * L.cols;
-    const int32_t* ro = L.ro + it.b;
-    r0 = min(max(ro[0], 0), L.rows);
-    m = max(min(max(ro[1], 0), L.rows) - r0, 0);
-    first = 2 * (int64_t)it.w + 1;
-    rest = 2 * (int64_t)it.w;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = blockDim.x >> 6, c = blockIdx.y;
+  Joined<LISTED> it;
+  if (!it.find(a, L, pc, blockIdx.x, parts) || (it.c0 + c) / L.group >= it.m) return;
+  float acc[V] = {}, l = 0.0f, top = -FLT_MAX;
+  for (int i = lane; i < it.n; i += 64) {
+    const f4 y = pc.ml[it.slot(L, i, c)];
+    if (y[1] != 0.0f) top = fmaxf(top, y[0]);
   }
-  const auto slot = [&](int i, int c) { return (i == 0 ? first : LISTED ? rest + i : rest + 2 * i) * L.cols + c; };
-  const int share = (blockDim.x >> 6) / per, mine = wave % share;  // waves a column
-  const int at0 = blockIdx.y * per;
-  for (int at = at0; at < L.cols && (c0 + at) / L.group < m; at += gridDim.y * per) {  // the same for all waves
-    const int c = at + wave / share;
-    float acc[V] = {}, l = 0.0f, top = -FLT_MAX;
-    for (int i = lane; i < n; i += 64) {
-      const f4 y = pc.ml[slot(i, c)];
-      if (y[1] != 0.0f) top = fmaxf(top, y[0]);
-    }
-    top = wave_max(top);
-    for (int i0 = mine; i0 < n; i0 += 8 * share) {
-      f4 x[8];
-      float v[8][V];
+  top = wave_max(top);
+  for (int i0 = wave; i0 < it.n; i0 += 8 * share) {
+    f4 x[8];
+    float v[8][V];
 #pragma unroll
-      for (int k = 0; k < 8; k++) {  // all loads before the first use
-        const int64_t p = slot(min(i0 + k * share, n - 1), c);
+    for (int k = 0; k < 8; k++) {  // all loads before the first use
+      const int64_t p = it.slot(L, min(i0 + k * share, it.n - 1), c);
+      x[k] = pc.ml[p];
+#pragma unroll
+      for (int j = 0; j < V; j++) v[k][j] = pc.acc[p * D + lane * V + j];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const bool some = i0 + k * share < it.n && x[k][1] != 0.0f;
+      const float f = some ? __builtin_amdgcn_exp2f((x[k][0] - top) * x[k][2]) : 0.0f;
+      l = __builtin_fmaf(f, some ? x[k][1] : 0.0f, l);
+#pragma unroll
+      for (int j = 0; j < V; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; j++) part[wave][lane * V + j] = acc[j];
+  if (lane == 0) pl[wave] = l;
+  __syncthreads();
+  if (wave != 0) return;
+  for (int k = 1; k < share; k++) {
+#pragma unroll
+    for (int j = 0; j < V; j++) acc[j] += part[k][lane * V + j];
+    l += pl[k];
+  }
+  T* dst = (T*)a.out.p + it.out_at(a, L, c) + lane * V;
+#pragma unroll
+  for (int j = 0; j < V; j++) dst[j] = E::put(l == 0.0f ? 0.0f : acc[j] / l);
+}
+
+// The same where items have few pieces or there are columns enough: D / 4 lanes a column, four dims each, pieces one after the other.
+// Nothing waits for the greatest reference of all pieces: sums that are there are scaled as it grows.  1333 rows of 32 heads, bf16, 55 MB
+// of pieces: 11.6 us (a wave a column as above 32 us).
+template <int D, class E, bool LISTED>
+__global__ void __launch_bounds__(256) k_pool_join(PoolAttn a, Lines L, PoolPieces pc, int parts) {
+  constexpr int LANES = D / 4, PER = 256 / LANES, AT_ONCE = 4;  // lanes a column, columns at a time, pieces at a time
+  typedef typename E::T T;
+  Joined<LISTED> it;
+  if (!it.find(a, L, pc, blockIdx.x, parts)) return;
+  const int c = blockIdx.y * PER + threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+  if (c >= L.cols || (it.c0 + c) / L.group >= it.m) return;
+  f4 acc = f4{0, 0, 0, 0};
+  float l = 0.0f, top = -FLT_MAX;
+  for (int i0 = 0; i0 < it.n; i0 += AT_ONCE) {
+    f4 x[AT_ONCE], v[AT_ONCE];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; k++) {
+      x[k] = v[k] = f4{0, 0, 0, 0};
+      if (i0 + k < it.n) {
+        const int64_t p = it.slot(L, i0 + k, c);
         x[k] = pc.ml[p];
-#pragma unroll
-        for (int j = 0; j < V; j++) v[k][j] = pc.acc[p * D + lane * V + j];
-      }
-#pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const bool some = i0 + k * share < n && x[k][1] != 0.0f;
-        const float f = some ? __builtin_amdgcn_exp2f((x[k][0] - top) * x[k][2]) : 0.0f;
-        l = __builtin_fmaf(f, some ? x[k][1] : 0.0f, l);
-#pragma unroll
-        for (int j = 0; j < V; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
+        v[k] = *(const f4*)(pc.acc + p * D + d);
       }
     }
-    if (share > 1) {
+    float now = top, scale = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; j++) part[wave][lane * V + j] = acc[j];
-      if (lane == 0) pl[wave] = l;
-      __syncthreads();
-      if (mine == 0)
-        for (int k = 1; k < share; k++) {
+    for (int k = 0; k < AT_ONCE; k++)
+      if (x[k][1] != 0.0f) now = fmaxf(now, x[k][0]), scale = x[k][2];  // (a column's scale is the same in all)
+    const float keep = __builtin_amdgcn_exp2f((top - now) * scale);
+    top = now;
+    l *= keep;
+    acc *= keep;
 #pragma unroll
-          for (int j = 0; j < V; j++) acc[j] += part[wave + k][lane * V + j];
-          l += pl[wave + k];
-        }
-      __syncthreads();
+    for (int k = 0; k < AT_ONCE; k++) {
+      const bool some = x[k][1] != 0.0f;
+      const float f = some ? __builtin_amdgcn_exp2f((x[k][0] - top) * x[k][2]) : 0.0f;
+      l = __builtin_fmaf(f, some ? x[k][1] : 0.0f, l);
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
     }
-    const int cc = c0 + c, r = cc / L.group;
-    if (r < m && mine == 0) {
-      T* dst = (T*)a.out.p + (int64_t)(r0 + r) * a.out.row + ((int64_t)h * L.group + cc % L.group) * a.out.head + lane * V;
+  }
+  T* dst = (T*)a.out.p + it.out_at(a, L, c) + d;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T o[4];
 #pragma unroll
-      for (int j = 0; j < V; j++) dst[j] = E::put(l == 0.0f ? 0.0f : acc[j] / l);
-    }
+  for (int j = 0; j < 4; j++) o[j] = E::put(acc[j] * inv);
+  if (vec_rows(a.out, sizeof(T))) {
+    if constexpr (sizeof(T) == 4) *(u32x4*)dst = *(u32x4*)o;
+    else *(u32x2*)dst = *(u32x2*)o;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) dst[j] = o[j];
   }
 }
 
@@ -1068,7 +1128,11 @@ constexpr int kMergeWaves = 4096;
 constexpr int kWhole = 4;  // tiles of an item that one wave does, without a merge
 constexpr int kLeast = 2;  // tiles a wave takes at least
 constexpr int kPromptLeast = 8;  // and a workgroup of k_pool_prompt
-constexpr int kManyColumns = 64;  // columns a sequence from which waves share tiles
+// Columns a sequence from which waves share tiles.  Both sides, in us, of one sequence of 4000 tokens and of eight of 2000: D = 128 f16
+// 25.0 | 26.3 and 39.6 | 38.2 with 32 columns, 31.6 | 26.4 and 46.0 | 41.0 with 64; D = 64 17.2 | 19.4 and 24.4 | 20.9 with 64;
+// D = 256 f16 23.4 | 27.9 and 32.0 | 29.9 with 64, 37.7 | 34.4 with 512; D = 256 fp32 40.9 | 46.8 with 128, 38.3 | 44.7 with 512, and with
+// 3600 at 5000 tokens 307 | 152.
+constexpr int many_columns(int hd, int terms) { return hd < 256 ? 64 : terms == 1 ? 128 : 1024; }
 constexpr int kOneTile = 16;  // columns a sequence up to which items have one tile of columns, above it two
 
 int64_t most_workers(int hd, int nt) { return (int64_t)compute_units() * 4 * pool_waves(hd, nt); }
@@ -1117,9 +1181,9 @@ hipError_t merge(hipStream_t st, const PoolAttn& a, const PoolPieces& pc, int64_
   const int each = (int)(pieces / items);
   int share = each >= 16 ? 16 : each >= 4 ? 4 : 1;
   while (share > 1 && items * columns * share > kMergeWaves) share /= 4;
-  const int per = share == 1 ? 4 : 1;
-  hipLaunchKernelGGL((k_pool_merge<D, E, LISTED>), dim3((unsigned)items, (unsigned)((columns + per - 1) / per)), dim3(share == 16 ? 1024 : 256),
-                     0, st, a, L, pc, per, parts);
+  constexpr int per = 1024 / D;
+  if (share == 1) hipLaunchKernelGGL((k_pool_join<D, E, LISTED>), dim3((unsigned)items, (unsigned)((columns + per - 1) / per)), dim3(256), 0, st, a, L, pc, parts);
+  else hipLaunchKernelGGL((k_pool_merge<D, E, LISTED>), dim3((unsigned)items, (unsigned)columns), dim3(64 * share), 0, st, a, L, pc, parts);
   return hipGetLastError();
 }
 
@@ -1140,13 +1204,13 @@ hipError_t attn_tiles(hipStream_t st, const PoolAttn& a) {
 
 template <int D, class E>
 hipError_t attn_prompt(hipStream_t st, const PoolAttn& a) {
-  constexpr int waves = prompt_waves(D, Terms<E>::n), cols = 32 * waves;
+  constexpr int cols = 16 * prompt_tiles(D, Terms<E>::n) * kShareWaves;
   const int64_t cap = std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0), tiles = (cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
   const int64_t most = compute_units(), want = (items * (tiles + kPromptStart) + kPromptLeast - 1) / kPromptLeast;
   const int workers = (int)std::min(most, want);
   const PoolPieces pc = pool_pieces(a.ws, items, 2 * workers, cols);
-  hipLaunchKernelGGL((k_pool_prompt<D, E>), dim3((unsigned)workers), dim3(64 * waves), 0, st, a, a.row_offsets, a.lengths, a.page_table, pc, workers,
+  hipLaunchKernelGGL((k_pool_prompt<D, E>), dim3((unsigned)workers), dim3(64 * kShareWaves), 0, st, a, a.row_offsets, a.lengths, a.page_table, pc, workers,
                      kPromptLeast);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess ? e : merge<D, E, false>(st, a, pc, items, workers, cols, 0);
@@ -1165,15 +1229,15 @@ hipError_t attn_listed(hipStream_t st, const PoolAttn& a) {
   return e != hipSuccess || c.parts == 1 ? e : merge<D, E, true>(st, a, pc, c.items, c.items * c.parts, 16, c.parts);
 }
 
-bool many_columns(const PoolAttn& a) {
+bool prompts(const PoolAttn& a, int many) {
   const int64_t group = a.n_q / a.c.n_kv;
-  return a.max_rows * group >= kManyColumns && a.rows * group >= (int64_t)kManyColumns * a.batch;
+  return a.max_rows * group >= many && a.rows * group >= (int64_t)many * a.batch;
 }
 
 template <int D, class E>
 hipError_t attn_dim(hipStream_t st, const PoolAttn& a) {
   if (a.blocks) return attn_listed<D, E>(st, a);
-  if (many_columns(a)) return attn_prompt<D, E>(st, a);
+  if (prompts(a, many_columns(D, Terms<E>::n))) return attn_prompt<D, E>(st, a);
   if constexpr (D != 256)
     if ((int64_t)a.max_rows * (a.n_q / a.c.n_kv) > kOneTile) return attn_tiles<D, 2, E>(st, a);
   return attn_tiles<D, 1, E>(st, a);
@@ -1190,7 +1254,7 @@ hipError_t attn_type(hipStream_t st, const PoolAttn& a) {
 
 size_t pool_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows) {
   // a call has at most two pieces a worker, of 32 columns at most; a list's parts are no more than the workers
-  const int64_t prompt = (int64_t)compute_units() * 32 * prompt_waves(hd, 1);
+  const int64_t prompt = (int64_t)compute_units() * 16 * prompt_tiles(hd, 1) * kShareWaves;
   const int64_t columns = 2 * std::max(std::max(most_workers(hd, 1) * 16, most_workers(hd, 2) * 32), prompt) + 64;
   return 256 + align256(sizeof(Begun) * attn_items(n_q, n_kv, batch, rows, 16)) + align256(sizeof(f4) * columns) + sizeof(float) * columns * hd;
 }
