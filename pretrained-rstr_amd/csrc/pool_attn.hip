@@ -893,7 +893,7 @@ __global__ void __launch_bounds__(64 * kShareWaves, kShareWaves / 4)
               for (int x = 0; x < TERMS; x++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t][u][x], acc[t][j], 0, 0, 0);
           }
         uint32_t odd = 0;
-        if (edge)
+        if (edge || tok0 < g_lo_last || tok0 + kStep > g_hi_first)  // also where this wave's own columns see all of the step
 #pragma unroll
           for (int i = 0; i < WAVES; i++) odd |= odd_at[buf][i];
         if (uniform(odd)) {  // values that mend() left out, for the columns that see them

@@ -786,3 +786,139 @@ def test_repeated_calls_are_equal(sess):
             outs.append(torch.empty_like(q))
             plan.run(0, q, offs, table, lens, outs[-1], max_rows=40)
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+# ---- sizes that choose another form ----------------------------------------------------------
+@pytest.mark.parametrize("pages", [700, 1024, 1025, 3001, 4097, 16384, 17003])
+@pytest.mark.parametrize("alike", [False, True])
+def test_select_sizes(sess, pages, alike):
+    """Lists from few blocks to more than a workgroup's registers hold; scores of a few values, so that many are equal."""
+    print("select sizes", pages, alike, flush=True)
+    n_q, n_kv, D, page = 4, 2, 64, 4
+    g = torch.Generator("cuda").manual_seed(pages)
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        b = x.open(hip.BlockBounds, x.pool)
+        lim = torch.as_tensor(b.device(0), device="cuda")
+        z = torch.randn(lim.shape, generator=g, device="cuda")
+        q = torch.randn(2, n_q, D, generator=g, device="cuda")
+        if alike:
+            z = torch.where(torch.arange(D, device="cuda") == 5, z.round(), 0.0)
+            q = q.round()
+        lim.copy_(z)
+        table = np.random.default_rng(pages).permutation(pages)[None]
+        lengths = [pages * page]
+        for top, first, last in ((1, 0, 1), (64, 1, 2), (pages // 2, 1, 1), (pages + 3, 2, 1)):
+            got = _select(x, b, q, table, lengths, [0, 2], top, first, last, n_q, n_kv).cpu().numpy()
+            want = P.select(P.as_f64(q), P.as_f64(lim), table, lengths, [0, 2], page, top, first, last)
+            assert np.array_equal(got, want), (top, np.argwhere(got != want)[:5])
+
+
+@pytest.mark.parametrize("D,n_q,n_kv,page", [(64, 8, 2, 12), (128, 8, 2, 16), (256, 4, 1, 64), (256, 8, 2, 4)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("window", [0, 213])
+def test_attention_of_prompts(sess, D, n_q, n_kv, page, dtype, window):
+    """Prompts whose waves share tiles, for every head size and type: pages that are gone, what is no number behind the lengths and at tokens
+    that some rows of a tile see and others do not."""
+    print("prompts", D, n_q, dtype, window, flush=True)
+    rng = np.random.default_rng(D + n_q)
+    lengths, news, dt = [701, 350, 0, 520], [701, 290, 2, 260], TYPES[dtype]
+    offsets = np.concatenate([[0], np.cumsum(news)])
+    rows = int(offsets[-1])
+    pages = sum(-(-n // page) for n in lengths) + 1
+    table = _table(rng, lengths, page, pages, -(-max(lengths) // page) + 2)
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        k, v = _filled(x, rng, n_kv, D, page, pages)
+        at = lambda b, t: (table[b, t // page], t % page)  # noqa: E731
+        for b, n in enumerate(lengths):
+            for t in range(n, -(-n // page) * page):
+                k[at(b, t)], v[at(b, t)] = float("nan"), float("inf")
+        v[at(0, 650)][0, 5], v[at(1, 200)][n_kv - 1, 7], v[at(3, 400)][0, D - 1] = float("inf"), float("nan"), float("-inf")
+        k[at(1, 120)][0, 3] = float("nan")
+        table[3, 130 // page] = -1
+        x.slab(0).copy_(k)
+        x.slab(1).copy_(v)
+        q = torch.tensor(rng.standard_normal((rows, n_q, D)), dtype=torch.float32).to(dt)
+        out = torch.empty(rows, n_q, D, dtype=dt, device="cuda")
+        _attend(x, q.cuda(), table, lengths, offsets, out, n_q, max_rows=max(news), window=window)
+        sel = np.unique(np.concatenate([rng.integers(0, rows, 40), [0, 1, 63, 64, 649, 650, 651, 700, 701, 840, 841, 990, 991, 993, rows - 1]]))
+        want, mag, size, seen, _ = _some_rows(P.as_f64(q), k, v, table, lengths, offsets, sel, D ** -0.5, window=window)
+        _near(out.cpu()[sel], want, _attn_tol(dt, D, want, mag, size, seen, float(v[v.isfinite()].abs().max()), prompt=True))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,length", [(64, 9001), (3, 20011), (17, 2100)])
+def test_attention_of_many_pieces(sess, dtype, rows, length):
+    """Few rows over a long context: many pieces an item, joined wave by wave and one after the other."""
+    print("pieces", dtype, rows, length, flush=True)
+    rng = np.random.default_rng(rows)
+    n_q, n_kv, D, page, dt = 32, 8, 64, 64, TYPES[dtype]
+    pages = -(-length // page)
+    table = _table(rng, [length], page, pages, pages)
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        k, v = _filled(x, rng, n_kv, D, page, pages)
+        q = torch.tensor(rng.standard_normal((rows, n_q, D)), dtype=torch.float32).to(dt)
+        out = torch.empty(rows, n_q, D, dtype=dt, device="cuda")
+        _attend(x, q.cuda(), table, [length], [0, rows], out, n_q)
+        sel = np.unique([0, 1, rows // 2, rows - 1])
+        want, mag, size, seen, _ = _some_rows(P.as_f64(q), k, v, table, [length], [0, rows], sel, D ** -0.5)
+        _near(out.cpu()[sel], want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=True))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n_q,n_kv,D", [(16, 8, 64), (8, 8, 128), (40, 4, 256)])
+def test_attention_of_blocks_for_many_rows(sess, dtype, n_q, n_kv, D):
+    """Rows enough that a wave takes a row's whole list."""
+    print("blocks of many rows", dtype, n_q, D, flush=True)
+    rng = np.random.default_rng(n_q)
+    page, dt, width = 16, TYPES[dtype], 40
+    news = [600 if n_kv == 4 else 300, 1]
+    lengths = [630, 200]
+    offsets = np.concatenate([[0], np.cumsum(news)])
+    rows = int(offsets[-1])
+    table = _table(rng, lengths, page, 60, width)
+    blocks = rng.integers(-1, width, (rows, n_kv, 9))
+    with Pooled(sess, n_kv, D, page, 60) as x:
+        k, v = _filled(x, rng, n_kv, D, page, 60)
+        q = torch.tensor(rng.standard_normal((rows, n_q, D)), dtype=torch.float32).to(dt)
+        out = torch.empty(rows, n_q, D, dtype=dt, device="cuda")
+        _attend(x, q.cuda(), table, lengths, offsets, out, n_q, blocks=_i32(blocks))
+        sel = np.unique(np.concatenate([rng.integers(0, rows, 20), [0, rows - 2, rows - 1]]))
+        want, mag, size, seen, _ = _some_rows(P.as_f64(q), k, v, table, lengths, offsets, sel, D ** -0.5, blocks=blocks[sel])
+        _near(out.cpu()[sel], want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max())))
+
+
+def test_two_plans_side_by_side(sess):
+    """Two plans and two selections at once on two streams, each with its own workspace, give what they give alone."""
+    rng = np.random.default_rng(4)
+    n_q, n_kv, D, page, pages, rows, top = 32, 8, 128, 16, 700, 24, 20
+    lengths = [9000, 1500]
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        _filled(x, rng, n_kv, D, page, pages)
+        table, lens = _i32(_table(rng, lengths, page, pages, 570)), _i32(lengths)
+        offs = [_i32([0, 23, 24]), _i32([0, 1, 24])]
+        bounds = x.open(hip.BlockBounds, x.pool)
+        bounds.update(0, _i32([0, 9000, 10500]), table, lens, 10500)
+        q = [torch.randn(rows, n_q, D, device="cuda").to(t) for t in (torch.float16, torch.float32)]
+        plans = [x.open(hip.PagedAttention, x.pool, n_q, 2, rows) for _ in range(2)]
+        sels = [x.open(hip.BlockSelect, bounds, n_q, 2, rows, 570) for _ in range(2)]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+
+        def results():
+            return [(torch.empty_like(a), torch.empty_like(a), torch.empty(rows, n_kv, top, dtype=torch.int32, device="cuda")) for a in q]
+
+        def one(i, r, stream):
+            plans[i].run(0, q[i], offs[i], table, lens, r[0], max_rows=23, stream=stream)
+            sels[i].run(0, q[i], offs[i], table, lens, r[2], stream=stream)
+            plans[i].run(0, q[i], offs[i], table, lens, r[1], max_rows=23, blocks=r[2], stream=stream)
+
+        alone = results()
+        for i in range(2):
+            one(i, alone[i], None)
+            torch.cuda.synchronize()
+        for _ in range(3):
+            both = results()
+            torch.cuda.synchronize()
+            for i in range(2):
+                one(i, both[i], streams[i])
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for r, s in zip(alone, both) for a, b in zip(r, s))
