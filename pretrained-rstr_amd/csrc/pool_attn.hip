@@ -47,7 +47,7 @@ __device__ __forceinline__ _Float16 first_term(float x) {
   return (_Float16)__builtin_amdgcn_cvt_pkrtz(x * (1.0f - 0x1p-12f), 0.0f)[0];
 }
 
-constexpr int pool_waves(int hd, int nt) { return hd == 256 ? 1 : 2; }
+constexpr int pool_waves(int hd) { return hd == 256 ? 1 : 2; }
 
 // What raw scores of queries that were brought down by 2^e are multiplied with: finite and not 0, so that it leaves the
 // difference of two equal scores 0 and that of a score and -infinity -infinity.
@@ -97,7 +97,7 @@ __device__ __forceinline__ V load_page(const void* p) {
 // LW > 0: a list of blocks; LW waves of a workgroup share a row's list and join their parts in LDS.
 constexpr int listed_threads(int lw) { return lw > 1 ? 64 * lw : 256; }
 template <int D, int NT, class E, int LW>
-__global__ void __launch_bounds__(listed_threads(LW), pool_waves(D, NT))
+__global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
     k_pool_attn(PoolAttn a, const int32_t* __restrict__ ro, const int32_t* __restrict__ lens, const int32_t* __restrict__ table,
                 PoolPieces pc, int workers, int least, bool whole, int parts) {
   typedef Dims<D> G;
@@ -1125,17 +1125,24 @@ __global__ void __launch_bounds__(256) k_pool_join(PoolAttn a, Lines L, PoolPiec
 
 // ---- launches ------------------------------------------------------------------------
 constexpr int kMergeWaves = 4096;
-constexpr int kWhole = 4;  // tiles of an item that one wave does, without a merge
-constexpr int kLeast = 2;  // tiles a wave takes at least
-constexpr int kPromptLeast = 8;  // and a workgroup of k_pool_prompt
+// Tiles of an item that one wave does, without a merge, and twice as many where items occupy half the card: 4 instead costs 34 us for 28 with
+// 128 sequences of 250 tokens, 1 instead 14.0 for 11.8 with one of 128; 16 always saves 55 -> 47 with 128 of 500, but costs 37 for 25 with 32.
+constexpr int kWhole = 8;
+// Tiles a wave takes at least.  1: 17.0 -> 15.6 us for one sequence of 1000 tokens, but 19.3 -> 23.7 for one of 8000; 4: 14.3 -> 18.2 for 300 tokens.
+constexpr int kLeast = 2;
+// And a workgroup of k_pool_prompt: 8 instead costs 22.8 us for 19.4 with 400 rows of 500 tokens, 16 28.7; all are alike from 2000 tokens on.
+constexpr int kPromptLeast = 4;
 // Columns a sequence from which waves share tiles.  Both sides, in us, of one sequence of 4000 tokens and of eight of 2000: D = 128 f16
 // 25.0 | 26.3 and 39.6 | 38.2 with 32 columns, 31.6 | 26.4 and 46.0 | 41.0 with 64; D = 64 17.2 | 19.4 and 24.4 | 20.9 with 64;
 // D = 256 f16 23.4 | 27.9 and 32.0 | 29.9 with 64, 37.7 | 34.4 with 512; D = 256 fp32 40.9 | 46.8 with 128, 38.3 | 44.7 with 512, and with
 // 3600 at 5000 tokens 307 | 152.
 constexpr int many_columns(int hd, int terms) { return hd < 256 ? 64 : terms == 1 ? 128 : 1024; }
-constexpr int kOneTile = 16;  // columns a sequence up to which items have one tile of columns, above it two
+// 16-bit queries: columns a sequence from which items have two tiles of 16 columns, where tables are long enough.  Two tiles | one, in us, 8 rows
+// of four heads a kv head: 24.4 | 27.0 for one sequence of 4000 tokens, 36.6 | 43.1 for 16 of 1000, but 67.6 | 59.6 for 128 of 300.  In fp32 one tile is
+// never slower (45.9 | 44.0 and 82.3 | 61.5).
+constexpr int kTwoTiles = 17, kTwoTilesFrom = 512;
 
-int64_t most_workers(int hd, int nt) { return (int64_t)compute_units() * 4 * pool_waves(hd, nt); }
+int64_t most_workers(int hd) { return (int64_t)compute_units() * 4 * pool_waves(hd); }
 
 PoolPieces pool_pieces(void* ws, int64_t items, int64_t pieces, int cols) {
   char* p = (char*)ws;
@@ -1156,15 +1163,16 @@ struct Cut {
   int waves, parts, tiles;
 };
 constexpr int listed_waves(int hd) { return hd == 256 ? 4 : 8; }
-// A wave an item where these fill the card, and where a list is short; else a workgroup an item, and where a wave would have more than
-// kListedTiles tiles several.
+// A wave an item where these occupy a quarter of the card, and where a list is short (selection and attention together, 100 rows of 8 kv heads: 114 us with
+// a wave an item, 134 with a workgroup, for lists of 64 blocks of 16 tokens, 55 and 72 for 16; 60 rows alike); else a workgroup an item, and where
+// a wave would have more than kListedTiles tiles several (16 instead of 2: 25 us for 12 + 4 with the join, one row, lists of 128 blocks).
 constexpr int kListedTiles = 2;
 Cut listed_cut(int n_q, int n_kv, int hd, int rows, int64_t tiles) {
   const int group = n_q / n_kv, ncts = (group + 15) / 16;
   Cut c{(int64_t)rows * n_kv * ncts, 1, 1, (int)tiles};
-  if (tiles <= kLeast || c.items >= most_workers(hd, 1)) return c;
+  if (tiles <= kLeast || 4 * c.items >= most_workers(hd)) return c;
   c.waves = listed_waves(hd);
-  const int64_t room = std::max<int64_t>(1, most_workers(hd, 1) / (c.items * c.waves));
+  const int64_t room = std::max<int64_t>(1, most_workers(hd) / (c.items * c.waves));
   const int64_t parts = std::min(room, (tiles + (int64_t)c.waves * kListedTiles - 1) / (c.waves * kListedTiles));
   c.tiles = (int)((tiles + parts * c.waves - 1) / (parts * c.waves));
   c.parts = (int)((tiles + (int64_t)c.tiles * c.waves - 1) / ((int64_t)c.tiles * c.waves));
@@ -1192,8 +1200,9 @@ hipError_t attn_tiles(hipStream_t st, const PoolAttn& a) {
   const int cols = 16 * NT;
   const int64_t cap = std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0), tiles = (cap + kTile - 1) / kTile;
   const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
-  const bool whole = tiles <= kWhole;
-  const int64_t most = most_workers(D, NT), want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
+  const int64_t most = most_workers(D);
+  const bool whole = tiles <= kWhole || (tiles <= 2 * kWhole && 2 * items >= most);
+  const int64_t want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
   const int64_t workers = whole ? (items + 3) / 4 * 4 : (std::min(most, want) + 3) / 4 * 4;
   const PoolPieces pc = pool_pieces(a.ws, items, 2 * workers, cols);
   hipLaunchKernelGGL((k_pool_attn<D, NT, E, 0>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths, a.page_table,
@@ -1238,8 +1247,8 @@ template <int D, class E>
 hipError_t attn_dim(hipStream_t st, const PoolAttn& a) {
   if (a.blocks) return attn_listed<D, E>(st, a);
   if (prompts(a, many_columns(D, Terms<E>::n))) return attn_prompt<D, E>(st, a);
-  if constexpr (D != 256)
-    if ((int64_t)a.max_rows * (a.n_q / a.c.n_kv) > kOneTile) return attn_tiles<D, 2, E>(st, a);
+  if constexpr (D != 256 && Terms<E>::n == 1)
+    if ((int64_t)a.max_rows * (a.n_q / a.c.n_kv) >= kTwoTiles && (int64_t)a.pps * a.c.page_size > kTwoTilesFrom) return attn_tiles<D, 2, E>(st, a);
   return attn_tiles<D, 1, E>(st, a);
 }
 
@@ -1255,7 +1264,7 @@ hipError_t attn_type(hipStream_t st, const PoolAttn& a) {
 size_t pool_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows) {
   // a call has at most two pieces a worker, of 32 columns at most; a list's parts are no more than the workers
   const int64_t prompt = (int64_t)compute_units() * 16 * prompt_tiles(hd, 1) * kShareWaves;
-  const int64_t columns = 2 * std::max(std::max(most_workers(hd, 1) * 16, most_workers(hd, 2) * 32), prompt) + 64;
+  const int64_t columns = 2 * std::max(most_workers(hd) * 32, prompt) + 64;
   return 256 + align256(sizeof(Begun) * attn_items(n_q, n_kv, batch, rows, 16)) + align256(sizeof(f4) * columns) + sizeof(float) * columns * hd;
 }
 
