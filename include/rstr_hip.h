@@ -553,7 +553,7 @@ int rstr_bounds_update(rstr_bounds* b, int32_t layer, int32_t batch, int32_t row
                        const int32_t* page_table, int32_t pages_per_seq, const int32_t* lengths, void* stream);
 
 /* Workspace for selections of up to max_batch sequences and max_rows query rows of n_q heads over page tables of up
- * to max_pages.  max_rows * n_kv < 2^24, and times the 64s of max_pages < 2^26.  One call at a time, as with attention plans. */
+ * to max_pages.  max_rows * n_kv < 2^24, and times the 32s of max_pages < 2^26.  One call at a time, as with attention plans. */
 int rstr_select_open(rstr_bounds* b, int32_t n_q, int32_t max_batch, int32_t max_rows, int32_t max_pages, rstr_select** out);
 /* Waits for the device. */
 int rstr_select_close(rstr_select* a);

@@ -141,9 +141,11 @@ template <int D, class E>
 hipError_t rope_dim(hipStream_t st, const RopeAppend& a) {
   const int size = sizeof(typename E::T);
   const bool vec = vec_rows(a.k, size) && vec_rows(a.v, size) && (a.n_q == 0 || (vec_rows(a.q, size) && vec_rows(a.q_out, size)));
-  const bool few = a.rows < 2048;
-  const unsigned grid = (unsigned)(few ? a.rows : (a.rows + 3) / 4);
-  auto f = few ? (vec ? k_rope_append<D, 1, E, true> : k_rope_append<D, 1, E, false>)
+  // One row a workgroup where its heads fill it (8000 rows of 48 heads of 128, fp32: 70 us, four rows a workgroup 76) or rows are few; where
+  // heads are few four (8000 rows of 12 heads of 64: 10.0 us, one row 14.2).
+  const bool one = a.rows < 2048 || (int64_t)(a.n_q + 2 * a.c.n_kv) * D / 16 >= 256;
+  const unsigned grid = (unsigned)(one ? a.rows : (a.rows + 3) / 4);
+  auto f = one ? (vec ? k_rope_append<D, 1, E, true> : k_rope_append<D, 1, E, false>)
                : (vec ? k_rope_append<D, 4, E, true> : k_rope_append<D, 4, E, false>);
   hipLaunchKernelGGL(f, dim3(grid), dim3(256), 0, st, a);
   return hipGetLastError();
@@ -269,11 +271,11 @@ __device__ double odd_score(const typename E::T* q, int64_t head, int group, con
   return 2.0 * best;
 }
 
-// A wave scores `per` blocks, up to 64, for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers
+// A wave scores kScoreBlocks blocks for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers
 // twice the larger of q lo and q hi is q (lo + hi) + |q| |hi - lo|, so a bound is converted once for all heads, and a product costs
 // two multiply-adds; where a sum is not finite the block is scored by the definition.
 template <int D, int HG, class E>
-__global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks, int per) {
+__global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks) {
   typedef typename E::T T;
   constexpr int CH = D / 8, PER = 64 / CH, AHEAD = 4;  // lanes of a block, blocks at a time, steps in flight
   const int lane = threadIdx.x & 63, c = lane % CH;
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* 
   const RowOf of(a.row_offsets, a.lengths, a.batch, a.rows, row);
   if (of.b < 0 || of.p < 0) return;
   const Choice ch(a, of.p);
-  const int j0 = chunk * per, n = min(per, ch.n - j0);
+  const int j0 = chunk * kScoreBlocks, n = min(kScoreBlocks, ch.n - j0);
   if (n <= 0) return;
   double* out = scores + rh * a.ws_blocks + j0;
   const int page = lane < n ? a.page_table[(int64_t)of.b * a.pps + ch.lo + j0 + lane] : -1;
@@ -610,17 +612,17 @@ hipError_t select_dim(hipStream_t st, const BlockSelect& a) {
   double* scores = (double*)a.ws;
   const int group = a.n_q / a.n_kv;
   const int64_t rh = (int64_t)a.rows * a.n_kv;
-  // 64 blocks a wave where that leaves the card full, else 32
-  const int per = rh * ((a.pps + 63) / 64) >= 16 * (int64_t)compute_units() ? 64 : kScoreBlocks;
-  const int chunks = (a.pps + per - 1) / per;
+  const int chunks = (a.pps + kScoreBlocks - 1) / kScoreBlocks;
   const int64_t units = rh * chunks;
   if (a.pps > a.top) {
     auto f = group == 1 ? k_block_scores<D, 1, E> : group == 2 ? k_block_scores<D, 2, E> : k_block_scores<D, 4, E>;
-    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, chunks, per);
+    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, chunks);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   const dim3 grid((unsigned)rh);
+  // The fewest threads and registers that hold the blocks: 1024 threads for tables of up to 1024 blocks 98 us for 90 (128 rows of 8 kv heads, the
+  // selection with its attention), 16 blocks a thread for up to 4096 75 for 67 (8 rows of 3750 blocks).
   if (a.pps <= 256 * 4) hipLaunchKernelGGL((k_block_pick<256, 4>), grid, dim3(256), 0, st, a, scores);
   else if (a.pps <= 1024 * 4) hipLaunchKernelGGL((k_block_pick<1024, 4>), grid, dim3(1024), 0, st, a, scores);
   else if (a.pps <= 1024 * 16) hipLaunchKernelGGL((k_block_pick<1024, 16>), grid, dim3(1024), 0, st, a, scores);
