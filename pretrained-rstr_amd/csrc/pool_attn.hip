@@ -33,6 +33,10 @@ namespace {
 // lanes and the rescaling of O are rare; p is below 2^14, and the factor 2^10 keeps small weights' bits: fp16's
 // subnormals begin 2^24 below the largest.  p is one fp16 term (f16, bf16) or two (fp32).  S, m, l and O are fp32.
 //
+// Memory bounds it: 128 sequences of 128 to 4608 tokens, 32 heads over 8 of 128, f16, read 1.24 GB in 219 us (5.7 TB/s), four of 9000 to
+// 131 000 733 MB in 132 (5.5), 33 of 5 to 8192 with 1 to 6 fp32 rows 556 MB in 111 (5.0).  Two waves a SIMD, each with the next tile's K and V in
+// registers: three waves spill (335, 200 and 193 us); loads that bypass the caches' order are worth 234 -> 220 in the first.
+//
 // The tiles of all (sequence, kv head, column tile) items form one line of units that is cut into equal parts, one
 // a wave, as in kv4_line.h; with a list of blocks every row and kv head is an item, and all have as many parts.
 constexpr int kStart = 4;  // what beginning an item costs, in tiles
@@ -572,6 +576,11 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
 // transposing reads of four tokens x 16 dims.  A row of a token is swizzled in LDS by its number, 16 bytes at a time, so that 16 tokens' same
 // dims lie in different banks; the loads into LDS write 1 KB in the lanes' order, so a lane asks for the piece that
 // belongs to its place.
+// 333 and 1000 rows at 333 and 9000 tokens, 32 heads over 8 of 128, bf16: 250 us, 560 TFLOP/s (four-row waves that load for themselves: 383).  No
+// one part of a step bounds it: without its exponentials it takes 219 us, without either product 204 and 214, without its loads 219;
+// matrix instructions are busy 22 % of the time, vector instructions 48 %, and the two waves that a SIMD has registers for wait for LDS and for
+// each other's step the rest.  A third buffer (256), the two halves of a workgroup half a step apart (293, 270), all operands read ahead
+// (283) and two workgroups of four waves (283) gain nothing.
 constexpr int kPromptStart = 8;  // what beginning an item costs, in tiles
 constexpr int kStep = 64;        // tokens at a time
 constexpr int kShareWaves = 8;  // two a SIMD, with half its registers each
@@ -1018,54 +1027,57 @@ struct Joined {
   }
 };
 
-// Joins the pieces of an item, in their order: a workgroup a column, its waves by piece.
+// Joins the pieces of an item, in their order: a workgroup a column (more where a sequence has more rows than the call said), its waves by piece.
 template <int D, class E, bool LISTED>
 __global__ void k_pool_merge(PoolAttn a, Lines L, PoolPieces pc, int parts) {
   constexpr int V = D / 64;  // dims a lane
   typedef typename E::T T;
   __shared__ float part[16][D];
   __shared__ float pl[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = blockDim.x >> 6, c = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = blockDim.x >> 6;
   Joined<LISTED> it;
-  if (!it.find(a, L, pc, blockIdx.x, parts) || (it.c0 + c) / L.group >= it.m) return;
-  float acc[V] = {}, l = 0.0f, top = -FLT_MAX;
-  for (int i = lane; i < it.n; i += 64) {
-    const f4 y = pc.ml[it.slot(L, i, c)];
-    if (y[1] != 0.0f) top = fmaxf(top, y[0]);
-  }
-  top = wave_max(top);
-  for (int i0 = wave; i0 < it.n; i0 += 8 * share) {
-    f4 x[8];
-    float v[8][V];
-#pragma unroll
-    for (int k = 0; k < 8; k++) {  // all loads before the first use
-      const int64_t p = it.slot(L, min(i0 + k * share, it.n - 1), c);
-      x[k] = pc.ml[p];
-#pragma unroll
-      for (int j = 0; j < V; j++) v[k][j] = pc.acc[p * D + lane * V + j];
+  if (!it.find(a, L, pc, blockIdx.x, parts)) return;
+  for (int c = blockIdx.y; c < L.cols && (it.c0 + c) / L.group < it.m; c += gridDim.y) {  // the same for all waves
+    float acc[V] = {}, l = 0.0f, top = -FLT_MAX;
+    for (int i = lane; i < it.n; i += 64) {
+      const f4 y = pc.ml[it.slot(L, i, c)];
+      if (y[1] != 0.0f) top = fmaxf(top, y[0]);
     }
+    top = wave_max(top);
+    for (int i0 = wave; i0 < it.n; i0 += 8 * share) {
+      f4 x[8];
+      float v[8][V];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const bool some = i0 + k * share < it.n && x[k][1] != 0.0f;
-      const float f = some ? __builtin_amdgcn_exp2f((x[k][0] - top) * x[k][2]) : 0.0f;
-      l = __builtin_fmaf(f, some ? x[k][1] : 0.0f, l);
+      for (int k = 0; k < 8; k++) {  // all loads before the first use
+        const int64_t p = it.slot(L, min(i0 + k * share, it.n - 1), c);
+        x[k] = pc.ml[p];
 #pragma unroll
-      for (int j = 0; j < V; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
+        for (int j = 0; j < V; j++) v[k][j] = pc.acc[p * D + lane * V + j];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const bool some = i0 + k * share < it.n && x[k][1] != 0.0f;
+        const float f = some ? __builtin_amdgcn_exp2f((x[k][0] - top) * x[k][2]) : 0.0f;
+        l = __builtin_fmaf(f, some ? x[k][1] : 0.0f, l);
+#pragma unroll
+        for (int j = 0; j < V; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
+      }
     }
+    __syncthreads();  // the column before has been read
+#pragma unroll
+    for (int j = 0; j < V; j++) part[wave][lane * V + j] = acc[j];
+    if (lane == 0) pl[wave] = l;
+    __syncthreads();
+    if (wave != 0) continue;
+    for (int k = 1; k < share; k++) {
+#pragma unroll
+      for (int j = 0; j < V; j++) acc[j] += part[k][lane * V + j];
+      l += pl[k];
+    }
+    T* dst = (T*)a.out.p + it.out_at(a, L, c) + lane * V;
+#pragma unroll
+    for (int j = 0; j < V; j++) dst[j] = E::put(l == 0.0f ? 0.0f : acc[j] / l);
   }
-#pragma unroll
-  for (int j = 0; j < V; j++) part[wave][lane * V + j] = acc[j];
-  if (lane == 0) pl[wave] = l;
-  __syncthreads();
-  if (wave != 0) return;
-  for (int k = 1; k < share; k++) {
-#pragma unroll
-    for (int j = 0; j < V; j++) acc[j] += part[k][lane * V + j];
-    l += pl[k];
-  }
-  T* dst = (T*)a.out.p + it.out_at(a, L, c) + lane * V;
-#pragma unroll
-  for (int j = 0; j < V; j++) dst[j] = E::put(l == 0.0f ? 0.0f : acc[j] / l);
 }
 
 // The same where items have few pieces or there are columns enough: D / 4 lanes a column, four dims each, pieces one after the other.
@@ -1077,49 +1089,51 @@ __global__ void __launch_bounds__(256) k_pool_join(PoolAttn a, Lines L, PoolPiec
   typedef typename E::T T;
   Joined<LISTED> it;
   if (!it.find(a, L, pc, blockIdx.x, parts)) return;
-  const int c = blockIdx.y * PER + threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
-  if (c >= L.cols || (it.c0 + c) / L.group >= it.m) return;
-  f4 acc = f4{0, 0, 0, 0};
-  float l = 0.0f, top = -FLT_MAX;
-  for (int i0 = 0; i0 < it.n; i0 += AT_ONCE) {
-    f4 x[AT_ONCE], v[AT_ONCE];
+  const int d = threadIdx.x % LANES * 4;
+  const bool ovec = vec_rows(a.out, sizeof(T));
+  for (int c = blockIdx.y * PER + threadIdx.x / LANES; c < L.cols && (it.c0 + c) / L.group < it.m; c += gridDim.y * PER) {
+    f4 acc = f4{0, 0, 0, 0};
+    float l = 0.0f, top = -FLT_MAX;
+    for (int i0 = 0; i0 < it.n; i0 += AT_ONCE) {
+      f4 x[AT_ONCE], v[AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; k++) {
-      x[k] = v[k] = f4{0, 0, 0, 0};
-      if (i0 + k < it.n) {
-        const int64_t p = it.slot(L, i0 + k, c);
-        x[k] = pc.ml[p];
-        v[k] = *(const f4*)(pc.acc + p * D + d);
+      for (int k = 0; k < AT_ONCE; k++) {
+        x[k] = v[k] = f4{0, 0, 0, 0};
+        if (i0 + k < it.n) {
+          const int64_t p = it.slot(L, i0 + k, c);
+          x[k] = pc.ml[p];
+          v[k] = *(const f4*)(pc.acc + p * D + d);
+        }
+      }
+      float now = top, scale = 0.0f;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; k++)
+        if (x[k][1] != 0.0f) now = fmaxf(now, x[k][0]), scale = x[k][2];  // (a column's scale is the same in all)
+      const float keep = __builtin_amdgcn_exp2f((top - now) * scale);
+      top = now;
+      l *= keep;
+      acc *= keep;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; k++) {
+        const bool some = x[k][1] != 0.0f;
+        const float f = some ? __builtin_amdgcn_exp2f((x[k][0] - top) * x[k][2]) : 0.0f;
+        l = __builtin_fmaf(f, some ? x[k][1] : 0.0f, l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
       }
     }
-    float now = top, scale = 0.0f;
+    T* dst = (T*)a.out.p + it.out_at(a, L, c) + d;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T o[4];
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; k++)
-      if (x[k][1] != 0.0f) now = fmaxf(now, x[k][0]), scale = x[k][2];  // (a column's scale is the same in all)
-    const float keep = __builtin_amdgcn_exp2f((top - now) * scale);
-    top = now;
-    l *= keep;
-    acc *= keep;
+    for (int j = 0; j < 4; j++) o[j] = E::put(acc[j] * inv);
+    if (ovec) {
+      if constexpr (sizeof(T) == 4) *(u32x4*)dst = *(u32x4*)o;
+      else *(u32x2*)dst = *(u32x2*)o;
+    } else {
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; k++) {
-      const bool some = x[k][1] != 0.0f;
-      const float f = some ? __builtin_amdgcn_exp2f((x[k][0] - top) * x[k][2]) : 0.0f;
-      l = __builtin_fmaf(f, some ? x[k][1] : 0.0f, l);
-#pragma unroll
-      for (int j = 0; j < 4; j++) acc[j] = __builtin_fmaf(f, some ? v[k][j] : 0.0f, acc[j]);
+      for (int j = 0; j < 4; j++) dst[j] = o[j];
     }
-  }
-  T* dst = (T*)a.out.p + it.out_at(a, L, c) + d;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T o[4];
-#pragma unroll
-  for (int j = 0; j < 4; j++) o[j] = E::put(acc[j] * inv);
-  if (vec_rows(a.out, sizeof(T))) {
-    if constexpr (sizeof(T) == 4) *(u32x4*)dst = *(u32x4*)o;
-    else *(u32x2*)dst = *(u32x2*)o;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; j++) dst[j] = o[j];
   }
 }
 

@@ -59,13 +59,11 @@ bool in_pages(const PoolLayer& c, const Rows& r, int64_t rows, int64_t heads, in
 constexpr int kMostHeads = 1 << 16;
 
 // What the attention, the bounds and the selection take alike: the sequences of a call.
-int sequences_args(rstr_session* s, int32_t batch, int32_t rows, const int32_t* row_offsets, const int32_t* page_table, int32_t pages_per_seq,
-                   const int32_t* lengths) {
+int sequences_args(rstr_session* s, const int32_t* row_offsets, const int32_t* page_table, int32_t pages_per_seq, const int32_t* lengths) {
   if (pages_per_seq <= 0) return fail(s, RSTR_E_INVALID, "page table width must be positive");
   TRY(check_ints(s, "row offsets", row_offsets));
   TRY(check_ints(s, "page table", page_table));
   TRY(check_ints(s, "lengths", lengths));
-  (void)batch, (void)rows;
   return RSTR_OK;
 }
 
@@ -196,7 +194,7 @@ extern "C" int rstr_pool_attn_run(rstr_pool_attn* a, int32_t layer, int32_t dtyp
   if (!std::isfinite(scale)) return fail(s, RSTR_E_INVALID, "scale must be finite");
   if (batch == 0 || rows == 0) return RSTR_OK;
   if (max_rows <= 0 || max_rows > rows) return fail(s, RSTR_E_INVALID, "rows per sequence must lie between 1 and the rows");
-  TRY(sequences_args(s, batch, rows, row_offsets, page_table, pages_per_seq, lengths));
+  TRY(sequences_args(s, row_offsets, page_table, pages_per_seq, lengths));
   const Rows qr{(void*)q, q_row, q_head}, o{out, out_row, out_head};
   TRY(check_rows(s, "query", qr, size));
   TRY(check_rows(s, "output", o, size));
@@ -298,7 +296,7 @@ extern "C" int rstr_bounds_update(rstr_bounds* b, int32_t layer, int32_t batch, 
   if (batch < 0 || rows < 0) return fail(s, RSTR_E_INVALID, "batch and row counts must not be negative");
   if ((int64_t)rows * v.c.n_kv >= 4 * kGridGroups) return fail(s, RSTR_E_INVALID, "too many rows for one call");
   if (batch == 0 || rows == 0) return RSTR_OK;
-  TRY(sequences_args(s, batch, rows, row_offsets, page_table, pages_per_seq, lengths));
+  TRY(sequences_args(s, row_offsets, page_table, pages_per_seq, lengths));
   BoundsUpdate a{pool_view(b->p, layer).c, b->base + layer * b->layer_elems, batch, rows, pages_per_seq, row_offsets, page_table, lengths};
   OnDevice dev(s->device);
   HIPCHK(s, dev.e);
@@ -322,7 +320,7 @@ extern "C" int rstr_select_open(rstr_bounds* b, int32_t n_q, int32_t max_batch, 
   if (!a) return fail(s, RSTR_E_OOM, "selection handle");
   OnDevice dev(s->device);
   HIPCHK(s, dev.e);
-  if (device_alloc(&a->ws, select_workspace(n_q, v.c.n_kv, v.c.hd, max_rows, max_pages)) != hipSuccess) {
+  if (device_alloc(&a->ws, select_workspace(v.c.n_kv, max_rows, max_pages)) != hipSuccess) {
     (void)hipGetLastError();
     return fail(s, RSTR_E_OOM, "selection workspace allocation failed");
   }
@@ -362,7 +360,7 @@ extern "C" int rstr_select_run(rstr_select* a, int32_t layer, int32_t dtype, int
     return fail(s, RSTR_E_INVALID, "the first blocks and the last, one at least, must fit in the list");
   if (batch == 0 || rows == 0) return RSTR_OK;
   if (pages_per_seq > a->blocks) return fail(s, RSTR_E_INVALID, "page table is wider than the selection's");
-  TRY(sequences_args(s, batch, rows, row_offsets, page_table, pages_per_seq, lengths));
+  TRY(sequences_args(s, row_offsets, page_table, pages_per_seq, lengths));
   const Rows qr{(void*)q, q_row, q_head};
   TRY(check_rows(s, "query", qr, size));
   TRY(check_ints(s, "blocks", blocks));
@@ -370,6 +368,7 @@ extern "C" int rstr_select_run(rstr_select* a, int32_t layer, int32_t dtype, int
   const struct { const void* p; size_t n; } in[] = {{row_offsets, (size_t)batch * 4 + 4}, {page_table, (size_t)batch * pages_per_seq * 4}, {lengths, (size_t)batch * 4}};
   for (const auto& x : in)
     if (ranges_meet(x.p, x.n, blocks, n)) return fail(s, RSTR_E_INVALID, "blocks overlap the sequences' tables");
+  if (ranges_meet(a->b->base, (size_t)a->b->layer_elems * 2 * v.layers, blocks, n)) return fail(s, RSTR_E_INVALID, "blocks overlap the bounds");
   if (ints_meet(blocks, (int64_t)n, qr, rows, a->n_q, v.c.hd, size)) return fail(s, RSTR_E_INVALID, "blocks overlap the queries");
   BlockSelect k{a->b->base + layer * a->b->layer_elems, v.c.n_kv, v.c.hd, v.c.page_size, v.c.pages, a->n_q, batch, rows, pages_per_seq,
                 blocks_per_row, first, last, qr, row_offsets, page_table, lengths, blocks, a->ws,

@@ -84,7 +84,7 @@ constexpr int kScoreBlocks = 32;  // blocks that a wave scores (64 where these f
 inline bool select_fits(int n_kv, int rows, int blocks) {  // grids hold it
   return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * ((blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26);
 }
-size_t select_workspace(int n_q, int n_kv, int hd, int rows, int blocks);
+size_t select_workspace(int n_kv, int rows, int blocks);
 hipError_t launch_block_select(hipStream_t st, int dtype, const BlockSelect& a);
 
 }  // namespace rstr

@@ -7,7 +7,9 @@ reference raises ``ex-info``.  No computation happens here; every call goes to
 the HIP library, and loading fails loudly if the library is missing.
 
 The operators on device arrays (:class:`Kv4Pool`, :class:`Kv4Attention`,
-:class:`Verifier`, :meth:`Session.step_maps`) take arrays that live on the
+:class:`Verifier`, :meth:`Session.step_maps`, and over the fp16 pages of a pool
+:meth:`Pool.rope_append`, :class:`PagedAttention`, :class:`BlockBounds` and
+:class:`BlockSelect`) take arrays that live on the
 session's GPU: torch tensors, or anything with their ``data_ptr()``, ``shape``,
 ``stride()``, ``dtype`` and ``device``.  They queue work and return.  A program
 that uses torch imports it before this library is loaded, so that both share

@@ -29,7 +29,7 @@ hipError_t rstr::launch_rope_append(hipStream_t st, int, const RopeAppend&) { re
 size_t rstr::pool_attn_workspace(int, int, int, int, int) { return 64; }
 hipError_t rstr::launch_pool_attn(hipStream_t st, int, const PoolAttn&) { return launched(st); }
 hipError_t rstr::launch_bounds_update(hipStream_t st, const BoundsUpdate&) { return launched(st); }
-size_t rstr::select_workspace(int, int, int, int, int) { return 64; }
+size_t rstr::select_workspace(int, int, int) { return 64; }
 hipError_t rstr::launch_block_select(hipStream_t st, int, const BlockSelect&) { return launched(st); }
 
 extern "C" {

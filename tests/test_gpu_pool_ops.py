@@ -922,3 +922,22 @@ def test_two_plans_side_by_side(sess):
                 one(i, both[i], streams[i])
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for r, s in zip(alone, both) for a, b in zip(r, s))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n_q,n_kv,D,rows,said", [(32, 8, 64, 40, 1), (8, 2, 128, 90, 3), (8, 2, 256, 300, 20), (16, 1, 128, 3, 1)])
+def test_attention_of_more_rows_than_said(sess, dtype, n_q, n_kv, D, rows, said):
+    """max_rows chooses the form only: sequences with more rows are computed whole."""
+    print("more rows than said", dtype, n_q, D, rows, said, flush=True)
+    rng = np.random.default_rng(rows)
+    page, dt, lengths, offsets = 64, TYPES[dtype], [5000, 800], [0, rows, 2 * rows]
+    pages = 79 + 13
+    table = _table(rng, lengths, page, pages, 80)
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        k, v = _filled(x, rng, n_kv, D, page, pages)
+        q = torch.tensor(rng.standard_normal((2 * rows, n_q, D)), dtype=torch.float32).to(dt)
+        out = torch.full((2 * rows, n_q, D), 7.0, dtype=dt, device="cuda")
+        _attend(x, q.cuda(), table, lengths, offsets, out, n_q, max_rows=said)
+        sel = np.unique([0, 1, 2, rows // 2, rows - 2, rows - 1, rows, rows + 1, 2 * rows - 1])
+        want, mag, size, seen, _ = _some_rows(P.as_f64(q), k, v, table, lengths, offsets, sel, D ** -0.5)
+        _near(out.cpu()[sel], want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=True))

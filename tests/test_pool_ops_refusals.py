@@ -268,6 +268,9 @@ def test_bounds_and_selection(dev):
         for name, a in (("ro", ints(3)), ("pt", ints((2, 7))), ("ln", ints(2))):
             refused(dev, hip.RstrError, "overlap the sequences' tables", lambda: run(blocks=x, **{name: inside(a, x, 4 * 29)}))
             run(blocks=x, **{name: inside(a, x, 4 * 30)})
+        x = ints((5, 2, 3))
+        x.data_ptr = lambda at=b.device(1).data_ptr(): at + 64  # of another layer
+        refused(dev, hip.RstrError, "overlap the bounds", lambda: run(blocks=x))
         q = Dev((5, 4, 128))
         refused(dev, hip.RstrError, "overlap the queries", lambda: run(q=q, blocks=inside(ints((5, 2, 3)), q, 4 * (5 * 4 * 128 - 1))))
         n = dev.fake_launches()
