@@ -80,7 +80,7 @@ struct BlockSelect {
   int ws_blocks;  // scores a row and kv head in the workspace
 };
 inline int select_stride(int blocks) { return (blocks + 15) / 16 * 16; }  // ws_blocks for tables of that many pages
-constexpr int kScoreBlocks = 32;  // blocks that a wave scores (64 where these fill the card: 81 us for 79, selection and attention of 32 sequences of 16000 tokens)
+constexpr int kScoreBlocks = 32;  // blocks that a wave scores, at least
 inline bool select_fits(int n_kv, int rows, int blocks) {  // grids hold it
   return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * ((blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26);
 }

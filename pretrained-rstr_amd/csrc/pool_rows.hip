@@ -66,8 +66,8 @@ __device__ __forceinline__ double group_sum(double v) {
 }
 
 // A thread takes 16 elements of a head: eight pairs that turn (or 16 that do not), a workgroup R rows, whose
-// angles it works out once for all heads.  Memory bounds it where rows are many: 16 411 rows of 48 heads of 128, bf16, 403 MB in 81 us (5.0 TB/s;
-// a copy reaches 4.96); below some 1000 rows it is one launch and one chain of waits (4.1 to 4.6 us).
+// angles it works out once for all heads.  Memory bounds it where rows are many: 16 411 rows of 48 heads of 128, bf16, 403 MB in 74 us (5.4 TB/s;
+// a copy of 2 GiB reaches 5.0); below some 1000 rows it is one launch and one chain of waits (4.1 to 4.6 us).
 template <int D, int R, class E, bool VEC>
 __global__ void __launch_bounds__(256) k_rope_append(RopeAppend a) {
   typedef typename E::T T;
@@ -273,13 +273,13 @@ __device__ double odd_score(const typename E::T* q, int64_t head, int group, con
   return 2.0 * best;
 }
 
-// A wave scores kScoreBlocks blocks for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers
+// A wave scores `per` blocks for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers
 // twice the larger of q lo and q hi is q (lo + hi) + |q| |hi - lo|, so a bound is converted once for all heads, and a product costs
 // two multiply-adds; where a sum is not finite the block is scored by the definition.  Four steps' bounds are in flight.  32 sequences of 2048 to
 // 16 384 tokens in pages of 16, 32 heads over 8 of 128, f16: 76 MB of bounds in 30 us, twice what reading them takes; by count half of that are conversions
 // and multiply-adds in 64 bits, which make the choice exact.  One sequence of 131 071: 34 MB in 13.8.
 template <int D, int HG, class E>
-__global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks) {
+__global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks, int per) {
   typedef typename E::T T;
   constexpr int CH = D / 8, PER = 64 / CH, AHEAD = 4;  // lanes of a block, blocks at a time, steps in flight
   const int lane = threadIdx.x & 63, c = lane % CH;
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* 
   const RowOf of(a.row_offsets, a.lengths, a.batch, a.rows, row);
   if (of.b < 0 || of.p < 0) return;
   const Choice ch(a, of.p);
-  const int j0 = chunk * kScoreBlocks, n = min(kScoreBlocks, ch.n - j0);
+  const int j0 = chunk * per, n = min(per, ch.n - j0);
   if (n <= 0) return;
   double* out = scores + rh * a.ws_blocks + j0;
   const int page = lane < n ? a.page_table[(int64_t)of.b * a.pps + ch.lo + j0 + lane] : -1;
@@ -617,11 +617,14 @@ hipError_t select_dim(hipStream_t st, const BlockSelect& a) {
   double* scores = (double*)a.ws;
   const int group = a.n_q / a.n_kv;
   const int64_t rh = (int64_t)a.rows * a.n_kv;
-  const int chunks = (a.pps + kScoreBlocks - 1) / kScoreBlocks;
+  // Twice as many blocks a wave where these waves fill the card (32 sequences of up to 1024 blocks: 30.3 us for 33.2; with one sequence, always
+  // twice as many: 27 -> 32 us for the selection and its attention).
+  const int per = rh * ((a.pps + 2 * kScoreBlocks - 1) / (2 * kScoreBlocks)) >= 16 * (int64_t)compute_units() ? 2 * kScoreBlocks : kScoreBlocks;
+  const int chunks = (a.pps + per - 1) / per;
   const int64_t units = rh * chunks;
   if (a.pps > a.top) {
     auto f = group == 1 ? k_block_scores<D, 1, E> : group == 2 ? k_block_scores<D, 2, E> : k_block_scores<D, 4, E>;
-    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, chunks);
+    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, chunks, per);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

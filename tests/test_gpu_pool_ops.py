@@ -941,3 +941,31 @@ def test_attention_of_more_rows_than_said(sess, dtype, n_q, n_kv, D, rows, said)
         sel = np.unique([0, 1, 2, rows // 2, rows - 2, rows - 1, rows, rows + 1, 2 * rows - 1])
         want, mag, size, seen, _ = _some_rows(P.as_f64(q), k, v, table, lengths, offsets, sel, D ** -0.5)
         _near(out.cpu()[sel], want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=True))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page", [4, 20, 100, 256, 1024])
+def test_attention_of_any_page_size(sess, dtype, D, page):
+    """Pages that are smaller and larger than what is read at a time, in every form; a query that is no number reaches its own row only."""
+    print("pages of", page, dtype, D, flush=True)
+    rng = np.random.default_rng(page + D)
+    n_q, n_kv, dt = 4, 1, TYPES[dtype]
+    lengths, news = [1500, 290], [280, 1]
+    offsets = np.concatenate([[0], np.cumsum(news)])
+    rows = int(offsets[-1])
+    pages = sum(-(-n // page) for n in lengths)
+    width = -(-1500 // page)
+    table = _table(rng, lengths, page, pages, width)
+    blocks = rng.integers(0, width, (rows, n_kv, 3))
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        k, v = _filled(x, rng, n_kv, D, page, pages)
+        q = torch.tensor(rng.standard_normal((rows, n_q, D)), dtype=torch.float32).to(dt)
+        q[17, 2, 5] = float("nan")
+        sel = np.unique(np.concatenate([rng.integers(0, rows, 8), [0, 16, 17, 18, 64, rows - 2, rows - 1]]))
+        for kw in (dict(max_rows=280), dict(max_rows=1), dict(max_rows=5, window=300), dict(max_rows=280, window=70), dict(blocks=blocks)):
+            out = torch.empty(rows, n_q, D, dtype=dt, device="cuda")
+            _attend(x, q.cuda(), table, lengths, offsets, out, n_q, **{**kw, **({"blocks": _i32(blocks)} if "blocks" in kw else {})})
+            plain = {n: (blocks[sel] if n == "blocks" else w) for n, w in kw.items() if n != "max_rows"}
+            want, mag, size, seen, _ = _some_rows(P.as_f64(q), k, v, table, lengths, offsets, sel, D ** -0.5, **plain)
+            _near(out.cpu()[sel], want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=True))
