@@ -23,6 +23,9 @@ the tokens it sees:
   step there, 2^-25, where the largest weight is at least 2^6 (the reference lags by 2^4 at most: 2^10 / 2^4): N * 2^-31 * max|v|.
   fp32: two terms as above, 1.25 * 2^-21 W, and N * 2^-31 * 2^-11 max|v|;
 - the sums over tokens: 32 terms and N / 32 products, and up to 64 pieces: (32 + N / 32 + 64) * 2^-23 W, the sum of the weights likewise;
+  with more pieces than 64, p of them, a chain has N / (32 p) products and p pieces of two products at least, which is no more than N / 32 + 64
+  either, and where a join scales what it has as it goes, one exponential (2^-22) for four pieces, eight products at least, of whose terms a chain
+  over p pieces leaves that many unused;
 - the quotient: 2 * 2^-24 W; the output's own rounding.
 """
 import numpy as np
