@@ -494,7 +494,9 @@ int rstr_verify_run(rstr_verify* v, int32_t dtype, int32_t batch, int32_t rows, 
  * with the position rotation on the way, attention of one or several new tokens
  * per sequence, and attention over those blocks of a context that a cheap score selects.  Rules of the
  * operators above; a block is a page.  Work of the session's own calls on the same pages is on its stream: the
- * caller orders the two.  A pool with open plans or bounds does not close (RSTR_E_STATE). */
+ * caller orders the two.  A pool with open plans or bounds does not close (RSTR_E_STATE).  An address that
+ * an entry gives out is not counted: closing its owner frees the memory, and who still uses the address then
+ * reads or writes what is no longer there.  A caller that hands it on closes the owner after the last use. */
 
 /* Device address of one slab (0: keys, 1: values) of a layer, fp16 [page][page_size][n_kv][head_dim], valid
  * until the pool is closed. */

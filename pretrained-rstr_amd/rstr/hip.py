@@ -18,8 +18,11 @@ one HIP runtime.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 import sys
+import threading
+import weakref
 
 import numpy as np
 
@@ -218,12 +221,54 @@ def _code(dtype):
     return c
 
 
+_lock = threading.RLock()   # views die on any thread, and inside any allocation
+_late = []                  # memory whose last user has left: freed at once, or when a capture has ended
+
+
+class _Stay:
+    """How long a handle's memory stays: while the handle is open, while views of it live, and while memory that
+    hangs on it (a pool's on its model, bounds' on their pool) stays.  ``free`` runs when the last of these has left,
+    then that of what it hung on."""
+
+    def __init__(self, free, *on):
+        self.free, self.on, self.users = free, on, 1
+        for x in on:
+            x.join()
+
+    def join(self):
+        with _lock:
+            self.users += 1
+
+    def leave(self):
+        with _lock:
+            self.users -= 1
+            if not self.users:
+                _late.append(self)
+        torch = sys.modules.get("torch")
+        if _late and torch is not None and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            return  # freeing waits for the device, which would end the capture: when the next one leaves
+        while True:
+            with _lock:
+                if not _late:
+                    return
+                x = _late.pop(0)
+            x.free()
+            for y in x.on:
+                y.leave()
+
+
 class DeviceView:
     """Device memory that the library owns, in the form the operators take
-    (and torch's ``as_tensor``); it keeps its owner alive, not open."""
+    (and torch's ``as_tensor``, whose tensors keep their view).  While it lives its memory does:
+    closing the owner, or what that hangs on, ends the handle for calls, and the memory is
+    freed once the last view of it has gone."""
 
     def __init__(self, ptr: int, shape, dtype: str, device: int, owner):
         self._ptr, self.shape, self.dtype, self.device, self._owner = ptr, tuple(shape), dtype, device, owner
+        stay = getattr(owner, "_stay", None)
+        if stay is not None:
+            stay.join()
+            weakref.finalize(self, stay.leave).atexit = False
 
     def data_ptr(self) -> int:
         return self._ptr
@@ -328,6 +373,7 @@ class Session:
         if rc != 0:
             raise RstrError(rc, lib().rstr_open_error().decode())
         self.h = h
+        self._stay = _Stay(functools.partial(lib().rstr_session_close, h))
         self.device = device
         self.children = []   # open models, pools, decoders (closed before the session)
 
@@ -345,14 +391,15 @@ class Session:
             raise RstrError(rc, lib().rstr_last_error(self.h).decode())
 
     def close(self):
+        """Closes what is open on it, then itself; memory that views of it still show is freed after them."""
         if self.h:
             order = {"Decoder": 0, "Prefill": 0, "Kv4Attention": 0, "Verifier": 0, "PagedAttention": 0, "BlockSelect": 0,
                      "BlockBounds": 1, "Pool": 2, "Kv4Pool": 2, "Model": 3}
             for obj in sorted(self.children, key=lambda o: order.get(type(o).__name__, 4)):
                 obj.close()
             self.children = []
-            lib().rstr_session_close(self.h)
             self.h = None
+            self._stay.leave()
 
     def tail(self, logits, emb):
         """The decode tail on given logits [rows][vocab] and embedding [vocab][d]
@@ -426,6 +473,7 @@ class Model:
                                        len(tensors), C.byref(h))
         sess.check(rc)
         self.h = h
+        self._stay = _Stay(functools.partial(lib().rstr_model_close, h), sess._stay)
         sess._adopt(self)
 
     @property
@@ -464,9 +512,11 @@ class Model:
         return wq, ws
 
     def close(self):
+        """Ends the handle; the weights are freed once no pool or decoder of it is left."""
         if self.h:
-            lib().rstr_model_close(self.h)
             self.h = None
+            _left(self)
+            self._stay.leave()
 
 
 class Pool:
@@ -478,6 +528,8 @@ class Pool:
         h = C.c_void_p()
         self.sess.check(lib().rstr_pool_open(model.h, page_size, physical_pages, C.byref(h)))
         self.h = h
+        self._stay = _Stay(functools.partial(lib().rstr_pool_close, h), model._stay)
+        self._readers = self._transfers = 0   # open plans and bounds; transfers in flight
         self.sess._adopt(self)
 
     @property
@@ -572,7 +624,7 @@ class Pool:
         h = C.c_void_p()
         self.sess.check(lib().rstr_chunk_export_submit(self.h, _p(pages), pages.size, int(start), int(token_count),
                                                       _p(out), C.byref(h)))
-        return Transfer(self.sess, h, out, (pages, out))
+        return Transfer(self.sess, h, out, (pages, out), self)
 
     def restore_submit(self, pages, start: int, token_count: int, payload) -> "Transfer":
         """Scatter a durable payload (fp16 bits as uint16, or float32) into the route's pages."""
@@ -591,7 +643,7 @@ class Pool:
         h = C.c_void_p()
         self.sess.check(lib().rstr_chunk_restore_submit(self.h, _p(pages), pages.size, int(start), int(token_count),
                                                        _p(payload), dtype, C.byref(h)))
-        return Transfer(self.sess, h, None, (pages, payload))
+        return Transfer(self.sess, h, None, (pages, payload), self)
 
     def chunk_bench(self, pages, start: int, token_count: int, mode: int, iters: int) -> float:
         """Average ms of the gather (mode 0) / scatter (mode 1) kernel alone."""
@@ -636,17 +688,24 @@ class Pool:
         return a.value, b.value
 
     def close(self):
-        """Frees the slabs; refused (RstrError) while chunk transfers are in flight, or plans or bounds open."""
+        """Ends the handle; refused (RstrError) while chunk transfers are in flight, or plans or bounds open.  The
+        slabs are freed once no view of them, and no decoder over them, is left."""
         if self.h:
-            self.sess.check(lib().rstr_pool_close(self.h))
+            if self._transfers:
+                raise RstrError(-4, "pool has chunk transfers in flight")
+            if self._readers:
+                raise RstrError(-4, "pool has open attention plans or block bounds")
             self.h = None
+            _left(self)
+            self._stay.leave()
 
 
 class Transfer:
     """A submitted chunk export/restore; keeps its host buffers alive until completion."""
 
-    def __init__(self, sess: Session, h, payload, retained):
-        self.sess, self.h, self.payload, self._retained = sess, h, payload, retained
+    def __init__(self, sess: Session, h, payload, retained, pool: Pool):
+        self.sess, self.h, self.payload, self._retained, self._pool = sess, h, payload, retained, pool
+        pool._transfers += 1
 
     def done(self) -> bool:
         if self.h is None:  # completed
@@ -662,6 +721,7 @@ class Transfer:
             raise RstrError(-4, "transfer already completed")
         st = TransferStats()
         h, self.h = self.h, None
+        self._pool._transfers -= 1
         self.sess.check(lib().rstr_transfer_complete(h, C.byref(st)))
         self._retained = None
         return {"bytes": int(st.bytes), "device_ms": float(st.device_ms),
@@ -679,6 +739,7 @@ class Decoder:
         self.sess.check(lib().rstr_decoder_open(model.h, pool.h, batch, pages_per_seq, maxpos, split,
                                                 C.byref(h)))
         self.h = h
+        self._stay = _Stay(functools.partial(lib().rstr_decoder_close, h), pool._stay, model._stay)
         self._keep = []
         self.sess._adopt(self)
 
@@ -773,9 +834,11 @@ class Decoder:
         return {k: (float(ms[i]), int(n[i])) for i, k in enumerate(KERNEL_CLASSES)}
 
     def close(self):
+        """Ends the handle; its memory is freed once no view of its logits is left."""
         if self.h:
-            lib().rstr_decoder_close(self.h)
             self.h = None
+            _left(self)
+            self._stay.leave()
 
 
 class Prefill:
@@ -790,6 +853,7 @@ class Prefill:
         self.sess.check(lib().rstr_prefill_open(model.h, pool.h, rows, pages_per_seq, maxpos, split,
                                                 C.byref(h)))
         self.h = h
+        self._stay = _Stay(functools.partial(lib().rstr_decoder_close, h), pool._stay, model._stay)
         self.sess._adopt(self)
 
     def set_graph(self, enabled: bool):
@@ -812,8 +876,9 @@ class Prefill:
 
     def close(self):
         if self.h:
-            lib().rstr_decoder_close(self.h)
             self.h = None
+            _left(self)
+            self._stay.leave()
 
 
 class Kv4Pool:
@@ -940,6 +1005,7 @@ class PagedAttention:
         h = C.c_void_p()
         self.sess.check(lib().rstr_pool_attn_open(pool.h, n_q, max_batch, max_rows, C.byref(h)))
         self.h = h
+        pool._readers += 1
         self.sess._adopt(self)
 
     def run(self, layer: int, q, row_offsets, page_table, lengths, out, max_rows: int | None = None, window: int = 0,
@@ -967,6 +1033,7 @@ class PagedAttention:
         if self.h:
             self.sess.check(lib().rstr_pool_attn_close(self.h))
             self.h = None
+            self.pool._readers -= 1
             _left(self)
 
 
@@ -978,6 +1045,9 @@ class BlockBounds:
         h = C.c_void_p()
         self.sess.check(lib().rstr_bounds_open(pool.h, C.byref(h)))
         self.h = h
+        self._stay = _Stay(functools.partial(lib().rstr_bounds_close, h), pool._stay)
+        self._selections = 0
+        pool._readers += 1
         self.sess._adopt(self)
 
     def update(self, layer: int, row_offsets, page_table, lengths, rows: int, stream=None):
@@ -995,11 +1065,15 @@ class BlockBounds:
         return DeviceView(p.value, (self.pool.physical_pages, c["n_kv"], 2, c["head_dim"]), "float16", self.sess.device, self)
 
     def close(self):
-        """Refused (RstrError) while selections are open."""
+        """Ends the handle; refused (RstrError) while selections are open.  The bounds are freed once no view of them
+        is left."""
         if self.h:
-            self.sess.check(lib().rstr_bounds_close(self.h))
+            if self._selections:
+                raise RstrError(-4, "block bounds have open selections")
             self.h = None
+            self.pool._readers -= 1
             _left(self)
+            self._stay.leave()
 
 
 class BlockSelect:
@@ -1012,6 +1086,7 @@ class BlockSelect:
         h = C.c_void_p()
         self.sess.check(lib().rstr_select_open(bounds.h, n_q, max_batch, max_rows, max_pages, C.byref(h)))
         self.h = h
+        bounds._selections += 1
         self.sess._adopt(self)
 
     def run(self, layer: int, q, row_offsets, page_table, lengths, blocks, first: int = 1, last: int = 1, stream=None):
@@ -1029,6 +1104,7 @@ class BlockSelect:
         if self.h:
             self.sess.check(lib().rstr_select_close(self.h))
             self.h = None
+            self.bounds._selections -= 1
             _left(self)
 
 
