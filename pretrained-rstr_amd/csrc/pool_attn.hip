@@ -51,6 +51,14 @@ __device__ __forceinline__ _Float16 first_term(float x) {
   return (_Float16)__builtin_amdgcn_cvt_pkrtz(x * (1.0f - 0x1p-12f), 0.0f)[0];
 }
 
+// The second: the rest, rounded; of an infinity that infinity again, as both products have to be it.
+__device__ __forceinline__ _Float16 second_term(float x, _Float16 first) {
+  return (_Float16)(fabsf(x) < INFINITY ? x - (float)first : x);
+}
+
+// The size of a query's element, for the largest that its row is brought to: an infinity has none, it stays one at any power of two.
+__device__ __forceinline__ float size_of(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
+
 constexpr int pool_waves(int hd) { return hd == 256 ? 1 : 2; }
 
 // What raw scores of queries that were brought down by 2^e are multiplied with: finite and not 0, so that it leaves the
@@ -249,10 +257,10 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
             for (int i = 0; i < 8; i++) x[s2][i] = 0.0f;
           }
 #pragma unroll
-          for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[s2][i]));
+          for (int i = 0; i < 8; i++) big = fmaxf(big, size_of(x[s2][i]));
         }
         big = xor_max<32>(xor_max<16>(big));
-        // (a largest of 0 or infinity has the exponent 0; the sign of the scale goes into the queries)
+        // (a largest of 0 has the exponent 0; the sign of the scale goes into the queries)
         const int e = __builtin_amdgcn_frexp_expf(big) - 15;
         kcol[t] = score_scale(a.scale, e);
 #pragma unroll
@@ -263,7 +271,7 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
             if (a.scale < 0.0f) y = -y;
             if constexpr (TERMS == 2) {
               q[t][0][s2][i] = first_term(y);
-              q[t][1][s2][i] = (_Float16)(y - (float)q[t][0][s2][i]);
+              q[t][1][s2][i] = second_term(y, q[t][0][s2][i]);
             } else {
               q[t][0][s2][i] = (_Float16)y;
             }
@@ -745,7 +753,7 @@ __global__ void __launch_bounds__(64 * kShareWaves, kShareWaves / 4)
             for (int k = 0; k < 8; k++) x[i][k] = 0.0f;
           }
 #pragma unroll
-          for (int k = 0; k < 8; k++) big = fmaxf(big, fabsf(x[i][k]));
+          for (int k = 0; k < 8; k++) big = fmaxf(big, size_of(x[i][k]));
         }
         big = xor_max<32>(xor_max<16>(big));
         const int e = __builtin_amdgcn_frexp_expf(big) - 15;
@@ -758,7 +766,7 @@ __global__ void __launch_bounds__(64 * kShareWaves, kShareWaves / 4)
             if (a.scale < 0.0f) y = -y;
             if constexpr (TERMS == 2) {
               q[t][0][i][k] = first_term(y);
-              q[t][1][i][k] = (_Float16)(y - (float)q[t][0][i][k]);
+              q[t][1][i][k] = second_term(y, q[t][0][i][k]);
             } else {
               q[t][0][i][k] = (_Float16)y;
             }
