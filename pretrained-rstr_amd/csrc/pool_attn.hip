@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
           for (int i = 0; i < 8; i++) big = fmaxf(big, size_of(x[s2][i]));
         }
         big = xor_max<32>(xor_max<16>(big));
-        // (a largest of 0 has the exponent 0; the sign of the scale goes into the queries)
+        // (a largest of 0 has the exponent 0; the sign of the scale goes into the queries, and a scale of 0 itself: 0 times an infinity is no number)
         const int e = __builtin_amdgcn_frexp_expf(big) - 15;
         kcol[t] = score_scale(a.scale, e);
 #pragma unroll
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             float y = __builtin_amdgcn_ldexpf(x[s2][i], -e);
-            if (a.scale < 0.0f) y = -y;
+            y = a.scale < 0.0f ? -y : a.scale == 0.0f ? y * 0.0f : y;
             if constexpr (TERMS == 2) {
               q[t][0][s2][i] = first_term(y);
               q[t][1][s2][i] = second_term(y, q[t][0][s2][i]);
@@ -763,7 +763,7 @@ __global__ void __launch_bounds__(64 * kShareWaves, kShareWaves / 4)
 #pragma unroll
           for (int k = 0; k < 8; k++) {
             float y = __builtin_amdgcn_ldexpf(x[i][k], -e);
-            if (a.scale < 0.0f) y = -y;
+            y = a.scale < 0.0f ? -y : a.scale == 0.0f ? y * 0.0f : y;
             if constexpr (TERMS == 2) {
               q[t][0][i][k] = first_term(y);
               q[t][1][i][k] = second_term(y, q[t][0][i][k]);

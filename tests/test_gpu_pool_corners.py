@@ -48,3 +48,26 @@ def test_attention_of_infinite_queries(sess, D, n_q, n_kv, page, dtype, news, mo
         vmax = float(v.abs().max())
         _near(out, want, _attn_tol(dt, D, want, mag, size, seen, vmax, prompt=most > 16))
         assert not out[0, 0].any() and not out[-1, 1].any()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 5, 300])
+@pytest.mark.parametrize("scale", [0.0, -0.0])
+def test_attention_of_scale_zero(sess, dtype, D, rows, scale):  # noqa: F811
+    """All tokens alike: their mean; and no number where a score is 0 times an infinity, of either sign, of a key or a query."""
+    rng = np.random.default_rng(D + rows)
+    n_q, n_kv, page, n, dt = 4, 2, 16, 300, TYPES[dtype]
+    with Pooled(sess, n_kv, D, page, 19) as x:
+        k, v = _filled(x, rng, n_kv, D, page, 19)
+        k[0, 3, 0, 7] = float("-inf")
+        x.slab(0).copy_(k)
+        q = torch.tensor(np.abs(rng.standard_normal((rows, n_q, D))) + 0.1, dtype=torch.float32)
+        q[-1, 3, 5] = float("inf")
+        q, out = q.to(dt), torch.empty(rows, n_q, D, dtype=dt, device="cuda")
+        _attend(x, q.cuda(), np.arange(19)[None], [n], [0, rows], out, n_q, scale=scale)
+        finite = torch.nan_to_num(q.float(), posinf=1.0)
+        want, mag, size, seen, _ = P.attention(P.as_f64(finite), np.maximum(P.as_f64(k), -9.0), P.as_f64(v), [list(range(19))], [n], [0, rows], 0, 0.0)
+        want[[r for r in range(rows) if n - rows + r >= 3], :2] = np.nan
+        want[-1, 3] = np.nan
+        _near(out, want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=rows > 16))
