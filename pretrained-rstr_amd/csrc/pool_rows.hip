@@ -207,8 +207,9 @@ __global__ void __launch_bounds__(256) k_bounds_update(BoundsUpdate a) {
 // ---- selection of blocks -----------------------------------------------------------------
 // A row's score of a block is the most that a product of one of the group's queries with a key inside the block's bounds can
 // be: s_j = max over the heads g of sum_d max(q_gd lo_jd, q_gd hi_jd).  Sums are in 64 bits, where products of fp16 with
-// fp16 or bf16 lose nothing: which of two blocks is taken is part of the result.
-// 1. k_block_scores: twice the scores.  2. k_block_pick: the border between what is taken and what is not, and the list in ascending order.
+// fp16 or bf16 lose nothing, and only the bound that a query takes enters them: which of two blocks is taken is part of the result, and
+// blocks whose bounds are alike where the queries take them are equal.
+// 1. k_block_scores: the scores.  2. k_block_pick: the border between what is taken and what is not, and the list in ascending order.
 
 // The blocks that a row's list is chosen from: those from `first` on up to, not with, the last ones.
 struct Choice {
@@ -270,12 +271,12 @@ __device__ double odd_score(const typename E::T* q, int64_t head, int group, con
     if (s != s) return INFINITY;
     best = s > best ? s : best;
   }
-  return 2.0 * best;
+  return best;
 }
 
 // A wave scores `per` blocks for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers
-// twice the larger of q lo and q hi is q (lo + hi) + |q| |hi - lo|, so a bound is converted once for all heads, and a product costs
-// two multiply-adds; where a sum is not finite the block is scored by the definition.  Four steps' bounds are in flight.  32 sequences of 2048 to
+// the larger of q lo and q hi is q hi where q is positive and q lo where it is not: a selection and a multiply-add a product (q (lo + hi) + |q| |hi - lo|, two
+// multiply-adds, would leave the rounding of the bound that is not taken in the sum); where a sum is not finite the block is scored by the definition.  Four steps' bounds are in flight.  32 sequences of 2048 to
 // 16 384 tokens in pages of 16, 32 heads over 8 of 128, f16: 76 MB of bounds in 30 us, twice what reading them takes; by count half of that are conversions
 // and multiply-adds in 64 bits, which make the choice exact.  One sequence of 131 071: 34 MB in 13.8.
 template <int D, int HG, class E>
@@ -326,16 +327,25 @@ __global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* 
       hi[i] = *(const u32x4*)(p + D);
     };
     const auto score = [&](int i, int step) {
-      double s[HG];
+      // (bounds that are not in order, as a caller may write them, count as their least and greatest; a NaN stays one)
+      h2 least[4], most[4], wide = {0, 0};
 #pragma unroll
-      for (int g = 0; g < HG; g++) s[g] = 0.0;
+      for (int k = 0; k < 4; k++) {
+        const uint32_t l = lo[i][k], h = hi[i][k];
+        least[k] = __builtin_elementwise_minimum(__builtin_bit_cast(h2, l), __builtin_bit_cast(h2, h));
+        most[k] = __builtin_elementwise_maximum(__builtin_bit_cast(h2, l), __builtin_bit_cast(h2, h));
+        wide = __builtin_elementwise_maximum(wide, most[k] - least[k]);
+      }
+      double s[HG];
+      // an infinity among the bounds that no query takes here may be a NaN by the definition (0 times it)
+      s[0] = (double)(((float)wide[0] + (float)wide[1]) * 0.0f);
+#pragma unroll
+      for (int g = 1; g < HG; g++) s[g] = 0.0;
 #pragma unroll
       for (int k = 0; k < 8; k++) {
-        const uint32_t wl = lo[i][k >> 1], wh = hi[i][k >> 1];
-        const double x = (double)(float)__builtin_bit_cast(h2, wl)[k & 1], y = (double)(float)__builtin_bit_cast(h2, wh)[k & 1];
-        const double sum = y + x, wide = __builtin_fabs(y - x);
+        const double x = (double)(float)least[k >> 1][k & 1], y = (double)(float)most[k >> 1][k & 1];
 #pragma unroll
-        for (int g = 0; g < HG; g++) s[g] = __builtin_fma(__builtin_fabs(q[g][k]), wide, __builtin_fma(q[g][k], sum, s[g]));
+        for (int g = 0; g < HG; g++) s[g] = __builtin_fma(q[g][k], q[g][k] > 0.0 ? y : x, s[g]);
       }
       double x = scatter_sum<CH, HG>(s);
       int odd = !(__builtin_fabs(x) < INFINITY);

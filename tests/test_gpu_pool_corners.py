@@ -6,7 +6,7 @@ import torch
 
 import pool_plain as P
 from rstr import hip
-from test_gpu_pool_ops import TYPES, Pooled, _attend, _attn_tol, _filled, _i32, _near, _table, sess  # noqa: F401
+from test_gpu_pool_ops import TYPES, Pooled, _attend, _attn_tol, _filled, _i32, _near, _select, _table, sess  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,81 @@ def test_attention_of_scale_zero(sess, dtype, D, rows, scale):  # noqa: F811
         want[[r for r in range(rows) if n - rows + r >= 3], :2] = np.nan
         want[-1, 3] = np.nan
         _near(out, want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=rows > 16))
+
+
+# ---- selection of blocks -----------------------------------------------------------------------
+def _scores(q, lim, ids):
+    """[heads][blocks] of one row and kv head by the definition: q [heads][D], lim [pages][2][D], ids [blocks]."""
+    ok = (ids >= 0) & (ids < len(lim))
+    lo, hi = lim[np.where(ok, ids, 0)].transpose(1, 0, 2)
+    with np.errstate(invalid="ignore"):
+        s = np.stack([np.maximum(x * lo, x * hi).sum(-1) for x in q])
+    s = np.where(np.isnan(s).any(0), np.inf, s.max(0))
+    return np.where(ok, s, -np.inf)
+
+
+def _lists(q, lim, table, cells, page, top, first, last, n_kv):
+    """The lists of rows that all have more blocks than these hold."""
+    out = np.zeros((len(cells), n_kv, top), np.int64)
+    group = q.shape[1] // n_kv
+    for r, (b, p) in enumerate(cells):
+        cur = p // page
+        for h in range(n_kv):
+            s = _scores(q[r, h * group:(h + 1) * group], lim[:, h], table[b, first:cur + 1 - last])
+            best = np.argsort(-s, kind="stable")[:top - first - last]
+            out[r, h] = np.concatenate([np.arange(first), first + np.sort(best), np.arange(cur + 1 - last, cur + 1)])
+    return out
+
+
+@pytest.mark.parametrize("n_q,n_kv,D", [(8, 2, 64), (4, 4, 128), (4, 2, 128), (12, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("wide", [1.0, 1000.0, 60000.0])
+def test_select_of_blocks_that_differ_where_no_query_looks(sess, n_q, n_kv, D, dtype, wide):  # noqa: F811
+    """Blocks that are alike in the bounds that the queries take, however the others differ, are equal: the first of them are taken."""
+    page, pages, n, dt = 4, 400, 390, TYPES[dtype]
+    g = torch.Generator().manual_seed(D + n_q)
+    sign = torch.where(torch.rand(n_kv, 1, D, generator=g) < 0.5, -1.0, 1.0)  # of all heads of a group
+    q = (torch.randn(2, n_kv, n_q // n_kv, D, generator=g).abs() + 0.01) * sign
+    q = q.reshape(2, n_q, D).to(dt)
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        b = x.open(hip.BlockBounds, x.pool)
+        lim = torch.as_tensor(b.device(0), device="cuda")
+        taken = torch.randn(n_kv, D, generator=g)
+        other = torch.rand(pages, n_kv, D, generator=g) * wide
+        lo = torch.where(sign[:, 0] > 0, taken - other, taken)
+        hi = torch.where(sign[:, 0] > 0, taken, taken + other)
+        lim.copy_(torch.stack([lo, hi], 2).half())
+        table = np.random.default_rng(D).permutation(pages)[None, :n]
+        for top, first, last in ((9, 1, 1), (300, 0, 2)):
+            got = _select(x, b, q.cuda(), table, [n * page], [0, 2], top, first, last, n_q, n_kv).cpu().numpy()
+            assert np.array_equal(got, np.broadcast_to(np.concatenate([np.arange(top - last), np.arange(n - last, n)]), got.shape))
+
+
+@pytest.mark.parametrize("n_q,n_kv,D,rows", [(8, 8, 64, 40), (16, 8, 128, 41), (32, 8, 128, 40), (12, 2, 256, 160), (48, 8, 64, 33)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("pages", [1000, 1024, 700])
+def test_select_for_many_rows(sess, n_q, n_kv, D, rows, dtype, pages):  # noqa: F811
+    """Calls whose scores fill the card, and one just below that (700): with blocks that are gone, NaN and infinite bounds
+    among the last of a wave, infinite ones that no query takes, and lists that end inside a wave's blocks."""
+    print("select for many rows", n_q, n_kv, D, rows, dtype, pages, flush=True)
+    if pages == 700:
+        rows = 4095 // (n_kv * 11)
+    page, dt, top, first, last = 4, TYPES[dtype], 40, 1, 2
+    rng = np.random.default_rng(pages + D)
+    lim = rng.standard_normal((pages, n_kv, 2, D)).astype(np.float32)
+    q = rng.standard_normal((rows, n_q, D)).astype(np.float32)
+    table = np.stack([rng.permutation(pages) for _ in range(2)])
+    lim[table[0, [62, 63, 64, 65]], :, 0, 5], lim[table[0, 127], :, :, 6] = np.nan, np.nan
+    lim[table[0, 128], :, 1, 7], lim[table[0, pages - 6], 0, 1, 8], lim[table[0, 300], -1, 0, 9] = np.inf, np.inf, -np.inf
+    q[:, :, 8], q[0, :, 9] = 0.0, np.abs(q[0, :, 9])
+    table[0, [40, 200]], table[1, [1, 64]] = [-1, pages], [2 ** 31 - 1, -7]
+    lengths, offsets = [pages * page, (pages - 30) * page - 3], [0, rows // 2, rows]
+    cells = P.cells(table, lengths, offsets, page, pages, rows)
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        b = x.open(hip.BlockBounds, x.pool)
+        device = torch.as_tensor(b.device(0), device="cuda")
+        device.copy_(torch.tensor(lim).half())
+        q = torch.tensor(q).to(dt)
+        got = _select(x, b, q.cuda(), table, lengths, offsets, top, first, last, n_q, n_kv).cpu().numpy()
+        want = _lists(P.as_f64(q), P.as_f64(device), table, cells, page, top, first, last, n_kv)
+        assert np.array_equal(got, want), np.argwhere(got != want)[:5]
