@@ -83,6 +83,7 @@ struct Part {
   int64_t piece;
   const int32_t* list;      // the row's blocks, or null
   int entries;              // pages (blocks) of it
+  int blocks;               // of a list: blocks of the table that begin at the row's token or before
 };
 
 template <int D>
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
         int id = -1;
         if (LISTED) {
           block = e < s.entries ? s.list[e] : -1;
-          if ((uint32_t)block < (uint32_t)a.pps) id = row[block];
+          if ((uint32_t)block < (uint32_t)s.blocks) id = row[block];  // (later ones hold nothing that the row sees, and their tokens may pass 32 bits)
           else block = 0;
         } else if (e < s.entries) {
           id = row[e];
@@ -545,7 +546,8 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
     s.m = 1;
     s.p0 = of.p;
     s.list = a.blocks + ((int64_t)row * n_kv + s.h) * a.top;
-    s.entries = of.p < 0 ? 0 : min(min(a.top, a.pps), of.p / ps + 1);
+    s.blocks = of.p < 0 ? 0 : min(a.pps, of.p / ps + 1);
+    s.entries = min(a.top, s.blocks);
     const int tiles = (int)(((int64_t)s.entries * ps + kTile - 1) / kTile);
     s.t0 = (LW > 1 ? part * LW + wave : part) * least;
     s.t1 = min(s.t0 + least, tiles);
@@ -572,6 +574,7 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
       s.piece = line.begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w;
       s.list = nullptr;
       s.entries = (int)(((int64_t)L.held(x.len) + ps - 1) / ps);
+      s.blocks = 0;
       work(s);
     }
   }
@@ -1249,7 +1252,8 @@ hipError_t attn_prompt(hipStream_t st, const PoolAttn& a) {
 
 template <int D, class E>
 hipError_t attn_listed(hipStream_t st, const PoolAttn& a) {
-  const int64_t entries = std::min<int64_t>(a.top, a.pps), tiles = (entries * a.c.page_size + kTile - 1) / kTile;
+  // (a row counts no more entries than blocks up to its own)
+  const int64_t entries = std::min<int64_t>(std::min(a.top, a.pps), 0x7FFFFFFF / a.c.page_size + 1), tiles = (entries * a.c.page_size + kTile - 1) / kTile;
   const Cut c = listed_cut(a.n_q, a.c.n_kv, D, a.rows, tiles);
   const int64_t groups = c.waves > 1 ? c.items * c.parts : (c.items + 3) / 4;
   const PoolPieces pc = pool_pieces(a.ws, 0, c.items * c.parts, 16);

@@ -73,6 +73,35 @@ def test_attention_of_scale_zero(sess, dtype, D, rows, scale):  # noqa: F811
         _near(out, want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max()), prompt=rows > 16))
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_of_listed_blocks_past_32_bits(sess, dtype, wide):  # noqa: F811
+    """Blocks whose first token would be 2^32 or more are behind every row, also where a list as long as the table names them."""
+    rng = np.random.default_rng(5)
+    n_q, n_kv, D, page, pages, dt, n = 2, 1, 64, 1 << 18, 2, TYPES[dtype], (1 << 18) + 70
+    width = (1 << 14) + 3
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        k, v = (torch.tensor(rng.standard_normal((pages, 128, n_kv, D))).half() for _ in "kv")
+        x.slab(0)[:, :128].copy_(k)
+        x.slab(1)[:, :128].copy_(v)
+        x.slab(1)[:, 128:].fill_(100.0)
+        table = np.zeros((1, width), np.int64)
+        table[0, 1] = 1
+        # rows at the last two of the sequence's tokens, and one at its block's first
+        q = torch.tensor(rng.standard_normal((70, n_q, D)), dtype=torch.float32).to(dt)
+        blocks = np.full((70, n_kv, width if wide else 2), -1)
+        blocks[:, 0, 0], blocks[:, 0, 1] = 1 << 14, 1
+        blocks[-1, 0, 1] = (1 << 14) + 2
+        out = torch.full((70, n_q, D), 5.0, dtype=dt, device="cuda")
+        _attend(x, q.cuda(), table, [n], [0, 70], out, n_q, blocks=_i32(blocks))
+        kk, vv = P.as_f64(k), P.as_f64(v)
+        short = np.ones((70, n_kv, 1), np.int64)  # the same by pages of 128 tokens: the second one alone
+        want, mag, size, seen, _ = P.attention(P.as_f64(q), kk, vv, [[0, 1]], [128 + 70], [0, 70], 0, D ** -0.5, short)
+        want[-1], mag[-1] = 0.0, 0.0
+        _near(out, want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max())))
+        assert not out[-1].any()
+
+
 # ---- selection of blocks -----------------------------------------------------------------------
 def _scores(q, lim, ids):
     """[heads][blocks] of one row and kv head by the definition: q [heads][D], lim [pages][2][D], ids [blocks]."""
