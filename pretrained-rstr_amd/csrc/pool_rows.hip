@@ -107,11 +107,14 @@ __global__ void __launch_bounds__(256) k_rope_append(RopeAppend a) {
       }
       sum = group_sum<TPH>(sum);
       if (gain) {
-        const float s = (float)(1.0 / __builtin_sqrt(sum * (1.0 / D) + (double)a.eps));
+        const double factor = 1.0 / __builtin_sqrt(sum * (1.0 / D) + (double)a.eps);
+        // in two factors, the first a power of two: for rows next to fp32's largest and smallest numbers theirs is no normal one
+        const float lift = factor > 0x1p126 ? 0x1p64f : factor < 0x1p-126 ? 0x1p-64f : 1.0f;
+        const float s = (float)(factor > 0x1p126 ? factor * 0x1p-64 : factor < 0x1p-126 ? factor * 0x1p64 : factor);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          x[0][i] = (x[0][i] * s) * (a.gain_offset + gain[o0 + i]);
-          x[1][i] = (x[1][i] * s) * (a.gain_offset + gain[o1 + i]);
+          x[0][i] = ((x[0][i] * lift) * s) * (a.gain_offset + gain[o0 + i]);
+          x[1][i] = ((x[1][i] * lift) * s) * (a.gain_offset + gain[o1 + i]);
         }
       }
     }

@@ -6,11 +6,34 @@ import torch
 
 import pool_plain as P
 from rstr import hip
-from test_gpu_pool_ops import TYPES, Pooled, _attend, _attn_tol, _filled, _i32, _near, _select, _table, sess  # noqa: F401
+from test_gpu_pool_ops import TYPES, Pooled, _rope_tol, _attend, _attn_tol, _filled, _i32, _near, _select, _table, sess  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
 SHAPES = [(64, 8, 2, 12), (128, 4, 1, 16), (256, 4, 2, 16)]  # head dim, heads, kv heads, page
+
+
+# ---- rotated append --------------------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [5, 2050])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norms_of_the_largest_and_smallest_rows(sess, D, rows, dtype):  # noqa: F811
+    """Rows whose norm's factor is no normal fp32 number; those of zeros (the second of five in bf16 too) are no numbers without an epsilon."""
+    rng = np.random.default_rng(D)
+    n_q, n_kv, page, dt = 2, 1, 16, TYPES[dtype]
+    size = torch.tensor([2.0 ** 126, 2.0 ** -149 * 1000, 2.0 ** -130, 1.0, 0.0])[torch.arange(rows) % 5][:, None, None]
+    q, k = ((torch.tensor(rng.standard_normal((rows, n, D)), dtype=torch.float32).clamp(-1.9, 1.9) * size).to(dt) for n in (n_q, n_kv))
+    gain = torch.tensor(rng.standard_normal(D), dtype=torch.float32)
+    freqs, positions = torch.tensor(1e4 ** -(np.arange(0, D, 2) / D)), rng.integers(0, 1000, rows)
+    with Pooled(sess, n_kv, D, page, rows // page + 1) as x:
+        out = torch.empty_like(q, device="cuda")
+        x.pool.rope_append(0, k.cuda(), k.cuda(), _i32(np.arange(rows)), _i32(positions), freqs.cuda(), q=q.cuda(), q_out=out,
+                           q_gain=gain.cuda(), k_gain=gain.cuda(), eps=0.0)
+        for got, y in ((out, q), (x.slab(0).reshape(-1, n_kv, D)[:rows], k)):
+            with np.errstate(invalid="ignore"):
+                want, mag = P.rotated(P.as_f64(y), positions, freqs.numpy(), gain.numpy())
+            assert np.array_equal(np.isnan(want), np.broadcast_to((P.as_f64(y) == 0).all(-1, keepdims=True), want.shape))
+            _near(got, want, np.nan_to_num(_rope_tol(got.dtype, want, mag, True)))
 
 
 # ---- attention -----------------------------------------------------------------------------
