@@ -1,12 +1,15 @@
 """Corners of the operators over the fp16 page pool on the GPU, against plain float64 forms.  Tolerances are those that
 test_gpu_pool_ops.py derives."""
+import weakref
+
 import numpy as np
 import pytest
 import torch
 
 import pool_plain as P
 from rstr import hip
-from test_gpu_pool_ops import TYPES, Pooled, _rope_tol, _attend, _attn_tol, _filled, _i32, _near, _select, _table, sess  # noqa: F401
+from test_gpu_pool_ops import (HEADS, TYPES, Pooled, _attend, _attn_tol, _filled, _i32, _laid, _near, _own, _rope_tol, _select, _some_rows,  # noqa: F401
+                               _table, sess)
 
 pytestmark = pytest.mark.gpu
 
@@ -34,6 +37,41 @@ def test_norms_of_the_largest_and_smallest_rows(sess, D, rows, dtype):  # noqa: 
                 want, mag = P.rotated(P.as_f64(y), positions, freqs.numpy(), gain.numpy())
             assert np.array_equal(np.isnan(want), np.broadcast_to((P.as_f64(y) == 0).all(-1, keepdims=True), want.shape))
             _near(got, want, np.nan_to_num(_rope_tol(got.dtype, want, mag, True)))
+
+
+@pytest.mark.parametrize("D,n_q,n_kv,rot,page", [(64, 5, 2, 64, 12), (128, 8, 2, 128, 16), (128, 3, 1, 48, 16), (256, 4, 1, 256, 4), (128, 2, 2, 0, 20)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("how", ["plain", "odd"])
+def test_rope_append_of_many_rows(sess, D, n_q, n_kv, rot, page, dtype, norm, how):  # noqa: F811
+    """Rows enough that a workgroup takes four, the last fewer: norms, parts of a head, slots that are none, any alignment."""
+    print("rope_append of many rows", D, n_q, rot, dtype, norm, how, flush=True)
+    rng = np.random.default_rng(D + rot + page)
+    dt, rows = TYPES[dtype], 2050
+    pages = -(-(rows + 9) // page)
+    q, k, v = (torch.tensor(rng.standard_normal((rows, h, D)) * 3, dtype=torch.float32).to(dt) for h in (n_q, n_kv, n_kv))
+    slots = rng.permutation(pages * page)[:rows].astype(np.int64)
+    gone = [3, 8, 9, 20, 2049]
+    slots[gone] = [-1, pages * page, 2 ** 31 - 1, -2 ** 31, -7]
+    pos = rng.integers(0, 1 << 20, rows)
+    freqs = None if rot == 0 else 500000.0 ** (-np.arange(0, rot, 2) / rot)
+    gains = [rng.standard_normal(D).astype(np.float32) for _ in "qk"] if norm else [None, None]
+    gq, gk = (None if g is None else torch.tensor(g).cuda() for g in gains)
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        for which in (0, 1):
+            x.slab(which).fill_(7.0)
+        out = _laid(torch.full((rows, n_q, D), 5.0, dtype=dt), how)
+        x.pool.rope_append(0, _laid(k, how), _laid(v, how), _i32(slots), None if rot == 0 else _i32(pos),
+                           None if rot == 0 else torch.tensor(freqs).cuda(), q=_laid(q, how), q_out=out, q_gain=gq, k_gain=gk, eps=1e-5,
+                           gain_offset=0.5)
+        y, mag = P.rotated(P.as_f64(q), pos, freqs, gains[0], 1e-5, 0.5)
+        _near(out, y, _rope_tol(dt, y, mag, norm))
+        y, mag = P.rotated(P.as_f64(k), pos, freqs, gains[1], 1e-5, 0.5)
+        keep = np.delete(np.arange(rows), gone)
+        for which, want, tol in ((0, y, _rope_tol(torch.float16, y, mag, norm)), (1, P.as_f64(v), _own(torch.float16, P.as_f64(v)))):
+            got = P.as_f64(x.slab(which)).reshape(-1, n_kv, D)
+            _near(got[slots[keep]], want[keep], tol[keep])
+            assert (got[np.setdiff1d(np.arange(pages * page), slots[keep])] == 7.0).all()
 
 
 # ---- attention -----------------------------------------------------------------------------
@@ -125,6 +163,50 @@ def test_attention_of_listed_blocks_past_32_bits(sess, dtype, wide):  # noqa: F8
         assert not out[-1].any()
 
 
+@pytest.mark.parametrize("n_q,n_kv,D,page", HEADS)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lengths,news", [([1, 300, 64, 131], [1, 1, 1, 1]), ([900, 33, 0, 5000], [2, 1, 1, 2]), ([20011], [3]), ([2100], [1])])
+def test_attention_of_few_rows_rounds_weights_once(sess, n_q, n_kv, D, page, dtype, lengths, news):  # noqa: F811
+    """Where rows do not share tiles the sum of the weights is that of the unrounded ones: 2^-11 of each weight, whole items and joined ones."""
+    rng = np.random.default_rng(n_q + D + page)
+    offsets = np.concatenate([[0], np.cumsum(news)])
+    rows, dt = int(offsets[-1]), TYPES[dtype]
+    pages, width = sum(-(-n // page) for n in lengths), -(-max(lengths) // page)
+    table = _table(rng, lengths, page, pages, width)
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        k, v = _filled(x, rng, n_kv, D, page, pages)
+        q = torch.tensor(rng.standard_normal((rows, n_q, D)), dtype=torch.float32).to(dt)
+        for window in (0, 300):
+            out = torch.empty(rows, n_q, D, dtype=dt, device="cuda")
+            _attend(x, q.cuda(), table, lengths, offsets, out, n_q, max_rows=max(news), window=window)
+            want, mag, size, seen, _ = P.attention(P.as_f64(q), P.as_f64(k), P.as_f64(v), table, lengths, offsets, window, D ** -0.5)
+            _near(out, want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max())))
+
+
+@pytest.mark.parametrize("n_q,n_kv,D,page", HEADS)
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("window", [1, 70, 400])
+def test_attention_of_listed_blocks_in_a_window(sess, n_q, n_kv, D, page, dtype, window):  # noqa: F811
+    """Of the listed blocks' tokens those in the window: for tokens, drafts and a prompt's rows; rows whose list holds none of them are 0."""
+    rng = np.random.default_rng(D + window)
+    lengths, news, dt = [700, 1, 300, 0], [3, 1, 150, 2], TYPES[dtype]
+    offsets = np.concatenate([[0], np.cumsum(news)])
+    rows, pages, width = int(offsets[-1]), sum(-(-n // page) for n in lengths) + 1, -(-700 // page)
+    table = _table(rng, lengths, page, pages, width)
+    blocks = np.full((rows, n_kv, 12), -1)
+    for r, (b, p) in enumerate(P.cells(table, lengths, offsets, page, pages, rows)):
+        for h in range(n_kv):
+            have = list(rng.permutation(max(p, 0) // page + 1))[:int(rng.integers(0, 12))]
+            blocks[r, h, :len(have)] = have
+    with Pooled(sess, n_kv, D, page, pages) as x:
+        k, v = _filled(x, rng, n_kv, D, page, pages)
+        q = torch.tensor(rng.standard_normal((rows, n_q, D)), dtype=torch.float32).to(dt)
+        out = torch.full((rows, n_q, D), 5.0, dtype=dt, device="cuda")
+        _attend(x, q.cuda(), table, lengths, offsets, out, n_q, max_rows=max(news), window=window, blocks=_i32(blocks))
+        want, mag, size, seen, _ = P.attention(P.as_f64(q), P.as_f64(k), P.as_f64(v), table, lengths, offsets, window, D ** -0.5, blocks)
+        _near(out, want, _attn_tol(dt, D, want, mag, size, seen, float(v.abs().max())))
+
+
 # ---- selection of blocks -----------------------------------------------------------------------
 def _scores(q, lim, ids):
     """[heads][blocks] of one row and kv head by the definition: q [heads][D], lim [pages][2][D], ids [blocks]."""
@@ -201,3 +283,31 @@ def test_select_for_many_rows(sess, n_q, n_kv, D, rows, dtype, pages):  # noqa: 
         got = _select(x, b, q.cuda(), table, lengths, offsets, top, first, last, n_q, n_kv).cpu().numpy()
         want = _lists(P.as_f64(q), P.as_f64(device), table, cells, page, top, first, last, n_kv)
         assert np.array_equal(got, want), np.argwhere(got != want)[:5]
+
+
+# ---- memory that is lent -------------------------------------------------------------------------
+def test_tensors_keep_what_they_show(sess):  # noqa: F811
+    """Tensors of pages, bounds and logits outlive their handles and the session, with their values; memory goes with the last of them."""
+    g = torch.Generator().manual_seed(1)
+    with hip.Session(0) as s:
+        x = Pooled(s, 2, 128, 16, 300, layers=2)
+        b = hip.BlockBounds(x.pool)
+        view = x.pool.pages_device(1, 1)
+        alive = weakref.ref(view)
+        made = [torch.as_tensor(view, device="cuda"), torch.as_tensor(x.pool.pages_device(0, 0), device="cuda"), torch.as_tensor(b.device(1), device="cuda")]
+        del view
+        assert alive() is not None  # a tensor holds its view, which holds the memory
+        values = [torch.randn(t.shape, generator=g).half() for t in made]
+        for t, y in zip(made, values):
+            t.copy_(y)
+        torch.cuda.synchronize()
+        b.close()
+        x.pool.close()
+        x.model.close()
+    other = torch.full((64 << 20,), 7.0, device="cuda")  # would land in memory that had been freed
+    for t, y in zip(made, values):
+        assert torch.equal(t.cpu(), y)
+        t.mul_(2.0)
+        assert torch.equal(t.cpu(), y * 2.0)
+    del t, made
+    assert alive() is None and bool((other == 7.0).all())
