@@ -77,12 +77,12 @@ struct BlockSelect {
   const int32_t *row_offsets, *page_table, *lengths;
   int32_t* blocks;
   void* ws;
-  int ws_blocks;  // scores a row and kv head in the workspace
+  int64_t ws_blocks;  // scores a row and kv head in the workspace
 };
-inline int select_stride(int blocks) { return (blocks + 15) / 16 * 16; }  // ws_blocks for tables of that many pages
+inline int64_t select_stride(int blocks) { return ((int64_t)blocks + 15) / 16 * 16; }  // ws_blocks for tables of that many pages
 constexpr int kScoreBlocks = 32;  // blocks that a wave scores, at least
 inline bool select_fits(int n_kv, int rows, int blocks) {  // grids hold it
-  return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * ((blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26);
+  return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * (((int64_t)blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26);
 }
 size_t select_workspace(int n_kv, int rows, int blocks);
 hipError_t launch_block_select(hipStream_t st, int dtype, const BlockSelect& a);

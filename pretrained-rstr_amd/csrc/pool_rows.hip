@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(THREADS) k_block_pick(BlockSelect a, const dou
   const int64_t rh = blockIdx.x;
   const int row = (int)(rh / a.n_kv);
   // scores, asked for before the row's candidates are known (in the workspace wherever they end)
-  const double* from = scores + rh * a.ws_blocks + min(tid * KPT, a.ws_blocks - KPT);
+  const double* from = scores + rh * a.ws_blocks + min(tid * KPT, (int)a.ws_blocks - KPT);
   double s[KPT];
 #pragma unroll
   for (int i = 0; i < KPT / 2; i++) ((u32x4*)s)[i] = a.pps > a.top ? ((const u32x4*)from)[i] : u32x4{0, 0, 0, 0};
@@ -632,8 +632,8 @@ hipError_t select_dim(hipStream_t st, const BlockSelect& a) {
   const int64_t rh = (int64_t)a.rows * a.n_kv;
   // Twice as many blocks a wave where these waves fill the card (32 sequences of up to 1024 blocks: 30.3 us for 33.2; with one sequence, always
   // twice as many: 27 -> 32 us for the selection and its attention).
-  const int per = rh * ((a.pps + 2 * kScoreBlocks - 1) / (2 * kScoreBlocks)) >= 16 * (int64_t)compute_units() ? 2 * kScoreBlocks : kScoreBlocks;
-  const int chunks = (a.pps + per - 1) / per;
+  const int per = rh * (((int64_t)a.pps + 2 * kScoreBlocks - 1) / (2 * kScoreBlocks)) >= 16 * (int64_t)compute_units() ? 2 * kScoreBlocks : kScoreBlocks;
+  const int chunks = (int)(((int64_t)a.pps + per - 1) / per);
   const int64_t units = rh * chunks;
   if (a.pps > a.top) {
     auto f = group == 1 ? k_block_scores<D, 1, E> : group == 2 ? k_block_scores<D, 2, E> : k_block_scores<D, 4, E>;
