@@ -162,7 +162,7 @@ struct Line {
         n = (int)min((int64_t)(per_item - at), u_end - u);
         begins = at == 0;
         ends = at + n == per_item;
-        pieces = ends ? 0 : (int)(quotient(u + per_item - 1, part) - w + 1);
+        pieces = ends ? 0 : pieces_to(quotient(u + per_item - 1, part), w);
         u += n;
         return true;
       }
@@ -232,8 +232,6 @@ struct RowOf {
 };
 
 // ---- host side ----------------------------------------------------------------------
-inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
-
 inline int compute_units() {
   static std::atomic<int> known[64];  // calls may come from several threads
   int dev = 0, n = 0;

@@ -55,6 +55,12 @@ __host__ __device__ inline Seq sequence(const Lines& L, int b) {
   return s;
 }
 
+// Pieces of an item that worker w begins and worker `last` ends.  The first lies in w's second place, the others in their workers' first.
+__host__ __device__ inline int pieces_to(int64_t last, int w) { return (int)(last - w + 1); }
+__host__ __device__ inline int64_t piece_place(int w, bool begins) { return 2 * (int64_t)w + (begins ? 1 : 0); }
+
+inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
 // Items of a call whose sequences are ordered, at most: column tiles that are full, and one a
 // sequence that is not.
 __host__ __device__ inline int64_t attn_items(int n_q, int n_kv, int batch, int rows, int cols) {

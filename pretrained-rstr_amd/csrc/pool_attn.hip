@@ -9,6 +9,7 @@
 #include "../../include/rstr_hip.h"
 #include "attn_line.h"
 #include "device_math.h"
+#include "pool_line.h"
 #include "pool_ops.h"
 
 namespace rstr {
@@ -39,8 +40,6 @@ namespace {
 //
 // The tiles of all (sequence, kv head, column tile) items form one line of units that is cut into equal parts, one
 // a wave, as in kv4_line.h; with a list of blocks every row and kv head is an item, and all have as many parts.
-constexpr int kStart = 4;  // what beginning an item costs, in tiles
-
 template <class E> struct Terms { static constexpr int n = 1; };
 template <> struct Terms<F32> { static constexpr int n = 2; };
 
@@ -58,8 +57,6 @@ __device__ __forceinline__ _Float16 second_term(float x, _Float16 first) {
 
 // The size of a query's element, for the largest that its row is brought to: an infinity has none, it stays one at any power of two.
 __device__ __forceinline__ float size_of(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
-
-constexpr int pool_waves(int hd) { return hd == 256 ? 1 : 2; }
 
 // What raw scores of queries that were brought down by 2^e are multiplied with: finite and not 0, so that it leaves the
 // difference of two equal scores 0 and that of a score and -infinity -infinity.
@@ -122,9 +119,9 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = uniform(threadIdx.x >> 6), w = uniform(blockIdx.x * (LW > 1 ? LW : 4) + wave);
   const int n_kv = a.c.n_kv, group = a.n_q / n_kv, ps = a.c.page_size;
-  const int cap = (int)min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0);
+  const int cap = token_cap(a.pps, ps);
   const int64_t row_bytes = (int64_t)n_kv * D * 2;
-  const uint32_t step_e = kTile / ps, step_off = kTile - step_e * ps;
+  const int step_e = kTile / ps, step_off = kTile - step_e * ps;
 
   const auto work = [&](const Part& s) {
     const auto end_seen = [&](int r) { return min(max(s.p0 + r + 1, 0), cap); };
@@ -176,35 +173,27 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
         page = (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
       };
       // entry and place of the lane's token of each half, and of the tile's first and last token
-      int ent[2], off[2], e_first = (int)((uint32_t)t0 * kTile / (uint32_t)ps), o_first = t0 * kTile - e_first * ps;
+      Place tok[2], first = place_of((uint32_t)t0 * kTile, ps);
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const uint32_t at = (uint32_t)t0 * kTile + 16 * j + col;
-        ent[j] = (int)(at / (uint32_t)ps);
-        off[j] = (int)(at - (uint32_t)ent[j] * ps);
-      }
-      look(e_first);
+      for (int j = 0; j < 2; j++) tok[j] = place_of((uint32_t)t0 * kTile + 16 * j + col, ps);
+      look(first.entry);
       int slot_k[2], slot_v[2], tok_v[2];  // slots of the lane's tokens (-1: none), position of its first token of V
       const auto slots = [&](int tile) {
-        if (uniform((int)((uint32_t)o_first + kTile - 1) / ps + e_first - e0) >= 64) look(e_first);
+        if (uniform(entries_to_end(first, e0, ps)) >= 64) look(first.entry);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          const int at = (ent[j] - e0) & 63, id = __shfl(page, at, 64);
-          slot_k[j] = id < 0 ? -1 : id * ps + off[j];
+          const int at = (tok[j].entry - e0) & 63, id = __shfl(page, at, 64);
+          slot_k[j] = id < 0 ? -1 : id * ps + tok[j].off;
           slot_v[j] = __shfl(slot_k[j], 4 * g, 64);
           if (LISTED) {
-            const int tok = __shfl(block, at, 64) * ps + off[j];
-            tok_v[j] = __shfl(tok, 4 * g, 64);
+            const int position = __shfl(block, at, 64) * ps + tok[j].off;
+            tok_v[j] = __shfl(position, 4 * g, 64);
           } else {
             tok_v[j] = tile * kTile + 16 * j + 4 * g;
           }
-          ent[j] += step_e;
-          off[j] += step_off;
-          if (off[j] >= ps) off[j] -= ps, ent[j]++;
+          forward(tok[j], step_e, step_off, ps);
         }
-        e_first += step_e;
-        o_first += step_off;
-        if (o_first >= ps) o_first -= ps, e_first++;
+        forward(first, step_e, step_off, ps);
       };
       const uint8_t* kbase = (const uint8_t*)a.c.k + (int64_t)s.h * D * 2 + 16 * g;
       const uint8_t* vbase = (const uint8_t*)a.c.v + (int64_t)s.h * D * 2 + 2 * G::PIECE * col;
@@ -571,7 +560,7 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
       s.t0 = x.lo + (whole ? 0 : max(line.at - kStart, 0));
       s.t1 = x.lo + (whole ? x.tiles : max(line.at + line.n - kStart, 0));
       s.whole = line.begins && line.ends;
-      s.piece = line.begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w;
+      s.piece = piece_place(w, line.begins);
       s.list = nullptr;
       s.entries = (int)(((int64_t)L.held(x.len) + ps - 1) / ps);
       s.blocks = 0;
@@ -592,12 +581,6 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
 // matrix instructions are busy 22 % of the time, vector instructions 48 %, and the two waves that a SIMD has registers for wait for LDS and for
 // each other's step the rest.  A third buffer (256), the two halves of a workgroup half a step apart (293, 270), all operands read ahead
 // (283) and two workgroups of four waves (283) gain nothing.
-constexpr int kPromptStart = 8;  // what beginning an item costs, in tiles
-constexpr int kStep = 64;        // tokens at a time
-constexpr int kShareWaves = 8;  // two a SIMD, with half its registers each
-// Tiles of 16 columns a wave: what these registers hold.  Four waves of two tiles instead: 167 us for 98 at D = 256, 556 for 449 in fp32
-// at D = 128 (1900 rows at 5000 tokens, 4 and 32 heads).
-constexpr int prompt_tiles(int hd, int terms) { return hd * terms >= 256 ? 1 : 2; }
 
 typedef short sv4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t* TablePtr;  // read-only for the kernel: scalar loads
@@ -623,7 +606,7 @@ __global__ void __launch_bounds__(64 * kShareWaves, kShareWaves / 4)
   // eight of them in turn)
   const int w = uniform((int)(workers % 8 == 0 ? (blockIdx.x % 8) * (workers / 8) + blockIdx.x / 8 : blockIdx.x));
   const int n_kv = a.c.n_kv, group = a.n_q / n_kv, ps = a.c.page_size;
-  const int cap = (int)min((int64_t)a.pps * ps, (int64_t)0x7FFFFFC0);
+  const int cap = token_cap(a.pps, ps);
   const int64_t row_bytes = (int64_t)n_kv * ROW;
   const Lines L{ro, lens, a.rows, n_kv, group, a.window, COLS, cap, kPromptStart, false};
   Line line(L, a.batch, w, workers, least);
@@ -689,22 +672,17 @@ __global__ void __launch_bounds__(64 * kShareWaves, kShareWaves / 4)
       const int n_pages = (int)(((int64_t)held + ps - 1) / ps);
       const int step_e = kStep / ps, step_off = kStep - step_e * ps;
       // page and place in it of the wave's fours of tokens, and the page's id, read a step ahead of its use
-      int pg[GROUPS], off[GROUPS], id[GROUPS], id_off[GROUPS];
+      Place four[GROUPS];
+      int id[GROUPS], id_off[GROUPS];
 #pragma unroll
-      for (int n = 0; n < GROUPS; n++) {
-        const int tok = t0 * kTile + wave * MINE + 4 * n;
-        pg[n] = tok / ps;
-        off[n] = tok - pg[n] * ps;
-      }
+      for (int n = 0; n < GROUPS; n++) four[n] = place_of((uint32_t)t0 * kTile + wave * MINE + 4 * n, ps);
       const auto look = [&] {
 #pragma unroll
         for (int n = 0; n < GROUPS; n++) {
-          const int v = rowp[min(pg[n], n_pages - 1)];
-          id[n] = pg[n] < n_pages ? v : -1;
-          id_off[n] = off[n];
-          pg[n] += step_e;
-          off[n] += step_off;
-          if (off[n] >= ps) off[n] -= ps, pg[n]++;
+          const int v = rowp[min(four[n].entry, n_pages - 1)];
+          id[n] = four[n].entry < n_pages ? v : -1;
+          id_off[n] = four[n].off;
+          forward(four[n], step_e, step_off, ps);
         }
       };
       const uint8_t* kbase = (const uint8_t*)a.c.k + (int64_t)h * ROW;
@@ -966,7 +944,7 @@ __global__ void __launch_bounds__(64 * kShareWaves, kShareWaves / 4)
       __syncthreads();  // the buffers are the next part's
     }
 
-    const int64_t piece = (begins ? 2 * (int64_t)w + 1 : 2 * (int64_t)w) * COLS;
+    const int64_t piece = piece_place(w, begins) * COLS;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const float sum = xor_add<32>(xor_add<16>(l[t]));
@@ -1026,8 +1004,8 @@ struct Joined {
       const int32_t* ro = L.ro + it.b;
       r0 = min(max(ro[0], 0), L.rows);
       m = max(min(max(ro[1], 0), L.rows) - r0, 0);
-      first = 2 * (int64_t)it.w + 1;
-      rest = 2 * (int64_t)it.w;
+      first = piece_place(it.w, true);
+      rest = piece_place(it.w, false);
     }
     return true;
   }
@@ -1150,64 +1128,16 @@ __global__ void __launch_bounds__(256) k_pool_join(PoolAttn a, Lines L, PoolPiec
 
 // ---- launches ------------------------------------------------------------------------
 constexpr int kMergeWaves = 4096;
-// Tiles of an item that one wave does, without a merge, and twice as many where items occupy half the card: 4 instead costs 34 us for 28 with
-// 128 sequences of 250 tokens, 1 instead 14.0 for 11.8 with one of 128; 16 always saves 55 -> 47 with 128 of 500, but costs 37 for 25 with 32.
-constexpr int kWhole = 8;
-// Tiles a wave takes at least.  1: 17.0 -> 15.6 us for one sequence of 1000 tokens, but 19.3 -> 23.7 for one of 8000; 4: 14.3 -> 18.2 for 300 tokens.
-constexpr int kLeast = 2;
-// And a workgroup of k_pool_prompt: 8 instead costs 22.8 us for 19.4 with 400 rows of 500 tokens, 16 28.7; all are alike from 2000 tokens on.
-constexpr int kPromptLeast = 4;
-// Columns a sequence from which waves share tiles.  Both sides, in us, of one sequence of 4000 tokens and of eight of 2000: D = 128 f16
-// 25.0 | 26.3 and 39.6 | 38.2 with 32 columns, 31.6 | 26.4 and 46.0 | 41.0 with 64; D = 64 17.2 | 19.4 and 24.4 | 20.9 with 64;
-// D = 256 f16 23.4 | 27.9 and 32.0 | 29.9 with 64, 37.7 | 34.4 with 512; D = 256 fp32 40.9 | 46.8 with 128, 38.3 | 44.7 with 512, and with
-// 3600 at 5000 tokens 307 | 152.
-constexpr int many_columns(int hd, int terms) { return hd < 256 ? 64 : terms == 1 ? 128 : 1024; }
-// 16-bit queries: columns a sequence from which items have two tiles of 16 columns, where tables are long enough.  Two tiles | one, in us, 8 rows
-// of four heads a kv head: 24.4 | 27.0 for one sequence of 4000 tokens, 36.6 | 43.1 for 16 of 1000, but 67.6 | 59.6 for 128 of 300.  In fp32 one tile is
-// never slower (45.9 | 44.0 and 82.3 | 61.5).
-constexpr int kTwoTiles = 17, kTwoTilesFrom = 512;
-
-int64_t most_workers(int hd) { return (int64_t)compute_units() * 4 * pool_waves(hd); }
-
-PoolPieces pool_pieces(void* ws, int64_t items, int64_t pieces, int cols) {
+PoolPieces pool_pieces(void* ws, int64_t items, int64_t columns, int hd) {
+  const PoolRoom r = pool_room(sizeof(Begun), items, columns, hd);
   char* p = (char*)ws;
-  PoolPieces pc;
-  pc.n_items = (int*)p;
-  p += 256;
-  pc.begun = (Begun*)p;
-  p += align256(sizeof(Begun) * items);
-  pc.ml = (f4*)p;
-  p += align256(sizeof(f4) * pieces * cols);
-  pc.acc = (float*)p;
-  return pc;
-}
-
-// How the items of lists of blocks are shared out: waves an item, workgroups an item, tiles a wave.
-struct Cut {
-  int64_t items;
-  int waves, parts, tiles;
-};
-constexpr int listed_waves(int hd) { return hd == 256 ? 4 : 8; }
-// A wave an item where these occupy a quarter of the card, and where a list is short (selection and attention together, 100 rows of 8 kv heads: 114 us with
-// a wave an item, 134 with a workgroup, for lists of 64 blocks of 16 tokens, 55 and 72 for 16; 60 rows alike); else a workgroup an item, and where
-// a wave would have more than kListedTiles tiles several (16 instead of 2: 25 us for 12 + 4 with the join, one row, lists of 128 blocks).
-constexpr int kListedTiles = 2;
-Cut listed_cut(int n_q, int n_kv, int hd, int rows, int64_t tiles) {
-  const int group = n_q / n_kv, ncts = (group + 15) / 16;
-  Cut c{(int64_t)rows * n_kv * ncts, 1, 1, (int)tiles};
-  if (tiles <= kLeast || 4 * c.items >= most_workers(hd)) return c;
-  c.waves = listed_waves(hd);
-  const int64_t room = std::max<int64_t>(1, most_workers(hd) / (c.items * c.waves));
-  const int64_t parts = std::min(room, (tiles + (int64_t)c.waves * kListedTiles - 1) / (c.waves * kListedTiles));
-  c.tiles = (int)((tiles + parts * c.waves - 1) / (parts * c.waves));
-  c.parts = (int)((tiles + (int64_t)c.tiles * c.waves - 1) / ((int64_t)c.tiles * c.waves));
-  return c;
+  return PoolPieces{(int*)p, (Begun*)(p + r.begun), (f4*)(p + r.ml), (float*)(p + r.acc)};
 }
 
 template <int D, class E, bool LISTED>
 hipError_t merge(hipStream_t st, const PoolAttn& a, const PoolPieces& pc, int64_t items, int64_t pieces, int cols, int parts) {
   const int group = a.n_q / a.c.n_kv;
-  const int cap = (int)std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0);
+  const int cap = token_cap(a.pps, a.c.page_size);
   const Lines L{a.row_offsets, a.lengths, a.rows, a.c.n_kv, group, a.window, cols, cap, kStart, false};
   // Waves a column: more where an item has many pieces, but not where there are columns enough to fill the card.
   const int64_t columns = std::min<int64_t>(cols, LISTED ? group : (int64_t)a.max_rows * group);
@@ -1221,61 +1151,42 @@ hipError_t merge(hipStream_t st, const PoolAttn& a, const PoolPieces& pc, int64_
 }
 
 template <int D, int NT, class E>
-hipError_t attn_tiles(hipStream_t st, const PoolAttn& a) {
-  const int cols = 16 * NT;
-  const int64_t cap = std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0), tiles = (cap + kTile - 1) / kTile;
-  const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
-  const int64_t most = most_workers(D);
-  const bool whole = tiles <= kWhole || (tiles <= 2 * kWhole && 2 * items >= most);
-  const int64_t want = whole ? items : (items * (tiles + kStart) + kLeast - 1) / kLeast;
-  const int64_t workers = whole ? (items + 3) / 4 * 4 : (std::min(most, want) + 3) / 4 * 4;
-  const PoolPieces pc = pool_pieces(a.ws, items, 2 * workers, cols);
-  hipLaunchKernelGGL((k_pool_attn<D, NT, E, 0>), dim3((unsigned)(workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths, a.page_table,
-                     pc, (int)workers, whole ? 1 : kLeast, whole, 0);
+hipError_t attn_tiles(hipStream_t st, const PoolAttn& a, const PoolForm& f) {
+  const PoolPieces pc = pool_pieces(a.ws, f.items, 2 * f.workers * f.cols, D);
+  hipLaunchKernelGGL((k_pool_attn<D, NT, E, 0>), dim3((unsigned)(f.workers / 4)), dim3(256), 0, st, a, a.row_offsets, a.lengths, a.page_table,
+                     pc, (int)f.workers, f.whole ? 1 : kLeast, f.whole, 0);
   const hipError_t e = hipGetLastError();
-  return e != hipSuccess || whole ? e : merge<D, E, false>(st, a, pc, items, workers, cols, 0);
+  return e != hipSuccess || f.whole ? e : merge<D, E, false>(st, a, pc, f.items, f.workers, f.cols, 0);
 }
 
 template <int D, class E>
-hipError_t attn_prompt(hipStream_t st, const PoolAttn& a) {
-  constexpr int cols = 16 * prompt_tiles(D, Terms<E>::n) * kShareWaves;
-  const int64_t cap = std::min<int64_t>((int64_t)a.pps * a.c.page_size, 0x7FFFFFC0), tiles = (cap + kTile - 1) / kTile;
-  const int64_t items = attn_items(a.n_q, a.c.n_kv, a.batch, a.rows, cols);
-  const int64_t most = compute_units(), want = (items * (tiles + kPromptStart) + kPromptLeast - 1) / kPromptLeast;
-  const int workers = (int)std::min(most, want);
-  const PoolPieces pc = pool_pieces(a.ws, items, 2 * workers, cols);
-  hipLaunchKernelGGL((k_pool_prompt<D, E>), dim3((unsigned)workers), dim3(64 * kShareWaves), 0, st, a, a.row_offsets, a.lengths, a.page_table, pc, workers,
-                     kPromptLeast);
+hipError_t attn_prompt(hipStream_t st, const PoolAttn& a, const PoolForm& f) {
+  const PoolPieces pc = pool_pieces(a.ws, f.items, 2 * f.workers * f.cols, D);
+  hipLaunchKernelGGL((k_pool_prompt<D, E>), dim3((unsigned)f.workers), dim3(64 * kShareWaves), 0, st, a, a.row_offsets, a.lengths, a.page_table, pc,
+                     (int)f.workers, kPromptLeast);
   const hipError_t e = hipGetLastError();
-  return e != hipSuccess ? e : merge<D, E, false>(st, a, pc, items, workers, cols, 0);
+  return e != hipSuccess ? e : merge<D, E, false>(st, a, pc, f.items, f.workers, f.cols, 0);
 }
 
 template <int D, class E>
 hipError_t attn_listed(hipStream_t st, const PoolAttn& a) {
-  // (a row counts no more entries than blocks up to its own)
-  const int64_t entries = std::min<int64_t>(std::min(a.top, a.pps), 0x7FFFFFFF / a.c.page_size + 1), tiles = (entries * a.c.page_size + kTile - 1) / kTile;
-  const Cut c = listed_cut(a.n_q, a.c.n_kv, D, a.rows, tiles);
-  const int64_t groups = c.waves > 1 ? c.items * c.parts : (c.items + 3) / 4;
-  const PoolPieces pc = pool_pieces(a.ws, 0, c.items * c.parts, 16);
+  const Cut c = listed_cut(a.n_q, a.c.n_kv, D, a.rows, a.top, a.pps, a.c.page_size, compute_units());
+  const PoolPieces pc = pool_pieces(a.ws, 0, c.items * c.parts * 16, D);
   auto f = c.waves > 1 ? k_pool_attn<D, 1, E, listed_waves(D)> : k_pool_attn<D, 1, E, 1>;
-  hipLaunchKernelGGL(f, dim3((unsigned)groups), dim3(64 * (c.waves > 1 ? c.waves : 4)), 0, st, a, a.row_offsets, a.lengths, a.page_table,
-                     pc, (int)groups, c.tiles, c.parts == 1, c.parts);
+  hipLaunchKernelGGL(f, dim3((unsigned)c.groups()), dim3(64 * (c.waves > 1 ? c.waves : 4)), 0, st, a, a.row_offsets, a.lengths, a.page_table,
+                     pc, (int)c.groups(), c.tiles, c.parts == 1, c.parts);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess || c.parts == 1 ? e : merge<D, E, true>(st, a, pc, c.items, c.items * c.parts, 16, c.parts);
-}
-
-bool prompts(const PoolAttn& a, int many) {
-  const int64_t group = a.n_q / a.c.n_kv;
-  return a.max_rows * group >= many && a.rows * group >= (int64_t)many * a.batch;
 }
 
 template <int D, class E>
 hipError_t attn_dim(hipStream_t st, const PoolAttn& a) {
   if (a.blocks) return attn_listed<D, E>(st, a);
-  if (prompts(a, many_columns(D, Terms<E>::n))) return attn_prompt<D, E>(st, a);
+  const PoolForm f = pool_form(D, Terms<E>::n, a.n_q, a.c.n_kv, a.batch, a.rows, a.max_rows, token_cap(a.pps, a.c.page_size), compute_units());
+  if (f.prompt) return attn_prompt<D, E>(st, a, f);
   if constexpr (D != 256 && Terms<E>::n == 1)
-    if ((int64_t)a.max_rows * (a.n_q / a.c.n_kv) >= kTwoTiles && (int64_t)a.pps * a.c.page_size > kTwoTilesFrom) return attn_tiles<D, 2, E>(st, a);
-  return attn_tiles<D, 1, E>(st, a);
+    if (f.nt == 2) return attn_tiles<D, 2, E>(st, a, f);
+  return attn_tiles<D, 1, E>(st, a, f);
 }
 
 template <class E>
@@ -1288,10 +1199,7 @@ hipError_t attn_type(hipStream_t st, const PoolAttn& a) {
 }  // namespace
 
 size_t pool_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows) {
-  // a call has at most two pieces a worker, of 32 columns at most; a list's parts are no more than the workers
-  const int64_t prompt = (int64_t)compute_units() * 16 * prompt_tiles(hd, 1) * kShareWaves;
-  const int64_t columns = 2 * std::max(most_workers(hd) * 32, prompt) + 64;
-  return 256 + align256(sizeof(Begun) * attn_items(n_q, n_kv, batch, rows, 16)) + align256(sizeof(f4) * columns) + sizeof(float) * columns * hd;
+  return pool_attn_room(sizeof(Begun), n_q, n_kv, hd, batch, rows, compute_units());
 }
 
 hipError_t launch_pool_attn(hipStream_t st, int dtype, const PoolAttn& a) {

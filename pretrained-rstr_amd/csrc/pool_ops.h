@@ -6,7 +6,7 @@
 #include <stdint.h>
 
 #include "kv4.h"
-#include "kv4_line.h"
+#include "pool_line.h"
 
 struct rstr_pool;
 struct rstr_session;
@@ -52,12 +52,6 @@ struct PoolAttn {
 };
 // Bytes of workspace that every call of up to `rows` query rows and `batch` sequences can need.
 size_t pool_attn_workspace(int n_q, int n_kv, int hd, int batch, int rows);
-// A grid holds fewer than 2^32 threads: of a merge with 256 an item (those with more have few items), and of a wave
-// an item of a list.
-inline bool pool_attn_fits(int n_q, int n_kv, int batch, int rows) {
-  const int64_t dense = attn_items(n_q, n_kv, batch, rows, 16), listed = (int64_t)rows * n_kv * ((n_q / n_kv + 15) / 16);
-  return (int64_t)rows * n_q <= 0x7FFFF000 && dense < (1 << 24) && listed < (1 << 24);
-}
 hipError_t launch_pool_attn(hipStream_t st, int dtype, const PoolAttn& a);
 
 // Bounds of one layer's blocks: fp16 [page][n_kv][2][hd], the least and the greatest key element of a channel.
@@ -79,11 +73,6 @@ struct BlockSelect {
   void* ws;
   int64_t ws_blocks;  // scores a row and kv head in the workspace
 };
-inline int64_t select_stride(int blocks) { return ((int64_t)blocks + 15) / 16 * 16; }  // ws_blocks for tables of that many pages
-constexpr int kScoreBlocks = 32;  // blocks that a wave scores, at least
-inline bool select_fits(int n_kv, int rows, int blocks) {  // grids hold it
-  return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * (((int64_t)blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26);
-}
 size_t select_workspace(int n_kv, int rows, int blocks);
 hipError_t launch_block_select(hipStream_t st, int dtype, const BlockSelect& a);
 

@@ -5,6 +5,7 @@
 #include "../../include/rstr_hip.h"
 #include "attn_line.h"
 #include "device_math.h"
+#include "pool_line.h"
 #include "pool_ops.h"
 
 namespace rstr {
@@ -630,14 +631,11 @@ hipError_t select_dim(hipStream_t st, const BlockSelect& a) {
   double* scores = (double*)a.ws;
   const int group = a.n_q / a.n_kv;
   const int64_t rh = (int64_t)a.rows * a.n_kv;
-  // Twice as many blocks a wave where these waves fill the card (32 sequences of up to 1024 blocks: 30.3 us for 33.2; with one sequence, always
-  // twice as many: 27 -> 32 us for the selection and its attention).
-  const int per = rh * (((int64_t)a.pps + 2 * kScoreBlocks - 1) / (2 * kScoreBlocks)) >= 16 * (int64_t)compute_units() ? 2 * kScoreBlocks : kScoreBlocks;
-  const int chunks = (int)(((int64_t)a.pps + per - 1) / per);
-  const int64_t units = rh * chunks;
+  const ScoreCut cut = score_cut(rh, a.pps, compute_units());
+  const int64_t units = rh * cut.chunks;
   if (a.pps > a.top) {
     auto f = group == 1 ? k_block_scores<D, 1, E> : group == 2 ? k_block_scores<D, 2, E> : k_block_scores<D, 4, E>;
-    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, chunks, per);
+    hipLaunchKernelGGL(f, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, scores, cut.chunks, cut.per);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
