@@ -1,5 +1,4 @@
-// device_args.h -- what the C entries of the operators on device arrays share: the session's device for a
-// call, its stream, and the checks of arrays that the host can see.
+// device_args.h -- what the C entries of the operators on device arrays share: the stream of a call, and the checks of arrays that the host can see.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -10,20 +9,6 @@
 
 namespace rstr {
 namespace {
-
-// The session's device for the length of a call; the caller's own comes back.
-struct OnDevice {
-  int was = -1;
-  hipError_t e;
-  explicit OnDevice(int device) {
-    e = hipGetDevice(&was);
-    if (e == hipSuccess && was != device) e = hipSetDevice(device);
-    else if (e == hipSuccess) was = -1;
-  }
-  ~OnDevice() {
-    if (was >= 0) (void)hipSetDevice(was);
-  }
-};
 
 inline hipStream_t on_stream(rstr_session* s, void* stream) {
   return stream == RSTR_SESSION_STREAM ? s->stream : (hipStream_t)stream;

@@ -334,9 +334,10 @@ extern "C" int rstr_session_open(int32_t device, rstr_session** out) {
   return RSTR_OK;
 }
 
+// Handles may close wherever the last view of their memory dies, so closing leaves the caller's device.
 extern "C" int rstr_session_close(rstr_session* s) {
   if (!s) return RSTR_OK;
-  hipSetDevice(s->device);
+  OnDevice dev(s->device);
   hipStreamSynchronize(s->stream);
   hipStreamDestroy(s->stream);
   delete s;
@@ -645,7 +646,7 @@ extern "C" int rstr_model_bind_raw(rstr_session* s, const rstr_model_desc* desc,
 
 extern "C" int rstr_model_close(rstr_model* m) {
   if (!m) return RSTR_OK;
-  hipSetDevice(m->s->device);
+  OnDevice dev(m->s->device);
   hipStreamSynchronize(m->s->stream);
   model_free(m);
   return RSTR_OK;
@@ -766,7 +767,7 @@ extern "C" int rstr_pool_close(rstr_pool* p) {
   if (!p) return RSTR_OK;
   if (p->open_transfers > 0) return fail(p->m->s, RSTR_E_STATE, "pool has chunk transfers in flight");
   if (p->held > 0) return fail(p->m->s, RSTR_E_STATE, "pool has open attention plans or block bounds");
-  hipSetDevice(p->m->s->device);
+  OnDevice dev(p->m->s->device);
   if (p->shared) (void)hipDeviceSynchronize();
   {
     std::lock_guard<std::mutex> lock(g_pools_mu);
@@ -1228,8 +1229,8 @@ extern "C" int rstr_prefill_open(rstr_model* m, rstr_pool* p, int32_t rows, int3
 
 extern "C" int rstr_decoder_close(rstr_decoder* d) {
   if (!d) return RSTR_OK;
-  hipSetDevice(d->m->s->device);
-  hipStreamSynchronize(d->m->s->stream);
+  OnDevice dev(d->m->s->device);
+  (void)hipDeviceSynchronize();  // (the logits may be read on any stream)
   decoder_free(d);
   return RSTR_OK;
 }

@@ -20,6 +20,20 @@ namespace rstr {
 // Leaves `msg` with the session (or with the thread's open error) and returns `code`.
 int fail(rstr_session* s, int code, const std::string& msg);
 
+// The session's device for the length of a call; the caller's own comes back.
+struct OnDevice {
+  int was = -1;
+  hipError_t e;
+  explicit OnDevice(int device) {
+    e = hipGetDevice(&was);
+    if (e == hipSuccess && was != device) e = hipSetDevice(device);
+    else if (e == hipSuccess) was = -1;
+  }
+  ~OnDevice() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
+
 // hipMalloc, tried again without the blocks that the pools of this GPU keep
 // for isolated attention when it does not fit.
 hipError_t device_alloc(void** p, size_t bytes);
