@@ -517,7 +517,8 @@ int rstr_pool_rope_append(rstr_pool* p, int32_t layer, int32_t rows, int32_t dty
                           const double* frequencies, const int32_t* positions, const int32_t* slots, void* stream);
 
 /* A plan for attention of up to max_batch sequences and max_rows query rows of n_q heads: the call's
- * workspace.  n_kv * (max_rows * (n_q / n_kv) / 16 + the smaller of max_rows and max_batch), and rows * n_kv, < 2^24.
+ * workspace.  n_kv * (max_rows * (n_q / n_kv) / 16 + the smaller of max_rows and max_batch) < 2^24, max_rows * n_kv times the 16s
+ * of n_q / n_kv (rounded up) < 2^24, max_rows * n_q < 2^31 - 4095, n_q up to 65536.
  * One plan serves one call at a time: calls (and graphs that hold them) that may run at once need a plan each. */
 int rstr_pool_attn_open(rstr_pool* p, int32_t n_q, int32_t max_batch, int32_t max_rows, rstr_pool_attn** out);
 /* Waits for the device. */
@@ -525,7 +526,8 @@ int rstr_pool_attn_close(rstr_pool_attn* a);
 /* Attention over one layer; sequences, rows, positions, window and what is not seen are those of rstr_kv4_attn_run:
  * out = sum softmax(scale * q . k_j) v_j over the tokens j <= p that the row at token p sees, in the type of q (f32:
  * products and sums in fp32 precision; f16, bf16: probabilities rounded to 11 bits; a query's elements are off by 2^-39 of
- * its largest where that is more).  A row that sees no token is 0, and so is one whose scores are all -infinity.  What is
+ * its largest where that is more).  A row that sees no token is 0, and so is one whose scores are all -infinity (an infinite element of a
+ * query gives scores by the formula: infinite ones, no number where the key's is 0).  What is
  * in a token that a row does not see, NaN and infinities among it, does not reach it.  (An infinite value whose weight is below
  * 2^-23 of the row's largest may give NaN.)
  * blocks NULL: all blocks.  Else int32 [rows][n_kv][blocks_per_row]: a row of a query and kv head sees only the tokens of
@@ -563,7 +565,8 @@ int rstr_select_close(rstr_select* a);
  * row at token p has the blocks 0 .. p / page_size (of its table).  Where they fit, all are listed; else the `first` first
  * ones, the `last` last ones (one at least: the row's own), and of those between them the ones of the highest score, of equal
  * ones the first.  A block's score is the most that a key inside its bounds can give: the largest over the group's
- * query heads of sum_d max(q_d lo_d, q_d hi_d), in 64 bits; a sum that is no number counts as infinity, a block whose
+ * query heads of sum_d max(q_d lo_d, q_d hi_d), in 64 bits (a bound that a query does not take leaves nothing in its
+ * sum); a sum that is no number counts as infinity, a block whose
  * page is outside the pool as -infinity.  A row without a position (more rows than tokens) lists none.  Rows behind row_offsets[batch] are
  * left as they are; where row_offsets decrease anywhere, nothing is written.  The list overlaps no input. */
 int rstr_select_run(rstr_select* a, int32_t layer, int32_t dtype, int32_t batch, int32_t rows, const void* q, int64_t q_row,

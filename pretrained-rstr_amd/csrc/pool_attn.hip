@@ -35,7 +35,7 @@ namespace {
 // subnormals begin 2^24 below the largest.  p is one fp16 term (f16, bf16) or two (fp32).  S, m, l and O are fp32.
 //
 // Memory bounds it: 128 sequences of 128 to 4608 tokens, 32 heads over 8 of 128, f16, read 1.24 GB in 219 us (5.7 TB/s), four of 9000 to
-// 131 000 733 MB in 132 (5.5), 33 of 5 to 8192 with 1 to 6 fp32 rows 556 MB in 111 (5.0).  Two waves a SIMD, each with the next tile's K and V in
+// 131 000 733 MB in 133 (5.5), 33 of 5 to 8192 with 1 to 6 fp32 rows 556 MB in 111 (5.0).  Two waves a SIMD, each with the next tile's K and V in
 // registers: three waves spill (335, 200 and 193 us); loads that bypass the caches' order are worth 234 -> 220 in the first.
 //
 // The tiles of all (sequence, kv head, column tile) items form one line of units that is cut into equal parts, one
@@ -576,11 +576,13 @@ __global__ void __launch_bounds__(listed_threads(LW), pool_waves(D))
 // transposing reads of four tokens x 16 dims.  A row of a token is swizzled in LDS by its number, 16 bytes at a time, so that 16 tokens' same
 // dims lie in different banks; the loads into LDS write 1 KB in the lanes' order, so a lane asks for the piece that
 // belongs to its place.
-// 333 and 1000 rows at 333 and 9000 tokens, 32 heads over 8 of 128, bf16: 250 us, 560 TFLOP/s (four-row waves that load for themselves: 383).  No
-// one part of a step bounds it: without its exponentials it takes 219 us, without either product 204 and 214, without its loads 219;
-// matrix instructions are busy 22 % of the time, vector instructions 48 %, and the two waves that a SIMD has registers for wait for LDS and for
+// 333 and 1000 rows at 333 and 9000 tokens, 32 heads over 8 of 128, bf16: 240 us with the join in calls back to back, 584 TFLOP/s; in launches that stand apart,
+// under the profiler, 253 and 13 for the join (four-row waves that load for themselves: 383).  No one part of a step bounds it: of then 250 us it
+// took 219 without its exponentials, 204 and 214 without either product, 219 without its loads;
+// matrix instructions are busy 25 % of the time, vector instructions 42 %, and the two waves that a SIMD has registers for wait for LDS and for
 // each other's step the rest.  A third buffer (256), the two halves of a workgroup half a step apart (293, 270), all operands read ahead
-// (283) and two workgroups of four waves (283) gain nothing.
+// (283) and two workgroups of four waves (283) gain nothing.  Head dim 64 has half the products to an exponential (vector 53 %, matrix 19 %); 256 one tile of columns a
+// wave, so that an operand read from LDS feeds one product (waits 59 %, matrix 21 %).
 
 typedef short sv4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t* TablePtr;  // read-only for the kernel: scalar loads

@@ -128,8 +128,8 @@ constexpr int kScoreBlocks = 32;  // blocks that a wave scores, at least
 inline bool select_fits(int n_kv, int rows, int blocks) {  // grids hold it
   return (int64_t)rows * n_kv < (1 << 24) && (double)rows * n_kv * (((int64_t)blocks + kScoreBlocks - 1) / kScoreBlocks) < (double)(1 << 26);
 }
-// Blocks a wave, and waves a row and kv head (`rh` of these).  Twice as many blocks a wave where these waves fill the card (32 sequences of up to 1024
-// blocks: 30.3 us for 33.2; with one sequence, always twice as many: 27 -> 32 us for the selection and its attention).
+// Blocks a wave, and waves a row and kv head (`rh` of these).  Twice as many blocks a wave where these waves fill the card (selection and attention of 32
+// sequences of up to 1024 blocks: 74.1 us for 77.2; of one sequence of 8192 blocks 46.1 for 45.4).
 struct ScoreCut {
   int per, chunks;
 };
@@ -154,7 +154,7 @@ __host__ __device__ inline void forward(Place& p, int step_entries, int step_off
   p.off += step_off;
   if (p.off >= page_size) p.off -= page_size, p.entry++;
 }
-// Does the tile that begins at `first` reach behind the 64 entries from `from` on?
+// Entries from `from` to that of the last token of the tile that begins at `first`: from 64 on, 64 entries from `from` on do not hold it.
 __host__ __device__ inline int entries_to_end(Place first, int from, int page_size) {
   return (int)((uint32_t)first.off + kTile - 1) / page_size + first.entry - from;
 }

@@ -281,8 +281,8 @@ __device__ double odd_score(const typename E::T* q, int64_t head, int group, con
 // A wave scores `per` blocks for one row and kv head, D / 8 lanes a block, HG heads of the group at a time.  With finite numbers
 // the larger of q lo and q hi is q hi where q is positive and q lo where it is not: a selection and a multiply-add a product (q (lo + hi) + |q| |hi - lo|, two
 // multiply-adds, would leave the rounding of the bound that is not taken in the sum); where a sum is not finite the block is scored by the definition.  Four steps' bounds are in flight.  32 sequences of 2048 to
-// 16 384 tokens in pages of 16, 32 heads over 8 of 128, f16: 76 MB of bounds in 30 us, twice what reading them takes; by count half of that are conversions
-// and multiply-adds in 64 bits, which make the choice exact.  One sequence of 131 071: 34 MB in 13.8.
+// 16 384 tokens in pages of 16, 32 heads over 8 of 128, f16: 76 MB of bounds in 33 us, twice what reading them takes; vector instructions are busy
+// half of that, with selections, conversions and multiply-adds in 64 bits.  One sequence of 131 071: 34 MB in 15.
 template <int D, int HG, class E>
 __global__ void __launch_bounds__(256, 4) k_block_scores(BlockSelect a, double* __restrict__ scores, int chunks, int per) {
   typedef typename E::T T;
